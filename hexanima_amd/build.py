@@ -20,7 +20,7 @@ MOSS_LIB = os.path.join(HERE, "libhexanima_moss.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 PROGRAMS = ["hxa_run", "hxa_blk"]
 SOURCES = ["gemm.hip", "gemm_f16.hip", "gemm_q8.hip", "gemm_q4.hip", "gemm_skinny.hip",
-           "attention.hip", "elementwise.hip", "runtime.hip", "dit.hip", "noalloc.hip"]
+           "attention.hip", "causal_attn.hip", "causal_heads.hip", "elementwise.hip", "runtime.hip", "dit.hip", "noalloc.hip"]
 
 ARCH = os.environ.get("HXA_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")

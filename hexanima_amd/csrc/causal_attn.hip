@@ -1,0 +1,974 @@
+// Causal attention with grouped heads: over packed prompts (hxa_attention_causal) and over a paged cache with a shared prefix
+// (hxa_attention_cached). fp16 / bf16 in and out, heads of 64, 128 or 256, fp32 softmax.
+//
+// Rows. The G = Hq / Hk query heads that read one key head are rows of one problem: row R of a sequence is token R / G, head
+// h G + R % G. A workgroup of 4 waves takes consecutive rows of one sequence and one key head, so a key tile is loaded once for all G
+// heads, and the rows of a tile span few tokens: less of the diagonal is computed to be masked.
+//
+// Online softmax: over 64-key tiles S = K Q^T, p = 2^(c S - c m) with c = scale log2(e) and the running maximum m, l += p,
+// O^T = V^T P^T. O and l are rescaled only when m grows by more than 5.5 nats (p <= e^5.5 otherwise, well within fp16).
+// p is rounded to the input type, as the matrix product takes it; S, m, l and O stay in fp32.
+//
+// Tiles move global -> LDS directly, rows of K and V as they lie in memory, double buffered, one barrier a tile. V is transposed
+// on its way out of LDS (ds_read_b64_tr_b16: 16 lanes that read 4 keys x 16 dims get 4 keys of one dim each), so no
+// caller has to keep V transposed. K row order and chunk swizzles are chosen so that the scores in the accumulators
+// are the B operand of the P V product and that the reads of 16 (32) lanes spread over the 64 LDS banks.
+//
+// Modes of a workgroup:
+//   rows (W = 4): 128 rows, 32 a wave, every wave all 64 keys of a tile (32x32x16 MFMAs)
+//   rows (W = 2): 64 rows, the two halves of the tile's keys to two waves each, joined at the end
+//   few rows:     16 rows, 16 keys of the tile to each wave (16x16 MFMAs), joined at the end; bound by reading the cache
+//
+// What a mask hides has no part in a result: hidden scores become -inf before the maximum; values of keys that no row of the workgroup sees are
+// zeroed in LDS (0 x NaN would be NaN), and values of keys that only some rows see are, where they are not finite, taken out of the
+// matrix product and added by the rows that see them (add_apart).
+#include <cmath>
+#include <mutex>
+
+#include "causal.h"
+#include "kernels.h"
+
+namespace {
+
+constexpr int KT = 64;              // keys a tile
+constexpr float L2E = 1.4426950408889634f;
+constexpr float RESCALE2 = 5.5f * L2E;  // growth of the maximum, in powers of two, that is left unscaled
+
+HXA_DEV float16_t mma32(half8_t a, half8_t b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+HXA_DEV float16_t mma32(bf8_t a, bf8_t b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+HXA_DEV float4_t mma16(half8_t a, half8_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+HXA_DEV float4_t mma16(bf8_t a, bf8_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+typedef short short4_t __attribute__((ext_vector_type(4)));
+HXA_DEV float4_t mma16h(half4_t a, half4_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+HXA_DEV float4_t mma16h(bf4_t a, bf4_t b, float4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4_t, a), __builtin_bit_cast(short4_t, b), c, 0, 0, 0);
+}
+typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+template <typename V4>
+HXA_DEV V4 read_tr(const uint8_t *p) {
+  return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *)(lds_void_t *)p));
+}
+HXA_DEV float max16(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48, which all get it
+  const int x = __builtin_bit_cast(int, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  v = fmaxf(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1]));
+  float lo, hi;
+  halves(v, lo, hi);
+  return fmaxf(lo, hi);
+}
+HXA_DEV float add16(float v) {
+  const int x = __builtin_bit_cast(int, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  v = __builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]);
+  float lo, hi;
+  halves(v, lo, hi);
+  return lo + hi;
+}
+
+// where the keys of a work item lie
+template <typename T>
+struct Keys {
+  const T *k, *v;   // contiguous: row 0 of the sequence and key head; paged: the pools
+  long ldk, ldv;    // contiguous: row strides
+  const int *prefix, *table;  // paged: the prefix's pages, the sequence's own
+  int P, page, npages, H, h;
+};
+
+// a work item: rows [r0, r0 + rows of the mode) of nrows rows that belong together, keys [x0, x1)
+struct Item {
+  int r0, nrows, G;
+  int tok0;  // row R is token tok0 + R / G of the call
+  int x0, x1;
+  // row R sees the keys x <= base + R / G (not causal: base), but none past cap, and those up to least in any case
+  int base, cap, least;
+  bool causal;
+};
+HXA_DEV int row_limit(const Item &it, int R) { return max(min(it.causal ? it.base + R / it.G : it.base, it.cap), it.least); }
+
+template <typename T, int HD>
+struct Geo {
+  static constexpr int RB = HD * 2;          // bytes of a row
+  static constexpr int TB = KT * RB;         // of a tile
+  static constexpr int CH = HD / 8;          // 16-byte chunks a row = lanes a row of a load
+  static constexpr int RPL = 64 / CH;        // rows of one wave-wide load (1 KB)
+  static constexpr int NLD = KT / RPL / 4;   // loads a wave and tile, for K and for V each
+  static constexpr int FLAGS = 4 * TB;       // LDS past the tiles: the flags of fix_v
+  static constexpr int LDS = 4 * TB + 64;
+};
+
+// The tile loader, for all modes: K row i of LDS holds key (PERM ? krow_key(i) : i) of the tile, chunk c of a row at c ^ fk(row);
+// V row i holds key i, chunk c at c ^ fv(row).
+template <typename T, int HD, bool PERM>
+struct Swz {
+  static HXA_DEV int fk(int row) { return HD == 64 ? (row >> 1) & 7 : row & 15; }
+  // PERM (rows modes): 32 lanes read 4 keys x 64 bytes; few rows: 8 keys x 32 bytes
+  static HXA_DEV int fv(int row) {
+    if (PERM) return HD == 64 ? (row & 2) << 1 : (row & 3) << 2;
+    return HD == 64 ? (row & 6) : (row & 7) << 1;
+  }
+};
+
+template <typename T, int HD, bool PERM, bool PAGED>
+struct Loader {
+  typedef Geo<T, HD> G_;
+  typedef Swz<T, HD, PERM> S_;
+  const Keys<T> &s;
+  const Item &it;
+  uint8_t *lds;
+  int lane, wave;
+  uint32_t koff[G_::NLD], voff[G_::NLD];  // contiguous: byte offsets within a whole tile; paged: chunk offsets within a row
+  int ent;         // paged: the page entry of this lane's key in the tile that is loaded next
+  uint32_t row;    // paged: page row of this lane's key in the tile loaded last (key = lane)
+  uint32_t prow;   // and in the one before
+  HXA_DEV Loader(const Keys<T> &s_, const Item &it_, uint8_t *lds_, int lane_, int wave_) : s(s_), it(it_), lds(lds_), lane(lane_), wave(wave_) {
+    row = prow = 0;
+    ent = -1;
+#pragma unroll
+    for (int j = 0; j < G_::NLD; j++) {
+      const int r = (j * 4 + wave) * G_::RPL + lane / G_::CH, c = lane % G_::CH;
+      const int kr = PERM ? krow_key(r) : r;
+      const int ck = c ^ S_::fk(r), cv = c ^ S_::fv(r);
+      koff[j] = PAGED ? ck * 16u : ((uint32_t)kr * (uint32_t)s.ldk + ck * 8) * 2u;
+      voff[j] = PAGED ? cv * 16u : ((uint32_t)r * (uint32_t)s.ldv + cv * 8) * 2u;
+    }
+    if (PAGED) entry(0);
+  }
+  HXA_DEV uint8_t *kbuf(int i) const { return lds + (i & 1) * G_::TB; }
+  HXA_DEV uint8_t *vbuf(int i) const { return lds + (2 + (i & 1)) * G_::TB; }
+  HXA_DEV void entry(int i) {  // look up the page of this lane's key of tile i
+    const int x = it.x0 + i * KT + lane;
+    ent = -1;
+    if (x < it.x1) {
+      const bool pre = x < s.P;
+      const unsigned y = pre ? x : x - s.P;
+      ent = (pre ? s.prefix : s.table)[y / (unsigned)s.page];
+    }
+  }
+  // tile i into its buffer; returns the mask of its keys that are there
+  HXA_DEV uint64_t load(int i) {
+    const int key0 = it.x0 + i * KT;
+    if constexpr (PAGED) {
+      const int x = key0 + lane;
+      const unsigned y = x < s.P ? x : x - s.P;
+      const bool ok = x < it.x1 && (unsigned)ent < (unsigned)s.npages;
+      prow = row;
+      row = ok ? ((uint32_t)ent * s.H + s.h) * s.page + y % (unsigned)s.page : 0;  // < 2^32: checked on the host
+      const uint64_t mask = __ballot(ok);
+      if (key0 + KT < it.x1) entry(i + 1);
+#pragma unroll
+      for (int j = 0; j < G_::NLD; j++) {
+        const int blk = j * 4 + wave, r = blk * G_::RPL + lane / G_::CH;
+        const uint32_t rk = __shfl((int)row, PERM ? krow_key(r) : r), rv = PERM ? (uint32_t)__shfl((int)row, r) : rk;
+        g2l16_opaque((const uint8_t *)s.k + (uint64_t)rk * G_::RB + koff[j], kbuf(i) + blk * 1024);
+        g2l16_opaque((const uint8_t *)s.v + (uint64_t)rv * G_::RB + voff[j], vbuf(i) + blk * 1024);
+      }
+      return mask;
+    } else {
+      const T *kt = s.k + (long)key0 * s.ldk, *vt = s.v + (long)key0 * s.ldv;
+      if (key0 + KT <= it.x1) {
+#pragma unroll
+        for (int j = 0; j < G_::NLD; j++) g2l16_sbase(kt, koff[j], kbuf(i) + (j * 4 + wave) * 1024);
+#pragma unroll
+        for (int j = 0; j < G_::NLD; j++) g2l16_sbase(vt, voff[j], vbuf(i) + (j * 4 + wave) * 1024);
+        return ~0ull;
+      }
+      const int last = it.x1 - 1 - key0;  // rows past the keys read the last one
+      int ln = lane;
+      asm volatile("" : "+v"(ln));  // opaque: the loop keeps none of these addresses in registers
+#pragma unroll
+      for (int j = 0; j < G_::NLD; j++) {
+        const int blk = j * 4 + wave, r = blk * G_::RPL + ln / G_::CH, c = ln % G_::CH;
+        const int kr = min(PERM ? krow_key(r) : r, last), vr = min(r, last);
+        g2l16_sbase(kt, ((uint32_t)kr * (uint32_t)s.ldk + (c ^ S_::fk(r)) * 8) * 2u, kbuf(i) + blk * 1024);
+        g2l16_sbase(vt, ((uint32_t)vr * (uint32_t)s.ldv + (c ^ S_::fv(r)) * 8) * 2u, vbuf(i) + blk * 1024);
+      }
+      return (2ull << last) - 1;
+    }
+  }
+  // global address of the value row of key f of the tile before the one loaded last (cur: of the one loaded last)
+  HXA_DEV const T *vrow(int i, int f, bool cur) const {
+    if constexpr (PAGED) return s.v + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(cur ? row : prow), f) * HD;
+    return s.v + (long)(it.x0 + i * KT + f) * s.ldv;
+  }
+};
+
+// The values of tile i where the mask cuts it: rows of keys that are not there (km) become zeros; so do rows that only some rows of
+// the workgroup see (keys past lim_min) and that hold an infinity or NaN: their mask is returned. Whole workgroup, ends with a barrier.
+template <typename T, int HD>
+HXA_DEV uint64_t fix_v(uint8_t *vb, uint8_t *flags, int key0, uint64_t km, int lim_min, int tid) {
+  constexpr int RB = HD * 2, N = RB / 4 / 16;
+  const int row = tid >> 2, lane = tid & 63;
+  uint8_t *p = vb + row * RB + (tid & 3) * (RB / 4);
+  const bool dead = !((km >> row) & 1);
+  bool bad = false;
+  if (!dead && key0 + row > lim_min) {
+    constexpr uint32_t E = HxaVec<T>::EXP, EL = E & 0xffff, EH = E & 0xffff0000u;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const uint4_t x = *(const uint4_t *)(p + 16 * i);
+#pragma unroll
+      for (int e = 0; e < 4; e++) bad |= (x[e] & EL) == EL || (x[e] & EH) == EH;
+    }
+  }
+  const uint64_t b = __ballot(bad);
+  if (dead || ((b >> (lane & 60)) & 15)) {
+#pragma unroll
+    for (int i = 0; i < N; i++) *(uint4_t *)(p + 16 * i) = (uint4_t){0, 0, 0, 0};
+  }
+  const uint64_t rows = __ballot(lane < 16 && ((b >> (4 * (lane & 15))) & 15)) & 0xffff;
+  if (lane == 0) ((uint16_t *)flags)[tid >> 6] = (uint16_t)rows;
+  reads_done_barrier();
+  const uint64_t f = *(const uint64_t *)flags;
+  return ((uint64_t)__builtin_amdgcn_readfirstlane((int)(f >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)f);
+}
+
+// ---- rows modes ----
+// One workgroup's rows against keys [x0, x1): the wave's O^T (lane (g, ql): row 32 rw + ql, dims 32 d + 8 i + 4 g .. + 3 in
+// acc[d][4 i ..]), its maximum m and its row sum l (of both halves of the lanes).
+template <typename T, int HD, int W, bool PAGED>
+HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, int head0, float c, uint8_t *lds, float16_t (&acc)[HD / 32],
+                       float &mrun, float &lsum) {
+  typedef Geo<T, HD> G_;
+  typedef typename HxaVec<T>::v8 v8;
+  typedef typename HxaVec<T>::v4 v4;
+  typedef Swz<T, HD, true> S_;
+  constexpr int NB = W == 4 ? 2 : 1;  // 32-key blocks of a tile for each wave
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = W == 4 ? wave : wave & 1, kh = W == 4 ? 0 : wave >> 1;
+  const int g = lane >> 5, ql = lane & 31;
+
+  const int R = it.r0 + rw * 32 + ql;
+  const bool qok = R < it.nrows;
+  const int Rc = qok ? R : it.nrows - 1;
+  const T *qp = q + (long)(it.tok0 + Rc / it.G) * ldq + (long)(head0 + Rc % it.G) * HD;
+  v8 qf[HD / 16];
+#pragma unroll
+  for (int i = 0; i < HD / 16; i++) qf[i] = *(const v8 *)(qp + i * 16 + 8 * g);
+  const int lim = row_limit(it, Rc);
+  const int last = it.nrows - 1;
+  const int lim_min = row_limit(it, it.r0);
+  const int wave_max = it.r0 + rw * 32 <= last ? row_limit(it, min(it.r0 + rw * 32 + 31, last)) : -1;
+
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++) acc[d] = (float16_t){};
+  mrun = -INFINITY;
+  lsum = 0.0f;
+  const int nt = (it.x1 - it.x0 + KT - 1) / KT;
+  if (nt <= 0) return;
+  Loader<T, HD, true, PAGED> ld(s, it, lds, lane, wave);
+  uint64_t km_next = ld.load(0);
+
+  // V^T fragment of 32 dims dblk, keys kb .. kb + 15 (kb a multiple of 16): lane (g, ql) dim 32 dblk + ql, keys kb + 8 g .. + 7
+  const int s4 = (lane & 15) >> 2, sub = (lane >> 4) & 1;
+  const int vkey = 8 * g + s4;
+  const int vlow = ((2 * sub + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;  // within 64 bytes
+  uint32_t vat[HD / 32];
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++) vat[d] = vkey * G_::RB + (((d << 2) ^ S_::fv(vkey)) << 4) + vlow;  // fv(vkey + 4) is the same
+  static_assert(HD == 64 || HD == 128 || HD == 256, "heads");
+
+  for (int i = 0; i < nt; i++) {
+    wait_vm<0>();
+    reads_done_barrier();  // tile i has landed; every wave is done with tile i - 1
+    const uint64_t km = km_next;
+    const int key0 = it.x0 + i * KT;
+    const bool more = i + 1 < nt;
+    if (more) km_next = ld.load(i + 1);
+    const bool cut = km != ~0ull || key0 + KT - 1 > lim_min;
+    uint64_t apart = 0;
+    if (cut) apart = fix_v<T, HD>(ld.vbuf(i), lds + G_::FLAGS, key0, km, lim_min, tid);
+    if (wave_max < key0 + 32 * kh) continue;
+    const uint8_t *kb = ld.kbuf(i), *vb = ld.vbuf(i);
+    float16_t S[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) S[b] = (float16_t){};
+#pragma unroll
+    for (int ds = 0; ds < HD / 16; ds++)
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        const int row = (b + kh) * 32 + ql, ch = 2 * ds + g;
+        S[b] = mma32(*(const v8 *)(kb + row * G_::RB + ((ch ^ S_::fk(row)) << 4)), qf[ds], S[b]);
+      }
+    if (cut) {
+      const int n = lim - key0;
+      const uint64_t see = (km & (n >= 63 ? ~0ull : n < 0 ? 0ull : (2ull << n) - 1)) >> (32 * kh + 8 * g);
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (!((see >> (32 * b + 16 * (r >> 3) + (r & 7))) & 1)) S[b][r] = -INFINITY;
+    }
+    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) m4[r & 3] = fmaxf(m4[r & 3], S[b][r]);
+    float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+    {
+      float lo, hi;
+      halves(mt, lo, hi);
+      mt = fmaxf(lo, hi);
+    }
+    const bool need = (mt - mrun) * c > RESCALE2;  // also when mrun is still -inf
+    if (__any(need)) {
+      const float alpha = need ? __builtin_amdgcn_exp2f((mrun - mt) * c) : 1.0f;
+      if (need) mrun = mt;
+      lsum *= alpha;
+#pragma unroll
+      for (int d = 0; d < HD / 32; d++) acc[d] *= alpha;
+    }
+    const float mb = mrun == -INFINITY ? 0.0f : mrun * c;
+    v8 pf[NB][2];
+    float ls[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(S[b][r], c, -mb));
+        pf[b][r >> 3][r & 7] = (T)p;
+        ls[r & 1] += p;
+      }
+    lsum += ls[0] + ls[1];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++) {
+          const uint8_t *at = vb + vat[d] + ((b + kh) * 32 + ks * 16) * G_::RB;
+          const v4 x = read_tr<v4>(at), y = read_tr<v4>(at + 4 * G_::RB);
+          const v8 vf = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[d] = mma32(vf, pf[b][ks], acc[d]);
+        }
+    // values that are not finite and that only some rows see: their keys one by one
+    while (apart) {
+      const int f = __builtin_ctzll(apart);
+      apart &= apart - 1;
+      const int fb = f - 32 * kh;
+      if (fb < 0 || fb >= 32 * NB) continue;
+      const T *vr = ld.vrow(i, f, !more);
+      float p = 0.0f;
+      const int idx = (fb >> 5) * 16 + ((fb >> 4) & 1) * 8 + (fb & 7);
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (idx == b * 16 + r) p = (float)pf[b][r >> 3][r & 7];
+      float lo, hi;
+      halves(p, lo, hi);
+      p = (fb >> 3) & 1 ? hi : lo;
+      if (lim >= key0 + f) {
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+          for (int e4 = 0; e4 < 4; e4++) {
+            const v4 v = *(const v4 *)(vr + 32 * d + 8 * e4 + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[d][4 * e4 + e] += p * (float)v[e];
+          }
+      }
+    }
+  }
+  float lo, hi;
+  halves(lsum, lo, hi);
+  lsum = lo + hi;
+  if constexpr (W == 2) {  // join the key halves: waves 2, 3 hand theirs to waves 0, 1
+    reads_done_barrier();
+    float4_t *ox = (float4_t *)lds + rw * (HD / 8 * 64);
+    float *ml = (float *)(lds + 2 * HD / 8 * 1024) + rw * 128;
+    if (kh == 1) {
+#pragma unroll
+      for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; e4++)
+          ox[(d * 4 + e4) * 64 + lane] = (float4_t){acc[d][4 * e4], acc[d][4 * e4 + 1], acc[d][4 * e4 + 2], acc[d][4 * e4 + 3]};
+      ml[lane] = mrun;
+      ml[64 + lane] = lsum;
+    }
+    reads_done_barrier();
+    if (kh == 0) {
+      const float m1 = ml[lane], l1 = ml[64 + lane], m = fmaxf(mrun, m1);
+      const float mz = m == -INFINITY ? 0.0f : m;
+      const float a0 = __builtin_amdgcn_exp2f((mrun - mz) * c), a1 = __builtin_amdgcn_exp2f((m1 - mz) * c);
+      lsum = lsum * a0 + l1 * a1;
+      mrun = m;
+#pragma unroll
+      for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; e4++) {
+          const float4_t o = ox[(d * 4 + e4) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[d][4 * e4 + e] = acc[d][4 * e4 + e] * a0 + o[e] * a1;
+        }
+    }
+  }
+}
+
+// what an item leaves: rows of o, or (part != nullptr) fp32 partials of slot `slot`: part[slot][row][hd] unscaled and
+// ml[slot][row] = (maximum in powers of two, sum), row = token Hq + head
+template <typename T>
+struct Out {
+  T *o;
+  long ldo;
+  float *part;
+  float2_t *ml;
+  long rows;  // T Hq
+  int slot, Hq;
+};
+
+// rows mode: the wave's accumulators to their rows
+template <typename T, int HD, int W>
+HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uint8_t *lds, float16_t (&acc)[HD / 32], float m, float l) {
+  typedef typename HxaVec<T>::v4 v4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int rw = W == 4 ? wave : wave & 1;
+  const int g = lane >> 5, ql = lane & 31, r0 = it.r0 + rw * 32;
+  if (out.part != nullptr) {
+    const int R = r0 + ql;
+    if ((W == 2 && wave >= 2) || R >= it.nrows) return;
+    const long at = (long)out.slot * out.rows + (long)(it.tok0 + R / it.G) * out.Hq + head0 + R % it.G;
+    if (g == 0) out.ml[at] = (float2_t){m == -INFINITY ? m : m * c, l};
+    if (l == 0.0f) return;  // (l is NaN where a score is: written)
+    float *p = out.part + at * HD;
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; e4++)
+        *(float4_t *)(p + 32 * d + 8 * e4 + 4 * g) =
+            (float4_t){acc[d][4 * e4], acc[d][4 * e4 + 1], acc[d][4 * e4 + 2], acc[d][4 * e4 + 3]};
+    return;
+  }
+  // whole rows: staged through LDS, 8-byte unit u of row r at u ^ (r % 16)
+  reads_done_barrier();  // every wave is done with the tiles (and the join)
+  if (W == 2 && wave >= 2) return;
+  constexpr int RB = HD * 2, UN = HD / 4;
+  uint8_t *stage = lds + rw * 32 * RB;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; e4++) {
+      v4 x;
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = (T)(acc[d][4 * e4 + e] * inv);
+      const int u = 8 * d + 2 * e4 + g;
+      *(v4 *)(stage + ql * RB + ((u ^ (ql & 15)) << 3)) = x;
+    }
+  constexpr int RPP = 64 / UN;  // rows a pass
+#pragma unroll 4
+  for (int p = 0; p < 32 / RPP; p++) {
+    const int r = p * RPP + lane / UN, u = lane % UN, R = r0 + r;
+    const v4 x = *(const v4 *)(stage + r * RB + ((u ^ (r & 15)) << 3));
+    if (R < it.nrows) *(v4 *)(out.o + (long)(it.tok0 + R / it.G) * out.ldo + (long)(head0 + R % it.G) * HD + 4 * u) = x;
+  }
+}
+
+// ---- few rows ----
+// 16 rows against keys [x0, x1), each wave 16 keys of every tile, and the result out
+template <typename T, int HD, bool PAGED>
+HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, int head0, float c, uint8_t *lds, const Out<T> &out) {
+  typedef Geo<T, HD> G_;
+  typedef typename HxaVec<T>::v8 v8;
+  typedef typename HxaVec<T>::v4 v4;
+  typedef Swz<T, HD, false> S_;
+  constexpr int ND = HD / 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int gi = lane >> 4, ql = lane & 15;
+  const int R = it.r0 + ql, last = it.nrows - 1, Rc = min(R, last);
+  float4_t acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) acc[d] = (float4_t){};
+  float mrun = -INFINITY, lsum = 0.0f;
+  const int nt = (it.x1 - it.x0 + KT - 1) / KT;
+  if (nt > 0) {
+    Loader<T, HD, false, PAGED> ld(s, it, lds, lane, wave);
+    uint64_t km_next = ld.load(0);
+    const T *qp = q + (long)(it.tok0 + Rc / it.G) * ldq + (long)(head0 + Rc % it.G) * HD;
+    v8 qf[HD / 32];
+#pragma unroll
+    for (int i = 0; i < HD / 32; i++) qf[i] = *(const v8 *)(qp + i * 32 + 8 * gi);
+    const int lim = row_limit(it, Rc), lim_min = row_limit(it, it.r0);
+    const int vkey = 16 * wave + 4 * gi + (ql >> 2);
+    const int krow = 16 * wave + ql;
+    for (int i = 0; i < nt; i++) {
+      wait_vm<0>();
+      reads_done_barrier();
+      const uint64_t km = km_next;
+      const int key0 = it.x0 + i * KT;
+      const bool more = i + 1 < nt;
+      if (more) km_next = ld.load(i + 1);
+      const bool cut = km != ~0ull || key0 + KT - 1 > lim_min;
+      uint64_t apart = 0;
+      if (cut) apart = fix_v<T, HD>(ld.vbuf(i), lds + G_::FLAGS, key0, km, lim_min, tid);
+      const uint8_t *kb = ld.kbuf(i) + krow * G_::RB, *vb = ld.vbuf(i) + vkey * G_::RB;
+      float4_t S = {};
+#pragma unroll
+      for (int ds = 0; ds < HD / 32; ds++) S = mma16(*(const v8 *)(kb + (((4 * ds + gi) ^ S_::fk(krow)) << 4)), qf[ds], S);
+      if (cut) {
+        const int n = lim - key0;
+        const uint64_t see = (km & (n >= 63 ? ~0ull : n < 0 ? 0ull : (2ull << n) - 1)) >> (16 * wave + 4 * gi);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (!((see >> r) & 1)) S[r] = -INFINITY;
+      }
+      const float mt = max16(fmaxf(fmaxf(S[0], S[1]), fmaxf(S[2], S[3])));
+      const bool need = (mt - mrun) * c > RESCALE2;
+      if (__any(need)) {
+        const float alpha = need ? __builtin_amdgcn_exp2f((mrun - mt) * c) : 1.0f;
+        if (need) mrun = mt;
+        lsum *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; d++) acc[d] *= alpha;
+      }
+      const float mb = mrun == -INFINITY ? 0.0f : mrun * c;
+      v4 pf;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(S[r], c, -mb));
+        pf[r] = (T)p;
+        lsum += p;
+      }
+#pragma unroll
+      for (int d = 0; d < ND; d++) {
+        const int ch = 2 * d + ((ql & 3) >> 1);
+        acc[d] = mma16h(read_tr<v4>(vb + ((ch ^ S_::fv(vkey)) << 4) + (ql & 1) * 8), pf, acc[d]);
+      }
+      while (apart) {
+        const int f = __builtin_ctzll(apart);
+        apart &= apart - 1;
+        if (f >> 4 != wave) continue;
+        const T *vr = ld.vrow(i, f, !more);
+        const int e0 = f & 3;
+        const float mine = e0 == 0 ? (float)pf[0] : e0 == 1 ? (float)pf[1] : e0 == 2 ? (float)pf[2] : (float)pf[3];
+        const float p = __shfl(mine, ((f >> 2) & 3) * 16 + ql);
+        if (lim >= key0 + f) {
+#pragma unroll
+          for (int d = 0; d < ND; d++) {
+            const v4 v = *(const v4 *)(vr + 16 * d + 4 * gi);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[d][e] += p * (float)v[e];
+          }
+        }
+      }
+    }
+    lsum = add16(lsum);
+  }
+  // join the four waves: wave w takes the dims [w HD / 4, (w + 1) HD / 4)
+  reads_done_barrier();
+  float4_t *ox = (float4_t *)lds;                    // [wave][d][lane]
+  float2_t *mlx = (float2_t *)(lds + ND * 4 * 1024);  // [wave][row]
+#pragma unroll
+  for (int d = 0; d < ND; d++) ox[(wave * ND + d) * 64 + lane] = acc[d];
+  if (gi == 0) mlx[wave * 16 + ql] = (float2_t){mrun, lsum};
+  reads_done_barrier();
+  float m = -INFINITY, l = 0.0f, a[4];
+#pragma unroll
+  for (int w = 0; w < 4; w++) m = fmaxf(m, mlx[w * 16 + ql][0]);
+  const float mz = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const float2_t x = mlx[w * 16 + ql];
+    a[w] = __builtin_amdgcn_exp2f((x[0] - mz) * c);
+    l += x[1] * a[w];
+  }
+  if (R >= it.nrows) return;
+  const long tok = it.tok0 + R / it.G;
+  const int head = head0 + R % it.G;
+  const long at = (long)out.slot * out.rows + tok * out.Hq + head;
+  if (out.part != nullptr) {
+    if (wave == 0 && gi == 0) out.ml[at] = (float2_t){m == -INFINITY ? m : m * c, l};
+    if (l == 0.0f) return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int d4 = 0; d4 < ND / 4; d4++) {
+    const int d = wave * (ND / 4) + d4;
+    float4_t o = {};
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float4_t x = ox[(w * ND + d) * 64 + lane];
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] += x[e] * a[w];
+    }
+    if (out.part != nullptr) {
+      *(float4_t *)(out.part + at * HD + 16 * d + 4 * gi) = o;
+    } else {
+      v4 x;
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = (T)(o[e] * inv);
+      *(v4 *)(out.o + tok * out.ldo + (long)head * HD + 16 * d + 4 * gi) = x;
+    }
+  }
+}
+
+// ---- which rows a block of the grid takes ----
+struct Block {
+  int seq, b, n;  // the sequence, its first row in the call and its tokens
+  int first;      // first row (token x G + head) of the block within the sequence; -1: none
+};
+// Blocks are numbered over the sequences in order, ceil(n G / RB) each, a sequence's from its end to its start (the longest first).
+// cu's entries are clamped into [0, T]. Whole wave.
+HXA_DEV Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int RB, int blk, int lane) {
+  int seen = 0;  // blocks of the sequences before `base`
+  for (int base = 0; base < nseq; base += 64) {
+    const int i = base + lane;
+    int b = 0, e = 0;
+    if (i < nseq) {
+      b = min(max(cu[i], 0), T);
+      e = min(max(cu[i + 1], b), T);
+    }
+    const int nb = (int)(((long)(e - b) * G + RB - 1) / RB);
+    int inc = nb;  // inclusive scan
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int x = __shfl_up(inc, d);
+      if (lane >= d) inc += x;
+    }
+    const uint64_t hit = __ballot(seen + inc > blk);
+    if (hit) {
+      const int w = __builtin_ctzll(hit);
+      Block r;
+      r.seq = base + w;
+      r.b = __builtin_amdgcn_readlane(b, w);
+      r.n = __builtin_amdgcn_readlane(e, w) - r.b;
+      const int cnt = __builtin_amdgcn_readlane(nb, w), before = seen + __builtin_amdgcn_readlane(inc, w) - cnt;
+      r.first = (cnt - 1 - (blk - before)) * RB;
+      return r;
+    }
+    seen += __builtin_amdgcn_readlane(inc, 63);
+  }
+  return Block{0, 0, 0, -1};
+}
+
+struct CausalArgs {
+  const void *q, *k, *v;
+  void *o;
+  long ldq, ldk, ldv, ldo;
+  const int *cu;
+  int T, nseq, G, Hk;
+  float c;
+};
+
+// waves a SIMD: two workgroups a CU, so that one's softmax runs beside the other's matrix products; heads of 256 take the
+// registers and LDS of a CU for one
+#define HXA_CAUSAL_BOUNDS __launch_bounds__(256, HD == 256 ? 1 : 2)
+
+template <typename T, int HD, int W>
+__global__ HXA_CAUSAL_BOUNDS void causal_kernel(CausalArgs p) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x & 63;
+  const int h = blockIdx.x % p.Hk, blk = blockIdx.x / p.Hk;  // key heads innermost: with 8 of them each XCD keeps its own head's keys
+  const Block b = find_block(p.cu, p.nseq, p.T, p.G, 32 * W, blk, lane);
+  if (b.first < 0) return;
+  const long row0 = b.b;
+  Keys<T> s{};
+  s.k = (const T *)p.k + row0 * p.ldk + (long)h * HD;
+  s.v = (const T *)p.v + row0 * p.ldv + (long)h * HD;
+  s.ldk = p.ldk;
+  s.ldv = p.ldv;
+  Item it;
+  it.r0 = b.first;
+  it.nrows = b.n * p.G;
+  it.G = p.G;
+  it.tok0 = b.b;
+  it.base = 0;
+  it.cap = b.n - 1;
+  it.least = -1;
+  it.causal = true;
+  it.x0 = 0;
+  it.x1 = row_limit(it, min(it.r0 + 32 * W, it.nrows) - 1) + 1;
+  float16_t acc[HD / 32];
+  float m, l;
+  rows_item<T, HD, W, false>(s, it, (const T *)p.q, p.ldq, h * p.G, p.c, lds, acc, m, l);
+  const Out<T> out{(T *)p.o, p.ldo, nullptr, nullptr, 0, 0, 0};
+  rows_out<T, HD, W>(out, it, h * p.G, p.c, lds, acc, m, l);
+}
+
+// ---- over the cache ----
+// The keys of a sequence are one list: the prefix (P keys), then its own. Work items of a launch, in grid order:
+//   shared: np_blocks blocks of all T G rows x np_split ranges of the prefix, without a mask (rows of unused tokens are computed and
+//           never read), partial slots [0, np_split)
+//   own:    n_blocks blocks of the sequences' rows x n_split ranges of n_chunk keys of [x_first, P + own), slots from np_split on
+struct CachedArgs {
+  hxa_kv_cache c;
+  const void *q;
+  void *o;
+  long ldq, ldo;
+  int T, G, Hq;
+  float cs;
+  int np_mode, np_blocks, np_split, np_chunk;
+  int n_mode, n_blocks, n_split, n_chunk;  // modes: 1 few rows (16), 2 rows (64), 4 rows (128)
+  int x_first;  // 0: own items take the prefix too
+  float *part;  // nullptr: straight to o (np_split = 0, n_split = 1)
+  float2_t *ml;
+};
+
+template <typename T, int HD>
+HXA_DEV void any_item(int mode, const Keys<T> &s, const Item &it, const CachedArgs &p, int head0, uint8_t *lds, const Out<T> &out) {
+  if (mode == 1) {
+    few_item<T, HD, true>(s, it, (const T *)p.q, p.ldq, head0, p.cs, lds, out);
+    return;
+  }
+  float16_t acc[HD / 32];
+  float m, l;
+  if (mode == 2) {
+    rows_item<T, HD, 2, true>(s, it, (const T *)p.q, p.ldq, head0, p.cs, lds, acc, m, l);
+    rows_out<T, HD, 2>(out, it, head0, p.cs, lds, acc, m, l);
+  } else {
+    rows_item<T, HD, 4, true>(s, it, (const T *)p.q, p.ldq, head0, p.cs, lds, acc, m, l);
+    rows_out<T, HD, 4>(out, it, head0, p.cs, lds, acc, m, l);
+  }
+}
+HXA_DEV int mode_rows(int mode) { return mode == 1 ? 16 : 32 * mode; }
+
+template <typename T, int HD>
+__global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x & 63;
+  const int h = blockIdx.x % p.c.H, rest = blockIdx.x / p.c.H, P = p.c.prefix_len;
+  Keys<T> s{};
+  s.k = (const T *)p.c.k;
+  s.v = (const T *)p.c.v;
+  s.prefix = p.c.prefix;
+  s.table = p.c.table;
+  s.P = P;
+  s.page = p.c.page;
+  s.npages = p.c.npages;
+  s.H = p.c.H;
+  s.h = h;
+  Item it;
+  it.G = p.G;
+  Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, 0, p.Hq};
+  int mode;
+  if (rest < p.np_blocks * p.np_split) {
+    const int split = rest / p.np_blocks;
+    mode = p.np_mode;
+    it.r0 = (rest % p.np_blocks) * mode_rows(mode);
+    it.nrows = p.T * p.G;
+    it.tok0 = 0;
+    it.x0 = split * p.np_chunk;
+    it.x1 = min(it.x0 + p.np_chunk, P);
+    it.base = it.cap = it.least = P - 1;
+    it.causal = false;
+    out.slot = split;
+  } else {
+    const int own = rest - p.np_blocks * p.np_split, split = own / p.n_blocks;
+    mode = p.n_mode;
+    const Block b = find_block(p.c.cu, p.c.nseq, p.T, p.G, mode_rows(mode), own % p.n_blocks, lane);
+    if (b.first < 0) return;
+    const long len = p.c.len[b.seq];
+    const int held = (int)min(max(len, 0L), (long)p.c.ldt * p.c.page);
+    s.table += (long)b.seq * p.c.ldt;
+    it.r0 = b.first;
+    it.nrows = b.n * p.G;
+    it.tok0 = b.b;
+    // own position of token j: len - n + j; a negative one sees the prefix alone
+    it.causal = true;
+    it.cap = P + held - 1;
+    it.least = P - 1;
+    const long base = (long)P + len - b.n;
+    it.base = (int)max(min(base, (long)it.cap), (long)P - 1 - b.n);
+    it.x0 = p.x_first + split * p.n_chunk;
+    it.x1 = min(row_limit(it, min(it.r0 + mode_rows(mode), it.nrows) - 1) + 1, it.x0 + p.n_chunk);
+    out.slot = p.np_split + split;
+  }
+  any_item<T, HD>(mode, s, it, p, h * p.G, lds, out);
+}
+
+// The partials of a row joined: weights 2^(m_s - m) against the common maximum, then one division and one rounding. HD / 4 lanes a
+// row. A slot whose sum is 0 saw no key and wrote no values.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs p, int nslots) {
+  typedef typename HxaVec<T>::v4 v4;
+  constexpr int LPR = HD / 4;
+  const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR, rows = (long)p.T * p.Hq;
+  if (row >= rows) return;
+  const int tok = (int)(row / p.Hq), head = (int)(row - (long)tok * p.Hq), u = threadIdx.x % LPR;
+  if (tok < p.c.cu[0] || tok >= p.c.cu[p.c.nseq]) return;
+  float m = -INFINITY;
+  for (int s = 0; s < nslots; s++) m = fmaxf(m, p.ml[s * rows + row][0]);
+  const float mz = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  float4_t o = {};
+  for (int s = 0; s < nslots; s++) {
+    const float2_t x = p.ml[s * rows + row];
+    if (x[1] == 0.0f) continue;
+    const float a = __builtin_amdgcn_exp2f(x[0] - mz);
+    l += x[1] * a;
+    const float4_t y = *(const float4_t *)(p.part + (s * rows + row) * HD + 4 * u);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] += y[e] * a;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  v4 x;
+#pragma unroll
+  for (int e = 0; e < 4; e++) x[e] = (T)(o[e] * inv);
+  *(v4 *)((T *)p.o + tok * p.ldo + (long)head * HD + 4 * u) = x;
+}
+
+int causal_ncu() {
+  static const int ncu = [] {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
+      return 256;
+    return n;
+  }();
+  return ncu;
+}
+
+// kernels that take more than 64 KB of LDS: allowed once a device
+int allow_lds(const void *f, int bytes, int id) {
+  static std::mutex mu;
+  static uint32_t done[HXA_MAX_DEVICES];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= HXA_MAX_DEVICES) return HXA_E_RESOURCE;
+  std::lock_guard<std::mutex> lk(mu);
+  if (done[dev] >> id & 1) return HXA_OK;
+  if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return HXA_E_HIP;
+  done[dev] |= 1u << id;
+  return HXA_OK;
+}
+// runs f with the kernel's types: f.template operator()<T, HD>(an index below 6)
+template <typename F>
+int by_type(int dtype, int hd, F f) {
+  if (dtype == HXA_DT_F16) {
+    if (hd == 64) return f(hxa_h{}, std::integral_constant<int, 64>{}, 0);
+    if (hd == 128) return f(hxa_h{}, std::integral_constant<int, 128>{}, 1);
+    return f(hxa_h{}, std::integral_constant<int, 256>{}, 2);
+  }
+  if (hd == 64) return f(hxa_b{}, std::integral_constant<int, 64>{}, 3);
+  if (hd == 128) return f(hxa_b{}, std::integral_constant<int, 128>{}, 4);
+  return f(hxa_b{}, std::integral_constant<int, 256>{}, 5);
+}
+int launched(const char *who) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? HXA_OK : hxa_set_error(HXA_E_HIP, "%s: %s", who, hipGetErrorString(e));
+}
+bool rows_ok(const void *p, long ld, int H, int hd) { return p != nullptr && (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld >= (long)H * hd; }
+
+long ceil_div(long a, long b) { return (a + b - 1) / b; }
+
+// workgroups that run at once
+int wg_slots(int hd) { return causal_ncu() * (hd == 256 ? 1 : 2); }
+
+// The launch of a call over the cache, from sizes that the host knows (T, the table's width, the prefix): how the lengths on
+// the device turn out does not change it, so a captured launch stays right.
+struct CachedPlan {
+  int np_mode, np_blocks, np_split, np_chunk, n_mode, n_blocks, n_split, n_chunk, x_first;
+};
+CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws) {
+  const int G = Hq / c.H;
+  const long RT = (long)T * G, slots = wg_slots(c.hd), P = c.prefix_len, cap = (long)c.ldt * c.page;
+  CachedPlan p{};
+  const long per_seq = ceil_div(RT, c.nseq);
+  p.n_mode = per_seq <= 16 ? 1 : per_seq <= 64 || (RT / 128 + c.nseq) * c.H < slots ? 2 : 4;
+  const int rb = p.n_mode == 1 ? 16 : 32 * p.n_mode;
+  p.n_blocks = (int)(RT / rb + c.nseq);
+  p.n_split = 1;
+  p.n_chunk = 1 << 30;
+  if (!ws) return p;
+  auto split = [&](long items, long keys, int &ns, int &chunk) {  // ranges of at least 4 tiles, until the items are two rounds
+    const long tiles = ceil_div(keys, KT), most = tiles / 4 > 1 ? tiles / 4 : 1;
+    long n = ceil_div(2 * slots, items);
+    n = n > most ? most : n;
+    const long per = ceil_div(tiles, n > 0 ? n : 1);
+    chunk = (int)((per > 0 ? per : 1) * KT);
+    ns = (int)(tiles > 0 ? ceil_div(tiles, per) : 1);
+  };
+  if (p.n_mode == 1 && c.nseq >= 2 && P >= 4 * KT) {  // the prefix once for all
+    p.np_mode = RT <= 16 ? 1 : RT <= 64 ? 2 : 4;
+    p.np_blocks = (int)ceil_div(RT, p.np_mode == 1 ? 16 : 32 * p.np_mode);
+    split((long)p.np_blocks * c.H, P, p.np_split, p.np_chunk);
+    p.x_first = (int)P;
+    split((long)p.n_blocks * c.H, cap, p.n_split, p.n_chunk);
+  } else {
+    split((long)p.n_blocks * c.H, P + cap, p.n_split, p.n_chunk);
+  }
+  return p;
+}
+long cached_ws(const CachedPlan &p, const hxa_kv_cache &c, int T, int Hq) {
+  const long slots = p.np_split + p.n_split;
+  return slots == 1 ? 0 : slots * T * Hq * (c.hd * 4L + 8);
+}
+
+}  // namespace
+
+extern "C" int hxa_attention_causal(int dtype, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, void *o, long ldo,
+                                    int T, const int *cu, int nseq, int Hq, int Hk, int hd, float scale, void *stream) {
+  if (dtype != HXA_DT_F16 && dtype != HXA_DT_BF16) return hxa_set_error(HXA_E_MODE, "attention_causal: dtype %d", dtype);
+  if (hd != 64 && hd != 128 && hd != 256) return hxa_set_error(HXA_E_MODE, "attention_causal: heads of %d", hd);
+  if (T < 0 || T > HXA_MAX_ROWS || nseq < 0 || Hq <= 0 || Hk <= 0 || Hq > HXA_MAX_HEADS || Hq % Hk || (long)T * Hq >= 1L << 31)
+    return hxa_set_error(HXA_E_ARG, "attention_causal: T=%d nseq=%d Hq=%d Hk=%d", T, nseq, Hq, Hk);
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return hxa_set_error(HXA_E_ARG, "attention_causal: scale %g", (double)scale);
+  if (T == 0 || nseq == 0) return HXA_OK;
+  if (!rows_ok(q, ldq, Hq, hd) || !rows_ok(k, ldk, Hk, hd) || !rows_ok(v, ldv, Hk, hd) || !rows_ok(o, ldo, Hq, hd))
+    return hxa_set_error(HXA_E_ARG, "attention_causal: pointers null or not 16-byte aligned, or strides (%ld %ld %ld %ld)", ldq, ldk, ldv, ldo);
+  if (ldk >= 1 << 24 || ldv >= 1 << 24) return hxa_set_error(HXA_E_ARG, "attention_causal: strides of %ld, %ld", ldk, ldv);
+  if (!cu || (uintptr_t)cu % 4) return hxa_set_error(HXA_E_ARG, "attention_causal: cu");
+  const int G = Hq / Hk;
+  const long RT = (long)T * G;
+  CausalArgs p{q, k, v, o, ldq, ldk, ldv, ldo, cu, T, nseq, G, Hk, scale * L2E};
+  // 64 rows a workgroup while 128 would leave workgroup places free
+  const bool half = (RT / 128 + 1) * Hk < wg_slots(hd);
+  const int rb = half ? 64 : 128;
+  const long wgs = (RT / rb + nseq) * Hk;
+  if (wgs >= 1L << 24) return hxa_set_error(HXA_E_ARG, "attention_causal: T=%d nseq=%d Hq=%d are too many blocks", T, nseq, Hq);
+  return by_type(dtype, hd, [&](auto ty, auto hdc, int id) -> int {
+    typedef decltype(ty) T_;
+    constexpr int HD = decltype(hdc)::value;
+    const auto f = half ? causal_kernel<T_, HD, 2> : causal_kernel<T_, HD, 4>;
+    const int r = allow_lds((const void *)f, Geo<T_, HD>::LDS, 2 * id + half);
+    if (r != HXA_OK) return hxa_set_error(r, "attention_causal: %d bytes of LDS", Geo<T_, HD>::LDS);
+    hxa_launch(f, dim3((unsigned)wgs), dim3(256), Geo<T_, HD>::LDS, (hipStream_t)stream, p);
+    return launched("attention_causal");
+  });
+}
+
+static int cached_check(const hxa_kv_cache *c, int T, int Hq) {
+  const int r = hxa_kv_check(c, T, "attention_cached");
+  if (r != HXA_OK) return r;
+  if (Hq <= 0 || Hq > HXA_MAX_HEADS || Hq % c->H || (long)T * Hq >= 1L << 31)
+    return hxa_set_error(HXA_E_ARG, "attention_cached: T=%d Hq=%d H=%d", T, Hq, c->H);
+  if (((long)T * Hq / c->H / 16 + c->nseq) * c->H >= 1L << 20)
+    return hxa_set_error(HXA_E_ARG, "attention_cached: T=%d nseq=%d H=%d are too many blocks", T, c->nseq, c->H);
+  return HXA_OK;
+}
+
+extern "C" long hxa_attention_cached_ws_bytes(const hxa_kv_cache *c, int T, int Hq) {
+  if (cached_check(c, T, Hq) != HXA_OK || T == 0 || c->nseq == 0) return 0;
+  return cached_ws(cached_plan(*c, T, Hq, true), *c, T, Hq);
+}
+
+extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long ldq, void *o, long ldo, int T, int Hq, float scale, void *ws,
+                                    long ws_bytes, void *stream) {
+  const int r = cached_check(c, T, Hq);
+  if (r != HXA_OK) return r;
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return hxa_set_error(HXA_E_ARG, "attention_cached: scale %g", (double)scale);
+  if (T == 0 || c->nseq == 0) return HXA_OK;
+  if (!rows_ok(q, ldq, Hq, c->hd) || !rows_ok(o, ldo, Hq, c->hd))
+    return hxa_set_error(HXA_E_ARG, "attention_cached: pointers null or not 16-byte aligned, or strides (%ld %ld)", ldq, ldo);
+  if ((uintptr_t)ws % 16) return hxa_set_error(HXA_E_ARG, "attention_cached: workspace not aligned");
+  CachedPlan pl = cached_plan(*c, T, Hq, true);
+  const long need = cached_ws(pl, *c, T, Hq);
+  if (need > 0 && (ws == nullptr || ws_bytes < need)) pl = cached_plan(*c, T, Hq, false);
+  const int nslots = pl.np_split + pl.n_split;
+  CachedArgs p{*c, q, o, ldq, ldo, T, Hq / c->H, Hq, scale * L2E, pl.np_mode, pl.np_blocks, pl.np_split, pl.np_chunk,
+               pl.n_mode, pl.n_blocks, pl.n_split, pl.n_chunk, pl.x_first, nullptr, nullptr};
+  if (nslots > 1) {
+    p.part = (float *)ws;
+    p.ml = (float2_t *)(p.part + (long)nslots * T * Hq * c->hd);
+  }
+  const long wgs = ((long)pl.np_blocks * pl.np_split + (long)pl.n_blocks * pl.n_split) * c->H;
+  const hipStream_t st = (hipStream_t)stream;
+  return by_type(c->dtype, c->hd, [&](auto ty, auto hdc, int id) -> int {
+    typedef decltype(ty) T_;
+    constexpr int HD = decltype(hdc)::value;
+    const auto f = cached_kernel<T_, HD>;
+    const int a = allow_lds((const void *)f, Geo<T_, HD>::LDS, 16 + id);
+    if (a != HXA_OK) return hxa_set_error(a, "attention_cached: %d bytes of LDS", Geo<T_, HD>::LDS);
+    hxa_launch(f, dim3((unsigned)wgs), dim3(256), Geo<T_, HD>::LDS, st, p);
+    if (nslots > 1)
+      hxa_launch(cached_merge_kernel<T_, HD>, dim3((unsigned)ceil_div((long)T * Hq, 1024 / HD)), dim3(256), 0, st, p, nslots);
+    return launched("attention_cached");
+  });
+}

@@ -20,6 +20,9 @@ SZ, U64 = C.c_size_t, C.c_uint64
 W_F16, W_Q8, W_Q4 = 0, 1, 2
 W_KTILED = 16  # OR'ed into a format: matrix stored k-tiled, [K/32][N][chunk]
 EPI_STORE, EPI_GELU_TANH, EPI_GELU_ERF, EPI_RESADD, EPI_STORE_T, EPI_SITU, EPI_PARTIAL, EPI_RESADD_SPLIT2, EPI_PARTIAL_F32 = range(9)
+DT_F16, DT_BF16 = 1, 2
+ROPE_HALF, ROPE_PAIRS = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = range(4)
 KIND_WEIGHTS_ANIMA, KIND_BLOB, KIND_WEIGHTS_MOSS = 0, 1, 2
 E_NAMES = {0: "OK", -1: "RESOURCE", -2: "LOCK", -5: "WEIGHTS", -6: "NOBLOB", -7: "BLOB", -10: "META", -11: "MODE",
            -12: "ARG", -13: "HIP"}
@@ -39,6 +42,17 @@ class BlockDims(C.Structure):
 class DitCfg(C.Structure):
     _fields_ = [("blk", BlockDims), ("nblocks", I), ("lat_c", I), ("lat_h", I), ("lat_w", I), ("temb", I),
                 ("ntxt_in", I), ("form", I)]
+
+
+class Rope(C.Structure):
+    """hxa_rope: rotary positions (freq: device pointer to rot / 2 fp32 frequencies)"""
+    _fields_ = [("freq", P), ("rot", I), ("layout", I), ("mscale", F)]
+
+
+class KvCache(C.Structure):
+    """hxa_kv_cache: a paged key / value cache and the plan of a call on it (device pointers)"""
+    _fields_ = [("dtype", I), ("H", I), ("hd", I), ("page", I), ("npages", I), ("k", P), ("v", P), ("prefix", P),
+                ("prefix_len", I), ("table", P), ("ldt", I), ("len", P), ("cu", P), ("nseq", I)]
 
 
 _SIGS = {
@@ -88,6 +102,12 @@ _SIGS = {
     "hxa_rmsrope": (I, [P, P, P, P, L, I, I, P, P, I, P]),
     "hxa_resadd2": (I, [P, L, P, P, L, I, I, P, P]),
     "hxa_dequant": (I, [I, P, P, P, I, I, P, P]),
+    "hxa_rope_freqs": (I, [I, C.c_double, I, C.c_double, C.c_double, C.c_double, C.c_double, P, P]),
+    "hxa_qk_norm_rope": (I, [I, P, L, I, P, L, I, I, I, P, P, F, P, C.POINTER(Rope), P, L, P, L, P]),
+    "hxa_kv_append": (I, [C.POINTER(KvCache), P, L, P, L, I, P, F, C.POINTER(Rope), P]),
+    "hxa_attention_causal": (I, [I, P, L, P, L, P, L, P, L, I, P, I, I, I, I, F, P]),
+    "hxa_attention_cached": (I, [C.POINTER(KvCache), P, L, P, L, I, I, F, P, L, P]),
+    "hxa_attention_cached_ws_bytes": (L, [C.POINTER(KvCache), I, I]),
     "hxa_fill_normal": (I, [P, I, SZ, U64, F, F, P]),
     "hxa_fill_uniform_int": (I, [P, I, SZ, U64, I, I, P]),
     "hxa_fill_const": (I, [P, I, SZ, F, P]),
@@ -318,3 +338,12 @@ def read_ws(d: BlockDims, ws: DeviceArray, which: int, rows: int, cols: int) -> 
     out = np.zeros((rows, ld), np.float16)
     check(lib().hxa_d2h(out.ctypes.data, p, ((rows - 1) * ld + cols) * 2), "read_ws")
     return np.ascontiguousarray(out[:, :cols])
+
+
+def rope_freqs(rot: int, base: float, scaling: int = ROPE_PLAIN, factor: float = 1.0, orig_len: float = 0.0,
+               beta_fast: float = 32.0, beta_slow: float = 1.0):
+    """hxa_rope_freqs -> (fp32 frequencies [rot / 2], mscale)"""
+    freq, m = np.empty(max(rot, 0) // 2, np.float32), F()
+    check(lib().hxa_rope_freqs(rot, base, scaling, factor, orig_len, beta_fast, beta_slow, freq.ctypes.data, C.byref(m)),
+          "rope_freqs")
+    return freq, m.value

@@ -232,6 +232,90 @@ int hxa_x32_to_rows(const float *tiles, float *x, int R, int C, void *stream);
 int hxa_rows_to_x32(const float *x, float *tiles, int R, int C, void *stream);
 
 /* ============================================================================================================
+ * 3b. The attention path of a causal text model (what conditions the DiT: grouped heads, per-head q / k norms, rotary
+ * positions, a paged key / value cache). No counterpart on the reference's accelerator: it runs its text encoders elsewhere.
+ * ============================================================================================================
+ * Rows are tokens; head h of a row is columns [h hd, (h + 1) hd). dtype HXA_DT_F16 or HXA_DT_BF16; hd 64, 128 or 256; row
+ * strides in elements, multiples of 8 and at least the row's heads; pointers 16-byte aligned; at most 2^25 rows, 4096 heads. Sums, softmax statistics and
+ * angles are held in 32 bits or more and every output is rounded once.
+ *
+ * A batch of sequences is packed: sequence i's tokens are rows cu[i] .. cu[i + 1] - 1 (cu: device, nseq + 1 ascending entries,
+ * cu[0] = 0, a sequence may be empty). Rows outside every sequence are neither read into a result nor written. cu, len, the page
+ * tables and pos stay on the device, so a captured graph follows what they hold when it is replayed; entries that
+ * are out of range never lead out of the buffers (what such an entry means is said with each function). The calls run on the
+ * current device, on whose memory every pointer must be. */
+#define HXA_DT_F16 1
+#define HXA_DT_BF16 2
+#define HXA_ROPE_HALF 0  /* pairs (i, i + rot / 2) */
+#define HXA_ROPE_PAIRS 1 /* pairs (2 i, 2 i + 1) */
+typedef struct {
+  const float *freq; /* device, rot / 2 radians a position (hxa_rope_freqs makes them) */
+  int rot;           /* rotated dims at the head's start, a multiple of 16 up to hd; the rest pass. 0: no rotation */
+  int layout;        /* HXA_ROPE_* */
+  float mscale;      /* cosines and sines are multiplied by it (1: a plain rotation) */
+} hxa_rope;
+/* Frequencies of rotary positions on the host: freq[i] = base^(-2 i / rot), rot / 2 of them, for contexts `factor` times as long
+ * as the trained `orig_len` positions:
+ *   HXA_ROPE_PLAIN  as they are
+ *   HXA_ROPE_LINEAR every position divided by factor
+ *   HXA_ROPE_BASE   base * factor^(rot / (rot - 2)) in the place of base: the slowest pair turns factor times slower, the fastest as before
+ *   HXA_ROPE_PARTS  by the turns r = orig_len freq[i] / (2 pi) a pair makes over the trained length: as they are from r = beta_fast on,
+ *                   divided by factor up to r = beta_slow, between them mixed by the share of log(r) (as parts of the pair index);
+ *                   *mscale = 0.1 ln(factor) + 1
+ * rot even and at least 2 (BASE: 4), base > 1, factor >= 1; orig_len > 0 and beta_fast > beta_slow > 0 for PARTS. Other modes set
+ * *mscale = 1; mscale may be NULL. Computed in 64 bits, each frequency rounded once. */
+#define HXA_ROPE_PLAIN 0
+#define HXA_ROPE_LINEAR 1
+#define HXA_ROPE_BASE 2
+#define HXA_ROPE_PARTS 3
+int hxa_rope_freqs(int rot, double base, int scaling, double factor, double orig_len, double beta_fast, double beta_slow,
+                   float *freq, float *mscale);
+/* Queries and keys in one pass: per head u = x * rsqrt(mean(x^2) + eps) * gain (gain [hd] fp32; NULL: u = x), then the rotation
+ * of rope (NULL: none) by the angles pos[t] * freq[i] (pos: device [T]; NULL: row t is at position t), which are formed in 64
+ * bits. q [T][ldq] of Hq heads to qo [T][ldqo], k of Hk heads to ko. In place (qo == q, ldqo == ldq, ko likewise) or apart;
+ * other overlaps are not allowed. Hq or Hk may be 0, its pointers NULL then. */
+int hxa_qk_norm_rope(int dtype, const void *q, long ldq, int Hq, const void *k, long ldk, int Hk, int T, int hd,
+                     const float *gq, const float *gk, float eps, const int *pos, const hxa_rope *rope, void *qo, long ldqo,
+                     void *ko, long ldko, void *stream);
+/* A paged cache of keys and values and the plan of a call on it. Pool page p holds `page` consecutive tokens of one sequence (or of
+ * the shared prefix), for each of H heads: k and v [npages][H][page][hd]. The keys of sequence i are the prefix_len tokens of
+ * the prefix (pages prefix[0 ..], ceil(prefix_len / page) entries, the same for every sequence), then its own len[i] tokens (pages
+ * table[i ldt ..]); len[i] counts the cu[i + 1] - cu[i] new tokens of this call, the last of them, at own positions
+ * len[i] - (cu[i + 1] - cu[i]) and up. Own positions at or past ldt * page are not in the cache. */
+typedef struct {
+  int dtype, H, hd;
+  int page, npages;  /* tokens a page (1 .. 65536), pages in the pool; npages * H * page < 2^32 */
+  void *k, *v;
+  const int *prefix; /* device; NULL when prefix_len is 0 */
+  int prefix_len;
+  const int *table;  /* device [nseq][ldt] */
+  int ldt;           /* entries a sequence; ldt * page + prefix_len < 2^30 */
+  const int *len;    /* device [nseq] */
+  const int *cu;     /* device [nseq + 1] */
+  int nseq;
+} hxa_kv_cache;
+/* The new tokens' keys and values into their sequences' own pages: k [T][ldk] with the norm gk (NULL: none) and the rotation rope
+ * (NULL: none) at position prefix_len + own position, as hxa_qk_norm_rope, v [T][ldv] as it is. A token whose own position is
+ * negative or past the table, or whose page is not in [0, npages), is left out. A page that is written may stand in one place of
+ * the table only. (The prefix itself is written through a plan of one sequence whose own pages are the prefix's.) */
+int hxa_kv_append(const hxa_kv_cache *c, const void *k, long ldk, const void *v, long ldv, int T, const float *gk, float eps,
+                  const hxa_rope *rope, void *stream);
+/* Causal attention over packed sequences: o[t] = softmax over the rows s <= t of t's own sequence of scale q[t] . k[s], times v[s];
+ * query head h reads key head h / (Hq / Hk) (Hq % Hk == 0). scale > 0. q, k, v, o [T][ld.]; ldk, ldv < 2^24. What the mask
+ * hides has no part in a row, infinities and NaN included. */
+int hxa_attention_causal(int dtype, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, void *o,
+                         long ldo, int T, const int *cu, int nseq, int Hq, int Hk, int hd, float scale, void *stream);
+/* Attention of the new tokens over the cache: the query at own position p sees the whole prefix and the own positions 0 .. p
+ * that the cache holds (so append first). Keys of a page that is not in [0, npages) are left out; a query that sees no key gets
+ * zeros. q, o [T][ld.] of Hq heads (a multiple of c->H). ws: hxa_attention_cached_ws_bytes(c, T, Hq) bytes, 16-byte aligned, for
+ * the partial results where the keys of few rows are split over the chip and where the prefix is read once for the whole batch; NULL or
+ * fewer bytes: one launch that splits nothing. The sums' order depends on the form, not on a run. Calls that
+ * share ws must not overlap. */
+int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long ldq, void *o, long ldo, int T, int Hq, float scale, void *ws,
+                         long ws_bytes, void *stream);
+long hxa_attention_cached_ws_bytes(const hxa_kv_cache *c, int T, int Hq); /* 0: the one-launch form is the best one */
+
+/* ============================================================================================================
  * 4. GPU block packs and the device-level block (weights resident in HBM)
  * ============================================================================================================ */
 /* A pack is one device allocation holding every weight of one block in the GPU layouts above, at offsets
