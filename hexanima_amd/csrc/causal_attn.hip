@@ -21,9 +21,11 @@
 //
 // What a mask hides has no part in a result: hidden scores become -inf before the maximum; values of keys that no row of the workgroup sees are
 // zeroed in LDS (0 x NaN would be NaN), and values of keys that only some rows see are, where they are not finite, taken out of the
-// matrix product and added by the rows that see them (add_apart).
+// matrix product and added, key by key, by the rows that see them at the end.
+#include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include "causal.h"
 #include "kernels.h"
@@ -48,6 +50,8 @@ template <typename V4>
 HXA_DEV V4 read_tr(const uint8_t *p) {
   return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *)(lds_void_t *)p));
 }
+HXA_DEV float sum2(half2_t h, float l) { return __builtin_amdgcn_fdot2(h, (half2_t){(hxa_h)1.0f, (hxa_h)1.0f}, l, false); }
+HXA_DEV float sum2(bf2_t h, float l) { return __builtin_amdgcn_fdot2_f32_bf16(h, (bf2_t){(hxa_b)1.0f, (hxa_b)1.0f}, l, false); }
 HXA_DEV float max16(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48, which all get it
   const int x = __builtin_bit_cast(int, v);
   const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
@@ -91,7 +95,8 @@ struct Geo {
   static constexpr int TB = KT * RB;         // of a tile
   static constexpr int CH = HD / 8;          // 16-byte chunks a row = lanes a row of a load
   static constexpr int RPL = 64 / CH;        // rows of one wave-wide load (1 KB)
-  static constexpr int NLD = KT / RPL / 4;   // loads a wave and tile, for K and for V each
+  static constexpr int NLD = KT / RPL / 4;   // loads a wave and tile, for K and for V each, of rows 4 RPL apart
+  static constexpr int NOFF = HD == 256 ? 2 : 1;  // of them different up to a whole number of 16 rows (permutation and swizzles repeat)
   static constexpr int FLAGS = 4 * TB;       // LDS past the tiles: the flags of fix_v
   static constexpr int LDS = 4 * TB + 64;
 };
@@ -116,15 +121,13 @@ struct Loader {
   const Item &it;
   uint8_t *lds;
   int lane, wave;
-  uint32_t koff[G_::NLD], voff[G_::NLD];  // contiguous: byte offsets within a whole tile; paged: chunk offsets within a row
-  int ent;         // paged: the page entry of this lane's key in the tile that is loaded next
-  uint32_t row;    // paged: page row of this lane's key in the tile loaded last (key = lane)
-  uint32_t prow;   // and in the one before
+  uint32_t koff[G_::NOFF], voff[G_::NOFF];  // contiguous: byte offsets within a whole tile; paged: chunk offsets within a row
+  int ent;           // paged: the page entry of this lane's key in the tile that is opened next
+  uint32_t krow[PAGED ? G_::NLD : 1], vrow[PAGED ? G_::NLD : 1];  // paged: page rows that this lane's loads of the tile opened last read
   HXA_DEV Loader(const Keys<T> &s_, const Item &it_, uint8_t *lds_, int lane_, int wave_) : s(s_), it(it_), lds(lds_), lane(lane_), wave(wave_) {
-    row = prow = 0;
     ent = -1;
 #pragma unroll
-    for (int j = 0; j < G_::NLD; j++) {
+    for (int j = 0; j < G_::NOFF; j++) {
       const int r = (j * 4 + wave) * G_::RPL + lane / G_::CH, c = lane % G_::CH;
       const int kr = PERM ? krow_key(r) : r;
       const int ck = c ^ S_::fk(r), cv = c ^ S_::fv(r);
@@ -144,51 +147,75 @@ struct Loader {
       ent = (pre ? s.prefix : s.table)[y / (unsigned)s.page];
     }
   }
-  // tile i into its buffer; returns the mask of its keys that are there
-  HXA_DEV uint64_t load(int i) {
+  // tile i: where its keys lie, and the mask of those that are there; its loads follow
+  HXA_DEV uint64_t open(int i) {
     const int key0 = it.x0 + i * KT;
     if constexpr (PAGED) {
       const int x = key0 + lane;
       const unsigned y = x < s.P ? x : x - s.P;
       const bool ok = x < it.x1 && (unsigned)ent < (unsigned)s.npages;
-      prow = row;
-      row = ok ? ((uint32_t)ent * s.H + s.h) * s.page + y % (unsigned)s.page : 0;  // < 2^32: checked on the host
+      const uint32_t row = ok ? ((uint32_t)ent * s.H + s.h) * s.page + y % (unsigned)s.page : 0;  // < 2^32: checked on the host
       const uint64_t mask = __ballot(ok);
       if (key0 + KT < it.x1) entry(i + 1);
 #pragma unroll
       for (int j = 0; j < G_::NLD; j++) {
-        const int blk = j * 4 + wave, r = blk * G_::RPL + lane / G_::CH;
-        const uint32_t rk = __shfl((int)row, PERM ? krow_key(r) : r), rv = PERM ? (uint32_t)__shfl((int)row, r) : rk;
-        g2l16_opaque((const uint8_t *)s.k + (uint64_t)rk * G_::RB + koff[j], kbuf(i) + blk * 1024);
-        g2l16_opaque((const uint8_t *)s.v + (uint64_t)rv * G_::RB + voff[j], vbuf(i) + blk * 1024);
+        const int r = (j * 4 + wave) * G_::RPL + lane / G_::CH;
+        krow[j] = __shfl((int)row, PERM ? krow_key(r) : r);
+        vrow[j] = PERM ? __shfl((int)row, r) : krow[j];
       }
       return mask;
     } else {
-      const T *kt = s.k + (long)key0 * s.ldk, *vt = s.v + (long)key0 * s.ldv;
-      if (key0 + KT <= it.x1) {
-#pragma unroll
-        for (int j = 0; j < G_::NLD; j++) g2l16_sbase(kt, koff[j], kbuf(i) + (j * 4 + wave) * 1024);
-#pragma unroll
-        for (int j = 0; j < G_::NLD; j++) g2l16_sbase(vt, voff[j], vbuf(i) + (j * 4 + wave) * 1024);
-        return ~0ull;
-      }
-      const int last = it.x1 - 1 - key0;  // rows past the keys read the last one
-      int ln = lane;
-      asm volatile("" : "+v"(ln));  // opaque: the loop keeps none of these addresses in registers
-#pragma unroll
-      for (int j = 0; j < G_::NLD; j++) {
-        const int blk = j * 4 + wave, r = blk * G_::RPL + ln / G_::CH, c = ln % G_::CH;
-        const int kr = min(PERM ? krow_key(r) : r, last), vr = min(r, last);
-        g2l16_sbase(kt, ((uint32_t)kr * (uint32_t)s.ldk + (c ^ S_::fk(r)) * 8) * 2u, kbuf(i) + blk * 1024);
-        g2l16_sbase(vt, ((uint32_t)vr * (uint32_t)s.ldv + (c ^ S_::fv(r)) * 8) * 2u, vbuf(i) + blk * 1024);
-      }
-      return (2ull << last) - 1;
+      const int n = it.x1 - key0;
+      return n >= KT ? ~0ull : (1ull << n) - 1;
     }
   }
-  // global address of the value row of key f of the tile before the one loaded last (cur: of the one loaded last)
-  HXA_DEV const T *vrow(int i, int f, bool cur) const {
-    if constexpr (PAGED) return s.v + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(cur ? row : prow), f) * HD;
-    return s.v + (long)(it.x0 + i * KT + f) * s.ldv;
+  // whether tile i lies below x1, so that its loads need no clamp (paged: never one)
+  HXA_DEV bool whole(int i) const { return PAGED || it.x0 + (i + 1) * KT <= it.x1; }
+  // load n of the 2 NLD of this wave for tile i, the one opened last: K's, then V's. WHOLE: whole(i)
+  template <bool WHOLE>
+  HXA_DEV void load(int i, int n) {
+    const bool V = n >= G_::NLD;
+    const int j = V ? n - G_::NLD : n, blk = j * 4 + wave;
+    uint8_t *to = (V ? vbuf(i) : kbuf(i)) + blk * 1024;
+    const uint32_t off = V ? voff[j % G_::NOFF] : koff[j % G_::NOFF];
+    if constexpr (PAGED) {
+      g2l16_opaque((const uint8_t *)(V ? s.v : s.k) + (uint64_t)(V ? vrow[j] : krow[j]) * G_::RB + off, to);
+    } else {
+      const int key0 = it.x0 + i * KT;
+      const long ld = V ? s.ldv : s.ldk;
+      const T *t = (V ? s.v : s.k) + (long)key0 * ld;
+      if (WHOLE) {
+        g2l16_sbase(t + (long)(j / G_::NOFF * G_::NOFF * 4 * G_::RPL) * ld, off, to);
+      } else {  // rows past the keys read the last one
+        int ln = lane;
+        asm volatile("" : "+v"(ln));  // opaque: the loop keeps none of these addresses in registers
+        const int r = blk * G_::RPL + ln / G_::CH, c = ln % G_::CH;
+        const int from = min(PERM && !V ? krow_key(r) : r, it.x1 - 1 - key0), ch = c ^ (V ? S_::fv(r) : S_::fk(r));
+        g2l16_sbase(t, ((uint32_t)from * (uint32_t)ld + ch * 8) * 2u, to);
+      }
+    }
+  }
+  HXA_DEV void load_all(int i) {
+    if (whole(i)) {
+#pragma unroll
+      for (int n = 0; n < 2 * G_::NLD; n++) load<true>(i, n);
+    } else {
+#pragma unroll
+      for (int n = 0; n < 2 * G_::NLD; n++) load<false>(i, n);
+    }
+  }
+  // the rows of key x, which is there
+  HXA_DEV void rows(int x, const T *&kr, const T *&vr) const {
+    if constexpr (PAGED) {
+      const unsigned y = x < s.P ? x : x - s.P;
+      const uint32_t e = (x < s.P ? s.prefix : s.table)[y / (unsigned)s.page];
+      const uint64_t r = (uint64_t)((e * s.H + s.h) * s.page + y % (unsigned)s.page) * HD;
+      kr = s.k + r;
+      vr = s.v + r;
+    } else {
+      kr = s.k + (long)x * s.ldk;
+      vr = s.v + (long)x * s.ldv;
+    }
   }
 };
 
@@ -232,7 +259,8 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
   typedef typename HxaVec<T>::v8 v8;
   typedef typename HxaVec<T>::v4 v4;
   typedef Swz<T, HD, true> S_;
-  constexpr int NB = W == 4 ? 2 : 1;  // 32-key blocks of a tile for each wave
+  constexpr int NB = W == 4 ? 2 : 1;       // 32-key blocks of a tile for each wave
+  constexpr int ND = HD / 32, AK = 2, AV = 3;  // dim blocks; fragments of K (V) read ahead
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = W == 4 ? wave : wave & 1, kh = W == 4 ? 0 : wave >> 1;
   const int g = lane >> 5, ql = lane & 31;
@@ -250,48 +278,64 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
   const int wave_max = it.r0 + rw * 32 <= last ? row_limit(it, min(it.r0 + rw * 32 + 31, last)) : -1;
 
 #pragma unroll
-  for (int d = 0; d < HD / 32; d++) acc[d] = (float16_t){};
+  for (int d = 0; d < ND; d++) acc[d] = (float16_t){};
   mrun = -INFINITY;
   lsum = 0.0f;
   const int nt = (it.x1 - it.x0 + KT - 1) / KT;
   if (nt <= 0) return;
   Loader<T, HD, true, PAGED> ld(s, it, lds, lane, wave);
-  uint64_t km_next = ld.load(0);
+  uint64_t km = ld.open(0);
+  ld.load_all(0);
 
-  // V^T fragment of 32 dims dblk, keys kb .. kb + 15 (kb a multiple of 16): lane (g, ql) dim 32 dblk + ql, keys kb + 8 g .. + 7
-  const int s4 = (lane & 15) >> 2, sub = (lane >> 4) & 1;
-  const int vkey = 8 * g + s4;
-  const int vlow = ((2 * sub + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;  // within 64 bytes
-  uint32_t vat[HD / 32];
+  // V^T fragment of 32 dims d, keys kb .. kb + 15 (kb a multiple of 16): lane (g, ql) dim 32 d + ql, keys kb + 8 g .. + 7; 16 lanes read
+  // 4 keys x 16 dims at a time
+  const int vkey = 8 * g + ((lane & 15) >> 2);
+  const int vlow = ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;  // within 64 bytes
+  uint32_t vat[ND];
 #pragma unroll
-  for (int d = 0; d < HD / 32; d++) vat[d] = vkey * G_::RB + (((d << 2) ^ S_::fv(vkey)) << 4) + vlow;  // fv(vkey + 4) is the same
-  static_assert(HD == 64 || HD == 128 || HD == 256, "heads");
+  for (int d = 0; d < ND; d++) vat[d] = vkey * G_::RB + (((d << 2) ^ S_::fv(vkey)) << 4) + vlow;  // fv(vkey + 4) is the same
 
-  for (int i = 0; i < nt; i++) {
-    wait_vm<0>();
-    reads_done_barrier();  // tile i has landed; every wave is done with tile i - 1
-    const uint64_t km = km_next;
+  // One tile for this wave. MAIN: every row sees all of it, and the next tile is whole: its loads are issued one beside each
+  // product of K (64 bytes a clock and CU: eight in a row hold a wave for 600 cycles). Fragments are read AK (AV) products ahead: without
+  // the fences each is read right before its use, a LDS latency a product.
+  auto tile = [&](int i, uint64_t kmi, bool cut, auto main) {
+    constexpr bool MAIN = decltype(main)::value;
     const int key0 = it.x0 + i * KT;
-    const bool more = i + 1 < nt;
-    if (more) km_next = ld.load(i + 1);
-    const bool cut = km != ~0ull || key0 + KT - 1 > lim_min;
-    uint64_t apart = 0;
-    if (cut) apart = fix_v<T, HD>(ld.vbuf(i), lds + G_::FLAGS, key0, km, lim_min, tid);
-    if (wave_max < key0 + 32 * kh) continue;
     const uint8_t *kb = ld.kbuf(i), *vb = ld.vbuf(i);
+    auto kfrag = [&](int ds, int b) {
+      const int row = (b + kh) * 32 + ql, ch = 2 * ds + g;
+      return *(const v8 *)(kb + row * G_::RB + ((ch ^ S_::fk(row)) << 4));
+    };
+    auto vfrag = [&](int n) {  // n = (16-key slice) ND + dims
+      const uint8_t *at = vb + vat[n % ND] + (kh * 32 + n / ND * 16) * G_::RB;
+      return __builtin_shufflevector(read_tr<v4>(at), read_tr<v4>(at + 4 * G_::RB), 0, 1, 2, 3, 4, 5, 6, 7);
+    };
     float16_t S[NB];
+    v8 kf[AK + 1][NB];
 #pragma unroll
-    for (int b = 0; b < NB; b++) S[b] = (float16_t){};
+    for (int ds = 0; ds < AK; ds++)
 #pragma unroll
-    for (int ds = 0; ds < HD / 16; ds++)
+      for (int b = 0; b < NB; b++) kf[ds][b] = kfrag(ds, b);
 #pragma unroll
-      for (int b = 0; b < NB; b++) {
-        const int row = (b + kh) * 32 + ql, ch = 2 * ds + g;
-        S[b] = mma32(*(const v8 *)(kb + row * G_::RB + ((ch ^ S_::fk(row)) << 4)), qf[ds], S[b]);
+    for (int ds = 0; ds < HD / 16; ds++) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (ds + AK < HD / 16) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) kf[(ds + AK) % (AK + 1)][b] = kfrag(ds + AK, b);
       }
-    if (cut) {
+      if constexpr (MAIN) ld.template load<true>(i + 1, ds);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < NB; b++) S[b] = mma32(kf[ds % (AK + 1)][b], qf[ds], ds == 0 ? (float16_t){} : S[b]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    v8 vf[AV + 1];
+#pragma unroll
+    for (int n = 0; n < AV; n++) vf[n] = vfrag(n);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!MAIN && cut) {
       const int n = lim - key0;
-      const uint64_t see = (km & (n >= 63 ? ~0ull : n < 0 ? 0ull : (2ull << n) - 1)) >> (32 * kh + 8 * g);
+      const uint64_t see = (kmi & (n >= 63 ? ~0ull : n < 0 ? 0ull : (2ull << n) - 1)) >> (32 * kh + 8 * g);
 #pragma unroll
       for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -315,67 +359,106 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
       if (need) mrun = mt;
       lsum *= alpha;
 #pragma unroll
-      for (int d = 0; d < HD / 32; d++) acc[d] *= alpha;
+      for (int d = 0; d < ND; d++) acc[d] *= alpha;
     }
     const float mb = mrun == -INFINITY ? 0.0f : mrun * c;
     v8 pf[NB][2];
     float ls[2] = {0.0f, 0.0f};
+    // two probabilities: rounded to the type, and their sum as rounded
+    auto expo2 = [&](int n) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(S[n >> 4][n & 15], c, -mb));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(S[n >> 4][(n & 15) + 1], c, -mb));
+      const typename HxaVec<T>::v2 h = {(T)p0, (T)p1};
+      pf[n >> 4][(n >> 3) & 1][n & 7] = h[0];
+      pf[n >> 4][(n >> 3) & 1][(n & 7) + 1] = h[1];
+      ls[(n >> 1) & 1] = sum2(h, ls[(n >> 1) & 1]);
+    };
+    // P V of a 32-key block beside the exponentials of the next one (in the compiler's order: fences as above change nothing, and cost 5%
+    // with heads of 64)
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+    for (int n = 0; n < 16; n += 2) expo2(n);
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(S[b][r], c, -mb));
-        pf[b][r >> 3][r & 7] = (T)p;
-        ls[r & 1] += p;
-      }
-    lsum += ls[0] + ls[1];
+    for (int n = 0; n < 2 * NB * ND; n++) {
+      if (n + AV < 2 * NB * ND) vf[(n + AV) % (AV + 1)] = vfrag(n + AV);
+      acc[n % ND] = mma32(vf[n % (AV + 1)], pf[n / (2 * ND)][n / ND & 1], acc[n % ND]);
+      if (NB == 2 && n < 2 * ND && (ND < 8 || n % 2 == 0)) {
 #pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-      for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-        for (int d = 0; d < HD / 32; d++) {
-          const uint8_t *at = vb + vat[d] + ((b + kh) * 32 + ks * 16) * G_::RB;
-          const v4 x = read_tr<v4>(at), y = read_tr<v4>(at + 4 * G_::RB);
-          const v8 vf = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-          acc[d] = mma32(vf, pf[b][ks], acc[d]);
-        }
-    // values that are not finite and that only some rows see: their keys one by one
-    while (apart) {
-      const int f = __builtin_ctzll(apart);
-      apart &= apart - 1;
-      const int fb = f - 32 * kh;
-      if (fb < 0 || fb >= 32 * NB) continue;
-      const T *vr = ld.vrow(i, f, !more);
-      float p = 0.0f;
-      const int idx = (fb >> 5) * 16 + ((fb >> 4) & 1) * 8 + (fb & 7);
-#pragma unroll
-      for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int r = 0; r < 16; r++)
-          if (idx == b * 16 + r) p = (float)pf[b][r >> 3][r & 7];
-      float lo, hi;
-      halves(p, lo, hi);
-      p = (fb >> 3) & 1 ? hi : lo;
-      if (lim >= key0 + f) {
-#pragma unroll
-        for (int d = 0; d < HD / 32; d++)
-#pragma unroll
-          for (int e4 = 0; e4 < 4; e4++) {
-            const v4 v = *(const v4 *)(vr + 32 * d + 8 * e4 + 4 * g);
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[d][4 * e4 + e] += p * (float)v[e];
-          }
+        for (int e = 0; e < (ND < 8 ? 8 / ND : 2); e += 2) expo2(16 + n * 8 / ND + e);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    lsum += ls[0] + ls[1];
+  };
+
+  int i = 0;
+  const int nmain = PAGED ? min((lim_min + 1 - it.x0) / KT, nt - 1) : min(lim_min + 1 - it.x0, it.x1 - it.x0 - KT) / KT;
+  while (i < nmain && km == ~0ull) {
+    wait_vm<0>();
+    reads_done_barrier();  // tile i has landed; every wave is done with tile i - 1
+    km = ld.open(i + 1);
+    tile(i, ~0ull, false, std::true_type{});
+    i++;
+  }
+  // flags of the tiles whose values fix_v took out: only the last three can hold keys that some rows see and some do not
+  uint64_t apart[3] = {0, 0, 0};
+  for (; i < nt; i++) {
+    wait_vm<0>();
+    reads_done_barrier();
+    const int key0 = it.x0 + i * KT;
+    const uint64_t kmi = km;
+    if (i + 1 < nt) {
+      km = ld.open(i + 1);
+      ld.load_all(i + 1);
+    }
+    const bool cut = kmi != ~0ull || key0 + KT - 1 > lim_min;
+    if (cut) {
+      const uint64_t f = fix_v<T, HD>(ld.vbuf(i), lds + G_::FLAGS, key0, kmi, lim_min, tid);
+      if (i == nt - 1) apart[0] = f;
+      if (i == nt - 2) apart[1] = f;
+      if (i == nt - 3) apart[2] = f;
+    }
+    if (wave_max >= key0 + 32 * kh) tile(i, kmi, cut, std::false_type{});
   }
   float lo, hi;
   halves(lsum, lo, hi);
   lsum = lo + hi;
-  if constexpr (W == 2) {  // join the key halves: waves 2, 3 hand theirs to waves 0, 1
+  if (apart[0] | apart[1] | apart[2]) {  // the values taken out, key by key, to the rows that see them
+    const float mb = mrun == -INFINITY ? 0.0f : mrun * c;
+#pragma unroll 1
+    for (int k = 0; k < 3; k++) {
+      uint64_t left = k == 0 ? apart[0] : k == 1 ? apart[1] : apart[2];
+      for (; left; left &= left - 1) {
+        const int f = __builtin_ctzll(left), x = it.x0 + (nt - 1 - k) * KT + f;
+        if (W == 2 && f >> 5 != kh) continue;
+        const T *kr, *vr;
+        ld.rows(x, kr, vr);
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HD / 16; j++) {
+          const v8 kk = *(const v8 *)(kr + 16 * j + 8 * g);
+#pragma unroll
+          for (int e = 0; e < 8; e++) dot = fmaf((float)kk[e], (float)qf[j][e], dot);
+        }
+        halves(dot, lo, hi);
+        const float p = __builtin_amdgcn_exp2f(fmaf(lo + hi, c, -mb));
+        if (lim >= x) {
+#pragma unroll
+          for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; e4++) {
+              const v4 v = *(const v4 *)(vr + 32 * d + 8 * e4 + 4 * g);
+#pragma unroll
+              for (int e = 0; e < 4; e++) acc[d][4 * e4 + e] += p * (float)v[e];
+            }
+        }
+      }
+    }
+  }
+  if constexpr (W == 2) {  // join the halves of the keys: the second half's waves hand theirs to the first's
+    constexpr int PART = HD / 8 * 64;  // float4 of a wave's accumulators
     reads_done_barrier();
-    float4_t *ox = (float4_t *)lds + rw * (HD / 8 * 64);
-    float *ml = (float *)(lds + 2 * HD / 8 * 1024) + rw * 128;
+    float4_t *ox = (float4_t *)lds + rw * PART;
+    float *ml = (float *)((float4_t *)lds + W * PART) + rw * 128;
     if (kh == 1) {
 #pragma unroll
       for (int d = 0; d < HD / 32; d++)
@@ -422,10 +505,11 @@ HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uin
   typedef typename HxaVec<T>::v4 v4;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int rw = W == 4 ? wave : wave & 1;
+  const bool second = W == 2 && wave >= 2;  // has handed its sums over
   const int g = lane >> 5, ql = lane & 31, r0 = it.r0 + rw * 32;
   if (out.part != nullptr) {
     const int R = r0 + ql;
-    if ((W == 2 && wave >= 2) || R >= it.nrows) return;
+    if (second || R >= it.nrows) return;
     const long at = (long)out.slot * out.rows + (long)(it.tok0 + R / it.G) * out.Hq + head0 + R % it.G;
     if (g == 0) out.ml[at] = (float2_t){m == -INFINITY ? m : m * c, l};
     if (l == 0.0f) return;  // (l is NaN where a score is: written)
@@ -440,7 +524,7 @@ HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uin
   }
   // whole rows: staged through LDS, 8-byte unit u of row r at u ^ (r % 16)
   reads_done_barrier();  // every wave is done with the tiles (and the join)
-  if (W == 2 && wave >= 2) return;
+  if (second) return;
   constexpr int RB = HD * 2, UN = HD / 4;
   uint8_t *stage = lds + rw * 32 * RB;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -482,7 +566,8 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
   const int nt = (it.x1 - it.x0 + KT - 1) / KT;
   if (nt > 0) {
     Loader<T, HD, false, PAGED> ld(s, it, lds, lane, wave);
-    uint64_t km_next = ld.load(0);
+    uint64_t km_next = ld.open(0);
+    ld.load_all(0);
     const T *qp = q + (long)(it.tok0 + Rc / it.G) * ldq + (long)(head0 + Rc % it.G) * HD;
     v8 qf[HD / 32];
 #pragma unroll
@@ -490,16 +575,23 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
     const int lim = row_limit(it, Rc), lim_min = row_limit(it, it.r0);
     const int vkey = 16 * wave + 4 * gi + (ql >> 2);
     const int krow = 16 * wave + ql;
+    uint64_t apart[2] = {0, 0};  // flags of the tiles whose values fix_v took out
     for (int i = 0; i < nt; i++) {
       wait_vm<0>();
       reads_done_barrier();
       const uint64_t km = km_next;
       const int key0 = it.x0 + i * KT;
       const bool more = i + 1 < nt;
-      if (more) km_next = ld.load(i + 1);
+      if (more) {
+        km_next = ld.open(i + 1);
+        ld.load_all(i + 1);
+      }
       const bool cut = km != ~0ull || key0 + KT - 1 > lim_min;
-      uint64_t apart = 0;
-      if (cut) apart = fix_v<T, HD>(ld.vbuf(i), lds + G_::FLAGS, key0, km, lim_min, tid);
+      if (cut) {
+        const uint64_t f = fix_v<T, HD>(ld.vbuf(i), lds + G_::FLAGS, key0, km, lim_min, tid);
+        if (i == nt - 1) apart[0] = f;
+        if (i == nt - 2) apart[1] = f;
+      }
       const uint8_t *kb = ld.kbuf(i) + krow * G_::RB, *vb = ld.vbuf(i) + vkey * G_::RB;
       float4_t S = {};
 #pragma unroll
@@ -533,25 +625,37 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
         const int ch = 2 * d + ((ql & 3) >> 1);
         acc[d] = mma16h(read_tr<v4>(vb + ((ch ^ S_::fv(vkey)) << 4) + (ql & 1) * 8), pf, acc[d]);
       }
-      while (apart) {
-        const int f = __builtin_ctzll(apart);
-        apart &= apart - 1;
-        if (f >> 4 != wave) continue;
-        const T *vr = ld.vrow(i, f, !more);
-        const int e0 = f & 3;
-        const float mine = e0 == 0 ? (float)pf[0] : e0 == 1 ? (float)pf[1] : e0 == 2 ? (float)pf[2] : (float)pf[3];
-        const float p = __shfl(mine, ((f >> 2) & 3) * 16 + ql);
-        if (lim >= key0 + f) {
+    }
+    lsum = add16(lsum);
+    if (apart[0] | apart[1]) {  // (16 rows span at most 16 tokens)
+      const float mb = mrun == -INFINITY ? 0.0f : mrun * c;
+#pragma unroll 1
+      for (int k = 0; k < 2; k++) {
+        uint64_t left = k == 0 ? apart[0] : apart[1];
+        for (; left; left &= left - 1) {
+          const int f = __builtin_ctzll(left), x = it.x0 + (nt - 1 - k) * KT + f;
+          if (f >> 4 != wave) continue;
+          const T *kr, *vr;
+          ld.rows(x, kr, vr);
+          float dot = 0.0f;
 #pragma unroll
-          for (int d = 0; d < ND; d++) {
-            const v4 v = *(const v4 *)(vr + 16 * d + 4 * gi);
+          for (int j = 0; j < HD / 32; j++) {
+            const v8 kk = *(const v8 *)(kr + 32 * j + 8 * gi);
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[d][e] += p * (float)v[e];
+            for (int e = 0; e < 8; e++) dot = fmaf((float)kk[e], (float)qf[j][e], dot);
+          }
+          const float p = __builtin_amdgcn_exp2f(fmaf(add16(dot), c, -mb));
+          if (lim >= x) {
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+              const v4 v = *(const v4 *)(vr + 16 * d + 4 * gi);
+#pragma unroll
+              for (int e = 0; e < 4; e++) acc[d][e] += p * (float)v[e];
+            }
           }
         }
       }
     }
-    lsum = add16(lsum);
   }
   // join the four waves: wave w takes the dims [w HD / 4, (w + 1) HD / 4)
   reads_done_barrier();
@@ -606,9 +710,57 @@ struct Block {
   int seq, b, n;  // the sequence, its first row in the call and its tokens
   int first;      // first row (token x G + head) of the block within the sequence; -1: none
 };
-// Blocks are numbered over the sequences in order, ceil(n G / RB) each, a sequence's from its end to its start (the longest first).
-// cu's entries are clamped into [0, T]. Whole wave.
-HXA_DEV Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int RB, int blk, int lane) {
+// Block `blk` of the grid: sequence i has ceil(n_i G / RB) blocks, and a block's keys grow with its place in the sequence, so places
+// are dealt from the highest down over all sequences (the longest first). Two workgroups share a CU: of the second
+// layer (blocks first .. 2 first - 1, `first` = CUs / key heads) the order is reversed, so that the longest block has the shortest
+// of them beside it. (4096 tokens, 16 / 8 heads: 512 workgroups, 96 us in falling order, XX so.) Above 64 sequences: in their order, each from its
+// end. cu's entries are clamped into [0, T]. Whole wave.
+HXA_DEV int wave_sum_i(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return __builtin_amdgcn_readlane(v, 63);
+}
+HXA_DEV Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int RB, int blk, int first, int lane) {
+  const Block none{0, 0, 0, -1};
+  if (nseq <= 64) {
+    int b = 0, e = 0;
+    if (lane < nseq) {
+      b = min(max(cu[lane], 0), T);
+      e = min(max(cu[lane + 1], b), T);
+    }
+    const int nb = (int)(((long)(e - b) * G + RB - 1) / RB);
+    const int total = nseq == 1 ? __builtin_amdgcn_readfirstlane(nb) : wave_sum_i(nb);
+    if (blk >= total) return none;
+    if (blk >= first && blk < 2 * first) blk = min(2 * first, total) - 1 - (blk - first);
+    int w = 0, j = total - 1 - blk;  // one sequence
+    if (nseq > 1) {
+      // S(L) = number of blocks at places >= L; the block's place j has S(j + 1) <= blk < S(j)
+      int lo = 0, hi = total, s_hi = 0;  // S(hi) <= blk < S(lo)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1, s = wave_sum_i(max(nb - mid, 0));
+        if (s <= blk) {
+          hi = mid;
+          s_hi = s;
+        } else {
+          lo = mid;
+        }
+      }
+      j = lo;
+      uint64_t at = __ballot(nb > j);
+      for (int k = blk - s_hi; k > 0; k--) at &= at - 1;
+      w = __builtin_ctzll(at);
+    }
+    Block r;
+    r.seq = w;
+    r.b = __builtin_amdgcn_readlane(b, w);
+    r.n = __builtin_amdgcn_readlane(e, w) - r.b;
+    r.first = j * RB;
+    return r;
+  }
   int seen = 0;  // blocks of the sequences before `base`
   for (int base = 0; base < nseq; base += 64) {
     const int i = base + lane;
@@ -645,7 +797,7 @@ struct CausalArgs {
   void *o;
   long ldq, ldk, ldv, ldo;
   const int *cu;
-  int T, nseq, G, Hk;
+  int T, nseq, G, Hk, first;
   float c;
 };
 
@@ -658,7 +810,7 @@ __global__ HXA_CAUSAL_BOUNDS void causal_kernel(CausalArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63;
   const int h = blockIdx.x % p.Hk, blk = blockIdx.x / p.Hk;  // key heads innermost: with 8 of them each XCD keeps its own head's keys
-  const Block b = find_block(p.cu, p.nseq, p.T, p.G, 32 * W, blk, lane);
+  const Block b = find_block(p.cu, p.nseq, p.T, p.G, 32 * W, blk, p.first, lane);
   if (b.first < 0) return;
   const long row0 = b.b;
   Keys<T> s{};
@@ -754,7 +906,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   } else {
     const int own = rest - p.np_blocks * p.np_split, split = own / p.n_blocks;
     mode = p.n_mode;
-    const Block b = find_block(p.c.cu, p.c.nseq, p.T, p.G, mode_rows(mode), own % p.n_blocks, lane);
+    const Block b = find_block(p.c.cu, p.c.nseq, p.T, p.G, mode_rows(mode), own % p.n_blocks, 1 << 29, lane);
     if (b.first < 0) return;
     const long len = p.c.len[b.seq];
     const int held = (int)min(max(len, 0L), (long)p.c.ldt * p.c.page);
@@ -775,30 +927,70 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   any_item<T, HD>(mode, s, it, p, h * p.G, lds, out);
 }
 
-// The partials of a row joined: weights 2^(m_s - m) against the common maximum, then one division and one rounding. HD / 4 lanes a
-// row. A slot whose sum is 0 saw no key and wrote no values.
+// The partials of a row joined: weights 2^(m_s - m) against the common maximum, then one division and one rounding. HD / 4 lanes
+// hold a row; sg of them side by side share its slots (nslots is up to some hundred where few rows read a long cache), each
+// with 8 slots' sums in flight, then 8 slots' values. A slot whose sum is 0 saw no key and holds no values.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs p, int nslots) {
+__global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs p, int nslots, int sg) {
   typedef typename HxaVec<T>::v4 v4;
-  constexpr int LPR = HD / 4;
-  const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR, rows = (long)p.T * p.Hq;
-  if (row >= rows) return;
-  const int tok = (int)(row / p.Hq), head = (int)(row - (long)tok * p.Hq), u = threadIdx.x % LPR;
-  if (tok < p.c.cu[0] || tok >= p.c.cu[p.c.nseq]) return;
-  float m = -INFINITY;
-  for (int s = 0; s < nslots; s++) m = fmaxf(m, p.ml[s * rows + row][0]);
-  const float mz = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
+  constexpr int LPR = HD / 4, N = 8;
+  __shared__ float4_t so[256];
+  __shared__ float2_t sml[256];
+  const int tid = threadIdx.x, u = tid % LPR, grp = tid / LPR % sg, rpw = 256 / LPR / sg;
+  const long row = (long)blockIdx.x * rpw + tid / LPR / sg, rows = (long)p.T * p.Hq;
+  const int tok = (int)min(row / p.Hq, (long)p.T - 1), head = (int)(row - row / p.Hq * p.Hq);
+  const bool mine = row < rows && tok >= p.c.cu[0] && tok < p.c.cu[p.c.nseq];
+  float m = -INFINITY, l = 0.0f;
   float4_t o = {};
-  for (int s = 0; s < nslots; s++) {
-    const float2_t x = p.ml[s * rows + row];
-    if (x[1] == 0.0f) continue;
-    const float a = __builtin_amdgcn_exp2f(x[0] - mz);
-    l += x[1] * a;
-    const float4_t y = *(const float4_t *)(p.part + (s * rows + row) * HD + 4 * u);
+  if (mine)
+    for (int s0 = grp; s0 < nslots; s0 += N * sg) {
+      float2_t x[N];
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] += y[e] * a;
+      for (int j = 0; j < N; j++) {
+        const int s = s0 + j * sg;
+        x[j] = s < nslots ? p.ml[s * rows + row] : (float2_t){-INFINITY, 0.0f};
+      }
+      float4_t y[N];
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        y[j] = x[j][1] != 0.0f ? *(const float4_t *)(p.part + ((s0 + j * sg) * rows + row) * HD + 4 * u) : (float4_t){};
+      float mt = m;
+#pragma unroll
+      for (int j = 0; j < N; j++) mt = fmaxf(mt, x[j][0]);
+      const float mz = mt == -INFINITY ? 0.0f : mt, b = __builtin_amdgcn_exp2f(m - mz);
+      m = mt;
+      l *= b;
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] *= b;
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const float a = x[j][1] != 0.0f ? __builtin_amdgcn_exp2f(x[j][0] - mz) : 0.0f;
+        l += x[j][1] * a;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += y[j][e] * a;
+      }
+    }
+  if (sg > 1) {
+    so[tid] = o;
+    sml[tid] = (float2_t){m, l};
+    __syncthreads();
+    if (grp != 0) return;
+    float mt = m;
+    for (int k = 1; k < sg; k++) mt = fmaxf(mt, sml[tid + k * LPR][0]);
+    const float mz = mt == -INFINITY ? 0.0f : mt, b = __builtin_amdgcn_exp2f(m - mz);
+    l *= b;
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] *= b;
+    for (int k = 1; k < sg; k++) {
+      const float2_t x = sml[tid + k * LPR];
+      const float4_t y = so[tid + k * LPR];
+      const float a = __builtin_amdgcn_exp2f(x[0] - mz);
+      l += x[1] * a;
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] += y[e] * a;
+    }
   }
+  if (!mine) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   v4 x;
 #pragma unroll
@@ -867,23 +1059,23 @@ CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws) {
   p.n_split = 1;
   p.n_chunk = 1 << 30;
   if (!ws) return p;
-  auto split = [&](long items, long keys, int &ns, int &chunk) {  // ranges of at least 4 tiles, until the items are two rounds
-    const long tiles = ceil_div(keys, KT), most = tiles / 4 > 1 ? tiles / 4 : 1;
-    long n = ceil_div(2 * slots, items);
-    n = n > most ? most : n;
-    const long per = ceil_div(tiles, n > 0 ? n : 1);
-    chunk = (int)((per > 0 ? per : 1) * KT);
-    ns = (int)(tiles > 0 ? ceil_div(tiles, per) : 1);
-  };
-  if (p.n_mode == 1 && c.nseq >= 2 && P >= 4 * KT) {  // the prefix once for all
+  const double target = 1.0;
+  const bool shared = p.n_mode == 1 && c.nseq >= 2 && P >= 4 * KT;
+  if (shared) {  // the prefix once for all
     p.np_mode = RT <= 16 ? 1 : RT <= 64 ? 2 : 4;
     p.np_blocks = (int)ceil_div(RT, p.np_mode == 1 ? 16 : 32 * p.np_mode);
-    split((long)p.np_blocks * c.H, P, p.np_split, p.np_chunk);
     p.x_first = (int)P;
-    split((long)p.n_blocks * c.H, cap, p.n_split, p.n_chunk);
-  } else {
-    split((long)p.n_blocks * c.H, P + cap, p.n_split, p.n_chunk);
   }
+  const long pt = ceil_div(P, KT), ct = ceil_div(cap, KT);
+  // tiles of the launch where the sequences are on average half as long as the table allows
+  const double tiles = (double)c.H * (shared ? (double)p.np_blocks * pt + p.n_blocks * ct * 0.5 : p.n_blocks * (pt + ct * 0.5));
+  const long chunk = std::max(1L, (long)std::ceil(tiles / (target * slots)));
+  auto ranges = [&](long n, int &ns, int &ck) {
+    ns = (int)std::max(1L, ceil_div(n, chunk));
+    ck = (int)(std::max(1L, ceil_div(n, ns)) * KT);
+  };
+  if (shared) ranges(pt, p.np_split, p.np_chunk);
+  ranges(ceil_div((shared ? 0 : P) + cap, KT), p.n_split, p.n_chunk);
   return p;
 }
 long cached_ws(const CachedPlan &p, const hxa_kv_cache &c, int T, int Hq) {
@@ -907,17 +1099,17 @@ extern "C" int hxa_attention_causal(int dtype, const void *q, long ldq, const vo
   if (!cu || (uintptr_t)cu % 4) return hxa_set_error(HXA_E_ARG, "attention_causal: cu");
   const int G = Hq / Hk;
   const long RT = (long)T * G;
-  CausalArgs p{q, k, v, o, ldq, ldk, ldv, ldo, cu, T, nseq, G, Hk, scale * L2E};
+  CausalArgs p{q, k, v, o, ldq, ldk, ldv, ldo, cu, T, nseq, G, Hk, std::max(1, causal_ncu() / Hk), scale * L2E};
   // 64 rows a workgroup while 128 would leave workgroup places free
-  const bool half = (RT / 128 + 1) * Hk < wg_slots(hd);
-  const int rb = half ? 64 : 128;
+  const int mode = (RT / 128 + nseq) * Hk < wg_slots(hd) ? 2 : 4;
+  const int rb = mode == 2 ? 64 : 128;
   const long wgs = (RT / rb + nseq) * Hk;
   if (wgs >= 1L << 24) return hxa_set_error(HXA_E_ARG, "attention_causal: T=%d nseq=%d Hq=%d are too many blocks", T, nseq, Hq);
   return by_type(dtype, hd, [&](auto ty, auto hdc, int id) -> int {
     typedef decltype(ty) T_;
     constexpr int HD = decltype(hdc)::value;
-    const auto f = half ? causal_kernel<T_, HD, 2> : causal_kernel<T_, HD, 4>;
-    const int r = allow_lds((const void *)f, Geo<T_, HD>::LDS, 2 * id + half);
+    const auto f = mode == 2 ? causal_kernel<T_, HD, 2> : causal_kernel<T_, HD, 4>;
+    const int r = allow_lds((const void *)f, Geo<T_, HD>::LDS, 2 * id + (mode == 2));
     if (r != HXA_OK) return hxa_set_error(r, "attention_causal: %d bytes of LDS", Geo<T_, HD>::LDS);
     hxa_launch(f, dim3((unsigned)wgs), dim3(256), Geo<T_, HD>::LDS, (hipStream_t)stream, p);
     return launched("attention_causal");
@@ -964,11 +1156,14 @@ extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long l
     typedef decltype(ty) T_;
     constexpr int HD = decltype(hdc)::value;
     const auto f = cached_kernel<T_, HD>;
-    const int a = allow_lds((const void *)f, Geo<T_, HD>::LDS, 16 + id);
+    const int a = allow_lds((const void *)f, Geo<T_, HD>::LDS, 18 + id);
     if (a != HXA_OK) return hxa_set_error(a, "attention_cached: %d bytes of LDS", Geo<T_, HD>::LDS);
     hxa_launch(f, dim3((unsigned)wgs), dim3(256), Geo<T_, HD>::LDS, st, p);
-    if (nslots > 1)
-      hxa_launch(cached_merge_kernel<T_, HD>, dim3((unsigned)ceil_div((long)T * Hq, 1024 / HD)), dim3(256), 0, st, p, nslots);
+    if (nslots > 1) {
+      int sg = 1;
+      while (sg * 4 < nslots && sg < 1024 / HD) sg *= 2;
+      hxa_launch(cached_merge_kernel<T_, HD>, dim3((unsigned)ceil_div((long)T * Hq, 1024 / HD / sg)), dim3(256), 0, st, p, nslots, sg);
+    }
     return launched("attention_cached");
   });
 }
