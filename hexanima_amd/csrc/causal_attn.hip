@@ -81,13 +81,28 @@ struct Keys {
 // a work item: rows [r0, r0 + rows of the mode) of nrows rows that belong together, keys [x0, x1)
 struct Item {
   int r0, nrows, G;
+  uint32_t gm;  // 2^32 / G, rounded down (2^32 - 1 for G = 1)
   int tok0;  // row R is token tok0 + R / G of the call
   int x0, x1;
   // row R sees the keys x <= base + R / G (not causal: base), but none past cap, and those up to least in any case
   int base, cap, least;
   bool causal;
 };
-HXA_DEV int row_limit(const Item &it, int R) { return max(min(it.causal ? it.base + R / it.G : it.base, it.cap), it.least); }
+// R / G and the rest: the product with the rounded reciprocal is at most one too small
+HXA_DEV int row_tok(const Item &it, int R, int &rest) {
+  int t = (int)__umulhi((uint32_t)R, it.gm);
+  rest = R - t * it.G;
+  if (rest >= it.G) {
+    rest -= it.G;
+    t++;
+  }
+  return t;
+}
+HXA_DEV int tok_limit(const Item &it, int tok) { return max(min(it.causal ? it.base + tok : it.base, it.cap), it.least); }
+HXA_DEV int row_limit(const Item &it, int R) {
+  int rest;
+  return tok_limit(it, row_tok(it, R, rest));
+}
 
 template <typename T, int HD>
 struct Geo {
@@ -229,13 +244,15 @@ HXA_DEV uint64_t fix_v(uint8_t *vb, uint8_t *flags, int key0, uint64_t km, int l
   const bool dead = !((km >> row) & 1);
   bool bad = false;
   if (!dead && key0 + row > lim_min) {
-    constexpr uint32_t E = HxaVec<T>::EXP, EL = E & 0xffff, EH = E & 0xffff0000u;
+    // a magnitude of at least the exponent's ones carries into the sign's place
+    uint32_t carry = 0;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const uint4_t x = *(const uint4_t *)(p + 16 * i);
 #pragma unroll
-      for (int e = 0; e < 4; e++) bad |= (x[e] & EL) == EL || (x[e] & EH) == EH;
+      for (int e = 0; e < 4; e++) carry |= (x[e] & 0x7fff7fffu) + (0x80008000u - HxaVec<T>::EXP);
     }
+    bad = (carry & 0x80008000u) != 0;
   }
   const uint64_t b = __ballot(bad);
   if (dead || ((b >> (lane & 60)) & 15)) {
@@ -268,11 +285,13 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
   const int R = it.r0 + rw * 32 + ql;
   const bool qok = R < it.nrows;
   const int Rc = qok ? R : it.nrows - 1;
-  const T *qp = q + (long)(it.tok0 + Rc / it.G) * ldq + (long)(head0 + Rc % it.G) * HD;
+  int rest;
+  const int tok = row_tok(it, Rc, rest);
+  const T *qp = q + (long)(it.tok0 + tok) * ldq + (long)(head0 + rest) * HD;
   v8 qf[HD / 16];
 #pragma unroll
   for (int i = 0; i < HD / 16; i++) qf[i] = *(const v8 *)(qp + i * 16 + 8 * g);
-  const int lim = row_limit(it, Rc);
+  const int lim = tok_limit(it, tok);
   const int last = it.nrows - 1;
   const int lim_min = row_limit(it, it.r0);
   const int wave_max = it.r0 + rw * 32 <= last ? row_limit(it, min(it.r0 + rw * 32 + 31, last)) : -1;
@@ -334,13 +353,24 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
     for (int n = 0; n < AV; n++) vf[n] = vfrag(n);
     __builtin_amdgcn_sched_barrier(0);
     if (!MAIN && cut) {
-      const int n = lim - key0;
-      const uint64_t see = (kmi & (n >= 63 ? ~0ull : n < 0 ? 0ull : (2ull << n) - 1)) >> (32 * kh + 8 * g);
+      // a row's limit hides the keys past x1 too (a range that ends before it ends with a tile); pages that are not there need the mask
+      const int n = lim - key0 - 32 * kh - 8 * g, left = it.x1 - key0;
+      if (!PAGED || kmi == (left >= KT ? ~0ull : (1ull << left) - 1)) {
 #pragma unroll
-      for (int b = 0; b < NB; b++)
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int r = 0; r < 16; r++)
-          if (!((see >> (32 * b + 16 * (r >> 3) + (r & 7))) & 1)) S[b][r] = -INFINITY;
+          for (int r = 0; r < 16; r++)
+            if (32 * b + 16 * (r >> 3) + (r & 7) > n) S[b][r] = -INFINITY;
+      } else {
+        const uint64_t see = kmi >> (32 * kh + 8 * g);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int k = 32 * b + 16 * (r >> 3) + (r & 7);
+            if (k > n || !((see >> k) & 1)) S[b][r] = -INFINITY;
+          }
+      }
     }
     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -503,6 +533,7 @@ struct Out {
 template <typename T, int HD, int W>
 HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uint8_t *lds, float16_t (&acc)[HD / 32], float m, float l) {
   typedef typename HxaVec<T>::v4 v4;
+  typedef typename HxaVec<T>::v8 v8;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int rw = W == 4 ? wave : wave & 1;
   const bool second = W == 2 && wave >= 2;  // has handed its sums over
@@ -510,7 +541,9 @@ HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uin
   if (out.part != nullptr) {
     const int R = r0 + ql;
     if (second || R >= it.nrows) return;
-    const long at = (long)out.slot * out.rows + (long)(it.tok0 + R / it.G) * out.Hq + head0 + R % it.G;
+    int rest;
+    const int tok = row_tok(it, R, rest);
+    const long at = (long)out.slot * out.rows + (long)(it.tok0 + tok) * out.Hq + head0 + rest;
     if (g == 0) out.ml[at] = (float2_t){m == -INFINITY ? m : m * c, l};
     if (l == 0.0f) return;  // (l is NaN where a score is: written)
     float *p = out.part + at * HD;
@@ -522,10 +555,11 @@ HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uin
             (float4_t){acc[d][4 * e4], acc[d][4 * e4 + 1], acc[d][4 * e4 + 2], acc[d][4 * e4 + 3]};
     return;
   }
-  // whole rows: staged through LDS, 8-byte unit u of row r at u ^ (r % 16)
+  // whole rows: staged through LDS, 16-byte chunk c of row r at c ^ sw(r)
   reads_done_barrier();  // every wave is done with the tiles (and the join)
   if (second) return;
-  constexpr int RB = HD * 2, UN = HD / 4;
+  constexpr int RB = HD * 2, CH = HD / 8;
+  auto sw = [](int r) { return HD == 64 ? (r >> 1) & 7 : r & 15; };
   uint8_t *stage = lds + rw * 32 * RB;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -535,16 +569,30 @@ HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uin
       v4 x;
 #pragma unroll
       for (int e = 0; e < 4; e++) x[e] = (T)(acc[d][4 * e4 + e] * inv);
-      const int u = 8 * d + 2 * e4 + g;
-      *(v4 *)(stage + ql * RB + ((u ^ (ql & 15)) << 3)) = x;
+      *(v4 *)(stage + ql * RB + (((4 * d + e4) ^ sw(ql)) << 4) + 8 * g) = x;
     }
-  constexpr int RPP = 64 / UN;  // rows a pass
-#pragma unroll 4
-  for (int p = 0; p < 32 / RPP; p++) {
-    const int r = p * RPP + lane / UN, u = lane % UN, R = r0 + r;
-    const v4 x = *(const v4 *)(stage + r * RB + ((u ^ (r & 15)) << 3));
-    if (R < it.nrows) *(v4 *)(out.o + (long)(it.tok0 + R / it.G) * out.ldo + (long)(head0 + R % it.G) * HD + 4 * u) = x;
-  }
+  constexpr int RPP = 64 / CH, N = 32 / RPP;  // rows a pass, passes
+  const int u = lane % CH, dt = RPP / it.G, dr = RPP - dt * it.G;  // from a lane's row to its next one
+  const int r = lane / CH, left = it.nrows - r0;
+  v8 x[N];
+#pragma unroll
+  for (int n = 0; n < N; n++) x[n] = *(const v8 *)(stage + (r + n * RPP) * RB + ((u ^ sw(r + n * RPP)) << 4));
+  int rest;
+  const int tok = row_tok(it, r0 + r, rest);
+  T *p = out.o + (long)(it.tok0 + tok) * out.ldo + (long)(head0 + rest) * HD + 8 * u;
+  const long step = dt * out.ldo + (long)dr * HD, wrap = out.ldo - (long)it.G * HD;
+  auto store = [&](auto all) {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      if (decltype(all)::value || r + n * RPP < left) *(v8 *)p = x[n];
+      rest += dr;
+      const bool w = rest >= it.G;
+      rest -= w ? it.G : 0;
+      p += step + (w ? wrap : 0);
+    }
+  };
+  if (left >= 32) store(std::true_type{});
+  else store(std::false_type{});
 }
 
 // ---- few rows ----
@@ -568,11 +616,13 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
     Loader<T, HD, false, PAGED> ld(s, it, lds, lane, wave);
     uint64_t km_next = ld.open(0);
     ld.load_all(0);
-    const T *qp = q + (long)(it.tok0 + Rc / it.G) * ldq + (long)(head0 + Rc % it.G) * HD;
+    int rest;
+  const int tok = row_tok(it, Rc, rest);
+  const T *qp = q + (long)(it.tok0 + tok) * ldq + (long)(head0 + rest) * HD;
     v8 qf[HD / 32];
 #pragma unroll
     for (int i = 0; i < HD / 32; i++) qf[i] = *(const v8 *)(qp + i * 32 + 8 * gi);
-    const int lim = row_limit(it, Rc), lim_min = row_limit(it, it.r0);
+    const int lim = tok_limit(it, tok), lim_min = row_limit(it, it.r0);
     const int vkey = 16 * wave + 4 * gi + (ql >> 2);
     const int krow = 16 * wave + ql;
     uint64_t apart[2] = {0, 0};  // flags of the tiles whose values fix_v took out
@@ -676,8 +726,9 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
     l += x[1] * a[w];
   }
   if (R >= it.nrows) return;
-  const long tok = it.tok0 + R / it.G;
-  const int head = head0 + R % it.G;
+  int rest;
+  const long tok = it.tok0 + row_tok(it, R, rest);
+  const int head = head0 + rest;
   const long at = (long)out.slot * out.rows + tok * out.Hq + head;
   if (out.part != nullptr) {
     if (wave == 0 && gi == 0) out.ml[at] = (float2_t){m == -INFINITY ? m : m * c, l};
@@ -710,57 +761,21 @@ struct Block {
   int seq, b, n;  // the sequence, its first row in the call and its tokens
   int first;      // first row (token x G + head) of the block within the sequence; -1: none
 };
-// Block `blk` of the grid: sequence i has ceil(n_i G / RB) blocks, and a block's keys grow with its place in the sequence, so places
-// are dealt from the highest down over all sequences (the longest first). Two workgroups share a CU: of the second
-// layer (blocks first .. 2 first - 1, `first` = CUs / key heads) the order is reversed, so that the longest block has the shortest
-// of them beside it. (4096 tokens, 16 / 8 heads: 512 workgroups, 96 us in falling order, XX so.) Above 64 sequences: in their order, each from its
-// end. cu's entries are clamped into [0, T]. Whole wave.
-HXA_DEV int wave_sum_i(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false);
+// Block `blk` of the grid: sequence i has ceil(n_i G / RB) blocks, and a block's keys grow with its place in the sequence. Up to 16
+// sequences, places are dealt from the highest down over all of them (the longest first). Two workgroups share a CU: of the second layer (blocks
+// first .. 2 first - 1, `first` = CUs / key heads) the order is reversed, so that the longest block has the shortest of
+// them beside it (4096 tokens, 32 / 8 heads: 149 -> 143 us). More sequences: in their order, each from its end. cu's entries are
+// clamped into [0, T]. Whole wave.
+HXA_DEV int wave_scan_i(int v) {  // inclusive
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
   v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-  return __builtin_amdgcn_readlane(v, 63);
+  return v;
 }
 HXA_DEV Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int RB, int blk, int first, int lane) {
-  const Block none{0, 0, 0, -1};
-  if (nseq <= 64) {
-    int b = 0, e = 0;
-    if (lane < nseq) {
-      b = min(max(cu[lane], 0), T);
-      e = min(max(cu[lane + 1], b), T);
-    }
-    const int nb = (int)(((long)(e - b) * G + RB - 1) / RB);
-    const int total = nseq == 1 ? __builtin_amdgcn_readfirstlane(nb) : wave_sum_i(nb);
-    if (blk >= total) return none;
-    if (blk >= first && blk < 2 * first) blk = min(2 * first, total) - 1 - (blk - first);
-    int w = 0, j = total - 1 - blk;  // one sequence
-    if (nseq > 1) {
-      // S(L) = number of blocks at places >= L; the block's place j has S(j + 1) <= blk < S(j)
-      int lo = 0, hi = total, s_hi = 0;  // S(hi) <= blk < S(lo)
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1, s = wave_sum_i(max(nb - mid, 0));
-        if (s <= blk) {
-          hi = mid;
-          s_hi = s;
-        } else {
-          lo = mid;
-        }
-      }
-      j = lo;
-      uint64_t at = __ballot(nb > j);
-      for (int k = blk - s_hi; k > 0; k--) at &= at - 1;
-      w = __builtin_ctzll(at);
-    }
-    Block r;
-    r.seq = w;
-    r.b = __builtin_amdgcn_readlane(b, w);
-    r.n = __builtin_amdgcn_readlane(e, w) - r.b;
-    r.first = j * RB;
-    return r;
-  }
   int seen = 0;  // blocks of the sequences before `base`
   for (int base = 0; base < nseq; base += 64) {
     const int i = base + lane;
@@ -769,25 +784,47 @@ HXA_DEV Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int
       b = min(max(cu[i], 0), T);
       e = min(max(cu[i + 1], b), T);
     }
-    const int nb = (int)(((long)(e - b) * G + RB - 1) / RB);
-    int inc = nb;  // inclusive scan
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int x = __shfl_up(inc, d);
-      if (lane >= d) inc += x;
+    const int nb = ((e - b) * G + RB - 1) / RB;  // (T G < 2^31 - RB: checked on the host)
+    const int inc = wave_scan_i(nb);
+    const int total = __builtin_amdgcn_readlane(inc, 63);
+    Block r{0, 0, 0, -1};
+    int w, j;
+    if (nseq <= 16) {
+      if (blk >= total) return r;
+      if (blk >= first && blk < 2 * first) blk = min(2 * first, total) - 1 - (blk - first);
+      w = 0;
+      j = total - 1 - blk;
+      if (nseq > 1) {
+        // S(L) = number of blocks at places >= L, 64 values of L a step; the block's place j has S(j + 1) <= blk < S(j)
+        int lo = 0, hi = total, s_hi = 0;
+        while (hi - lo > 1) {
+          const int step = (hi - lo + 63) >> 6, L = lo + (lane + 1) * step;
+          int s = 0;
+          for (int q = 0; q < nseq; q++) s += max(__builtin_amdgcn_readlane(nb, q) - L, 0);
+          const int k = __popcll(__ballot(s > blk));
+          s_hi = __builtin_amdgcn_readlane(s, min(k, 63));
+          lo += k * step;
+          hi = min(lo + step, hi);
+        }
+        j = lo;
+        uint64_t at = __ballot(nb > j);
+        for (int k = blk - s_hi; k > 0; k--) at &= at - 1;
+        w = __builtin_ctzll(at);
+      }
+    } else {
+      const uint64_t hit = __ballot(seen + inc > blk);
+      if (!hit) {
+        seen += total;
+        continue;
+      }
+      w = __builtin_ctzll(hit);
+      j = seen + __builtin_amdgcn_readlane(inc, w) - 1 - blk;  // blocks of the sequence behind this one
     }
-    const uint64_t hit = __ballot(seen + inc > blk);
-    if (hit) {
-      const int w = __builtin_ctzll(hit);
-      Block r;
-      r.seq = base + w;
-      r.b = __builtin_amdgcn_readlane(b, w);
-      r.n = __builtin_amdgcn_readlane(e, w) - r.b;
-      const int cnt = __builtin_amdgcn_readlane(nb, w), before = seen + __builtin_amdgcn_readlane(inc, w) - cnt;
-      r.first = (cnt - 1 - (blk - before)) * RB;
-      return r;
-    }
-    seen += __builtin_amdgcn_readlane(inc, 63);
+    r.seq = base + w;
+    r.b = __builtin_amdgcn_readlane(b, w);
+    r.n = __builtin_amdgcn_readlane(e, w) - r.b;
+    r.first = j * RB;
+    return r;
   }
   return Block{0, 0, 0, -1};
 }
@@ -798,6 +835,7 @@ struct CausalArgs {
   long ldq, ldk, ldv, ldo;
   const int *cu;
   int T, nseq, G, Hk, first;
+  uint32_t gm;
   float c;
 };
 
@@ -822,6 +860,7 @@ __global__ HXA_CAUSAL_BOUNDS void causal_kernel(CausalArgs p) {
   it.r0 = b.first;
   it.nrows = b.n * p.G;
   it.G = p.G;
+  it.gm = p.gm;
   it.tok0 = b.b;
   it.base = 0;
   it.cap = b.n - 1;
@@ -847,6 +886,8 @@ struct CachedArgs {
   void *o;
   long ldq, ldo;
   int T, G, Hq;
+  uint32_t gm;
+  int first;
   float cs;
   int np_mode, np_blocks, np_split, np_chunk;
   int n_mode, n_blocks, n_split, n_chunk;  // modes: 1 few rows (16), 2 rows (64), 4 rows (128)
@@ -890,6 +931,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   s.h = h;
   Item it;
   it.G = p.G;
+  it.gm = p.gm;
   Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, 0, p.Hq};
   int mode;
   if (rest < p.np_blocks * p.np_split) {
@@ -906,7 +948,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   } else {
     const int own = rest - p.np_blocks * p.np_split, split = own / p.n_blocks;
     mode = p.n_mode;
-    const Block b = find_block(p.c.cu, p.c.nseq, p.T, p.G, mode_rows(mode), own % p.n_blocks, 1 << 29, lane);
+    const Block b = find_block(p.c.cu, p.c.nseq, p.T, p.G, mode_rows(mode), own % p.n_blocks, p.first, lane);
     if (b.first < 0) return;
     const long len = p.c.len[b.seq];
     const int held = (int)min(max(len, 0L), (long)p.c.ldt * p.c.page);
@@ -1038,6 +1080,7 @@ int launched(const char *who) {
 }
 bool rows_ok(const void *p, long ld, int H, int hd) { return p != nullptr && (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld >= (long)H * hd; }
 
+uint32_t recip(int G) { return G == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)G); }
 long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
 // workgroups that run at once
@@ -1089,7 +1132,7 @@ extern "C" int hxa_attention_causal(int dtype, const void *q, long ldq, const vo
                                     int T, const int *cu, int nseq, int Hq, int Hk, int hd, float scale, void *stream) {
   if (dtype != HXA_DT_F16 && dtype != HXA_DT_BF16) return hxa_set_error(HXA_E_MODE, "attention_causal: dtype %d", dtype);
   if (hd != 64 && hd != 128 && hd != 256) return hxa_set_error(HXA_E_MODE, "attention_causal: heads of %d", hd);
-  if (T < 0 || T > HXA_MAX_ROWS || nseq < 0 || Hq <= 0 || Hk <= 0 || Hq > HXA_MAX_HEADS || Hq % Hk || (long)T * Hq >= 1L << 31)
+  if (T < 0 || T > HXA_MAX_ROWS || nseq < 0 || Hq <= 0 || Hk <= 0 || Hq > HXA_MAX_HEADS || Hq % Hk || (long)T * Hq >= 1L << 30)
     return hxa_set_error(HXA_E_ARG, "attention_causal: T=%d nseq=%d Hq=%d Hk=%d", T, nseq, Hq, Hk);
   if (!(scale > 0.0f) || !std::isfinite(scale)) return hxa_set_error(HXA_E_ARG, "attention_causal: scale %g", (double)scale);
   if (T == 0 || nseq == 0) return HXA_OK;
@@ -1099,7 +1142,7 @@ extern "C" int hxa_attention_causal(int dtype, const void *q, long ldq, const vo
   if (!cu || (uintptr_t)cu % 4) return hxa_set_error(HXA_E_ARG, "attention_causal: cu");
   const int G = Hq / Hk;
   const long RT = (long)T * G;
-  CausalArgs p{q, k, v, o, ldq, ldk, ldv, ldo, cu, T, nseq, G, Hk, std::max(1, causal_ncu() / Hk), scale * L2E};
+  CausalArgs p{q, k, v, o, ldq, ldk, ldv, ldo, cu, T, nseq, G, Hk, std::max(1, causal_ncu() / Hk), recip(G), scale * L2E};
   // 64 rows a workgroup while 128 would leave workgroup places free
   const int mode = (RT / 128 + nseq) * Hk < wg_slots(hd) ? 2 : 4;
   const int rb = mode == 2 ? 64 : 128;
@@ -1119,7 +1162,7 @@ extern "C" int hxa_attention_causal(int dtype, const void *q, long ldq, const vo
 static int cached_check(const hxa_kv_cache *c, int T, int Hq) {
   const int r = hxa_kv_check(c, T, "attention_cached");
   if (r != HXA_OK) return r;
-  if (Hq <= 0 || Hq > HXA_MAX_HEADS || Hq % c->H || (long)T * Hq >= 1L << 31)
+  if (Hq <= 0 || Hq > HXA_MAX_HEADS || Hq % c->H || (long)T * Hq >= 1L << 30)
     return hxa_set_error(HXA_E_ARG, "attention_cached: T=%d Hq=%d H=%d", T, Hq, c->H);
   if (((long)T * Hq / c->H / 16 + c->nseq) * c->H >= 1L << 20)
     return hxa_set_error(HXA_E_ARG, "attention_cached: T=%d nseq=%d H=%d are too many blocks", T, c->nseq, c->H);
@@ -1144,7 +1187,7 @@ extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long l
   const long need = cached_ws(pl, *c, T, Hq);
   if (need > 0 && (ws == nullptr || ws_bytes < need)) pl = cached_plan(*c, T, Hq, false);
   const int nslots = pl.np_split + pl.n_split;
-  CachedArgs p{*c, q, o, ldq, ldo, T, Hq / c->H, Hq, scale * L2E, pl.np_mode, pl.np_blocks, pl.np_split, pl.np_chunk,
+  CachedArgs p{*c, q, o, ldq, ldo, T, Hq / c->H, Hq, recip(Hq / c->H), std::max(1, causal_ncu() / c->H), scale * L2E, pl.np_mode, pl.np_blocks, pl.np_split, pl.np_chunk,
                pl.n_mode, pl.n_blocks, pl.n_split, pl.n_chunk, pl.x_first, nullptr, nullptr};
   if (nslots > 1) {
     p.part = (float *)ws;
