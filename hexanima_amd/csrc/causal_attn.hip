@@ -76,6 +76,8 @@ struct Keys {
   long ldk, ldv;    // contiguous: row strides
   const int *prefix, *table;  // paged: the prefix's pages, the sequence's own
   int P, page, npages, H, h;
+  int shift;  // log2(page) where it is a power of two (a division is 40 instructions, twice a tile), -1 otherwise
+  HXA_DEV unsigned slot(unsigned y) const { return shift >= 0 ? y >> shift : y / (unsigned)page; }
 };
 
 // a work item: rows [r0, r0 + rows of the mode) of nrows rows that belong together, keys [x0, x1)
@@ -159,7 +161,7 @@ struct Loader {
     if (x < it.x1) {
       const bool pre = x < s.P;
       const unsigned y = pre ? x : x - s.P;
-      ent = (pre ? s.prefix : s.table)[y / (unsigned)s.page];
+      ent = (pre ? s.prefix : s.table)[s.slot(y)];
     }
   }
   // tile i: where its keys lie, and the mask of those that are there; its loads follow
@@ -169,7 +171,7 @@ struct Loader {
       const int x = key0 + lane;
       const unsigned y = x < s.P ? x : x - s.P;
       const bool ok = x < it.x1 && (unsigned)ent < (unsigned)s.npages;
-      const uint32_t row = ok ? ((uint32_t)ent * s.H + s.h) * s.page + y % (unsigned)s.page : 0;  // < 2^32: checked on the host
+      const uint32_t row = ok ? ((uint32_t)ent * s.H + s.h) * s.page + (y - s.slot(y) * s.page) : 0;  // < 2^32: checked on the host
       const uint64_t mask = __ballot(ok);
       if (key0 + KT < it.x1) entry(i + 1);
 #pragma unroll
@@ -223,8 +225,8 @@ struct Loader {
   HXA_DEV void rows(int x, const T *&kr, const T *&vr) const {
     if constexpr (PAGED) {
       const unsigned y = x < s.P ? x : x - s.P;
-      const uint32_t e = (x < s.P ? s.prefix : s.table)[y / (unsigned)s.page];
-      const uint64_t r = (uint64_t)((e * s.H + s.h) * s.page + y % (unsigned)s.page) * HD;
+      const uint32_t e = (x < s.P ? s.prefix : s.table)[s.slot(y)];
+      const uint64_t r = (uint64_t)((e * s.H + s.h) * s.page + (y - s.slot(y) * s.page)) * HD;
       kr = s.k + r;
       vr = s.v + r;
     } else {
@@ -876,10 +878,12 @@ __global__ HXA_CAUSAL_BOUNDS void causal_kernel(CausalArgs p) {
 }
 
 // ---- over the cache ----
-// The keys of a sequence are one list: the prefix (P keys), then its own. Work items of a launch, in grid order:
-//   shared: np_blocks blocks of all T G rows x np_split ranges of the prefix, without a mask (rows of unused tokens are computed and
-//           never read), partial slots [0, np_split)
-//   own:    n_blocks blocks of the sequences' rows x n_split ranges of n_chunk keys of [x_first, P + own), slots from np_split on
+// The keys of a sequence are one list: the prefix (P keys), then its own. The items of a key head, in grid order:
+//   shared: np_blocks blocks of all T G rows x ranges of the prefix, without a mask (rows of unused tokens are computed and
+//           never read); partial slots [0, sp_max)
+//   own:    the blocks of the sequences' rows x ranges of their keys [x_first, P + own), slots from sp_max on
+// How long the ranges are follows from the lengths as they are on the device: every workgroup adds the tiles of the whole launch up and
+// cuts them into as many items as run at once, so one long sequence among short ones does not decide the time.
 struct CachedArgs {
   hxa_kv_cache c;
   const void *q;
@@ -887,14 +891,117 @@ struct CachedArgs {
   long ldq, ldo;
   int T, G, Hq;
   uint32_t gm;
-  int first;
+  int shift;
   float cs;
-  int np_mode, np_blocks, np_split, np_chunk;
-  int n_mode, n_blocks, n_split, n_chunk;  // modes: 1 few rows (16), 2 rows (64), 4 rows (128)
-  int x_first;  // 0: own items take the prefix too
-  float *part;  // nullptr: straight to o (np_split = 0, n_split = 1)
+  int np_mode, np_blocks, sp_max;  // sp_max 0: nothing is shared
+  int n_mode, s_max;               // modes: 1 few rows (16), 2 rows (64), 4 rows (128)
+  int x_first;    // 0: own items take the prefix too
+  int budget;     // items a key head that run at once
+  int least;      // tiles an item is worth
+  float *part;    // nullptr: straight to o (sp_max = 0, s_max = 1)
   float2_t *ml;
 };
+__host__ HXA_DEV int mode_rows(int mode) { return mode == 1 ? 16 : 32 * mode; }
+
+// what item `q` of a key head is; split < 0: there is none
+struct Work {
+  bool shared;
+  int split, nsplit, chunk;  // range of `chunk` tiles
+  int block;                 // shared: the block of rows
+  int seq, b, n, len, first; // own: the sequence, its rows in the call, its length, the first row of the block
+};
+HXA_DEV Work find_work(const CachedArgs &p, int q, int lane) {
+  const hxa_kv_cache &c = p.c;
+  const int RB = mode_rows(p.n_mode), pt = p.sp_max ? (c.prefix_len + KT - 1) / KT : 0;
+  const long cap = (long)c.ldt * c.page;
+  int b = 0, n = 0, len = 0, nb = 0, tiles = 0;
+  auto load = [&](int base) {  // this lane's sequence: its blocks, and the tiles of each
+    const int i = base + lane;
+    b = n = len = nb = tiles = 0;
+    if (i < c.nseq) {
+      b = min(max(c.cu[i], 0), p.T);
+      n = min(max(c.cu[i + 1], b), p.T) - b;
+      len = c.len[i];
+      nb = (n * p.G + RB - 1) / RB;
+      tiles = nb ? (int)((min(max((long)len, 0L), cap) + c.prefix_len - p.x_first + KT - 1) / KT) : 0;
+    }
+  };
+  auto max_all = [](int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(v, 63);
+  };
+  uint64_t all = (uint64_t)p.np_blocks * pt * 5 / 4;  // a tile of 128 rows takes about 5/4 of one of 16 (4600 cycles, 3800)
+  int blocks = p.np_blocks, longest = 0;
+  for (int base = 0; base < c.nseq; base += 64) {
+    load(base);
+    const uint64_t x = (uint64_t)nb * (uint32_t)tiles;  // below 2^26 x 2^24: two sums of 26 bits
+    all += (uint32_t)__builtin_amdgcn_readlane(wave_scan_i((int)(x & 0x3ffffff)), 63);
+    if (__any(x >> 26)) all += (uint64_t)(uint32_t)__builtin_amdgcn_readlane(wave_scan_i((int)(x >> 26)), 63) << 26;
+    blocks += __any(nb > 1) ? __builtin_amdgcn_readlane(wave_scan_i(nb), 63) : __popcll(__ballot(nb > 0));
+    longest = max(longest, max_all(tiles));
+  }
+  // every block has one range that is not full: those are taken off what runs at once, where they leave enough; else some
+  // workgroups follow others, and shorter ranges even the ends out
+  const uint32_t places = p.budget - blocks > p.budget / 2 ? p.budget - blocks : p.budget + p.budget / 2;
+  // x / d rounded up, at most 2^24 (more tiles than a range has); below 2^24 the product with the reciprocal is off by one at most
+  auto ceil_of = [](uint64_t x, uint32_t d) {
+    if (x >= 1u << 24) {
+      const uint64_t y = (x + d - 1) / d;
+      return (uint32_t)(y < 1u << 24 ? y : 1u << 24);
+    }
+    const uint32_t n = (uint32_t)x;
+    uint32_t y = (uint32_t)((float)n * __builtin_amdgcn_rcpf((float)d));
+    const int left = (int)(n - y * d);
+    if (left > 0) y += left > (int)d ? 2 : 1;
+    if (left < 0 && left <= -(int)d) y--;
+    return y;
+  };
+  uint32_t chunk = p.s_max == 1 && p.sp_max == 0 ? 1u << 24 : max(ceil_of(all, places), (uint32_t)p.least);
+  chunk = max(chunk, ceil_of(longest, p.s_max));
+  Work w{};
+  w.split = -1;
+  if (p.sp_max) {
+    const uint32_t cp = max((chunk * 4 + 4) / 5, ceil_of(pt, p.sp_max));
+    const int ns = (int)ceil_of(pt, cp);
+    if (q < ns * p.np_blocks) {
+      w.shared = true;
+      w.split = q / p.np_blocks;
+      w.block = q - w.split * p.np_blocks;
+      w.nsplit = ns;
+      w.chunk = (int)cp;
+      return w;
+    }
+    q -= ns * p.np_blocks;
+  }
+  int seen = 0;
+  for (int base = 0; base < c.nseq; base += 64) {
+    if (c.nseq > 64) load(base);
+    const int ns = max((int)ceil_of(tiles, chunk), 1), cnt = nb * ns, inc = wave_scan_i(cnt);
+    const uint64_t hit = __ballot(seen + inc > q);
+    if (!hit) {
+      seen += __builtin_amdgcn_readlane(inc, 63);
+      continue;
+    }
+    const int l = __builtin_ctzll(hit);
+    q -= seen + __builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(cnt, l);
+    w.nsplit = __builtin_amdgcn_readlane(ns, l);
+    const int block = q / w.nsplit;
+    w.split = q - block * w.nsplit;
+    w.chunk = (int)chunk;
+    w.seq = base + l;
+    w.b = __builtin_amdgcn_readlane(b, l);
+    w.n = __builtin_amdgcn_readlane(n, l);
+    w.len = __builtin_amdgcn_readlane(len, l);
+    w.first = block * RB;
+    return w;
+  }
+  return w;
+}
 
 template <typename T, int HD>
 HXA_DEV void any_item(int mode, const Keys<T> &s, const Item &it, const CachedArgs &p, int head0, uint8_t *lds, const Out<T> &out) {
@@ -912,8 +1019,6 @@ HXA_DEV void any_item(int mode, const Keys<T> &s, const Item &it, const CachedAr
     rows_out<T, HD, 4>(out, it, head0, p.cs, lds, acc, m, l);
   }
 }
-HXA_DEV int mode_rows(int mode) { return mode == 1 ? 16 : 32 * mode; }
-
 template <typename T, int HD>
 __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -926,6 +1031,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   s.table = p.c.table;
   s.P = P;
   s.page = p.c.page;
+  s.shift = p.shift;
   s.npages = p.c.npages;
   s.H = p.c.H;
   s.h = h;
@@ -933,38 +1039,46 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   it.G = p.G;
   it.gm = p.gm;
   Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, 0, p.Hq};
-  int mode;
-  if (rest < p.np_blocks * p.np_split) {
-    const int split = rest / p.np_blocks;
-    mode = p.np_mode;
-    it.r0 = (rest % p.np_blocks) * mode_rows(mode);
+  const Work w = find_work(p, rest, lane);
+  if (w.split < 0) return;
+  const int mode = w.shared ? p.np_mode : p.n_mode;
+  int slot_end;
+  if (w.shared) {
+    it.r0 = w.block * mode_rows(mode);
     it.nrows = p.T * p.G;
     it.tok0 = 0;
-    it.x0 = split * p.np_chunk;
-    it.x1 = min(it.x0 + p.np_chunk, P);
+    it.x0 = w.split * w.chunk * KT;
+    it.x1 = min(it.x0 + w.chunk * KT, P);
     it.base = it.cap = it.least = P - 1;
     it.causal = false;
-    out.slot = split;
+    out.slot = w.split;
+    slot_end = p.sp_max;
   } else {
-    const int own = rest - p.np_blocks * p.np_split, split = own / p.n_blocks;
-    mode = p.n_mode;
-    const Block b = find_block(p.c.cu, p.c.nseq, p.T, p.G, mode_rows(mode), own % p.n_blocks, p.first, lane);
-    if (b.first < 0) return;
-    const long len = p.c.len[b.seq];
+    const long len = w.len;
     const int held = (int)min(max(len, 0L), (long)p.c.ldt * p.c.page);
-    s.table += (long)b.seq * p.c.ldt;
-    it.r0 = b.first;
-    it.nrows = b.n * p.G;
-    it.tok0 = b.b;
+    s.table += (long)w.seq * p.c.ldt;
+    it.r0 = w.first;
+    it.nrows = w.n * p.G;
+    it.tok0 = w.b;
     // own position of token j: len - n + j; a negative one sees the prefix alone
     it.causal = true;
     it.cap = P + held - 1;
     it.least = P - 1;
-    const long base = (long)P + len - b.n;
-    it.base = (int)max(min(base, (long)it.cap), (long)P - 1 - b.n);
-    it.x0 = p.x_first + split * p.n_chunk;
-    it.x1 = min(row_limit(it, min(it.r0 + mode_rows(mode), it.nrows) - 1) + 1, it.x0 + p.n_chunk);
-    out.slot = p.np_split + split;
+    const long base = (long)P + len - w.n;
+    it.base = (int)max(min(base, (long)it.cap), (long)P - 1 - w.n);
+    const int end = row_limit(it, min(it.r0 + mode_rows(mode), it.nrows) - 1) + 1;
+    it.x0 = p.x_first + (int)min((long)w.split * w.chunk * KT, 1L << 30);
+    it.x1 = (int)min((long)end, it.x0 + (long)w.chunk * KT);
+    out.slot = p.sp_max + w.split;
+    slot_end = p.sp_max + p.s_max;
+  }
+  if (out.part != nullptr && w.split == w.nsplit - 1) {  // slots that no range fills: sums of nothing
+    const int rows = min(mode_rows(mode), it.nrows - it.r0);
+    for (int k = threadIdx.x; k < rows * (slot_end - out.slot - 1); k += 256) {
+      int head;
+      const int sl = k / rows, tok = row_tok(it, it.r0 + k - sl * rows, head);
+      out.ml[(out.slot + 1 + sl) * out.rows + (long)(it.tok0 + tok) * p.Hq + h * p.G + head] = (float2_t){-INFINITY, 0.0f};
+    }
   }
   any_item<T, HD>(mode, s, it, p, h * p.G, lds, out);
 }
@@ -1088,41 +1202,40 @@ int wg_slots(int hd) { return causal_ncu() * (hd == 256 ? 1 : 2); }
 
 // The launch of a call over the cache, from sizes that the host knows (T, the table's width, the prefix): how the lengths on
 // the device turn out does not change it, so a captured launch stays right.
+//   Rows a workgroup: 16 where a sequence has no more on average, else 64, else 128 (at 65 .. 96 rows one workgroup of 128 takes 0.97 us a
+//   tile, two of 64 take 1.26).
+//   Shared prefix: where sequences bring few rows, there are at least two of them and the prefix is worth four tiles.
+//   Ranges of keys: with few rows as many as run at once. With more rows a partial result is as wide as a row's output is in fp32, so keys are
+//   split only where the blocks fill less than 5/8 of the places (32 prompts of 75 rows behind 1000 tokens, 456 blocks of 512 places: split
+//   in two 65 us, whole 51).
 struct CachedPlan {
-  int np_mode, np_blocks, np_split, np_chunk, n_mode, n_blocks, n_split, n_chunk, x_first;
+  int np_mode, np_blocks, sp_max, n_mode, n_blocks, s_max, x_first, budget, least;
 };
 CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws) {
   const int G = Hq / c.H;
   const long RT = (long)T * G, slots = wg_slots(c.hd), P = c.prefix_len, cap = (long)c.ldt * c.page;
   CachedPlan p{};
   const long per_seq = ceil_div(RT, c.nseq);
-  p.n_mode = per_seq <= 16 ? 1 : per_seq <= 64 || (RT / 128 + c.nseq) * c.H < slots ? 2 : 4;
+  p.n_mode = per_seq <= 16 ? 1 : per_seq <= 64 ? 2 : 4;
   const int rb = p.n_mode == 1 ? 16 : 32 * p.n_mode;
   p.n_blocks = (int)(RT / rb + c.nseq);
-  p.n_split = 1;
-  p.n_chunk = 1 << 30;
+  p.budget = (int)std::max(1L, slots / c.H);
+  p.least = p.n_mode == 1 ? 1 : 4;
+  p.s_max = 1;
   if (!ws) return p;
-  const double target = 1.0;
-  const bool shared = p.n_mode == 1 && c.nseq >= 2 && P >= 4 * KT;
-  if (shared) {  // the prefix once for all
+  if (p.n_mode == 1 && c.nseq >= 2 && P >= 4 * KT) {
     p.np_mode = RT <= 16 ? 1 : RT <= 64 ? 2 : 4;
-    p.np_blocks = (int)ceil_div(RT, p.np_mode == 1 ? 16 : 32 * p.np_mode);
+    p.np_blocks = (int)ceil_div(RT, mode_rows(p.np_mode));
+    p.sp_max = (int)std::min(32L, ceil_div(P, KT));
     p.x_first = (int)P;
   }
-  const long pt = ceil_div(P, KT), ct = ceil_div(cap, KT);
-  // tiles of the launch where the sequences are on average half as long as the table allows
-  const double tiles = (double)c.H * (shared ? (double)p.np_blocks * pt + p.n_blocks * ct * 0.5 : p.n_blocks * (pt + ct * 0.5));
-  const long chunk = std::max(1L, (long)std::ceil(tiles / (target * slots)));
-  auto ranges = [&](long n, int &ns, int &ck) {
-    ns = (int)std::max(1L, ceil_div(n, chunk));
-    ck = (int)(std::max(1L, ceil_div(n, ns)) * KT);
-  };
-  if (shared) ranges(pt, p.np_split, p.np_chunk);
-  ranges(ceil_div((shared ? 0 : P) + cap, KT), p.n_split, p.n_chunk);
+  const long tiles = ceil_div(cap + P - p.x_first, KT), blocks = ceil_div(RT, rb) + c.nseq / 2;
+  if (p.n_mode == 1) p.s_max = (int)std::max(1L, std::min(32L, tiles));
+  else if (blocks * c.H * 8 < slots * 5) p.s_max = (int)std::max(1L, std::min({8L, tiles / p.least, ceil_div(slots, blocks * c.H)}));
   return p;
 }
 long cached_ws(const CachedPlan &p, const hxa_kv_cache &c, int T, int Hq) {
-  const long slots = p.np_split + p.n_split;
+  const long slots = p.sp_max + p.s_max;
   return slots == 1 ? 0 : slots * T * Hq * (c.hd * 4L + 8);
 }
 
@@ -1186,14 +1299,15 @@ extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long l
   CachedPlan pl = cached_plan(*c, T, Hq, true);
   const long need = cached_ws(pl, *c, T, Hq);
   if (need > 0 && (ws == nullptr || ws_bytes < need)) pl = cached_plan(*c, T, Hq, false);
-  const int nslots = pl.np_split + pl.n_split;
-  CachedArgs p{*c, q, o, ldq, ldo, T, Hq / c->H, Hq, recip(Hq / c->H), std::max(1, causal_ncu() / c->H), scale * L2E, pl.np_mode, pl.np_blocks, pl.np_split, pl.np_chunk,
-               pl.n_mode, pl.n_blocks, pl.n_split, pl.n_chunk, pl.x_first, nullptr, nullptr};
+  const int nslots = pl.sp_max + pl.s_max;
+  CachedArgs p{*c, q, o, ldq, ldo, T, Hq / c->H, Hq, recip(Hq / c->H), (c->page & (c->page - 1)) ? -1 : __builtin_ctz(c->page), scale * L2E, pl.np_mode, pl.np_blocks, pl.sp_max,
+               pl.n_mode, pl.s_max, pl.x_first, pl.budget, pl.least, nullptr, nullptr};
   if (nslots > 1) {
     p.part = (float *)ws;
     p.ml = (float2_t *)(p.part + (long)nslots * T * Hq * c->hd);
   }
-  const long wgs = ((long)pl.np_blocks * pl.np_split + (long)pl.n_blocks * pl.n_split) * c->H;
+  // blocks, and as many ranges more as run at once (find_work's chunk is at least all tiles / (3/2 budget))
+  const long wgs = ((long)pl.np_blocks + pl.n_blocks + (nslots > 1 ? pl.budget + pl.budget / 2 : 0)) * c->H;
   const hipStream_t st = (hipStream_t)stream;
   return by_type(c->dtype, c->hd, [&](auto ty, auto hdc, int id) -> int {
     typedef decltype(ty) T_;
