@@ -96,7 +96,7 @@ def test_qk_in_place_without_gains_or_positions(hip, dtype):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("hd,H,new,past,prefix,page", [
     (128, 8, [1] * 70, [0, 5, 15, 16, 17] * 14, 100, 16), (64, 3, [0, 40, 1, 0, 129], [7, 0, 33, 4, 1], 0, 32),
-    (256, 2, [5], [12345], 1000, 1), (128, 1, [64, 64], [0, 1], 3, 64)])
+    (256, 2, [5], [12345], 1000, 1), (128, 1, [64, 64], [0, 1], 3, 64), (64, 1, [1, 0, 2] * 1500, [0, 0, 3] * 1500, 0, 4)])
 def test_kv_append(hip, dtype, hd, H, new, past, prefix, page):
     say("append", dtype, hd, H, len(new), prefix, page)
     rng = np.random.default_rng(hd + len(new))
@@ -240,6 +240,11 @@ CACHED = [  # hd, Hq, H, new, past, prefix, page
     (128, 256, 128, [130, 70], [30, 0], 70, 16),            # 128-row blocks
     (256, 96, 96, [129, 200], [30, 0], 0, 64),
     (64, 140, 140, [300], [100], 20, 16),
+    (128, 2, 1, [40] + [1] * 30, [5] + [40] * 30, 70, 16),  # on average few rows, one sequence with five blocks of them
+    (128, 4, 2, [1], [3000], 0, 16),                        # more tiles than a row has partial results
+    (64, 4, 2, [1, 1, 1], [2500, 0, 70], 2500, 32),         # and a shared prefix of more
+    (128, 8, 8, [1] * 200, [i % 50 for i in range(200)], 0, 8),  # more blocks than run at once
+    (64, 8, 4, [1] * 150, [(i * 37) % 300 for i in range(150)], 280, 16),
 ]
 
 
@@ -314,6 +319,44 @@ def test_cached_lengths_out_of_range(hip):
             got, _ = run_cached(hip, c, q, hd ** -0.5, ws)
             close(got, o, attend_bound(o, a, vmax, n, hd, smax, F16), "lengths")
             assert prefix or (got[:2] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------- far ends of large buffers
+def test_offsets_past_32_bits(hip):
+    """pools of 5 GB with the pages at their end, and key rows 16 MB apart: append, then attention over the cache and over the prompt"""
+    L, rng = hip.lib(), np.random.default_rng(6)
+    Hq, H, hd, page, n = 4, 2, 128, 64, 130
+    npages = 5 * 2 ** 30 // (H * page * hd * 2)
+    kc, vc = hip.DeviceArray((npages * H * page * hd,), np.uint16), hip.DeviceArray((npages * H * page * hd,), np.uint16)
+    pages = np.array([npages - 1, npages - 3, npages - 2], np.int32)
+    ld = 2 ** 23
+    k, v = narrow(rng.standard_normal((n, H * hd)), F16), narrow(rng.standard_normal((n, H * hd)), F16)
+    q = narrow(rng.standard_normal((n, Hq * hd)), F16)
+    big = hip.DeviceArray((n * ld,), np.uint16)  # k and v of a row side by side, 2.2 GB
+    big2 = hip.DeviceArray((300 * ld,), np.uint16)  # 5 GB: rows 170 .. 299
+    for t in range(n):
+        row = np.concatenate([k[t], v[t]])
+        hip.check(L.hxa_h2d(big.at(2 * t * ld), row.ctypes.data, row.nbytes))
+        hip.check(L.hxa_h2d(big2.at(2 * (170 + t) * ld), row.ctypes.data, row.nbytes))
+    dq, do, do2 = dev(hip, q), hip.DeviceArray((n, Hq * hd), np.uint16), hip.DeviceArray((300, Hq * hd), np.uint16)
+    d = [dev(hip, np.array(a, np.int32)) for a in ([0, n], pages, [n], [170, 300])]
+    c = hip.KvCache(F16, H, hd, page, npages, kc.ptr, vc.ptr, None, 0, d[1].ptr, 3, d[2].ptr, d[0].ptr, 1)
+    hip.check(L.hxa_kv_append(C.byref(c), big.ptr, ld, big.at(2 * H * hd), ld, n, None, 0.0, None, None))
+    hip.check(L.hxa_attention_cached(C.byref(c), dq.ptr, Hq * hd, do.ptr, Hq * hd, n, Hq, hd ** -0.5, None, 0, None))
+    q2 = np.zeros((300, Hq * hd), np.uint16)
+    q2[170:] = q
+    dq2 = dev(hip, q2)
+    hip.check(L.hxa_attention_causal(F16, dq2.ptr, Hq * hd, big2.ptr, ld, big2.at(2 * H * hd), ld, do2.ptr, Hq * hd, 300, d[3].ptr, 1, Hq, H, hd,
+                                     hd ** -0.5, None))
+    hip.sync()
+    qq, kk, vv = (widen(x, F16).reshape(n, -1, hd) for x in (q, k, v))
+    o, bound = np.zeros((n, Hq, hd)), np.zeros((n, Hq, hd))
+    for h in range(Hq):
+        o[:, h], a = attend(qq[:, h], kk[:, h // 2], vv[:, h // 2], hd ** -0.5, np.tril(np.ones((n, n), bool)))
+        smax = (np.abs(qq[:, h]) @ np.abs(kk[:, h // 2]).T).max() * hd ** -0.5
+        bound[:, h] = attend_bound(o[:, h], a, np.abs(vv).max(), n, hd, smax, F16)
+    close(widen(do.numpy(), F16).reshape(n, Hq, hd), o, bound, "cached")
+    close(widen(do2.numpy()[170:], F16).reshape(n, Hq, hd), o, bound, "causal")
 
 
 # --------------------------------------------------------------------------------------------------------- as it is used
