@@ -76,8 +76,15 @@ struct Keys {
   long ldk, ldv;    // contiguous: row strides
   const int *prefix, *table;  // paged: the prefix's pages, the sequence's own
   int P, page, npages, H, h;
-  int shift;  // log2(page) where it is a power of two (a division is 40 instructions, twice a tile), -1 otherwise
-  HXA_DEV unsigned slot(unsigned y) const { return shift >= 0 ? y >> shift : y / (unsigned)page; }
+  uint32_t pm;  // 2^32 / page, as Item's gm
+  // place of token y in its table, and in the page
+  HXA_DEV unsigned slot(unsigned y, unsigned &in_page) const {
+    unsigned n = __umulhi(y, pm);
+    in_page = y - n * page;
+    const bool one = in_page >= (unsigned)page;
+    in_page -= one ? page : 0;
+    return n + one;
+  }
 };
 
 // a work item: rows [r0, r0 + rows of the mode) of nrows rows that belong together, keys [x0, x1)
@@ -140,9 +147,11 @@ struct Loader {
   int lane, wave;
   uint32_t koff[G_::NOFF], voff[G_::NOFF];  // contiguous: byte offsets within a whole tile; paged: chunk offsets within a row
   int ent;           // paged: the page entry of this lane's key in the tile that is opened next
+  unsigned in_page;  // and the key's place in that page
   uint32_t krow[PAGED ? G_::NLD : 1], vrow[PAGED ? G_::NLD : 1];  // paged: page rows that this lane's loads of the tile opened last read
   HXA_DEV Loader(const Keys<T> &s_, const Item &it_, uint8_t *lds_, int lane_, int wave_) : s(s_), it(it_), lds(lds_), lane(lane_), wave(wave_) {
     ent = -1;
+    in_page = 0;
 #pragma unroll
     for (int j = 0; j < G_::NOFF; j++) {
       const int r = (j * 4 + wave) * G_::RPL + lane / G_::CH, c = lane % G_::CH;
@@ -161,17 +170,15 @@ struct Loader {
     if (x < it.x1) {
       const bool pre = x < s.P;
       const unsigned y = pre ? x : x - s.P;
-      ent = (pre ? s.prefix : s.table)[s.slot(y)];
+      ent = (pre ? s.prefix : s.table)[s.slot(y, in_page)];
     }
   }
   // tile i: where its keys lie, and the mask of those that are there; its loads follow
   HXA_DEV uint64_t open(int i) {
     const int key0 = it.x0 + i * KT;
     if constexpr (PAGED) {
-      const int x = key0 + lane;
-      const unsigned y = x < s.P ? x : x - s.P;
-      const bool ok = x < it.x1 && (unsigned)ent < (unsigned)s.npages;
-      const uint32_t row = ok ? ((uint32_t)ent * s.H + s.h) * s.page + (y - s.slot(y) * s.page) : 0;  // < 2^32: checked on the host
+      const bool ok = (unsigned)ent < (unsigned)s.npages;  // (-1 past x1)
+      const uint32_t row = ok ? ((uint32_t)ent * s.H + s.h) * s.page + in_page : 0;  // < 2^32: checked on the host
       const uint64_t mask = __ballot(ok);
       if (key0 + KT < it.x1) entry(i + 1);
 #pragma unroll
@@ -225,8 +232,9 @@ struct Loader {
   HXA_DEV void rows(int x, const T *&kr, const T *&vr) const {
     if constexpr (PAGED) {
       const unsigned y = x < s.P ? x : x - s.P;
-      const uint32_t e = (x < s.P ? s.prefix : s.table)[s.slot(y)];
-      const uint64_t r = (uint64_t)((e * s.H + s.h) * s.page + (y - s.slot(y) * s.page)) * HD;
+      unsigned in;
+      const uint32_t e = (x < s.P ? s.prefix : s.table)[s.slot(y, in)];
+      const uint64_t r = (uint64_t)((e * s.H + s.h) * s.page + in) * HD;
       kr = s.k + r;
       vr = s.v + r;
     } else {
@@ -890,8 +898,7 @@ struct CachedArgs {
   void *o;
   long ldq, ldo;
   int T, G, Hq;
-  uint32_t gm;
-  int shift;
+  uint32_t gm, pm;
   float cs;
   int np_mode, np_blocks, sp_max;  // sp_max 0: nothing is shared
   int n_mode, s_max;               // modes: 1 few rows (16), 2 rows (64), 4 rows (128)
@@ -1031,7 +1038,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   s.table = p.c.table;
   s.P = P;
   s.page = p.c.page;
-  s.shift = p.shift;
+  s.pm = p.pm;
   s.npages = p.c.npages;
   s.H = p.c.H;
   s.h = h;
@@ -1300,7 +1307,7 @@ extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long l
   const long need = cached_ws(pl, *c, T, Hq);
   if (need > 0 && (ws == nullptr || ws_bytes < need)) pl = cached_plan(*c, T, Hq, false);
   const int nslots = pl.sp_max + pl.s_max;
-  CachedArgs p{*c, q, o, ldq, ldo, T, Hq / c->H, Hq, recip(Hq / c->H), (c->page & (c->page - 1)) ? -1 : __builtin_ctz(c->page), scale * L2E, pl.np_mode, pl.np_blocks, pl.sp_max,
+  CachedArgs p{*c, q, o, ldq, ldo, T, Hq / c->H, Hq, recip(Hq / c->H), recip(c->page), scale * L2E, pl.np_mode, pl.np_blocks, pl.sp_max,
                pl.n_mode, pl.s_max, pl.x_first, pl.budget, pl.least, nullptr, nullptr};
   if (nslots > 1) {
     p.part = (float *)ws;
