@@ -528,7 +528,7 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
 }
 
 // what an item leaves: rows of o, or (part != nullptr) fp32 partials of slot `slot`: part[slot][row][hd] unscaled and
-// ml[slot][row] = (maximum in powers of two, sum), row = token Hq + head
+// ml[row][slot] = (maximum in powers of two, sum), row = token Hq + head
 template <typename T>
 struct Out {
   T *o;
@@ -536,7 +536,7 @@ struct Out {
   float *part;
   float2_t *ml;
   long rows;  // T Hq
-  int slot, Hq;
+  int slot, nslots, Hq;
 };
 
 // rows mode: the wave's accumulators to their rows
@@ -553,10 +553,10 @@ HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uin
     if (second || R >= it.nrows) return;
     int rest;
     const int tok = row_tok(it, R, rest);
-    const long at = (long)out.slot * out.rows + (long)(it.tok0 + tok) * out.Hq + head0 + rest;
-    if (g == 0) out.ml[at] = (float2_t){m == -INFINITY ? m : m * c, l};
+    const long row = (long)(it.tok0 + tok) * out.Hq + head0 + rest;
+    if (g == 0) out.ml[row * out.nslots + out.slot] = (float2_t){m == -INFINITY ? m : m * c, l};
     if (l == 0.0f) return;  // (l is NaN where a score is: written)
-    float *p = out.part + at * HD;
+    float *p = out.part + (out.slot * out.rows + row) * HD;
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
 #pragma unroll
@@ -739,9 +739,9 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
   int rest;
   const long tok = it.tok0 + row_tok(it, R, rest);
   const int head = head0 + rest;
-  const long at = (long)out.slot * out.rows + tok * out.Hq + head;
+  const long row = tok * out.Hq + head, at = out.slot * out.rows + row;
   if (out.part != nullptr) {
-    if (wave == 0 && gi == 0) out.ml[at] = (float2_t){m == -INFINITY ? m : m * c, l};
+    if (wave == 0 && gi == 0) out.ml[row * out.nslots + out.slot] = (float2_t){m == -INFINITY ? m : m * c, l};
     if (l == 0.0f) return;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -881,7 +881,7 @@ __global__ HXA_CAUSAL_BOUNDS void causal_kernel(CausalArgs p) {
   float16_t acc[HD / 32];
   float m, l;
   rows_item<T, HD, W, false>(s, it, (const T *)p.q, p.ldq, h * p.G, p.c, lds, acc, m, l);
-  const Out<T> out{(T *)p.o, p.ldo, nullptr, nullptr, 0, 0, 0};
+  const Out<T> out{(T *)p.o, p.ldo, nullptr, nullptr, 0, 0, 0, 0};
   rows_out<T, HD, W>(out, it, h * p.G, p.c, lds, acc, m, l);
 }
 
@@ -1045,7 +1045,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   Item it;
   it.G = p.G;
   it.gm = p.gm;
-  Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, 0, p.Hq};
+  Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, 0, p.sp_max + p.s_max, p.Hq};
   const Work w = find_work(p, rest, lane);
   if (w.split < 0) return;
   const int mode = w.shared ? p.np_mode : p.n_mode;
@@ -1081,84 +1081,62 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   }
   if (out.part != nullptr && w.split == w.nsplit - 1) {  // slots that no range fills: sums of nothing
     const int rows = min(mode_rows(mode), it.nrows - it.r0);
-    for (int k = threadIdx.x; k < rows * (slot_end - out.slot - 1); k += 256) {
+    const int free = slot_end - out.slot - 1;
+    for (int k = threadIdx.x; k < rows * free; k += 256) {
       int head;
-      const int sl = k / rows, tok = row_tok(it, it.r0 + k - sl * rows, head);
-      out.ml[(out.slot + 1 + sl) * out.rows + (long)(it.tok0 + tok) * p.Hq + h * p.G + head] = (float2_t){-INFINITY, 0.0f};
+      const int row = k / free, tok = row_tok(it, it.r0 + row, head);
+      out.ml[((long)(it.tok0 + tok) * p.Hq + h * p.G + head) * out.nslots + out.slot + 1 + k - row * free] = (float2_t){-INFINITY, 0.0f};
     }
   }
   any_item<T, HD>(mode, s, it, p, h * p.G, lds, out);
 }
 
-// The partials of a row joined: weights 2^(m_s - m) against the common maximum, then one division and one rounding. HD / 4 lanes
-// hold a row; sg of them side by side share its slots (nslots is up to some hundred where few rows read a long cache), each
-// with 8 slots' sums in flight, then 8 slots' values. A slot whose sum is 0 saw no key and holds no values.
+// The partials of a row joined by a wave: lane s has the maximum and the sum of slot s (at most 64 of them), which give its weight
+// 2^(m_s - m); then HD / 64 dims a lane over the slots that saw a key, eight of them in flight; one division, one rounding. A slot whose
+// sum is 0 saw none and holds no values. (64 tokens of 32 heads with 32 + 24 slots, a third of them used: 5 us; with the slots'
+// sums strided by rows and shared by 8 groups of lanes 8.8.)
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs p, int nslots, int sg) {
-  typedef typename HxaVec<T>::v4 v4;
-  constexpr int LPR = HD / 4, N = 8;
-  __shared__ float4_t so[256];
-  __shared__ float2_t sml[256];
-  const int tid = threadIdx.x, u = tid % LPR, grp = tid / LPR % sg, rpw = 256 / LPR / sg;
-  const long row = (long)blockIdx.x * rpw + tid / LPR / sg, rows = (long)p.T * p.Hq;
-  const int tok = (int)min(row / p.Hq, (long)p.T - 1), head = (int)(row - row / p.Hq * p.Hq);
-  const bool mine = row < rows && tok >= p.c.cu[0] && tok < p.c.cu[p.c.nseq];
-  float m = -INFINITY, l = 0.0f;
-  float4_t o = {};
-  if (mine)
-    for (int s0 = grp; s0 < nslots; s0 += N * sg) {
-      float2_t x[N];
+__global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs p) {
+  constexpr int E = HD / 64, N = 8;
+  typedef float fe __attribute__((ext_vector_type(E)));
+  const int lane = threadIdx.x & 63, nslots = p.sp_max + p.s_max;
+  const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), rows = (uint32_t)p.T * p.Hq;
+  if (row >= rows) return;
+  const int tok = (int)(row / (uint32_t)p.Hq), head = (int)(row - (uint32_t)tok * p.Hq);
+  if (tok < p.c.cu[0] || tok >= p.c.cu[p.c.nseq]) return;
+  const float2_t x = lane < nslots ? p.ml[(long)row * nslots + lane] : (float2_t){-INFINITY, 0.0f};
+  float m = x[0];
 #pragma unroll
-      for (int j = 0; j < N; j++) {
-        const int s = s0 + j * sg;
-        x[j] = s < nslots ? p.ml[s * rows + row] : (float2_t){-INFINITY, 0.0f};
-      }
-      float4_t y[N];
+  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  const float w = x[1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x[0] - (m == -INFINITY ? 0.0f : m));
+  const float l = wave_sum(x[1] * w);
+  uint64_t left = __ballot(x[1] != 0.0f);
+  fe o = {};
+  while (left) {
+    fe y[N];
+    float a[N];
 #pragma unroll
-      for (int j = 0; j < N; j++)
-        y[j] = x[j][1] != 0.0f ? *(const float4_t *)(p.part + ((s0 + j * sg) * rows + row) * HD + 4 * u) : (float4_t){};
-      float mt = m;
-#pragma unroll
-      for (int j = 0; j < N; j++) mt = fmaxf(mt, x[j][0]);
-      const float mz = mt == -INFINITY ? 0.0f : mt, b = __builtin_amdgcn_exp2f(m - mz);
-      m = mt;
-      l *= b;
-#pragma unroll
-      for (int e = 0; e < 4; e++) o[e] *= b;
-#pragma unroll
-      for (int j = 0; j < N; j++) {
-        const float a = x[j][1] != 0.0f ? __builtin_amdgcn_exp2f(x[j][0] - mz) : 0.0f;
-        l += x[j][1] * a;
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[e] += y[j][e] * a;
+    for (int j = 0; j < N; j++) {
+      y[j] = (fe){};
+      a[j] = 0.0f;
+      if (left) {
+        const int s = __builtin_ctzll(left);
+        left &= left - 1;
+        y[j] = *(const fe *)(p.part + ((long)s * rows + row) * HD + E * lane);
+        a[j] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s));
       }
     }
-  if (sg > 1) {
-    so[tid] = o;
-    sml[tid] = (float2_t){m, l};
-    __syncthreads();
-    if (grp != 0) return;
-    float mt = m;
-    for (int k = 1; k < sg; k++) mt = fmaxf(mt, sml[tid + k * LPR][0]);
-    const float mz = mt == -INFINITY ? 0.0f : mt, b = __builtin_amdgcn_exp2f(m - mz);
-    l *= b;
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] *= b;
-    for (int k = 1; k < sg; k++) {
-      const float2_t x = sml[tid + k * LPR];
-      const float4_t y = so[tid + k * LPR];
-      const float a = __builtin_amdgcn_exp2f(x[0] - mz);
-      l += x[1] * a;
+    for (int j = 0; j < N; j++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[e] += y[e] * a;
-    }
+      for (int e = 0; e < E; e++) o[e] += y[j][e] * a[j];
   }
-  if (!mine) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  v4 x;
+  typedef T te __attribute__((ext_vector_type(E)));
+  te z;
 #pragma unroll
-  for (int e = 0; e < 4; e++) x[e] = (T)(o[e] * inv);
-  *(v4 *)((T *)p.o + tok * p.ldo + (long)head * HD + 4 * u) = x;
+  for (int e = 0; e < E; e++) z[e] = (T)(o[e] * inv);
+  *(te *)((T *)p.o + tok * p.ldo + (long)head * HD + E * lane) = z;
 }
 
 int causal_ncu() {
@@ -1323,11 +1301,7 @@ extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long l
     const int a = allow_lds((const void *)f, Geo<T_, HD>::LDS, 18 + id);
     if (a != HXA_OK) return hxa_set_error(a, "attention_cached: %d bytes of LDS", Geo<T_, HD>::LDS);
     hxa_launch(f, dim3((unsigned)wgs), dim3(256), Geo<T_, HD>::LDS, st, p);
-    if (nslots > 1) {
-      int sg = 1;
-      while (sg * 4 < nslots && sg < 1024 / HD) sg *= 2;
-      hxa_launch(cached_merge_kernel<T_, HD>, dim3((unsigned)ceil_div((long)T * Hq, 1024 / HD / sg)), dim3(256), 0, st, p, nslots, sg);
-    }
+    if (nslots > 1) hxa_launch(cached_merge_kernel<T_, HD>, dim3((unsigned)ceil_div((long)T * Hq, 4)), dim3(256), 0, st, p);
     return launched("attention_cached");
   });
 }
