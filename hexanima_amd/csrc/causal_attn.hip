@@ -627,8 +627,8 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
     uint64_t km_next = ld.open(0);
     ld.load_all(0);
     int rest;
-  const int tok = row_tok(it, Rc, rest);
-  const T *qp = q + (long)(it.tok0 + tok) * ldq + (long)(head0 + rest) * HD;
+    const int tok = row_tok(it, Rc, rest);
+    const T *qp = q + (long)(it.tok0 + tok) * ldq + (long)(head0 + rest) * HD;
     v8 qf[HD / 32];
 #pragma unroll
     for (int i = 0; i < HD / 32; i++) qf[i] = *(const v8 *)(qp + i * 32 + 8 * gi);
@@ -889,7 +889,8 @@ __global__ HXA_CAUSAL_BOUNDS void causal_kernel(CausalArgs p) {
 // The keys of a sequence are one list: the prefix (P keys), then its own. The items of a key head, in grid order:
 //   shared: np_blocks blocks of all T G rows x ranges of the prefix, without a mask (rows of unused tokens are computed and
 //           never read); partial slots [0, sp_max)
-//   own:    the blocks of the sequences' rows x ranges of their keys [x_first, P + own), slots from sp_max on
+//   own:    the blocks of rb of the sequences' rows, the last one in the mode that its rows need, x ranges of their keys
+//           [x_first, P + own), slots from sp_max on
 // How long the ranges are follows from the lengths as they are on the device: every workgroup adds the tiles of the whole launch up and
 // cuts them into as many items as run at once, so one long sequence among short ones does not decide the time.
 struct CachedArgs {
@@ -901,14 +902,16 @@ struct CachedArgs {
   uint32_t gm, pm;
   float cs;
   int np_mode, np_blocks, sp_max;  // sp_max 0: nothing is shared
-  int n_mode, s_max;               // modes: 1 few rows (16), 2 rows (64), 4 rows (128)
+  int rb_log, s_max;  // rows a block of a sequence: 64 or 128
   int x_first;    // 0: own items take the prefix too
   int budget;     // items a key head that run at once
   int least;      // tiles an item is worth
   float *part;    // nullptr: straight to o (sp_max = 0, s_max = 1)
   float2_t *ml;
 };
+// modes: 1 few rows (16), 2 rows (64), 4 rows (128); the one for `rows` rows that belong together, or for the first of more than 128
 __host__ HXA_DEV int mode_rows(int mode) { return mode == 1 ? 16 : 32 * mode; }
+__host__ HXA_DEV int rows_mode(long rows) { return rows <= 16 ? 1 : rows <= 64 ? 2 : 4; }
 
 // what item `q` of a key head is; split < 0: there is none
 struct Work {
@@ -919,7 +922,7 @@ struct Work {
 };
 HXA_DEV Work find_work(const CachedArgs &p, int q, int lane) {
   const hxa_kv_cache &c = p.c;
-  const int RB = mode_rows(p.n_mode), pt = p.sp_max ? (c.prefix_len + KT - 1) / KT : 0;
+  const int rb = 1 << p.rb_log, pt = p.sp_max ? (c.prefix_len + KT - 1) / KT : 0;
   const long cap = (long)c.ldt * c.page;
   int b = 0, n = 0, len = 0, nb = 0, tiles = 0;
   auto load = [&](int base) {  // this lane's sequence: its blocks, and the tiles of each
@@ -929,7 +932,7 @@ HXA_DEV Work find_work(const CachedArgs &p, int q, int lane) {
       b = min(max(c.cu[i], 0), p.T);
       n = min(max(c.cu[i + 1], b), p.T) - b;
       len = c.len[i];
-      nb = (n * p.G + RB - 1) / RB;
+      nb = (n * p.G + rb - 1) >> p.rb_log;
       tiles = nb ? (int)((min(max((long)len, 0L), cap) + c.prefix_len - p.x_first + KT - 1) / KT) : 0;
     }
   };
@@ -944,13 +947,15 @@ HXA_DEV Work find_work(const CachedArgs &p, int q, int lane) {
   };
   uint64_t all = (uint64_t)p.np_blocks * pt * 5 / 4;  // a tile of 128 rows takes about 5/4 of one of 16 (4600 cycles, 3800)
   int blocks = p.np_blocks, longest = 0;
+  bool whole = false;  // up to 64 sequences, and one has a whole block
   for (int base = 0; base < c.nseq; base += 64) {
     load(base);
-    const uint64_t x = (uint64_t)nb * (uint32_t)tiles;  // below 2^26 x 2^24: two sums of 26 bits
+    const uint64_t x = (uint64_t)nb * (uint32_t)tiles;  // below 2^24 x 2^24: two sums of 26 bits
     all += (uint32_t)__builtin_amdgcn_readlane(wave_scan_i((int)(x & 0x3ffffff)), 63);
     if (__any(x >> 26)) all += (uint64_t)(uint32_t)__builtin_amdgcn_readlane(wave_scan_i((int)(x >> 26)), 63) << 26;
     blocks += __any(nb > 1) ? __builtin_amdgcn_readlane(wave_scan_i(nb), 63) : __popcll(__ballot(nb > 0));
     longest = max(longest, max_all(tiles));
+    whole |= c.nseq <= 64 && __any(n * p.G >= rb);
   }
   // every block has one range that is not full: those are taken off what runs at once, where they leave enough; else some
   // workgroups follow others, and shorter ranges even the ends out
@@ -985,27 +990,33 @@ HXA_DEV Work find_work(const CachedArgs &p, int q, int lane) {
     }
     q -= ns * p.np_blocks;
   }
+  // the whole blocks of all sequences, then what is left of each: the short items even the end of the launch out (32 prompts of 300 rows
+  // behind 1000 keys, 768 blocks on 512 places: 66 -> 61 us). More than 64 sequences keep their order: a second pass over their
+  // lengths costs each of 201 x 8 items more (109 -> 118 us).
   int seen = 0;
-  for (int base = 0; base < c.nseq; base += 64) {
-    if (c.nseq > 64) load(base);
-    const int ns = max((int)ceil_of(tiles, chunk), 1), cnt = nb * ns, inc = wave_scan_i(cnt);
-    const uint64_t hit = __ballot(seen + inc > q);
-    if (!hit) {
-      seen += __builtin_amdgcn_readlane(inc, 63);
-      continue;
+  for (int rest = whole ? 0 : 1; rest < 2; rest++) {
+    for (int base = 0; base < c.nseq; base += 64) {
+      if (c.nseq > 64) load(base);
+      const int ns = max((int)ceil_of(tiles, chunk), 1), full = whole ? nb - ((n * p.G & (rb - 1)) != 0) : 0;
+      const int cnt = (rest ? nb - full : full) * ns, inc = wave_scan_i(cnt);
+      const uint64_t hit = __ballot(seen + inc > q);
+      if (!hit) {
+        seen += __builtin_amdgcn_readlane(inc, 63);
+        continue;
+      }
+      const int l = __builtin_ctzll(hit);
+      q -= seen + __builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(cnt, l);
+      w.nsplit = __builtin_amdgcn_readlane(ns, l);
+      const int block = q / w.nsplit;
+      w.split = q - block * w.nsplit;
+      w.chunk = (int)chunk;
+      w.seq = base + l;
+      w.b = __builtin_amdgcn_readlane(b, l);
+      w.n = __builtin_amdgcn_readlane(n, l);
+      w.len = __builtin_amdgcn_readlane(len, l);
+      w.first = (block + (rest ? __builtin_amdgcn_readlane(full, l) : 0)) << p.rb_log;
+      return w;
     }
-    const int l = __builtin_ctzll(hit);
-    q -= seen + __builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(cnt, l);
-    w.nsplit = __builtin_amdgcn_readlane(ns, l);
-    const int block = q / w.nsplit;
-    w.split = q - block * w.nsplit;
-    w.chunk = (int)chunk;
-    w.seq = base + l;
-    w.b = __builtin_amdgcn_readlane(b, l);
-    w.n = __builtin_amdgcn_readlane(n, l);
-    w.len = __builtin_amdgcn_readlane(len, l);
-    w.first = block * RB;
-    return w;
   }
   return w;
 }
@@ -1048,9 +1059,9 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, 0, p.sp_max + p.s_max, p.Hq};
   const Work w = find_work(p, rest, lane);
   if (w.split < 0) return;
-  const int mode = w.shared ? p.np_mode : p.n_mode;
-  int slot_end;
+  int mode, slot_end;
   if (w.shared) {
+    mode = p.np_mode;
     it.r0 = w.block * mode_rows(mode);
     it.nrows = p.T * p.G;
     it.tok0 = 0;
@@ -1066,6 +1077,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
     s.table += (long)w.seq * p.c.ldt;
     it.r0 = w.first;
     it.nrows = w.n * p.G;
+    mode = rows_mode(min(it.nrows - it.r0, 1 << p.rb_log));
     it.tok0 = w.b;
     // own position of token j: len - n + j; a negative one sees the prefix alone
     it.causal = true;
@@ -1187,41 +1199,43 @@ int wg_slots(int hd) { return causal_ncu() * (hd == 256 ? 1 : 2); }
 
 // The launch of a call over the cache, from sizes that the host knows (T, the table's width, the prefix): how the lengths on
 // the device turn out does not change it, so a captured launch stays right.
-//   Rows a workgroup: 16 where a sequence has no more on average, else 64, else 128 (at 65 .. 96 rows one workgroup of 128 takes 0.97 us a
-//   tile, two of 64 take 1.26).
-//   Shared prefix: where sequences bring few rows, there are at least two of them and the prefix is worth four tiles.
-//   Ranges of keys: with few rows as many as run at once. With more rows a partial result is as wide as a row's output is in fp32, so keys are
+//   Rows a workgroup: 64 where the average sequence has no more, else 128 (at 65 .. 96 rows one workgroup of 128 takes 0.97 us a
+//   tile, two of 64 take 1.26); for what is left of a sequence 16 or 64 where that is enough, which is found on the device (a prompt of 1000
+//   tokens and 63 single ones over 800 each behind 500, 32 / 8 heads: 89 -> 60 us against 128 rows for all).
+//   Shared prefix: where sequences bring at most 16 rows, there are at least two of them and the prefix is worth four tiles. No more
+//   slots than ranges find_work's chunk can make.
+//   Ranges of keys: with few rows as many as run at once, but none that would bring the partials past 1 GB. With more rows a partial result is as wide as a row's output is in fp32, so keys are
 //   split only where the blocks fill less than 5/8 of the places (32 prompts of 75 rows behind 1000 tokens, 456 blocks of 512 places: split
 //   in two 65 us, whole 51).
 struct CachedPlan {
-  int np_mode, np_blocks, sp_max, n_mode, n_blocks, s_max, x_first, budget, least;
+  int np_mode, np_blocks, sp_max, rb_log, n_blocks, s_max, x_first, budget, least;
 };
+long cached_ws(const CachedPlan &p, const hxa_kv_cache &c, int T, int Hq) {
+  const long slots = p.sp_max + p.s_max;
+  return slots == 1 ? 0 : slots * T * Hq * (c.hd * 4L + 8);
+}
 CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws) {
   const int G = Hq / c.H;
   const long RT = (long)T * G, slots = wg_slots(c.hd), P = c.prefix_len, cap = (long)c.ldt * c.page;
   CachedPlan p{};
-  const long per_seq = ceil_div(RT, c.nseq);
-  p.n_mode = per_seq <= 16 ? 1 : per_seq <= 64 ? 2 : 4;
-  const int rb = p.n_mode == 1 ? 16 : 32 * p.n_mode;
-  p.n_blocks = (int)(RT / rb + c.nseq);
+  const int mode = rows_mode(ceil_div(RT, c.nseq));
+  p.rb_log = mode == 4 ? 7 : 6;
+  p.n_blocks = (int)((RT >> p.rb_log) + c.nseq);
   p.budget = (int)std::max(1L, slots / c.H);
-  p.least = p.n_mode == 1 ? 1 : 4;
+  p.least = mode == 1 ? 1 : 4;
   p.s_max = 1;
   if (!ws) return p;
-  if (p.n_mode == 1 && c.nseq >= 2 && P >= 4 * KT) {
-    p.np_mode = RT <= 16 ? 1 : RT <= 64 ? 2 : 4;
+  if (mode == 1 && c.nseq >= 2 && P >= 4 * KT) {
+    p.np_mode = rows_mode(RT);
     p.np_blocks = (int)ceil_div(RT, mode_rows(p.np_mode));
-    p.sp_max = (int)std::min(32L, ceil_div(P, KT));
+    p.sp_max = (int)std::min({32L, ceil_div(P, KT), ceil_div(p.budget + p.budget / 2, p.np_blocks) + 1});
     p.x_first = (int)P;
   }
-  const long tiles = ceil_div(cap + P - p.x_first, KT), blocks = ceil_div(RT, rb) + c.nseq / 2;
-  if (p.n_mode == 1) p.s_max = (int)std::max(1L, std::min(32L, tiles));
+  const long tiles = ceil_div(cap + P - p.x_first, KT), blocks = ceil_div(RT, mode_rows(mode)) + c.nseq / 2;
+  if (mode == 1) p.s_max = (int)std::max(1L, std::min(32L, tiles));
   else if (blocks * c.H * 8 < slots * 5) p.s_max = (int)std::max(1L, std::min({8L, tiles / p.least, ceil_div(slots, blocks * c.H)}));
+  while (p.s_max > 1 && cached_ws(p, c, T, Hq) > 1L << 30) p.s_max /= 2;
   return p;
-}
-long cached_ws(const CachedPlan &p, const hxa_kv_cache &c, int T, int Hq) {
-  const long slots = p.sp_max + p.s_max;
-  return slots == 1 ? 0 : slots * T * Hq * (c.hd * 4L + 8);
 }
 
 }  // namespace
@@ -1262,7 +1276,9 @@ static int cached_check(const hxa_kv_cache *c, int T, int Hq) {
   if (r != HXA_OK) return r;
   if (Hq <= 0 || Hq > HXA_MAX_HEADS || Hq % c->H || (long)T * Hq >= 1L << 30)
     return hxa_set_error(HXA_E_ARG, "attention_cached: T=%d Hq=%d H=%d", T, Hq, c->H);
-  if (((long)T * Hq / c->H / 16 + c->nseq) * c->H >= 1L << 20)
+  // grids of fewer than 2^24 workgroups; the join's waves, one for each of T Hq rows, are fewer than 2^26 where there is one
+  const long RT = (long)T * (Hq / c->H);
+  if ((RT / 64 + c->nseq) * c->H >= 1L << 21)
     return hxa_set_error(HXA_E_ARG, "attention_cached: T=%d nseq=%d H=%d are too many blocks", T, c->nseq, c->H);
   return HXA_OK;
 }
@@ -1286,7 +1302,7 @@ extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long l
   if (need > 0 && (ws == nullptr || ws_bytes < need)) pl = cached_plan(*c, T, Hq, false);
   const int nslots = pl.sp_max + pl.s_max;
   CachedArgs p{*c, q, o, ldq, ldo, T, Hq / c->H, Hq, recip(Hq / c->H), recip(c->page), scale * L2E, pl.np_mode, pl.np_blocks, pl.sp_max,
-               pl.n_mode, pl.s_max, pl.x_first, pl.budget, pl.least, nullptr, nullptr};
+               pl.rb_log, pl.s_max, pl.x_first, pl.budget, pl.least, nullptr, nullptr};
   if (nslots > 1) {
     p.part = (float *)ws;
     p.ml = (float2_t *)(p.part + (long)nslots * T * Hq * c->hd);

@@ -148,6 +148,25 @@ def test_workspace_follows_the_sizes(hip):
     assert size(100000, 4, nseq=8) == 0
 
 
+def test_workspace_stays_bounded(hip):
+    """many rows: fewer partial results a row instead of more memory, down to one for the prefix's first ranges and one for the own keys"""
+    L = hip.lib()
+    row = lambda Hq: Hq * (128 * 4 + 8)
+    for n in (64, 1000, 5000, 40000, 200000):
+        for P in (0, 4096):
+            nb = L.hxa_attention_cached_ws_bytes(C.byref(plan(hip, nseq=n, prefix_len=P, ldt=500)), n, 8)
+            assert nb % (n * row(8)) == 0 and nb <= max(2 ** 30, 4 * n * row(8)), (n, P, nb)
+            assert n > 64 or nb > 0
+    assert cached_call(hip, 2 ** 18) == 0 and cached_call(hip, 2 ** 20) == -12  # 2^15 (2^17) blocks of 64 rows for each of 32 heads
+
+
+def cached_call(hip, T):
+    """the error of a call over the cache with T tokens of 256 heads, refused for its pointers where the size is not"""
+    L, c = hip.lib(), plan(hip, H=32)
+    rc = L.hxa_attention_cached(C.byref(c), None, 2 ** 15, FAKE, 2 ** 15, T, 256, 0.1, None, 0, None)
+    return 0 if "pointers" in hip.last_error() else rc
+
+
 def test_the_tests_own_definitions():
     """attend and norm_rope against sums written out; narrow and widen against numpy's and a known bf16 rounding"""
     rng = np.random.default_rng(0)

@@ -321,6 +321,86 @@ def test_cached_lengths_out_of_range(hip):
             assert prefix or (got[:2] == 0).all()
 
 
+MIXED = [  # hd, Hq, H, new, past, prefix, page: prompts beside single tokens, whole blocks of rows and rests of every kind
+    (128, 8, 2, [130, 1, 64, 1, 0, 33, 1, 4, 5], [20, 300, 0, 64, 10, 100, 0, 7, 9], 70, 16),   # 128-row blocks; rests of 8, 4, 16, 20 rows
+    (64, 4, 1, [150] + [1] * 70 + [17, 33], [0] + [30] * 70 + [5, 0], 300, 32),                # 64-row blocks, more than 64 sequences
+    (128, 64, 64, [80, 1, 64, 16, 128, 17], [3, 90, 0, 200, 64, 1], 0, 16),                    # one row a token and head
+    (256, 4, 2, [70, 1, 1, 8, 9], [40, 500, 0, 1, 63], 130, 64),
+]
+
+
+@pytest.mark.parametrize("with_ws", [True, False])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix,page", MIXED)
+def test_cached_prompts_beside_single_tokens(hip, dtype, hd, Hq, H, new, past, prefix, page, with_ws):
+    say("mixed", dtype, hd, Hq, H, with_ws)
+    rng = np.random.default_rng(hd + Hq)
+    c = Cache(hip, rng, new, past, prefix, page, H, hd, dtype)
+    q = queries(rng, int(c.cu[-1]), Hq, hd, dtype)
+    got, _ = run_cached(hip, c, q, hd ** -0.5, with_ws)
+    o, a, n, smax, vmax = c.expect(q, hd ** -0.5)
+    close(got, o, attend_bound(o, a, vmax, n, hd, smax, dtype), "mixed")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix", [(128, 8, 4, [1] * 7, [900, 0, 64, 300, 1, 20, 500], 400), (64, 4, 2, [60, 3], [200, 700], 100)])
+def test_cached_steep_scores(hip, dtype, hd, Hq, H, new, past, prefix):
+    """scores of tens to hundreds: the maximum moves from range to range, and most partial results weigh nothing"""
+    rng = np.random.default_rng(31)
+    c = Cache(hip, rng, new, past, prefix, 16, H, hd, dtype)
+    q = queries(rng, int(c.cu[-1]), Hq, hd, dtype, std=8.0)
+    o, a, n, smax, vmax = c.expect(q, 1.0)
+    close(run_cached(hip, c, q, 1.0)[0], o, attend_bound(o, a, vmax, n, hd, smax, dtype), "steep")
+
+
+def test_cached_prefix_alone(hip):
+    """a table without entries: every query sees the prefix, and without a prefix nothing"""
+    rng = np.random.default_rng(14)
+    hd, Hq, H = 128, 4, 2
+    for prefix, new in ((300, [1, 1, 2]), (40, [50, 30]), (0, [1, 3])):
+        c = Cache(hip, rng, new, [0] * len(new), prefix, 16, H, hd, F16)
+        q = queries(rng, int(c.cu[-1]), Hq, hd, F16)
+        c.ldt, c.table = 0, np.zeros((len(new), 0), np.int32)
+        none = Cache.__new__(Cache)
+        none.__dict__.update(c.__dict__)
+        none.lens, none.past = [0] * len(new), [10 ** 6] * len(new)
+        o, a, n, smax, vmax = none.expect(q, hd ** -0.5)
+        for ws in (True, False):
+            got, _ = run_cached(hip, c, q, hd ** -0.5, ws)
+            close(got, o, attend_bound(o, a, vmax, n, hd, smax, F16), "prefix alone")
+            assert prefix or (got == 0).all()
+
+
+def test_two_streams_at_once(hip):
+    """calls in flight on two streams, each with its own workspace and output, give what they give alone, bit for bit"""
+    rng = np.random.default_rng(77)
+    L, hd, Hq, H = hip.lib(), 128, 8, 2
+    jobs = []
+    for new, past, prefix in (([1] * 20, [400] * 20, 600), ([1] * 3, [3000, 20, 900], 256)):
+        c = Cache(hip, rng, new, past, prefix, 16, H, hd, BF16)
+        q = queries(rng, len(new), Hq, hd, BF16)
+        st = C.c_void_p()
+        hip.check(L.hxa_stream_create(C.byref(st)))
+        plan = c.upload()
+        nb = L.hxa_attention_cached_ws_bytes(C.byref(plan), len(new), Hq)
+        jobs.append((c, plan, dev(hip, narrow(q, BF16)), dev(hip, np.zeros((len(new), Hq * hd), np.uint16)), hip.DeviceArray((nb,), np.uint8), nb, st,
+                     len(new)))
+    go = lambda j, st: hip.check(L.hxa_attention_cached(C.byref(j[1]), j[2].ptr, Hq * hd, j[3].ptr, Hq * hd, j[7], Hq, hd ** -0.5, j[4].ptr, j[5], st))
+    alone = []
+    for j in jobs:
+        go(j, None)
+        hip.sync()
+        alone.append(j[3].numpy().copy())
+        j[3].upload(np.zeros_like(alone[-1]))
+    for _ in range(10):
+        for j in jobs:
+            go(j, j[6])
+    hip.sync()
+    for j, want in zip(jobs, alone):
+        assert np.array_equal(j[3].numpy(), want) and (want != 0).any()
+        hip.check(L.hxa_stream_destroy(j[6]))
+
+
 # ------------------------------------------------------------------------------------------------- far ends of large buffers
 def test_offsets_past_32_bits(hip):
     """pools of 5 GB with the pages at their end, and key rows 16 MB apart: append, then attention over the cache and over the prompt"""
