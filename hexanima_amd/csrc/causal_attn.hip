@@ -69,6 +69,13 @@ HXA_DEV float add16(float v) {
   return lo + hi;
 }
 
+// the thread, opaque: what follows from it is computed again for each item, not kept in registers across them
+HXA_DEV int this_thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // where the keys of a work item lie
 template <typename T>
 struct Keys {
@@ -125,8 +132,8 @@ struct Geo {
   static constexpr int LDS = 4 * TB + 64;
 };
 
-// The tile loader, for all modes: K row i of LDS holds key (PERM ? krow_key(i) : i) of the tile, chunk c of a row at c ^ fk(row);
-// V row i holds key i, chunk c at c ^ fv(row).
+// The tile loader, for all modes: row i of LDS, of K and of V, holds key (PERM ? krow_key(i) : i) of the tile; chunk c of a row is at
+// c ^ fk(row) in K, c ^ fv(row) in V. (One order for both, so a page row is looked up once for its key and its value.)
 template <typename T, int HD, bool PERM>
 struct Swz {
   static HXA_DEV int fk(int row) { return HD == 64 ? (row >> 1) & 7 : row & 15; }
@@ -148,7 +155,7 @@ struct Loader {
   uint32_t koff[G_::NOFF], voff[G_::NOFF];  // contiguous: byte offsets within a whole tile; paged: chunk offsets within a row
   int ent;           // paged: the page entry of this lane's key in the tile that is opened next
   unsigned in_page;  // and the key's place in that page
-  uint32_t krow[PAGED ? G_::NLD : 1], vrow[PAGED ? G_::NLD : 1];  // paged: page rows that this lane's loads of the tile opened last read
+  uint32_t row[PAGED ? G_::NLD : 1];  // paged: page rows that this lane's loads of the tile opened last read
   HXA_DEV Loader(const Keys<T> &s_, const Item &it_, uint8_t *lds_, int lane_, int wave_) : s(s_), it(it_), lds(lds_), lane(lane_), wave(wave_) {
     ent = -1;
     in_page = 0;
@@ -158,7 +165,7 @@ struct Loader {
       const int kr = PERM ? krow_key(r) : r;
       const int ck = c ^ S_::fk(r), cv = c ^ S_::fv(r);
       koff[j] = PAGED ? ck * 16u : ((uint32_t)kr * (uint32_t)s.ldk + ck * 8) * 2u;
-      voff[j] = PAGED ? cv * 16u : ((uint32_t)r * (uint32_t)s.ldv + cv * 8) * 2u;
+      voff[j] = PAGED ? cv * 16u : ((uint32_t)kr * (uint32_t)s.ldv + cv * 8) * 2u;
     }
     if (PAGED) entry(0);
   }
@@ -178,14 +185,13 @@ struct Loader {
     const int key0 = it.x0 + i * KT;
     if constexpr (PAGED) {
       const bool ok = (unsigned)ent < (unsigned)s.npages;  // (-1 past x1)
-      const uint32_t row = ok ? ((uint32_t)ent * s.H + s.h) * s.page + in_page : 0;  // < 2^32: checked on the host
+      const uint32_t at = ok ? ((uint32_t)ent * s.H + s.h) * s.page + in_page : 0;  // < 2^32: checked on the host
       const uint64_t mask = __ballot(ok);
       if (key0 + KT < it.x1) entry(i + 1);
 #pragma unroll
       for (int j = 0; j < G_::NLD; j++) {
         const int r = (j * 4 + wave) * G_::RPL + lane / G_::CH;
-        krow[j] = __shfl((int)row, PERM ? krow_key(r) : r);
-        vrow[j] = PERM ? __shfl((int)row, r) : krow[j];
+        row[j] = __shfl((int)at, PERM ? krow_key(r) : r);
       }
       return mask;
     } else {
@@ -203,7 +209,7 @@ struct Loader {
     uint8_t *to = (V ? vbuf(i) : kbuf(i)) + blk * 1024;
     const uint32_t off = V ? voff[j % G_::NOFF] : koff[j % G_::NOFF];
     if constexpr (PAGED) {
-      g2l16_opaque((const uint8_t *)(V ? s.v : s.k) + (uint64_t)(V ? vrow[j] : krow[j]) * G_::RB + off, to);
+      g2l16_opaque((const uint8_t *)(V ? s.v : s.k) + (uint64_t)row[j] * G_::RB + off, to);
     } else {
       const int key0 = it.x0 + i * KT;
       const long ld = V ? s.ldv : s.ldk;
@@ -214,7 +220,7 @@ struct Loader {
         int ln = lane;
         asm volatile("" : "+v"(ln));  // opaque: the loop keeps none of these addresses in registers
         const int r = blk * G_::RPL + ln / G_::CH, c = ln % G_::CH;
-        const int from = min(PERM && !V ? krow_key(r) : r, it.x1 - 1 - key0), ch = c ^ (V ? S_::fv(r) : S_::fk(r));
+        const int from = min(PERM ? krow_key(r) : r, it.x1 - 1 - key0), ch = c ^ (V ? S_::fv(r) : S_::fk(r));
         g2l16_sbase(t, ((uint32_t)from * (uint32_t)ld + ch * 8) * 2u, to);
       }
     }
@@ -246,14 +252,14 @@ struct Loader {
 
 // The values of tile i where the mask cuts it: rows of keys that are not there (km) become zeros; so do rows that only some rows of
 // the workgroup see (keys past lim_min) and that hold an infinity or NaN: their mask is returned. Whole workgroup, ends with a barrier.
-template <typename T, int HD>
+template <typename T, int HD, bool PERM>
 HXA_DEV uint64_t fix_v(uint8_t *vb, uint8_t *flags, int key0, uint64_t km, int lim_min, int tid) {
   constexpr int RB = HD * 2, N = RB / 4 / 16;
-  const int row = tid >> 2, lane = tid & 63;
-  uint8_t *p = vb + row * RB + (tid & 3) * (RB / 4);
-  const bool dead = !((km >> row) & 1);
+  const int key = tid >> 2, lane = tid & 63;
+  uint8_t *p = vb + (PERM ? krow_key(key) : key) * RB + (tid & 3) * (RB / 4);  // (krow_key is its own inverse)
+  const bool dead = !((km >> key) & 1);
   bool bad = false;
-  if (!dead && key0 + row > lim_min) {
+  if (!dead && key0 + key > lim_min) {
     // a magnitude of at least the exponent's ones carries into the sign's place
     uint32_t carry = 0;
 #pragma unroll
@@ -288,7 +294,7 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
   typedef Swz<T, HD, true> S_;
   constexpr int NB = W == 4 ? 2 : 1;       // 32-key blocks of a tile for each wave
   constexpr int ND = HD / 32, AK = 2, AV = 3;  // dim blocks; fragments of K (V) read ahead
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = this_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = W == 4 ? wave : wave & 1, kh = W == 4 ? 0 : wave >> 1;
   const int g = lane >> 5, ql = lane & 31;
 
@@ -317,12 +323,12 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
   ld.load_all(0);
 
   // V^T fragment of 32 dims d, keys kb .. kb + 15 (kb a multiple of 16): lane (g, ql) dim 32 d + ql, keys kb + 8 g .. + 7; 16 lanes read
-  // 4 keys x 16 dims at a time
-  const int vkey = 8 * g + ((lane & 15) >> 2);
+  // 4 keys x 16 dims at a time: rows 4 g .. + 3 and 4 g + 8 .. + 3
+  const int vrow = 4 * g + ((lane & 15) >> 2);
   const int vlow = ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;  // within 64 bytes
   uint32_t vat[ND];
 #pragma unroll
-  for (int d = 0; d < ND; d++) vat[d] = vkey * G_::RB + (((d << 2) ^ S_::fv(vkey)) << 4) + vlow;  // fv(vkey + 4) is the same
+  for (int d = 0; d < ND; d++) vat[d] = vrow * G_::RB + (((d << 2) ^ S_::fv(vrow)) << 4) + vlow;  // fv(vrow + 8) is the same
 
   // One tile for this wave. MAIN: every row sees all of it, and the next tile is whole: its loads are issued one beside each
   // product of K (64 bytes a clock and CU: eight in a row hold a wave for 600 cycles). Fragments are read AK (AV) products ahead: without
@@ -337,7 +343,7 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
     };
     auto vfrag = [&](int n) {  // n = (16-key slice) ND + dims
       const uint8_t *at = vb + vat[n % ND] + (kh * 32 + n / ND * 16) * G_::RB;
-      return __builtin_shufflevector(read_tr<v4>(at), read_tr<v4>(at + 4 * G_::RB), 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_shufflevector(read_tr<v4>(at), read_tr<v4>(at + 8 * G_::RB), 0, 1, 2, 3, 4, 5, 6, 7);
     };
     float16_t S[NB];
     v8 kf[AK + 1][NB];
@@ -452,7 +458,7 @@ HXA_DEV void rows_item(const Keys<T> &s, const Item &it, const T *q, long ldq, i
     }
     const bool cut = kmi != ~0ull || key0 + KT - 1 > lim_min;
     if (cut) {
-      const uint64_t f = fix_v<T, HD>(ld.vbuf(i), lds + G_::FLAGS, key0, kmi, lim_min, tid);
+      const uint64_t f = fix_v<T, HD, true>(ld.vbuf(i), lds + G_::FLAGS, key0, kmi, lim_min, tid);
       if (i == nt - 1) apart[0] = f;
       if (i == nt - 2) apart[1] = f;
       if (i == nt - 3) apart[2] = f;
@@ -544,7 +550,7 @@ template <typename T, int HD, int W>
 HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uint8_t *lds, float16_t (&acc)[HD / 32], float m, float l) {
   typedef typename HxaVec<T>::v4 v4;
   typedef typename HxaVec<T>::v8 v8;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = this_thread(), lane = tid & 63, wave = tid >> 6;
   const int rw = W == 4 ? wave : wave & 1;
   const bool second = W == 2 && wave >= 2;  // has handed its sums over
   const int g = lane >> 5, ql = lane & 31, r0 = it.r0 + rw * 32;
@@ -614,7 +620,7 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
   typedef typename HxaVec<T>::v4 v4;
   typedef Swz<T, HD, false> S_;
   constexpr int ND = HD / 16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = this_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int gi = lane >> 4, ql = lane & 15;
   const int R = it.r0 + ql, last = it.nrows - 1, Rc = min(R, last);
   float4_t acc[ND];
@@ -648,7 +654,7 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
       }
       const bool cut = km != ~0ull || key0 + KT - 1 > lim_min;
       if (cut) {
-        const uint64_t f = fix_v<T, HD>(ld.vbuf(i), lds + G_::FLAGS, key0, km, lim_min, tid);
+        const uint64_t f = fix_v<T, HD, false>(ld.vbuf(i), lds + G_::FLAGS, key0, km, lim_min, tid);
         if (i == nt - 1) apart[0] = f;
         if (i == nt - 2) apart[1] = f;
       }
@@ -886,13 +892,18 @@ __global__ HXA_CAUSAL_BOUNDS void causal_kernel(CausalArgs p) {
 }
 
 // ---- over the cache ----
-// The keys of a sequence are one list: the prefix (P keys), then its own. The items of a key head, in grid order:
+// The keys of a sequence are one list: the prefix (P keys), then its own. The work of a key head, in grid order:
 //   shared: np_blocks blocks of all T G rows x ranges of the prefix, without a mask (rows of unused tokens are computed and
 //           never read); partial slots [0, sp_max)
-//   own:    the blocks of rb of the sequences' rows, the last one in the mode that its rows need, x ranges of their keys
+//   own:    the blocks of rb of the sequences' rows, the last one in the mode that its rows need, over their keys
 //           [x_first, P + own), slots from sp_max on
-// How long the ranges are follows from the lengths as they are on the device: every workgroup adds the tiles of the whole launch up and
-// cuts them into as many items as run at once, so one long sequence among short ones does not decide the time.
+// Split (with a workspace), the own blocks' tiles are one list that is cut into as many equal pieces as run at once beside the shared
+// ranges, wherever the cuts fall: a workgroup's piece may end one block, take others whole and begin another. A block counts SEG tiles
+// more than it has, for its setup and its result. With few blocks every piece begins in its own block instead, where that costs fewer than
+// SEG tiles: the second setup of a piece takes longer than they do. The cuts follow from the lengths as they are on the device, so
+// neither one long sequence among short ones nor a few items more than places decide the time (128 sequences, 32 / 8 heads, 500 keys behind 300:
+// 71 -> 65 us against pieces in their own blocks, 1024 of 300 behind 600: 458 -> 315; 16 of 1000: 18.8 us so, 20.2 cut anywhere).
+// Not split, an item is a block.
 struct CachedArgs {
   hxa_kv_cache c;
   const void *q;
@@ -903,122 +914,186 @@ struct CachedArgs {
   float cs;
   int np_mode, np_blocks, sp_max;  // sp_max 0: nothing is shared
   int rb_log, s_max;  // rows a block of a sequence: 64 or 128
-  int x_first;    // 0: own items take the prefix too
+  int x_first;    // 0: own blocks take the prefix too
   int budget;     // items a key head that run at once
   int least;      // tiles an item is worth
-  float *part;    // nullptr: straight to o (sp_max = 0, s_max = 1)
+  float *part;    // nullptr: nothing is split, straight to o
   float2_t *ml;
 };
+constexpr int SEG = 2;
+typedef int int4_t __attribute__((ext_vector_type(4)));
 // modes: 1 few rows (16), 2 rows (64), 4 rows (128); the one for `rows` rows that belong together, or for the first of more than 128
 __host__ HXA_DEV int mode_rows(int mode) { return mode == 1 ? 16 : 32 * mode; }
 __host__ HXA_DEV int rows_mode(long rows) { return rows <= 16 ? 1 : rows <= 64 ? 2 : 4; }
 
-// what item `q` of a key head is; split < 0: there is none
+// x / d rounded up, at most 2^24 (more tiles than a range has); below 2^24 the product with the reciprocal is off by one at most
+HXA_DEV uint32_t ceil_of(uint32_t x, uint32_t d) {
+  if (x >= 1u << 24) return min((x - 1) / d + 1, 1u << 24);
+  uint32_t y = (uint32_t)((float)x * __builtin_amdgcn_rcpf((float)d));
+  const int left = (int)(x - y * d);
+  if (left > 0) y += left > (int)d ? 2 : 1;
+  if (left < 0 && left <= -(int)d) y--;
+  return y;
+}
+HXA_DEV int floor_of(uint32_t x, uint32_t d) {
+  if (x >= 1u << 24) return (int)(x / d);
+  int y = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+  const int left = (int)(x - (uint32_t)y * d);
+  return left < 0 ? y - 1 : left >= (int)d ? y + 1 : y;
+}
+HXA_DEV int max_all(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+// 64 sequences of the batch, one a lane: first row in the call, tokens, length, blocks, and tiles of a block (0 without rows)
+struct Lanes {
+  int b, n, len, nb, tiles;
+  HXA_DEV void sizes(const CachedArgs &p) {
+    const long cap = (long)p.c.ldt * p.c.page;
+    nb = (n * p.G + (1 << p.rb_log) - 1) >> p.rb_log;
+    tiles = nb ? (int)((min(max((long)len, 0L), cap) + p.c.prefix_len - p.x_first + KT - 1) / KT) : 0;
+  }
+  HXA_DEV void load(const CachedArgs &p, int base, int lane) {
+    const int i = base + lane;
+    b = n = len = 0;
+    if (i < p.c.nseq) {
+      b = min(max(p.c.cu[i], 0), p.T);
+      n = min(max(p.c.cu[i + 1], b), p.T) - b;
+      len = p.c.len[i];
+    }
+    sizes(p);
+  }
+};
+// what a workgroup does next: a range of the prefix for all rows, or tiles [t0, t1) of a block of a sequence
 struct Work {
   bool shared;
-  int split, nsplit, chunk;  // range of `chunk` tiles
-  int block;                 // shared: the block of rows
-  int seq, b, n, len, first; // own: the sequence, its rows in the call, its length, the first row of the block
+  int slot, t0, t1;
+  bool last;                 // the block's last range: it fills the slots behind its own
+  int block;
+  int seq, b, n, len;        // own: the sequence, its rows in the call, its length
 };
-HXA_DEV Work find_work(const CachedArgs &p, int q, int lane) {
-  const hxa_kv_cache &c = p.c;
-  const int rb = 1 << p.rb_log, pt = p.sp_max ? (c.prefix_len + KT - 1) / KT : 0;
-  const long cap = (long)c.ldt * c.page;
-  int b = 0, n = 0, len = 0, nb = 0, tiles = 0;
-  auto load = [&](int base) {  // this lane's sequence: its blocks, and the tiles of each
-    const int i = base + lane;
-    b = n = len = nb = tiles = 0;
-    if (i < c.nseq) {
-      b = min(max(c.cu[i], 0), p.T);
-      n = min(max(c.cu[i + 1], b), p.T) - b;
-      len = c.len[i];
-      nb = (n * p.G + rb - 1) >> p.rb_log;
-      tiles = nb ? (int)((min(max((long)len, 0L), cap) + c.prefix_len - p.x_first + KT - 1) / KT) : 0;
-    }
-  };
-  auto max_all = [](int v) {
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
-    return __builtin_amdgcn_readlane(v, 63);
-  };
-  uint64_t all = (uint64_t)p.np_blocks * pt * 5 / 4;  // a tile of 128 rows takes about 5/4 of one of 16 (4600 cycles, 3800)
-  int blocks = p.np_blocks, longest = 0;
-  bool whole = false;  // up to 64 sequences, and one has a whole block
-  for (int base = 0; base < c.nseq; base += 64) {
-    load(base);
-    const uint64_t x = (uint64_t)nb * (uint32_t)tiles;  // below 2^24 x 2^24: two sums of 26 bits
-    all += (uint32_t)__builtin_amdgcn_readlane(wave_scan_i((int)(x & 0x3ffffff)), 63);
-    if (__any(x >> 26)) all += (uint64_t)(uint32_t)__builtin_amdgcn_readlane(wave_scan_i((int)(x >> 26)), 63) << 26;
-    blocks += __any(nb > 1) ? __builtin_amdgcn_readlane(wave_scan_i(nb), 63) : __popcll(__ballot(nb > 0));
-    longest = max(longest, max_all(tiles));
-    whole |= c.nseq <= 64 && __any(n * p.G >= rb);
-  }
-  // every block has one range that is not full: those are taken off what runs at once, where they leave enough; else some
-  // workgroups follow others, and shorter ranges even the ends out
-  const uint32_t places = p.budget - blocks > p.budget / 2 ? p.budget - blocks : p.budget + p.budget / 2;
-  // x / d rounded up, at most 2^24 (more tiles than a range has); below 2^24 the product with the reciprocal is off by one at most
-  auto ceil_of = [](uint64_t x, uint32_t d) {
-    if (x >= 1u << 24) {
-      const uint64_t y = (x + d - 1) / d;
-      return (uint32_t)(y < 1u << 24 ? y : 1u << 24);
-    }
-    const uint32_t n = (uint32_t)x;
-    uint32_t y = (uint32_t)((float)n * __builtin_amdgcn_rcpf((float)d));
-    const int left = (int)(n - y * d);
-    if (left > 0) y += left > (int)d ? 2 : 1;
-    if (left < 0 && left <= -(int)d) y--;
-    return y;
-  };
-  uint32_t chunk = p.s_max == 1 && p.sp_max == 0 ? 1u << 24 : max(ceil_of(all, places), (uint32_t)p.least);
-  chunk = max(chunk, ceil_of(longest, p.s_max));
-  Work w{};
-  w.split = -1;
-  if (p.sp_max) {
-    const uint32_t cp = max((chunk * 4 + 4) / 5, ceil_of(pt, p.sp_max));
-    const int ns = (int)ceil_of(pt, cp);
-    if (q < ns * p.np_blocks) {
-      w.shared = true;
-      w.split = q / p.np_blocks;
-      w.block = q - w.split * p.np_blocks;
-      w.nsplit = ns;
-      w.chunk = (int)cp;
-      return w;
-    }
-    q -= ns * p.np_blocks;
-  }
-  // the whole blocks of all sequences, then what is left of each: the short items even the end of the launch out (32 prompts of 300 rows
-  // behind 1000 keys, 768 blocks on 512 places: 66 -> 61 us). More than 64 sequences keep their order: a second pass over their
-  // lengths costs each of 201 x 8 items more (109 -> 118 us).
+// the walk of a workgroup over its piece [pos, end) of the list; the lanes' sequences, and the list's end behind each (inc, from `seen` on), wait
+// in LDS while a block is computed
+struct Walk {
+  int pos, end, chunk, base, seen;
+  bool own_pieces;  // a block is a whole number of pieces in the list
+  HXA_DEV int eff(int tiles) const { return own_pieces ? (int)ceil_of(max(tiles, 1), chunk) * chunk : tiles + SEG; }
+};
+HXA_DEV void take(Work &w, const Lanes &s, int l, int base) {
+  w.seq = base + l;
+  w.b = __builtin_amdgcn_readlane(s.b, l);
+  w.n = __builtin_amdgcn_readlane(s.n, l);
+  w.len = __builtin_amdgcn_readlane(s.len, l);
+}
+// item `q` of a key head, not split: the whole blocks of all sequences, then what is left of each: the short items even the end of the launch
+// out (32 prompts of 300 rows behind 1000 keys, 768 blocks on 512 places: 66 -> 61 us). More than 64 sequences keep their order: a second
+// pass over their lengths costs each of 201 x 8 items more (109 -> 118 us).
+HXA_DEV bool find_block_of(const CachedArgs &p, int q, int lane, Work &w) {
+  const int rb = 1 << p.rb_log;
+  Lanes s;
+  s.load(p, 0, lane);
+  const bool whole = p.c.nseq <= 64 && __any(s.n * p.G >= rb);
   int seen = 0;
   for (int rest = whole ? 0 : 1; rest < 2; rest++) {
-    for (int base = 0; base < c.nseq; base += 64) {
-      if (c.nseq > 64) load(base);
-      const int ns = max((int)ceil_of(tiles, chunk), 1), full = whole ? nb - ((n * p.G & (rb - 1)) != 0) : 0;
-      const int cnt = (rest ? nb - full : full) * ns, inc = wave_scan_i(cnt);
+    for (int base = 0; base < p.c.nseq; base += 64) {
+      if (base > 0) s.load(p, base, lane);
+      const int full = whole ? s.nb - ((s.n * p.G & (rb - 1)) != 0) : 0;
+      const int cnt = rest ? s.nb - full : full, inc = wave_scan_i(cnt);
       const uint64_t hit = __ballot(seen + inc > q);
       if (!hit) {
         seen += __builtin_amdgcn_readlane(inc, 63);
         continue;
       }
       const int l = __builtin_ctzll(hit);
-      q -= seen + __builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(cnt, l);
-      w.nsplit = __builtin_amdgcn_readlane(ns, l);
-      const int block = q / w.nsplit;
-      w.split = q - block * w.nsplit;
-      w.chunk = (int)chunk;
-      w.seq = base + l;
-      w.b = __builtin_amdgcn_readlane(b, l);
-      w.n = __builtin_amdgcn_readlane(n, l);
-      w.len = __builtin_amdgcn_readlane(len, l);
-      w.first = (block + (rest ? __builtin_amdgcn_readlane(full, l) : 0)) << p.rb_log;
-      return w;
+      take(w, s, l, base);
+      w.block = q - seen - __builtin_amdgcn_readlane(inc, l) + __builtin_amdgcn_readlane(cnt, l) + (rest ? __builtin_amdgcn_readlane(full, l) : 0);
+      w.t0 = 0;
+      w.t1 = 1 << 24;
+      return true;
     }
   }
-  return w;
+  return false;
+}
+// the work at the walk's place; pos < end
+HXA_DEV bool next_work(const CachedArgs &p, Walk &k, Lanes &s, int each, int inc, int lane, int4_t *stash, Work &w) {
+  uint64_t hit;
+  while (!(hit = __ballot(k.seen + inc > k.pos))) {
+    k.seen += __builtin_amdgcn_readlane(inc, 63);
+    k.base += 64;
+    if (k.base >= p.c.nseq) return false;
+    s.load(p, k.base, lane);
+    each = k.eff(s.tiles);
+    inc = wave_scan_i(s.nb * each);
+  }
+  *stash = (int4_t){s.b, s.n, s.len, inc};
+  const int l = __builtin_ctzll(hit), seg = k.own_pieces ? 0 : SEG;
+  take(w, s, l, k.base);
+  const int eff = __builtin_amdgcn_readlane(each, l), nb = __builtin_amdgcn_readlane(s.nb, l);
+  int at = k.pos - (k.seen + __builtin_amdgcn_readlane(inc, l) - nb * eff);
+  w.block = at < eff ? 0 : floor_of(at, eff);
+  at -= w.block * eff;  // the walk's place in the block: 0, or the first of a piece
+  const int stop = k.pos - at + eff;
+  w.slot = p.sp_max + (at == 0 ? 0 : (int)ceil_of(at, k.chunk));
+  w.t0 = max(at - seg, 0);
+  w.t1 = max(min(k.end, stop) - k.pos + at - seg, 0);
+  w.last = stop <= k.end;
+  k.pos = min(k.end, stop);
+  return true;
+}
+// the first work of item `q` of a key head, split
+HXA_DEV bool first_work(const CachedArgs &p, int q, int lane, int4_t *stash, Walk &k, Work &w) {
+  const int pt = p.sp_max ? (p.c.prefix_len + KT - 1) / KT : 0;
+  Lanes s;
+  int own = 0, blocks = 0, longest = 0;
+  for (int base = (p.c.nseq - 1) & ~63; base >= 0; base -= 64) {  // sums below 2^30: checked on the host
+    s.load(p, base, lane);
+    own += __builtin_amdgcn_readlane(wave_scan_i(s.nb * s.tiles), 63);
+    blocks += __any(s.nb > 1) ? __builtin_amdgcn_readlane(wave_scan_i(s.nb), 63) : __popcll(__ballot(s.nb > 0));
+    longest = max(longest, max_all(s.tiles));
+  }
+  // a tile of 128 rows takes about 5/4 of one of 16 (4600 cycles, 3800)
+  const uint32_t pre = (uint32_t)p.np_blocks * pt * 5 / 4;
+  uint32_t chunk = max(ceil_of(own + SEG * blocks + pre, p.budget), (uint32_t)p.least);
+  // no more pieces of a block than slots
+  if (longest + SEG - 1 > (long)chunk * (p.s_max - 1)) chunk = ceil_of(longest + SEG - 1, p.s_max - 1);
+  k.own_pieces = false;
+  const int taken = blocks + p.np_blocks;  // every block has one piece that is not full
+  if (2 * taken <= p.budget) {
+    uint32_t whole = max(ceil_of(own + pre, p.budget - taken), (uint32_t)p.least);
+    if (longest > (long)whole * p.s_max) whole = ceil_of(longest, p.s_max);
+    k.own_pieces = whole < chunk + SEG;
+    if (k.own_pieces) chunk = whole;
+  }
+  if (p.sp_max) {
+    const uint32_t cp = max((chunk * 4 + 4) / 5, ceil_of(pt, p.sp_max));
+    const int ns = (int)ceil_of(pt, cp);
+    if (q < ns * p.np_blocks) {
+      w.shared = true;
+      w.slot = q / p.np_blocks;
+      w.block = q - w.slot * p.np_blocks;
+      w.t0 = w.slot * (int)cp;
+      w.t1 = w.t0 + (int)cp;
+      w.last = w.slot == ns - 1;
+      k.pos = k.end = 0;
+      return true;
+    }
+    q -= ns * p.np_blocks;
+  }
+  const int total = k.own_pieces ? 1 << 30 : own + SEG * blocks;
+  if ((uint64_t)q * chunk >= (uint32_t)total) return false;
+  k.chunk = (int)chunk;
+  k.pos = q * (int)chunk;
+  k.end = min(k.pos + (int)chunk, total);
+  k.base = k.seen = 0;
+  w.shared = false;
+  const int each = k.eff(s.tiles);
+  return next_work(p, k, s, each, wave_scan_i(s.nb * each), lane, stash, w);
 }
 
 template <typename T, int HD>
@@ -1041,66 +1116,77 @@ template <typename T, int HD>
 __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63;
-  const int h = blockIdx.x % p.c.H, rest = blockIdx.x / p.c.H, P = p.c.prefix_len;
-  Keys<T> s{};
-  s.k = (const T *)p.c.k;
-  s.v = (const T *)p.c.v;
-  s.prefix = p.c.prefix;
-  s.table = p.c.table;
-  s.P = P;
-  s.page = p.c.page;
-  s.pm = p.pm;
-  s.npages = p.c.npages;
-  s.H = p.c.H;
-  s.h = h;
-  Item it;
-  it.G = p.G;
-  it.gm = p.gm;
-  Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, 0, p.sp_max + p.s_max, p.Hq};
-  const Work w = find_work(p, rest, lane);
-  if (w.split < 0) return;
-  int mode, slot_end;
-  if (w.shared) {
-    mode = p.np_mode;
-    it.r0 = w.block * mode_rows(mode);
-    it.nrows = p.T * p.G;
-    it.tok0 = 0;
-    it.x0 = w.split * w.chunk * KT;
-    it.x1 = min(it.x0 + w.chunk * KT, P);
-    it.base = it.cap = it.least = P - 1;
-    it.causal = false;
-    out.slot = w.split;
-    slot_end = p.sp_max;
-  } else {
-    const long len = w.len;
-    const int held = (int)min(max(len, 0L), (long)p.c.ldt * p.c.page);
-    s.table += (long)w.seq * p.c.ldt;
-    it.r0 = w.first;
-    it.nrows = w.n * p.G;
-    mode = rows_mode(min(it.nrows - it.r0, 1 << p.rb_log));
-    it.tok0 = w.b;
-    // own position of token j: len - n + j; a negative one sees the prefix alone
-    it.causal = true;
-    it.cap = P + held - 1;
-    it.least = P - 1;
-    const long base = (long)P + len - w.n;
-    it.base = (int)max(min(base, (long)it.cap), (long)P - 1 - w.n);
-    const int end = row_limit(it, min(it.r0 + mode_rows(mode), it.nrows) - 1) + 1;
-    it.x0 = p.x_first + (int)min((long)w.split * w.chunk * KT, 1L << 30);
-    it.x1 = (int)min((long)end, it.x0 + (long)w.chunk * KT);
-    out.slot = p.sp_max + w.split;
-    slot_end = p.sp_max + p.s_max;
-  }
-  if (out.part != nullptr && w.split == w.nsplit - 1) {  // slots that no range fills: sums of nothing
-    const int rows = min(mode_rows(mode), it.nrows - it.r0);
-    const int free = slot_end - out.slot - 1;
-    for (int k = threadIdx.x; k < rows * free; k += 256) {
-      int head;
-      const int row = k / free, tok = row_tok(it, it.r0 + row, head);
-      out.ml[((long)(it.tok0 + tok) * p.Hq + h * p.G + head) * out.nslots + out.slot + 1 + k - row * free] = (float2_t){-INFINITY, 0.0f};
+  const int h = blockIdx.x % p.c.H, q = blockIdx.x / p.c.H, P = p.c.prefix_len;
+  Walk k{};
+  Work w{};
+  int4_t *stash = (int4_t *)(lds + Geo<T, HD>::LDS) + threadIdx.x;  // the lanes' sequences while a block is computed
+  if (p.part == nullptr ? !find_block_of(p, q, lane, w) : !first_work(p, q, lane, stash, k, w)) return;
+  for (;;) {
+    Keys<T> s{};
+    s.k = (const T *)p.c.k;
+    s.v = (const T *)p.c.v;
+    s.prefix = p.c.prefix;
+    s.table = p.c.table;
+    s.P = P;
+    s.page = p.c.page;
+    s.pm = p.pm;
+    s.npages = p.c.npages;
+    s.H = p.c.H;
+    s.h = h;
+    Item it;
+    it.G = p.G;
+    it.gm = p.gm;
+    int mode, slot_end;
+    if (w.shared) {
+      mode = p.np_mode;
+      it.r0 = w.block * mode_rows(mode);
+      it.nrows = p.T * p.G;
+      it.tok0 = 0;
+      it.x0 = w.t0 * KT;
+      it.x1 = min(w.t1 * KT, P);
+      it.base = it.cap = it.least = P - 1;
+      it.causal = false;
+      slot_end = p.sp_max;
+    } else {
+      const long len = w.len;
+      const int held = (int)min(max(len, 0L), (long)p.c.ldt * p.c.page);
+      s.table += (long)w.seq * p.c.ldt;
+      it.r0 = w.block << p.rb_log;
+      it.nrows = w.n * p.G;
+      mode = rows_mode(min(it.nrows - it.r0, 1 << p.rb_log));
+      it.tok0 = w.b;
+      // own position of token j: len - n + j; a negative one sees the prefix alone
+      it.causal = true;
+      it.cap = P + held - 1;
+      it.least = P - 1;
+      const long base = (long)P + len - w.n;
+      it.base = (int)max(min(base, (long)it.cap), (long)P - 1 - w.n);
+      const int end = row_limit(it, min(it.r0 + mode_rows(mode), it.nrows) - 1) + 1;
+      it.x0 = p.x_first + w.t0 * KT;
+      it.x1 = (int)min((long)end, p.x_first + (long)w.t1 * KT);
+      slot_end = p.sp_max + p.s_max;
     }
+    if (p.part != nullptr && w.last) {  // slots that no range fills: sums of nothing
+      const int rows = min(mode_rows(mode), it.nrows - it.r0);
+      const int free = slot_end - w.slot - 1;
+      for (int j = threadIdx.x; j < rows * free; j += 256) {
+        int head;
+        const int row = j / free, tok = row_tok(it, it.r0 + row, head);
+        p.ml[((long)(it.tok0 + tok) * p.Hq + h * p.G + head) * (p.sp_max + p.s_max) + w.slot + 1 + j - row * free] = (float2_t){-INFINITY, 0.0f};
+      }
+    }
+    const Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, w.slot, p.sp_max + p.s_max, p.Hq};
+    any_item<T, HD>(mode, s, it, p, h * p.G, lds, out);
+    if (k.pos >= k.end) return;
+    reads_done_barrier();  // every wave is done with the LDS
+    Lanes y;
+    const int4_t x = *stash;
+    y.b = x[0];
+    y.n = x[1];
+    y.len = x[2];
+    y.sizes(p);
+    if (!next_work(p, k, y, k.eff(y.tiles), x[3], lane, stash, w)) return;
   }
-  any_item<T, HD>(mode, s, it, p, h * p.G, lds, out);
 }
 
 // The partials of a row joined by a wave: lane s has the maximum and the sum of slot s (at most 64 of them), which give its weight
@@ -1228,13 +1314,17 @@ CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws) {
   if (mode == 1 && c.nseq >= 2 && P >= 4 * KT) {
     p.np_mode = rows_mode(RT);
     p.np_blocks = (int)ceil_div(RT, mode_rows(p.np_mode));
-    p.sp_max = (int)std::min({32L, ceil_div(P, KT), ceil_div(p.budget + p.budget / 2, p.np_blocks) + 1});
+    p.sp_max = (int)std::min({32L, ceil_div(P, KT), ceil_div(p.budget, p.np_blocks) + 1});
     p.x_first = (int)P;
   }
+  // a list that is cut anywhere: a block of so many ranges touches one workgroup more
   const long tiles = ceil_div(cap + P - p.x_first, KT), blocks = ceil_div(RT, mode_rows(mode)) + c.nseq / 2;
-  if (mode == 1) p.s_max = (int)std::max(1L, std::min(32L, tiles));
-  else if (blocks * c.H * 8 < slots * 5) p.s_max = (int)std::max(1L, std::min({8L, tiles / p.least, ceil_div(slots, blocks * c.H)}));
-  while (p.s_max > 1 && cached_ws(p, c, T, Hq) > 1L << 30) p.s_max /= 2;
+  if (mode == 1) p.s_max = (int)std::min(31L, tiles);
+  else if (blocks * c.H * 8 < slots * 5) p.s_max = (int)std::min({8L, tiles / p.least, ceil_div(slots, blocks * c.H)});
+  p.s_max = std::max(1, p.s_max);
+  if (p.s_max > 1 || p.sp_max > 0) p.s_max++;
+  while (p.s_max > 2 && cached_ws(p, c, T, Hq) > 1L << 30) p.s_max = p.s_max / 2 + 1;
+  if ((p.n_blocks * (tiles + SEG) + ceil_div(P, KT) * p.np_blocks * 2) >= 1L << 29) p.sp_max = p.np_blocks = p.x_first = 0, p.s_max = 1;
   return p;
 }
 
@@ -1307,16 +1397,18 @@ extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long l
     p.part = (float *)ws;
     p.ml = (float2_t *)(p.part + (long)nslots * T * Hq * c->hd);
   }
-  // blocks, and as many ranges more as run at once (find_work's chunk is at least all tiles / (3/2 budget))
-  const long wgs = ((long)pl.np_blocks + pl.n_blocks + (nslots > 1 ? pl.budget + pl.budget / 2 : 0)) * c->H;
+  // split: a range of the prefix for each of its blocks and pieces of the rest, as many as run at once (first_work's chunk is at least all
+  // tiles / budget), and two roundings up
+  const long wgs = (nslots > 1 ? (long)pl.np_blocks + pl.budget + 2 : pl.n_blocks) * c->H;
   const hipStream_t st = (hipStream_t)stream;
   return by_type(c->dtype, c->hd, [&](auto ty, auto hdc, int id) -> int {
     typedef decltype(ty) T_;
     constexpr int HD = decltype(hdc)::value;
     const auto f = cached_kernel<T_, HD>;
-    const int a = allow_lds((const void *)f, Geo<T_, HD>::LDS, 18 + id);
-    if (a != HXA_OK) return hxa_set_error(a, "attention_cached: %d bytes of LDS", Geo<T_, HD>::LDS);
-    hxa_launch(f, dim3((unsigned)wgs), dim3(256), Geo<T_, HD>::LDS, st, p);
+    constexpr int LDS = Geo<T_, HD>::LDS + 4096;
+    const int a = allow_lds((const void *)f, LDS, 12 + id);
+    if (a != HXA_OK) return hxa_set_error(a, "attention_cached: %d bytes of LDS", LDS);
+    hxa_launch(f, dim3((unsigned)wgs), dim3(256), LDS, st, p);
     if (nslots > 1) hxa_launch(cached_merge_kernel<T_, HD>, dim3((unsigned)ceil_div((long)T * Hq, 4)), dim3(256), 0, st, p);
     return launched("attention_cached");
   });
