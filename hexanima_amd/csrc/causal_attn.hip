@@ -19,6 +19,12 @@
 //   rows (W = 2): 64 rows, the two halves of the tile's keys to two waves each, joined at the end
 //   few rows:     16 rows, 16 keys of the tile to each wave (16x16 MFMAs), joined at the end; bound by reading the cache
 //
+// Bound, and measured (32 query heads on 8 key heads of 128, bf16):
+//   prompts: the matrix instructions, at the board's power limit from ~8000 tokens on (16384 tokens 1.92 ms, 1.15 PFLOP/s); a shorter batch by its
+//            longest block, whose tiles follow each other (a tile of 128 rows 2300 cycles alone, 3050 with two workgroups a CU, of them 1024 MFMAs)
+//   single tokens: reading the keys (16 tokens over 90000 keys behind 32768 shared ones 99 us, 5.1 TB/s; 64 over 30000 behind 4096 40 us)
+// Two workgroups a CU, one's softmax beside the other's matrix products, did better than one that interleaves the tiles' phases itself.
+//
 // What a mask hides has no part in a result: hidden scores become -inf before the maximum; values of keys that no row of the workgroup sees are
 // zeroed in LDS (0 x NaN would be NaN), and values of keys that only some rows see are, where they are not finite, taken out of the
 // matrix product and added, key by key, by the rows that see them at the end.
@@ -1289,7 +1295,7 @@ int wg_slots(int hd) { return causal_ncu() * (hd == 256 ? 1 : 2); }
 //   tile, two of 64 take 1.26); for what is left of a sequence 16 or 64 where that is enough, which is found on the device (a prompt of 1000
 //   tokens and 63 single ones over 800 each behind 500, 32 / 8 heads: 89 -> 60 us against 128 rows for all).
 //   Shared prefix: where sequences bring at most 16 rows, there are at least two of them and the prefix is worth four tiles. No more
-//   slots than ranges find_work's chunk can make.
+//   slots than ranges first_work's chunk can make.
 //   Ranges of keys: with few rows as many as run at once, but none that would bring the partials past 1 GB. With more rows a partial result is as wide as a row's output is in fp32, so keys are
 //   split only where the blocks fill less than 5/8 of the places (32 prompts of 75 rows behind 1000 tokens, 456 blocks of 512 places: split
 //   in two 65 us, whole 51).

@@ -7,7 +7,9 @@
 //
 // Bound by HBM: 2 bytes read and 2 written per value (kv_append: the same for k and v). hd / 16 lanes hold a head, 16 values
 // each as two 16-byte loads; a lane's two chunks are partners of the rotation in either layout, so it needs no exchange, and the 8 angles a
-// lane needs are the same for every head of the token: a wave takes one token and forms them once.
+// lane needs are the same for every head of the token: a wave takes one token and forms them once. 8192 tokens of 32 + 8 heads of 128: 37.0 us,
+// 4.5 TB/s; 9001 tokens of 8 heads appended: 16.1 us, 4.6 TB/s (a large copy 4.8). Few tokens take the launch and three or four
+// dependent loads, 3 .. 4 us.
 #include <cmath>
 
 #include "causal.h"
@@ -163,7 +165,8 @@ struct AppendArgs {
   HeadRot r;
 };
 
-// one wave a token: its sequence (a search of cu), its page row, then k's heads and v's
+// One wave a token: its sequence (a search of cu), its page row, then k's heads and v's. A pool's rows of one token are H pieces of
+// 2 hd bytes a page apart, whole cache lines each, so their order costs nothing.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs p) {
   constexpr int LPH = HD / 16, HPW = 64 / LPH;
