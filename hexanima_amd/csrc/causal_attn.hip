@@ -1296,9 +1296,12 @@ int wg_slots(int hd) { return causal_ncu() * (hd == 256 ? 1 : 2); }
 //   tokens and 63 single ones over 800 each behind 500, 32 / 8 heads: 89 -> 60 us against 128 rows for all).
 //   Shared prefix: where sequences bring at most 16 rows, there are at least two of them and the prefix is worth four tiles. No more
 //   slots than ranges first_work's chunk can make.
-//   Ranges of keys: with few rows as many as run at once, but none that would bring the partials past 1 GB. With more rows a partial result is as wide as a row's output is in fp32, so keys are
-//   split only where the blocks fill less than 5/8 of the places (32 prompts of 75 rows behind 1000 tokens, 456 blocks of 512 places: split
-//   in two 65 us, whole 51).
+//   Not split where the table and the prefix hold at most 6 tiles of keys, or 16 where the blocks fill a quarter of the places: a second
+//   launch and what the ranges set up take longer than the tiles one after the other (single tokens, 16 / 8 heads of 128, us split, whole: one
+//   sequence of 4 tiles 8.9, 7.4, of 8 9.2, 10.0; 16 of 4 9.6, 7.7, of 8 13.6, 11.1, of 16 19.5, 18.4; 64 of 4 18.2, 14.9, of 16 48.5, 43.1).
+//   Ranges of keys: with few rows as many as run at once, but none that would bring the partials past 1 GB. With more rows a partial
+//   result is as wide as a row's output is in fp32, so keys are split only where the blocks fill less than 5/8 of the places (32 prompts of
+//   75 tokens behind 1000, 16 / 8 heads, 456 blocks of 512 places: split in two 65 us, whole 51).
 struct CachedPlan {
   int np_mode, np_blocks, sp_max, rb_log, n_blocks, s_max, x_first, budget, least;
 };
@@ -1316,7 +1319,8 @@ CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws) {
   p.budget = (int)std::max(1L, slots / c.H);
   p.least = mode == 1 ? 1 : 4;
   p.s_max = 1;
-  if (!ws) return p;
+  const long blocks = ceil_div(RT, mode_rows(mode)) + c.nseq / 2, most = ceil_div(cap + P, KT);
+  if (!ws || most <= 6) return p;
   if (mode == 1 && c.nseq >= 2 && P >= 4 * KT) {
     p.np_mode = rows_mode(RT);
     p.np_blocks = (int)ceil_div(RT, mode_rows(p.np_mode));
@@ -1324,8 +1328,8 @@ CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws) {
     p.x_first = (int)P;
   }
   // a list that is cut anywhere: a block of so many ranges touches one workgroup more
-  const long tiles = ceil_div(cap + P - p.x_first, KT), blocks = ceil_div(RT, mode_rows(mode)) + c.nseq / 2;
-  if (mode == 1) p.s_max = (int)std::min(31L, tiles);
+  const long tiles = ceil_div(cap + P - p.x_first, KT);
+  if (mode == 1) p.s_max = most <= 16 && blocks * c.H * 4 >= slots && p.sp_max == 0 ? 1 : (int)std::min(31L, tiles);
   else if (blocks * c.H * 8 < slots * 5) p.s_max = (int)std::min({8L, tiles / p.least, ceil_div(slots, blocks * c.H)});
   p.s_max = std::max(1, p.s_max);
   if (p.s_max > 1 || p.sp_max > 0) p.s_max++;

@@ -148,6 +148,16 @@ def test_workspace_follows_the_sizes(hip):
     assert size(100000, 4, nseq=8) == 0
 
 
+def test_short_tables_are_not_split(hip):
+    """up to 6 tiles of 64 keys take no workspace, nor up to 16 where the blocks are many; a prefix counts with them"""
+    L = hip.lib()
+    size = lambda T, Hq, **kw: L.hxa_attention_cached_ws_bytes(C.byref(plan(hip, **kw)), T, Hq)
+    assert size(1, 4, nseq=1, prefix_len=0, ldt=24) == 0 and size(1, 4, nseq=1, prefix_len=0, ldt=25) > 0
+    assert size(1, 4, nseq=1, prefix_len=65, ldt=20) > 0 and size(1, 4, nseq=1, prefix_len=64, ldt=20) == 0
+    assert size(64, 4, nseq=64, prefix_len=0, ldt=64, H=4) == 0 and size(64, 4, nseq=64, prefix_len=0, ldt=65, H=4) > 0
+    assert size(8, 4, nseq=8, prefix_len=0, ldt=64, H=4) > 0 and size(64, 4, nseq=64, prefix_len=256, ldt=48, H=4) > 0
+
+
 def test_workspace_stays_bounded(hip):
     """many rows: fewer partial results a row instead of more memory, down to one for the prefix's first ranges and one for the own keys"""
     L = hip.lib()
