@@ -198,6 +198,24 @@ def test_causal_infinities_and_nan_stay_behind_the_mask(hip, dtype, hd, Hq, Hk):
     assert np.isfinite(want[150:220]).all() and np.isnan(want[220:, :, 9]).any()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_scores_of_minus_infinity(hip, dtype, hd):
+    """a row that sees nothing but scores of -infinity gets zeros; beside finite ones such a key weighs nothing"""
+    b = Packed(hip, np.random.default_rng(2), [3], 1, 1, hd, dtype)
+    b.q[:, 0] = narrow(np.float32(-1), dtype)
+    b.q[0, 1:hd] = 0
+    b.k[0, :hd] = 0
+    b.k[0, 0] = narrow(np.float32(np.inf), dtype)
+    got = run_causal(hip, b, 0.1)
+    q, k, v = (b.heads(x, 1)[:, 0] for x in (b.q, b.k, b.v))
+    k[0] = 0
+    o, a = attend(q, k, v, 0.1, np.tril(np.ones((3, 3), bool)) & (np.arange(3) > 0))
+    smax = float((np.abs(q) @ np.abs(k).T).max()) * 0.1
+    close(got[:, 0], o, attend_bound(o, a, np.abs(v).max(), 3, hd, smax, dtype), "without the first key")
+    assert (got[0] == 0).all() and (o[1:] != 0).any()
+
+
 # ------------------------------------------------------------------------------------------------------------- cached
 def run_cached(hip, c, q, scale, with_ws=True, stream=None):
     n, Hq = q.shape[0], q.shape[1]
