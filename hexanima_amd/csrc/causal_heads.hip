@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs p) {
   const hxa_kv_cache &c = p.c;
   const int i = wave_count_le(c.cu + 1, c.nseq, t, lane);
   if (i >= c.nseq) return;
-  const int b = c.cu[i], e = c.cu[i + 1];
+  const int b = c.cu[i], e = min(c.cu[i + 1], p.T);  // past T: cut there, as in the attention
   const long at = (long)c.len[i] - (e - (long)t);
   if (t < b || at < 0 || at >= (long)c.ldt * c.page) return;
   const int own = (int)at, slot = own / c.page, row = own - slot * c.page;

@@ -240,7 +240,7 @@ int hxa_rows_to_x32(const float *x, float *tiles, int R, int C, void *stream);
  * angles are held in 32 bits or more and every output is rounded once.
  *
  * A batch of sequences is packed: sequence i's tokens are rows cu[i] .. cu[i + 1] - 1 (cu: device, nseq + 1 ascending entries,
- * cu[0] = 0, a sequence may be empty). Rows outside every sequence are neither read into a result nor written. cu, len, the page
+ * cu[0] = 0, a sequence may be empty; entries past T count as T). Rows outside every sequence are neither read into a result nor written. cu, len, the page
  * tables and pos stay on the device, so a captured graph follows what they hold when it is replayed; entries that
  * are out of range never lead out of the buffers (what such an entry means is said with each function). The calls run on the
  * current device, on whose memory every pointer must be. */

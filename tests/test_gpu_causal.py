@@ -371,6 +371,30 @@ def test_cached_steep_scores(hip, dtype, hd, Hq, H, new, past, prefix):
     close(run_cached(hip, c, q, 1.0)[0], o, attend_bound(o, a, vmax, n, hd, smax, dtype), "steep")
 
 
+def test_sequences_past_the_last_row_end_there(hip):
+    """cu[nseq] above T, as a graph captured for fewer rows may find it: the last sequence has the rows that there are"""
+    rng = np.random.default_rng(23)
+    hd, Hq, H = 128, 4, 2
+    b = Packed(hip, rng, [70, 90], Hq, H, hd, F16, tail=0)
+    want = run_causal(hip, b, 0.1)
+    b.cu = np.array([0, 70, 10 ** 6], np.int32)
+    assert np.array_equal(run_causal(hip, b, 0.1), want) and (want[159] != 0).any()
+    L = hip.lib()
+    pools = []
+    for end in (160, 2 ** 31 - 1):
+        c = Cache(hip, np.random.default_rng(5), [70, 90], [5, 0], 30, 16, H, hd, F16, empty=True)
+        c.cu[2] = end
+        c.lens = [75, 90]
+        plan = c.upload()
+        k, v = dev(hip, b.k), dev(hip, b.v)
+        hip.check(L.hxa_kv_append(C.byref(plan), k.ptr, b.ldk, v.ptr, b.ldv, 160, None, 0.0, None, None))
+        dq, do = dev(hip, b.q), dev(hip, np.zeros((160, b.ldo), np.uint16))
+        hip.check(L.hxa_attention_cached(C.byref(plan), dq.ptr, b.ldq, do.ptr, b.ldo, 160, Hq, 0.1, None, 0, None))
+        hip.sync()
+        pools.append((c.d["k"].numpy().copy(), c.d["v"].numpy().copy(), do.numpy().copy()))
+    assert all(np.array_equal(x, y) for x, y in zip(*pools))
+
+
 def test_cached_prefix_alone(hip):
     """a table without entries: every query sees the prefix, and without a prefix nothing"""
     rng = np.random.default_rng(14)
