@@ -34,11 +34,11 @@
 #include <type_traits>
 
 #include "causal.h"
+#include "causal_walk.h"
 #include "kernels.h"
 
 namespace {
 
-constexpr int KT = 64;              // keys a tile
 constexpr float L2E = 1.4426950408889634f;
 constexpr float RESCALE2 = 5.5f * L2E;  // growth of the maximum, in powers of two, that is left unscaled
 
@@ -779,15 +779,6 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
 }
 
 // ---- which rows a block of the grid takes ----
-struct Block {
-  int seq, b, n;  // the sequence, its first row in the call and its tokens
-  int first;      // first row (token x G + head) of the block within the sequence; -1: none
-};
-// Block `blk` of the grid: sequence i has ceil(n_i G / RB) blocks, and a block's keys grow with its place in the sequence. Up to 16
-// sequences, places are dealt from the highest down over all of them (the longest first). Two workgroups share a CU: of the second layer (blocks
-// first .. 2 first - 1, `first` = CUs / key heads) the order is reversed, so that the longest block has the shortest of
-// them beside it (4096 tokens, 32 / 8 heads: 149 -> 143 us). More sequences: in their order, each from its end. cu's entries are
-// clamped into [0, T]. Whole wave.
 HXA_DEV int wave_scan_i(int v) {  // inclusive
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
@@ -797,59 +788,35 @@ HXA_DEV int wave_scan_i(int v) {  // inclusive
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
   return v;
 }
-HXA_DEV Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int RB, int blk, int first, int lane) {
-  int seen = 0;  // blocks of the sequences before `base`
-  for (int base = 0; base < nseq; base += 64) {
-    const int i = base + lane;
-    int b = 0, e = 0;
-    if (i < nseq) {
-      b = min(max(cu[i], 0), T);
-      e = min(max(cu[i + 1], b), T);
-    }
-    const int nb = ((e - b) * G + RB - 1) / RB;  // (T G < 2^31 - RB: checked on the host)
-    const int inc = wave_scan_i(nb);
-    const int total = __builtin_amdgcn_readlane(inc, 63);
-    Block r{0, 0, 0, -1};
-    int w, j;
-    if (nseq <= 16) {
-      if (blk >= total) return r;
-      if (blk >= first && blk < 2 * first) blk = min(2 * first, total) - 1 - (blk - first);
-      w = 0;
-      j = total - 1 - blk;
-      if (nseq > 1) {
-        // S(L) = number of blocks at places >= L, 64 values of L a step; the block's place j has S(j + 1) <= blk < S(j)
-        int lo = 0, hi = total, s_hi = 0;
-        while (hi - lo > 1) {
-          const int step = (hi - lo + 63) >> 6, L = lo + (lane + 1) * step;
-          int s = 0;
-          for (int q = 0; q < nseq; q++) s += max(__builtin_amdgcn_readlane(nb, q) - L, 0);
-          const int k = __popcll(__ballot(s > blk));
-          s_hi = __builtin_amdgcn_readlane(s, min(k, 63));
-          lo += k * step;
-          hi = min(lo + step, hi);
-        }
-        j = lo;
-        uint64_t at = __ballot(nb > j);
-        for (int k = blk - s_hi; k > 0; k--) at &= at - 1;
-        w = __builtin_ctzll(at);
-      }
-    } else {
-      const uint64_t hit = __ballot(seen + inc > blk);
-      if (!hit) {
-        seen += total;
-        continue;
-      }
-      w = __builtin_ctzll(hit);
-      j = seen + __builtin_amdgcn_readlane(inc, w) - 1 - blk;  // blocks of the sequence behind this one
-    }
-    r.seq = base + w;
-    r.b = __builtin_amdgcn_readlane(b, w);
-    r.n = __builtin_amdgcn_readlane(e, w) - r.b;
-    r.first = j * RB;
-    return r;
-  }
-  return Block{0, 0, 0, -1};
+HXA_DEV int max_all(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(v, 63);
 }
+typedef int int4_t __attribute__((ext_vector_type(4)));
+// causal_walk.h's wave: a lane's value is a register, its stash 16 bytes of LDS
+struct Wave {
+  typedef int I;
+  typedef int4_t *Stash;
+  static HXA_DEV int lanes(int base) { return base + (threadIdx.x & 63); }
+  template <typename F, typename... A>
+  static HXA_DEV int map(F f, A... a) { return f(a...); }
+  template <typename F>
+  static HXA_DEV uint64_t ballot(F f, int a) { return __ballot(f(a)); }
+  static HXA_DEV int get(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+  static HXA_DEV int scan(int v) { return wave_scan_i(v); }
+  static HXA_DEV int most(int v) { return max_all(v); }
+  static HXA_DEV float rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+  static HXA_DEV void keep(int4_t *at, int a, int b, int c, int d) { *at = (int4_t){a, b, c, d}; }
+  static HXA_DEV void kept(const int4_t *at, int &a, int &b, int &c, int &d) {
+    const int4_t x = *at;
+    a = x[0], b = x[1], c = x[2], d = x[3];
+  }
+};
 
 struct CausalArgs {
   const void *q, *k, *v;
@@ -868,9 +835,8 @@ struct CausalArgs {
 template <typename T, int HD, int W>
 __global__ HXA_CAUSAL_BOUNDS void causal_kernel(CausalArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int lane = threadIdx.x & 63;
   const int h = blockIdx.x % p.Hk, blk = blockIdx.x / p.Hk;  // key heads innermost: with 8 of them each XCD keeps its own head's keys
-  const Block b = find_block(p.cu, p.nseq, p.T, p.G, 32 * W, blk, p.first, lane);
+  const Block b = find_block<Wave>(p.cu, p.nseq, p.T, p.G, 32 * W, blk, p.first);
   if (b.first < 0) return;
   const long row0 = b.b;
   Keys<T> s{};
@@ -898,210 +864,16 @@ __global__ HXA_CAUSAL_BOUNDS void causal_kernel(CausalArgs p) {
 }
 
 // ---- over the cache ----
-// The keys of a sequence are one list: the prefix (P keys), then its own. The work of a key head, in grid order:
-//   shared: np_blocks blocks of all T G rows x ranges of the prefix, without a mask (rows of unused tokens are computed and
-//           never read); partial slots [0, sp_max)
-//   own:    the blocks of rb of the sequences' rows, the last one in the mode that its rows need, over their keys
-//           [x_first, P + own), slots from sp_max on
-// Split (with a workspace), the own blocks' tiles are one list that is cut into as many equal pieces as run at once beside the shared
-// ranges, wherever the cuts fall: a workgroup's piece may end one block, take others whole and begin another. A block counts SEG tiles
-// more than it has, for its setup and its result. With few blocks every piece begins in its own block instead, where that costs fewer than
-// SEG tiles: the second setup of a piece takes longer than they do. The cuts follow from the lengths as they are on the device, so
-// neither one long sequence among short ones nor a few items more than places decide the time (128 sequences, 32 / 8 heads, 500 keys behind 300:
-// 71 -> 65 us against pieces in their own blocks, 1024 of 300 behind 600: 458 -> 315; 16 of 1000: 18.8 us so, 20.2 cut anywhere).
-// Not split, an item is a block.
-struct CachedArgs {
-  hxa_kv_cache c;
+struct CachedArgs : CachedWork {
   const void *q;
   void *o;
   long ldq, ldo;
-  int T, G, Hq;
+  int Hq;
   uint32_t gm, pm;
   float cs;
-  int np_mode, np_blocks, sp_max;  // sp_max 0: nothing is shared
-  int rb_log, s_max;  // rows a block of a sequence: 64 or 128
-  int x_first;    // 0: own blocks take the prefix too
-  int budget;     // items a key head that run at once
-  int least;      // tiles an item is worth
   float *part;    // nullptr: nothing is split, straight to o
   float2_t *ml;
 };
-constexpr int SEG = 2;
-typedef int int4_t __attribute__((ext_vector_type(4)));
-// modes: 1 few rows (16), 2 rows (64), 4 rows (128); the one for `rows` rows that belong together, or for the first of more than 128
-__host__ HXA_DEV int mode_rows(int mode) { return mode == 1 ? 16 : 32 * mode; }
-__host__ HXA_DEV int rows_mode(long rows) { return rows <= 16 ? 1 : rows <= 64 ? 2 : 4; }
-
-// x / d rounded up, at most 2^24 (more tiles than a range has); below 2^24 the product with the reciprocal is off by one at most
-HXA_DEV uint32_t ceil_of(uint32_t x, uint32_t d) {
-  if (x >= 1u << 24) return min((x - 1) / d + 1, 1u << 24);
-  uint32_t y = (uint32_t)((float)x * __builtin_amdgcn_rcpf((float)d));
-  const int left = (int)(x - y * d);
-  if (left > 0) y += left > (int)d ? 2 : 1;
-  if (left < 0 && left <= -(int)d) y--;
-  return y;
-}
-HXA_DEV int floor_of(uint32_t x, uint32_t d) {
-  if (x >= 1u << 24) return (int)(x / d);
-  int y = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
-  const int left = (int)(x - (uint32_t)y * d);
-  return left < 0 ? y - 1 : left >= (int)d ? y + 1 : y;
-}
-HXA_DEV int max_all(int v) {
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
-  return __builtin_amdgcn_readlane(v, 63);
-}
-
-// 64 sequences of the batch, one a lane: first row in the call, tokens, length, blocks, and tiles of a block (0 without rows)
-struct Lanes {
-  int b, n, len, nb, tiles;
-  HXA_DEV void sizes(const CachedArgs &p) {
-    const long cap = (long)p.c.ldt * p.c.page;
-    nb = (n * p.G + (1 << p.rb_log) - 1) >> p.rb_log;
-    tiles = nb ? (int)((min(max((long)len, 0L), cap) + p.c.prefix_len - p.x_first + KT - 1) / KT) : 0;
-  }
-  HXA_DEV void load(const CachedArgs &p, int base, int lane) {
-    const int i = base + lane;
-    b = n = len = 0;
-    if (i < p.c.nseq) {
-      b = min(max(p.c.cu[i], 0), p.T);
-      n = min(max(p.c.cu[i + 1], b), p.T) - b;
-      len = p.c.len[i];
-    }
-    sizes(p);
-  }
-};
-// what a workgroup does next: a range of the prefix for all rows, or tiles [t0, t1) of a block of a sequence
-struct Work {
-  bool shared;
-  int slot, t0, t1;
-  bool last;                 // the block's last range: it fills the slots behind its own
-  int block;
-  int seq, b, n, len;        // own: the sequence, its rows in the call, its length
-};
-// the walk of a workgroup over its piece [pos, end) of the list; the lanes' sequences, and the list's end behind each (inc, from `seen` on), wait
-// in LDS while a block is computed
-struct Walk {
-  int pos, end, chunk, base, seen;
-  bool own_pieces;  // a block is a whole number of pieces in the list
-  HXA_DEV int eff(int tiles) const { return own_pieces ? (int)ceil_of(max(tiles, 1), chunk) * chunk : tiles + SEG; }
-};
-HXA_DEV void take(Work &w, const Lanes &s, int l, int base) {
-  w.seq = base + l;
-  w.b = __builtin_amdgcn_readlane(s.b, l);
-  w.n = __builtin_amdgcn_readlane(s.n, l);
-  w.len = __builtin_amdgcn_readlane(s.len, l);
-}
-// item `q` of a key head, not split: the whole blocks of all sequences, then what is left of each: the short items even the end of the launch
-// out (32 prompts of 300 rows behind 1000 keys, 768 blocks on 512 places: 66 -> 61 us). More than 64 sequences keep their order: a second
-// pass over their lengths costs each of 201 x 8 items more (109 -> 118 us).
-HXA_DEV bool find_block_of(const CachedArgs &p, int q, int lane, Work &w) {
-  const int rb = 1 << p.rb_log;
-  Lanes s;
-  s.load(p, 0, lane);
-  const bool whole = p.c.nseq <= 64 && __any(s.n * p.G >= rb);
-  int seen = 0;
-  for (int rest = whole ? 0 : 1; rest < 2; rest++) {
-    for (int base = 0; base < p.c.nseq; base += 64) {
-      if (base > 0) s.load(p, base, lane);
-      const int full = whole ? s.nb - ((s.n * p.G & (rb - 1)) != 0) : 0;
-      const int cnt = rest ? s.nb - full : full, inc = wave_scan_i(cnt);
-      const uint64_t hit = __ballot(seen + inc > q);
-      if (!hit) {
-        seen += __builtin_amdgcn_readlane(inc, 63);
-        continue;
-      }
-      const int l = __builtin_ctzll(hit);
-      take(w, s, l, base);
-      w.block = q - seen - __builtin_amdgcn_readlane(inc, l) + __builtin_amdgcn_readlane(cnt, l) + (rest ? __builtin_amdgcn_readlane(full, l) : 0);
-      w.t0 = 0;
-      w.t1 = 1 << 24;
-      return true;
-    }
-  }
-  return false;
-}
-// the work at the walk's place; pos < end
-HXA_DEV bool next_work(const CachedArgs &p, Walk &k, Lanes &s, int each, int inc, int lane, int4_t *stash, Work &w) {
-  uint64_t hit;
-  while (!(hit = __ballot(k.seen + inc > k.pos))) {
-    k.seen += __builtin_amdgcn_readlane(inc, 63);
-    k.base += 64;
-    if (k.base >= p.c.nseq) return false;
-    s.load(p, k.base, lane);
-    each = k.eff(s.tiles);
-    inc = wave_scan_i(s.nb * each);
-  }
-  *stash = (int4_t){s.b, s.n, s.len, inc};
-  const int l = __builtin_ctzll(hit), seg = k.own_pieces ? 0 : SEG;
-  take(w, s, l, k.base);
-  const int eff = __builtin_amdgcn_readlane(each, l), nb = __builtin_amdgcn_readlane(s.nb, l);
-  int at = k.pos - (k.seen + __builtin_amdgcn_readlane(inc, l) - nb * eff);
-  w.block = at < eff ? 0 : floor_of(at, eff);
-  at -= w.block * eff;  // the walk's place in the block: 0, or the first of a piece
-  const int stop = k.pos - at + eff;
-  w.slot = p.sp_max + (at == 0 ? 0 : (int)ceil_of(at, k.chunk));
-  w.t0 = max(at - seg, 0);
-  w.t1 = max(min(k.end, stop) - k.pos + at - seg, 0);
-  w.last = stop <= k.end;
-  k.pos = min(k.end, stop);
-  return true;
-}
-// the first work of item `q` of a key head, split
-HXA_DEV bool first_work(const CachedArgs &p, int q, int lane, int4_t *stash, Walk &k, Work &w) {
-  const int pt = p.sp_max ? (p.c.prefix_len + KT - 1) / KT : 0;
-  Lanes s;
-  int own = 0, blocks = 0, longest = 0;
-  for (int base = (p.c.nseq - 1) & ~63; base >= 0; base -= 64) {  // sums below 2^30: checked on the host
-    s.load(p, base, lane);
-    own += __builtin_amdgcn_readlane(wave_scan_i(s.nb * s.tiles), 63);
-    blocks += __any(s.nb > 1) ? __builtin_amdgcn_readlane(wave_scan_i(s.nb), 63) : __popcll(__ballot(s.nb > 0));
-    longest = max(longest, max_all(s.tiles));
-  }
-  // a tile of 128 rows takes about 5/4 of one of 16 (4600 cycles, 3800)
-  const uint32_t pre = (uint32_t)p.np_blocks * pt * 5 / 4;
-  uint32_t chunk = max(ceil_of(own + SEG * blocks + pre, p.budget), (uint32_t)p.least);
-  // no more pieces of a block than slots
-  if (longest + SEG - 1 > (long)chunk * (p.s_max - 1)) chunk = ceil_of(longest + SEG - 1, p.s_max - 1);
-  k.own_pieces = false;
-  const int taken = blocks + p.np_blocks;  // every block has one piece that is not full
-  if (2 * taken <= p.budget) {
-    uint32_t whole = max(ceil_of(own + pre, p.budget - taken), (uint32_t)p.least);
-    if (longest > (long)whole * p.s_max) whole = ceil_of(longest, p.s_max);
-    k.own_pieces = whole < chunk + SEG;
-    if (k.own_pieces) chunk = whole;
-  }
-  if (p.sp_max) {
-    const uint32_t cp = max((chunk * 4 + 4) / 5, ceil_of(pt, p.sp_max));
-    const int ns = (int)ceil_of(pt, cp);
-    if (q < ns * p.np_blocks) {
-      w.shared = true;
-      w.slot = q / p.np_blocks;
-      w.block = q - w.slot * p.np_blocks;
-      w.t0 = w.slot * (int)cp;
-      w.t1 = w.t0 + (int)cp;
-      w.last = w.slot == ns - 1;
-      k.pos = k.end = 0;
-      return true;
-    }
-    q -= ns * p.np_blocks;
-  }
-  const int total = k.own_pieces ? 1 << 30 : own + SEG * blocks;
-  if ((uint64_t)q * chunk >= (uint32_t)total) return false;
-  k.chunk = (int)chunk;
-  k.pos = q * (int)chunk;
-  k.end = min(k.pos + (int)chunk, total);
-  k.base = k.seen = 0;
-  w.shared = false;
-  const int each = k.eff(s.tiles);
-  return next_work(p, k, s, each, wave_scan_i(s.nb * each), lane, stash, w);
-}
-
 template <typename T, int HD>
 HXA_DEV void any_item(int mode, const Keys<T> &s, const Item &it, const CachedArgs &p, int head0, uint8_t *lds, const Out<T> &out) {
   if (mode == 1) {
@@ -1121,12 +893,11 @@ HXA_DEV void any_item(int mode, const Keys<T> &s, const Item &it, const CachedAr
 template <typename T, int HD>
 __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int lane = threadIdx.x & 63;
   const int h = blockIdx.x % p.c.H, q = blockIdx.x / p.c.H, P = p.c.prefix_len;
   Walk k{};
   Work w{};
   int4_t *stash = (int4_t *)(lds + Geo<T, HD>::LDS) + threadIdx.x;  // the lanes' sequences while a block is computed
-  if (p.part == nullptr ? !find_block_of(p, q, lane, w) : !first_work(p, q, lane, stash, k, w)) return;
+  if (p.part == nullptr ? !find_block_of<Wave>(p, q, w) : !first_work<Wave>(p, q, stash, k, w)) return;
   for (;;) {
     Keys<T> s{};
     s.k = (const T *)p.c.k;
@@ -1144,7 +915,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
     it.gm = p.gm;
     int mode, slot_end;
     if (w.shared) {
-      mode = p.np_mode;
+      mode = p.p.np_mode;
       it.r0 = w.block * mode_rows(mode);
       it.nrows = p.T * p.G;
       it.tok0 = 0;
@@ -1152,14 +923,14 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
       it.x1 = min(w.t1 * KT, P);
       it.base = it.cap = it.least = P - 1;
       it.causal = false;
-      slot_end = p.sp_max;
+      slot_end = p.p.sp_max;
     } else {
       const long len = w.len;
       const int held = (int)min(max(len, 0L), (long)p.c.ldt * p.c.page);
       s.table += (long)w.seq * p.c.ldt;
-      it.r0 = w.block << p.rb_log;
+      it.r0 = w.block << p.p.rb_log;
       it.nrows = w.n * p.G;
-      mode = rows_mode(min(it.nrows - it.r0, 1 << p.rb_log));
+      mode = rows_mode(min(it.nrows - it.r0, 1 << p.p.rb_log));
       it.tok0 = w.b;
       // own position of token j: len - n + j; a negative one sees the prefix alone
       it.causal = true;
@@ -1168,9 +939,9 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
       const long base = (long)P + len - w.n;
       it.base = (int)max(min(base, (long)it.cap), (long)P - 1 - w.n);
       const int end = row_limit(it, min(it.r0 + mode_rows(mode), it.nrows) - 1) + 1;
-      it.x0 = p.x_first + w.t0 * KT;
-      it.x1 = (int)min((long)end, p.x_first + (long)w.t1 * KT);
-      slot_end = p.sp_max + p.s_max;
+      it.x0 = p.p.x_first + w.t0 * KT;
+      it.x1 = (int)min((long)end, p.p.x_first + (long)w.t1 * KT);
+      slot_end = p.p.sp_max + p.p.s_max;
     }
     if (p.part != nullptr && w.last) {  // slots that no range fills: sums of nothing
       const int rows = min(mode_rows(mode), it.nrows - it.r0);
@@ -1178,20 +949,14 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
       for (int j = threadIdx.x; j < rows * free; j += 256) {
         int head;
         const int row = j / free, tok = row_tok(it, it.r0 + row, head);
-        p.ml[((long)(it.tok0 + tok) * p.Hq + h * p.G + head) * (p.sp_max + p.s_max) + w.slot + 1 + j - row * free] = (float2_t){-INFINITY, 0.0f};
+        p.ml[((long)(it.tok0 + tok) * p.Hq + h * p.G + head) * (p.p.sp_max + p.p.s_max) + w.slot + 1 + j - row * free] = (float2_t){-INFINITY, 0.0f};
       }
     }
-    const Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, w.slot, p.sp_max + p.s_max, p.Hq};
+    const Out<T> out{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, w.slot, p.p.sp_max + p.p.s_max, p.Hq};
     any_item<T, HD>(mode, s, it, p, h * p.G, lds, out);
     if (k.pos >= k.end) return;
     reads_done_barrier();  // every wave is done with the LDS
-    Lanes y;
-    const int4_t x = *stash;
-    y.b = x[0];
-    y.n = x[1];
-    y.len = x[2];
-    y.sizes(p);
-    if (!next_work(p, k, y, k.eff(y.tiles), x[3], lane, stash, w)) return;
+    if (!further_work<Wave>(p, k, stash, w)) return;
   }
 }
 
@@ -1203,7 +968,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs p) {
   constexpr int E = HD / 64, N = 8;
   typedef float fe __attribute__((ext_vector_type(E)));
-  const int lane = threadIdx.x & 63, nslots = p.sp_max + p.s_max;
+  const int lane = threadIdx.x & 63, nslots = p.p.sp_max + p.p.s_max;
   const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), rows = (uint32_t)p.T * p.Hq;
   if (row >= rows) return;
   const int tok = (int)(row / (uint32_t)p.Hq), head = (int)(row - (uint32_t)tok * p.Hq);
@@ -1284,59 +1049,9 @@ int launched(const char *who) {
 bool rows_ok(const void *p, long ld, int H, int hd) { return p != nullptr && (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld >= (long)H * hd; }
 
 uint32_t recip(int G) { return G == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)G); }
-long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
 // workgroups that run at once
 int wg_slots(int hd) { return causal_ncu() * (hd == 256 ? 1 : 2); }
-
-// The launch of a call over the cache, from sizes that the host knows (T, the table's width, the prefix): how the lengths on
-// the device turn out does not change it, so a captured launch stays right.
-//   Rows a workgroup: 64 where the average sequence has no more, else 128 (at 65 .. 96 rows one workgroup of 128 takes 0.97 us a
-//   tile, two of 64 take 1.26); for what is left of a sequence 16 or 64 where that is enough, which is found on the device (a prompt of 1000
-//   tokens and 63 single ones over 800 each behind 500, 32 / 8 heads: 89 -> 60 us against 128 rows for all).
-//   Shared prefix: where sequences bring at most 16 rows, there are at least two of them and the prefix is worth four tiles. No more
-//   slots than ranges first_work's chunk can make.
-//   Not split where the table and the prefix hold at most 6 tiles of keys, or 16 where the blocks fill a quarter of the places: a second
-//   launch and what the ranges set up take longer than the tiles one after the other (single tokens, 16 / 8 heads of 128, us split, whole: one
-//   sequence of 4 tiles 8.9, 7.4, of 8 9.2, 10.0; 16 of 4 9.6, 7.7, of 8 13.6, 11.1, of 16 19.5, 18.4; 64 of 4 18.2, 14.9, of 16 48.5, 43.1).
-//   Ranges of keys: with few rows as many as run at once, but none that would bring the partials past 1 GB. With more rows a partial
-//   result is as wide as a row's output is in fp32, so keys are split only where the blocks fill less than 5/8 of the places (32 prompts of
-//   75 tokens behind 1000, 16 / 8 heads, 456 blocks of 512 places: split in two 65 us, whole 51).
-struct CachedPlan {
-  int np_mode, np_blocks, sp_max, rb_log, n_blocks, s_max, x_first, budget, least;
-};
-long cached_ws(const CachedPlan &p, const hxa_kv_cache &c, int T, int Hq) {
-  const long slots = p.sp_max + p.s_max;
-  return slots == 1 ? 0 : slots * T * Hq * (c.hd * 4L + 8);
-}
-CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws) {
-  const int G = Hq / c.H;
-  const long RT = (long)T * G, slots = wg_slots(c.hd), P = c.prefix_len, cap = (long)c.ldt * c.page;
-  CachedPlan p{};
-  const int mode = rows_mode(ceil_div(RT, c.nseq));
-  p.rb_log = mode == 4 ? 7 : 6;
-  p.n_blocks = (int)((RT >> p.rb_log) + c.nseq);
-  p.budget = (int)std::max(1L, slots / c.H);
-  p.least = mode == 1 ? 1 : 4;
-  p.s_max = 1;
-  const long blocks = ceil_div(RT, mode_rows(mode)) + c.nseq / 2, most = ceil_div(cap + P, KT);
-  if (!ws || most <= 6) return p;
-  if (mode == 1 && c.nseq >= 2 && P >= 4 * KT) {
-    p.np_mode = rows_mode(RT);
-    p.np_blocks = (int)ceil_div(RT, mode_rows(p.np_mode));
-    p.sp_max = (int)std::min({32L, ceil_div(P, KT), ceil_div(p.budget, p.np_blocks) + 1});
-    p.x_first = (int)P;
-  }
-  // a list that is cut anywhere: a block of so many ranges touches one workgroup more
-  const long tiles = ceil_div(cap + P - p.x_first, KT);
-  if (mode == 1) p.s_max = most <= 16 && blocks * c.H * 4 >= slots && p.sp_max == 0 ? 1 : (int)std::min(31L, tiles);
-  else if (blocks * c.H * 8 < slots * 5) p.s_max = (int)std::min({8L, tiles / p.least, ceil_div(slots, blocks * c.H)});
-  p.s_max = std::max(1, p.s_max);
-  if (p.s_max > 1 || p.sp_max > 0) p.s_max++;
-  while (p.s_max > 2 && cached_ws(p, c, T, Hq) > 1L << 30) p.s_max = p.s_max / 2 + 1;
-  if ((p.n_blocks * (tiles + SEG) + ceil_div(P, KT) * p.np_blocks * 2) >= 1L << 29) p.sp_max = p.np_blocks = p.x_first = 0, p.s_max = 1;
-  return p;
-}
 
 }  // namespace
 
@@ -1385,7 +1100,7 @@ static int cached_check(const hxa_kv_cache *c, int T, int Hq) {
 
 extern "C" long hxa_attention_cached_ws_bytes(const hxa_kv_cache *c, int T, int Hq) {
   if (cached_check(c, T, Hq) != HXA_OK || T == 0 || c->nseq == 0) return 0;
-  return cached_ws(cached_plan(*c, T, Hq, true), *c, T, Hq);
+  return cached_ws(cached_plan(*c, T, Hq, true, wg_slots(c->hd)), *c, T, Hq);
 }
 
 extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long ldq, void *o, long ldo, int T, int Hq, float scale, void *ws,
@@ -1397,19 +1112,16 @@ extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long l
   if (!rows_ok(q, ldq, Hq, c->hd) || !rows_ok(o, ldo, Hq, c->hd))
     return hxa_set_error(HXA_E_ARG, "attention_cached: pointers null or not 16-byte aligned, or strides (%ld %ld)", ldq, ldo);
   if ((uintptr_t)ws % 16) return hxa_set_error(HXA_E_ARG, "attention_cached: workspace not aligned");
-  CachedPlan pl = cached_plan(*c, T, Hq, true);
+  CachedPlan pl = cached_plan(*c, T, Hq, true, wg_slots(c->hd));
   const long need = cached_ws(pl, *c, T, Hq);
-  if (need > 0 && (ws == nullptr || ws_bytes < need)) pl = cached_plan(*c, T, Hq, false);
+  if (need > 0 && (ws == nullptr || ws_bytes < need)) pl = cached_plan(*c, T, Hq, false, wg_slots(c->hd));
   const int nslots = pl.sp_max + pl.s_max;
-  CachedArgs p{*c, q, o, ldq, ldo, T, Hq / c->H, Hq, recip(Hq / c->H), recip(c->page), scale * L2E, pl.np_mode, pl.np_blocks, pl.sp_max,
-               pl.rb_log, pl.s_max, pl.x_first, pl.budget, pl.least, nullptr, nullptr};
+  CachedArgs p{{*c, T, Hq / c->H, pl}, q, o, ldq, ldo, Hq, recip(Hq / c->H), recip(c->page), scale * L2E, nullptr, nullptr};
   if (nslots > 1) {
     p.part = (float *)ws;
     p.ml = (float2_t *)(p.part + (long)nslots * T * Hq * c->hd);
   }
-  // split: a range of the prefix for each of its blocks and pieces of the rest, as many as run at once (first_work's chunk is at least all
-  // tiles / budget), and two roundings up
-  const long wgs = (nslots > 1 ? (long)pl.np_blocks + pl.budget + 2 : pl.n_blocks) * c->H;
+  const long wgs = cached_items(pl) * c->H;
   const hipStream_t st = (hipStream_t)stream;
   return by_type(c->dtype, c->hd, [&](auto ty, auto hdc, int id) -> int {
     typedef decltype(ty) T_;

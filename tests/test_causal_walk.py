@@ -1,0 +1,100 @@
+"""Which rows and keys the workgroups of the causal attention kernels take (csrc/causal_walk.h), on the CPU: the kernels' own source with a wave
+of 64 values in an array. Every block of every sequence is taken once, every tile of every block lies in one piece, every piece has a slot
+of its own, and no work lies behind the grid."""
+import ctypes as C
+import os
+import random
+import subprocess
+
+import numpy as np
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("walk") / "walk.so")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-o", so, os.path.join(HERE, "causal_walk_host.cpp")], check=True)
+    lib = C.CDLL(so)
+    lib.host_find_block.restype = lib.host_cached.restype = C.c_long
+    return lib
+
+
+def ints(x):
+    return np.asarray(x, np.int32)
+
+
+def ptr(a):
+    return a.ctypes.data_as(C.c_void_p)
+
+
+def prompts(host, lens, G, RB, first, T=None):
+    """mistakes in the blocks of sequences of these lengths, and each block's place in its sequence (-1: none)"""
+    cu = ints(np.cumsum([0] + list(lens)))
+    T = int(cu[-1]) if T is None else T
+    grid = T * G // RB + len(lens)
+    order = np.empty(max(grid, 1), np.int32)
+    return host.host_find_block(ptr(cu), len(lens), T, G, RB, first, C.c_long(grid), ptr(order)), order[:grid]
+
+
+def parts(r, total, n):
+    """total into n parts, some of them empty"""
+    cut = sorted(r.randint(0, total) for _ in range(n - 1))
+    return [b - a for a, b in zip([0] + cut, cut + [total])]
+
+
+@pytest.mark.parametrize("nseq", [1, 2, 3, 7, 15, 16, 17, 63, 64, 65, 130])
+@pytest.mark.parametrize("RB", [64, 128])
+def test_every_block_of_prompts_once(host, nseq, RB):
+    r = random.Random(nseq * RB)
+    for total in [0, 1, RB - 1, RB, RB + 1, 63 * RB, 64 * RB, 64 * RB + 1, 65 * RB, 300 * RB, 1000 * RB + 7, 4000 * RB - 5] + [
+            r.randint(1, 3000 * RB) for _ in range(10)]:
+        G = r.choice([1, 2, 5, 8])
+        lens = parts(r, total // G, nseq)
+        for first in (256 // r.choice([1, 2, 8, 12]), 1):
+            bad, _ = prompts(host, lens, G, RB, first)
+            assert bad == 0, (lens, G, RB, first)
+
+
+def test_prompts_past_the_rows(host):
+    """entries of cu past T count as T"""
+    for lens in ([100, 200], [50] * 20, [10] * 70):
+        for T in (0, 60, 299):
+            assert prompts(host, lens, 3, 64, 32, T)[0] == 0
+
+
+def cached(host, hd, Hq, H, new, length, page, ldt, prefix, ws=1, places=None, rcp=0):
+    """mistakes in a key head's items over the cache, and the host's plan"""
+    cu, ln = ints(np.cumsum([0] + list(new))), ints(length)
+    plan = np.zeros(9, np.int32)
+    bad = host.host_cached(hd, Hq, H, int(cu[-1]), len(new), ptr(cu), ptr(ln), page, ldt, prefix, ws,
+                           C.c_long(places or (256 if hd == 256 else 512)), rcp, ptr(plan))
+    names = ("np_mode", "np_blocks", "sp_max", "rb_log", "s_max", "x_first", "budget", "least", "n_blocks")
+    return bad, dict(zip(names, plan.tolist()))
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_every_tile_over_the_cache_once(host, seed):
+    """batches of one to many tokens a sequence, short and long, with and without a prefix; reciprocals rounded either way"""
+    r = random.Random(seed)
+    split = shared = 0
+    for _ in range(120):
+        nseq = r.choice([1, 2, 3, 16, 17, 63, 64, 65, 128, 200])
+        hd, H = r.choice([64, 128, 256]), r.choice([1, 2, 3, 4, 8, 12, 40, 64, 128])
+        G, page = r.choice([1, 2, 4, 5, 8]), r.choice([1, 7, 16, 64, 128])
+        kind = r.random()
+        new = [1] * nseq if kind < 0.4 else [r.choice([0, 1, 2, 5, 40, 129, 400]) for _ in range(nseq)] if kind < 0.8 else parts(r, r.randint(1, 2000), nseq)
+        if sum(new) == 0:
+            new[0] = 1
+        most = r.choice([10, 300, 4000, 60000])
+        length = [n + r.randint(0, most) if r.random() < 0.9 else r.choice([-5, 0, 10 ** 9]) for n in new]
+        ldt = -(-max([1] + [x for x in length if x < 10 ** 9]) // page) + r.randint(0, 3)
+        prefix = r.choice([0, 0, r.randint(1, 300), r.randint(256, 40000)])
+        ws = r.random() < 0.8
+        for rcp in (-1, 0, 1):
+            bad, plan = cached(host, hd, G * H, H, new, length, page, ldt, prefix, ws, rcp=rcp)
+            assert bad == 0, (hd, G, H, new, length, page, ldt, prefix, ws, rcp, plan)
+        split += plan["s_max"] > 1
+        shared += plan["sp_max"] > 0
+    assert split > 20 and shared > 5
