@@ -49,7 +49,8 @@ HXA_ANY Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int
       w = 0;
       j = total - 1 - blk;
       if (nseq > 1) {
-        // S(L) = number of blocks at places >= L, 64 values of L a step; the block's place j has S(j + 1) <= blk < S(j)
+        // S(L) = number of blocks at places >= L, 64 values of L a step; the block's place j has S(j + 1) <= blk < S(j). Throughout
+        // S(lo) > blk >= S(hi) = s_hi; the last step of a round may reach past hi, whose S then stays.
         int lo = 0, hi = total, s_hi = 0;
         while (hi - lo > 1) {
           const int step = (hi - lo + 63) >> 6;
@@ -60,9 +61,11 @@ HXA_ANY Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int
             s = W::map([&](int x, int at) { return x + imax(n - at, 0); }, s, L);
           }
           const int k = __builtin_popcountll(W::ballot([&](int x) { return x > blk; }, s));
-          s_hi = W::get(s, imin(k, 63));
           lo += k * step;
-          hi = imin(lo + step, hi);
+          if (lo + step <= hi) {  // (so k < 64: the last L is hi at least, where S <= blk)
+            hi = lo + step;
+            s_hi = W::get(s, k);
+          }
         }
         j = lo;
         uint64_t at = W::ballot([&](int n) { return n > j; }, nb);

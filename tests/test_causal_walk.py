@@ -57,6 +57,18 @@ def test_every_block_of_prompts_once(host, nseq, RB):
             assert bad == 0, (lens, G, RB, first)
 
 
+@pytest.mark.parametrize("nseq", [2, 3, 5, 8, 16])
+def test_every_block_of_long_batches_once(host, nseq):
+    """more blocks than one round of the place search tells apart (64), and than two do (4096), on both sides of the borders"""
+    r = random.Random(nseq)
+    for total in (64, 65, 4095, 4096, 4097, 64 * 65 - 1, 64 * 65, 64 * 65 + 1, 5000, 8192, 9999):
+        even = [total // nseq + (i < total % nseq) for i in range(nseq)]
+        for blocks in (even, [total - 2 * (nseq - 1)] + [2] * (nseq - 1), parts(r, total, nseq), parts(r, total, nseq)):
+            for first in (256, 32, 1):
+                bad, _ = prompts(host, [64 * b - (b > 1) for b in blocks], 1, 64, first)
+                assert bad == 0, (blocks, first)
+
+
 def test_prompts_past_the_rows(host):
     """entries of cu past T count as T"""
     for lens in ([100, 200], [50] * 20, [10] * 70):
