@@ -122,13 +122,10 @@ struct CachedWork {
 HXA_ANY int mode_rows(int mode) { return mode == 1 ? 16 : 32 * mode; }
 HXA_ANY int rows_mode(long rows) { return rows <= 16 ? 1 : rows <= 64 ? 2 : 4; }
 
-// x / d rounded up, at most 2^24 (more tiles than a range has); below 2^24 the product with the reciprocal is off by one at most
+// x / d rounded up; below 2^24 the product with the reciprocal is off by one at most
 template <class W>
 HXA_ANY uint32_t ceil_of(uint32_t x, uint32_t d) {
-  if (x >= 1u << 24) {
-    const uint32_t y = (x - 1) / d + 1;
-    return y < 1u << 24 ? y : 1u << 24;
-  }
+  if (x >= 1u << 24) return (x - 1) / d + 1;
   uint32_t y = (uint32_t)((float)x * W::rcp((float)d));
   const int left = (int)(x - y * d);
   if (left > 0) y += left > (int)d ? 2 : 1;
@@ -354,7 +351,9 @@ inline CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws, lon
   p.s_max = imax(1, p.s_max);
   if (p.s_max > 1 || p.sp_max > 0) p.s_max++;
   while (p.s_max > 2 && cached_ws(p, c, T, Hq) > 1L << 30) p.s_max = p.s_max / 2 + 1;
-  if ((p.n_blocks * (tiles + SEG) + ceil_div(P, KT) * p.np_blocks * 2) >= 1L << 29) p.sp_max = p.np_blocks = p.x_first = 0, p.s_max = 1;
+  // a piece stays below 2^24 tiles (all tiles / half the budget at the most), so that its keys are counted in 31 bits, and the list below 2^29
+  const long list = p.n_blocks * (tiles + SEG) + ceil_div(P, KT) * p.np_blocks * 2;
+  if (list >= least(1L << 29, (long)p.budget << 23)) p.sp_max = p.np_blocks = p.x_first = 0, p.s_max = 1;
   return p;
 }
 // workgroups a key head. Split: a range of the prefix for each of its blocks and pieces of the rest, as many as run at once (first_work's

@@ -134,6 +134,7 @@ extern "C" long host_cached(int hd, int Hq, int H, int T, int nseq, const int *c
   auto piece = [&](Own &o, const Work &w, int slot0, int slots, const char *what) {
     EXPECT(!o.last, "%s block %d: work behind its last", what, w.block);
     EXPECT(w.slot == slot0 + o.slot && o.slot < slots, "%s block %d: slot %d, %d before", what, w.block, w.slot, o.slot);
+    EXPECT((long)w.t1 * KT <= 0x7fffffff, "%s block %d: %d tiles", what, w.block, w.t1);
     EXPECT(w.t0 == o.t && w.t1 >= w.t0, "%s block %d: tiles %d .. %d behind %d", what, w.block, w.t0, w.t1, o.t);
     o.slot++;
     o.t = w.t1;

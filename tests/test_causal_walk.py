@@ -110,3 +110,24 @@ def test_every_tile_over_the_cache_once(host, seed):
         split += plan["s_max"] > 1
         shared += plan["sp_max"] > 0
     assert split > 20 and shared > 5
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_pieces_of_very_long_lists_fit_the_grid(host, seed):
+    """few places a key head and tiles by the hundred million: whatever the plan, its items cover them"""
+    r = random.Random(100 + seed)
+    todo = [(256, 64, 1, 2048, 50000, 0), (256, 256, 4, 100, 400000, 0), (128, 512, 1, 31, 2 ** 20, 10 ** 6), (64, 64, 2, 2, 2 ** 24 - 1, 0),
+            (128, 4, 1, 2, 1, 2 ** 30 - 65), (64, 8, 1, 31, 2 ** 24 - 2 ** 23, 2 ** 29 - 64)]
+    for _ in range(60):
+        tiles = int(2 ** r.uniform(10, 24)) - 1
+        todo.append((r.choice([64, 128, 256]), r.choice([1, 8, 64, 256, 512, 2048]), r.choice([1, 3, 8]), r.choice([1, 2, 40, 300, 3000]), max(tiles, 1),
+                     r.choice([0, r.randint(256, 2 ** 30 - 64 * tiles - 65) if 2 ** 30 - 64 * tiles > 400 else 0])))
+    sizes = []
+    for hd, H, G, nseq, tiles, prefix in todo:
+        new = [r.choice([1, 1, 1, 3]) for _ in range(nseq)]
+        for length in ([64 * tiles] * nseq, [r.randint(n, max(64 * tiles, n)) for n in new]):
+            for rcp in (-1, 1):
+                bad, plan = cached(host, hd, G * H, H, new, length, 64, tiles, prefix, rcp=rcp)
+                assert bad == 0, (hd, H, G, nseq, tiles, prefix, rcp, plan)
+        sizes.append((plan["s_max"] > 1, plan["n_blocks"] * tiles / plan["budget"]))
+    assert any(x and n > 2 ** 21 for x, n in sizes) and any(not x and n > 2 ** 24 for x, n in sizes)
