@@ -551,6 +551,19 @@ struct Out {
   int slot, nslots, Hq;
 };
 
+HXA_DEV bool is_minus_0(float x) { return __builtin_bit_cast(uint32_t, x) == 0x80000000u; }
+
+// whether an accumulator of the lanes `mask`, which hold a row together, is NaN
+template <typename A, int N>
+HXA_DEV bool zero_times_bad(const A (&acc)[N], uint64_t mask) {
+  bool bad = false;
+#pragma unroll
+  for (int d = 0; d < N; d++)
+#pragma unroll
+    for (int e = 0; e < (int)(sizeof(A) / 4); e++) bad |= acc[d][e] != acc[d][e];
+  return (__ballot(bad) & mask) != 0;
+}
+
 // rows mode: the wave's accumulators to their rows
 template <typename T, int HD, int W>
 HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uint8_t *lds, float16_t (&acc)[HD / 32], float m, float l) {
@@ -566,8 +579,11 @@ HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uin
     int rest;
     const int tok = row_tok(it, R, rest);
     const long row = (long)(it.tok0 + tok) * out.Hq + head0 + rest;
-    if (g == 0) out.ml[row * out.nslots + out.slot] = (float2_t){m == -INFINITY ? m : m * c, l};
-    if (l == 0.0f) return;  // (l is NaN where a score is: written)
+    // a sum of 0: scores of -infinity alone (NaN scores give NaN). Their values weigh nothing, but 0 times one that is not finite is NaN: such
+    // a partial is kept, under a sum of -0
+    const bool kept = l == 0.0f && zero_times_bad(acc, 0x100000001ull << ql);
+    if (g == 0) out.ml[row * out.nslots + out.slot] = (float2_t){m == -INFINITY ? m : m * c, kept ? -0.0f : l};
+    if (l == 0.0f && !kept) return;
     float *p = out.part + (out.slot * out.rows + row) * HD;
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
@@ -584,6 +600,10 @@ HXA_DEV void rows_out(const Out<T> &out, const Item &it, int head0, float c, uin
   auto sw = [](int r) { return HD == 64 ? (r >> 1) & 7 : r & 15; };
   uint8_t *stage = lds + rw * 32 * RB;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (l == 0.0f) {  // no key, or scores of -infinity alone: zeros, whatever the values
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++) acc[d] = (float16_t){};
+  }
 #pragma unroll
   for (int d = 0; d < HD / 32; d++)
 #pragma unroll
@@ -735,17 +755,21 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
   float2_t *mlx = (float2_t *)(lds + ND * 4 * 1024);  // [wave][row]
 #pragma unroll
   for (int d = 0; d < ND; d++) ox[(wave * ND + d) * 64 + lane] = acc[d];
-  if (gi == 0) mlx[wave * 16 + ql] = (float2_t){mrun, lsum};
+  // a sum of -0: as in rows_out
+  const bool bad = lsum == 0.0f && zero_times_bad(acc, 0x1000100010001ull << ql);
+  if (gi == 0) mlx[wave * 16 + ql] = (float2_t){mrun, bad ? -0.0f : lsum};
   reads_done_barrier();
   float m = -INFINITY, l = 0.0f, a[4];
 #pragma unroll
   for (int w = 0; w < 4; w++) m = fmaxf(m, mlx[w * 16 + ql][0]);
   const float mz = m == -INFINITY ? 0.0f : m;
+  bool kept = false;
 #pragma unroll
   for (int w = 0; w < 4; w++) {
     const float2_t x = mlx[w * 16 + ql];
     a[w] = __builtin_amdgcn_exp2f((x[0] - mz) * c);
     l += x[1] * a[w];
+    kept |= is_minus_0(x[1]);
   }
   if (R >= it.nrows) return;
   int rest;
@@ -753,8 +777,8 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
   const int head = head0 + rest;
   const long row = tok * out.Hq + head, at = out.slot * out.rows + row;
   if (out.part != nullptr) {
-    if (wave == 0 && gi == 0) out.ml[row * out.nslots + out.slot] = (float2_t){m == -INFINITY ? m : m * c, l};
-    if (l == 0.0f) return;
+    if (wave == 0 && gi == 0) out.ml[row * out.nslots + out.slot] = (float2_t){m == -INFINITY ? m : m * c, l == 0.0f && kept ? -0.0f : l};
+    if (l == 0.0f && !kept) return;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -772,7 +796,7 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
     } else {
       v4 x;
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = (T)(o[e] * inv);
+      for (int e = 0; e < 4; e++) x[e] = l == 0.0f ? (T)0.0f : (T)(o[e] * inv);
       *(v4 *)(out.o + tok * out.ldo + (long)head * HD + 16 * d + 4 * gi) = x;
     }
   }
@@ -962,7 +986,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_kernel(CachedArgs p) {
 
 // The partials of a row joined by a wave: lane s has the maximum and the sum of slot s (at most 64 of them), which give its weight
 // 2^(m_s - m); then HD / 64 dims a lane over the slots that saw a key, eight of them in flight; one division, one rounding. A slot whose
-// sum is 0 saw none and holds no values. (64 tokens of 32 heads with 32 + 24 slots, a third of them used: 5 us; with the slots'
+// sum is +0 saw none and holds no values; one whose sum is -0 holds NaN where it has weights of 0 on values that are not finite. (64 tokens of 32 heads with 32 + 24 slots, a third of them used: 5 us; with the slots'
 // sums strided by rows and shared by 8 groups of lanes 8.8.)
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs p) {
@@ -979,7 +1003,7 @@ __global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs p) {
   for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
   const float w = x[1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x[0] - (m == -INFINITY ? 0.0f : m));
   const float l = wave_sum(x[1] * w);
-  uint64_t left = __ballot(x[1] != 0.0f);
+  uint64_t left = __ballot(x[1] != 0.0f || is_minus_0(x[1]));
   fe o = {};
   while (left) {
     fe y[N];
@@ -1004,7 +1028,7 @@ __global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs p) {
   typedef T te __attribute__((ext_vector_type(E)));
   te z;
 #pragma unroll
-  for (int e = 0; e < E; e++) z[e] = (T)(o[e] * inv);
+  for (int e = 0; e < E; e++) z[e] = l == 0.0f ? (T)0.0f : (T)(o[e] * inv);
   *(te *)((T *)p.o + tok * p.ldo + (long)head * HD + E * lane) = z;
 }
 

@@ -302,13 +302,14 @@ int hxa_kv_append(const hxa_kv_cache *c, const void *k, long ldk, const void *v,
                   const hxa_rope *rope, void *stream);
 /* Causal attention over packed sequences: o[t] = softmax over the rows s <= t of t's own sequence of scale q[t] . k[s], times v[s];
  * query head h reads key head h / (Hq / Hk) (Hq % Hk == 0). scale > 0. q, k, v, o [T][ld.]; ldk, ldv < 2^24. What the mask
- * hides has no part in a row, infinities and NaN included; a row whose scores are all -infinity gets zeros. o overlaps none of q, k, v. T * Hq < 2^30, and fewer than 2^24 workgroups:
+ * hides has no part in a row, infinities and NaN included. A row whose scores are all -infinity gets zeros, whatever the values; beside
+ * finite scores such a key adds 0 times its value (NaN where that is not finite). o overlaps none of q, k, v. T * Hq < 2^30, and fewer than 2^24 workgroups:
  * (T Hq / Hk / 128 + nseq) Hk (64 for 128 where that is below the places on the chip). */
 int hxa_attention_causal(int dtype, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, void *o,
                          long ldo, int T, const int *cu, int nseq, int Hq, int Hk, int hd, float scale, void *stream);
 /* Attention of the new tokens over the cache: the query at own position p sees the whole prefix and the own positions 0 .. p
  * that the cache holds (so append first). Keys of a page that is not in [0, npages) are left out; a query that sees no key, or
- * only scores of -infinity, gets zeros. q, o [T][ld.] of Hq heads (a multiple of c->H). ws: hxa_attention_cached_ws_bytes(c, T, Hq) bytes, 16-byte aligned, for
+ * only scores of -infinity, gets zeros, as in hxa_attention_causal. q, o [T][ld.] of Hq heads (a multiple of c->H). ws: hxa_attention_cached_ws_bytes(c, T, Hq) bytes, 16-byte aligned, for
  * the partial results where the keys of few rows are split over the chip and where the prefix is read once for the whole batch; NULL or
  * fewer bytes: one launch that splits nothing. The sums' order depends on the form, not on a run. Calls that
  * share ws must not overlap in time, graphs' replays included; o overlaps neither q, the pools nor ws. T * Hq < 2^30, and

@@ -2,8 +2,8 @@
 import numpy as np
 import pytest
 
-from tests._causal import BF16, F16, Packed, close
-from tests.test_gpu_causal import expect_causal, hip, run_causal, say  # noqa: F401 (hip is a fixture)
+from tests._causal import BF16, F16, Cache, Packed, attend_bound, close, narrow
+from tests.test_gpu_causal import expect_causal, hip, queries, run_cached, run_causal, say  # noqa: F401 (hip is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -16,3 +16,59 @@ def test_more_than_4096_blocks_a_key_head(hip, dtype, Hq, lens):
     b = Packed(hip, np.random.default_rng(Hq), lens, Hq, 1, 64, dtype)
     want, bound = expect_causal(b, 0.125)
     close(run_causal(hip, b, 0.125), want, bound, "many blocks")
+
+
+def bits(x, dtype):
+    return narrow(np.float32(x), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,Hq,Hk", [(64, 3, 1), (128, 4, 2), (256, 2, 1), (64, 256, 256), (128, 128, 128), (256, 64, 64)])
+def test_scores_of_minus_infinity_over_values_that_are_not_finite(hip, dtype, hd, Hq, Hk):
+    """a row whose scores are all -infinity is zeros, whatever the values; beside finite scores such a key adds 0 times its value"""
+    say("-inf", dtype, hd, Hq, Hk)
+    n = 150
+    b = Packed(hip, np.random.default_rng(3), [n, 70], Hq, Hk, hd, dtype)
+    b.q[:b.n, np.arange(Hq) * hd] = bits(-1, dtype)
+    b.k[:100, np.arange(Hk) * hd] = bits(np.inf, dtype)
+    b.v[5, 3], b.v[50, 7], b.v[90, hd - 1] = bits(np.inf, dtype), bits(np.nan, dtype), bits(-np.inf, dtype)
+    want, bound = expect_causal(b, hd ** -0.5)
+    want[:100], bound[:100] = 0, 0
+    got = run_causal(hip, b, hd ** -0.5)
+    close(got, want, bound, "-inf")
+    assert np.isnan(want[100:n, 0][:, [3, 7, hd - 1]]).all() and np.isfinite(want[100:n, 0, 0]).all()
+
+
+MINUS_INF = [  # hd, Hq, H, new, past, prefix: partial results of 16 rows; of 64 and 128 rows over a shared prefix; of 64 rows
+    (128, 16, 8, [1, 1], [1500, 700], 0), (64, 4, 1, [1, 2], [1500, 700], 0), (256, 4, 2, [1, 1], [1500, 700], 300),
+    (128, 8, 2, [1] * 8, [100, 300] * 4, 1000), (64, 8, 2, [1] * 40, [100, 300] * 20, 515), (256, 6, 2, [1] * 50, [100, 30] * 25, 400),
+    (128, 4, 2, [20, 30], [1500, 200], 0), (256, 2, 1, [40, 30], [700, 200], 100), (128, 128, 128, [150, 130], [300, 20], 0)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix", MINUS_INF)
+def test_cached_scores_of_minus_infinity_over_values_that_are_not_finite(hip, dtype, hd, Hq, H, new, past, prefix):
+    """the same over the cache, and the same with and without a workspace: the prefix and the older half of each sequence score -infinity; then
+    everything does"""
+    say("cached -inf", dtype, hd, Hq, H, prefix)
+    page = 16
+    for all_keys in (False, True):
+        c = Cache(hip, np.random.default_rng(7), new, past, prefix, page, H, hd, dtype)
+        q = queries(np.random.default_rng(8), sum(new), Hq, hd, dtype)
+        q[:, :, 0] = -1
+        c.k[c.prefix, :, :, 0] = bits(np.inf, dtype)
+        c.v[c.prefix[3:4], 0, 2, 9] = bits(np.inf, dtype)
+        for i, n in enumerate(c.lens):
+            for t in range(n if all_keys else past[i] // 2):
+                c.k[c.table[i, t // page], :, t % page, 0] = bits(np.inf, dtype)
+            c.v[c.table[i, 0], 0, 1, 4] = bits([np.inf, np.nan][i % 2], dtype)
+        scale = hd ** -0.5
+        o, a, m, smax, vmax = c.expect(q, scale)
+        bound = attend_bound(o, a, vmax, m, hd, smax, dtype)
+        if all_keys:
+            o[:], bound[:] = 0, 0
+        else:
+            assert np.isnan(o[:, 0, 4]).all() and np.isfinite(o[:, 0, 0]).all() and (prefix == 0 or np.isnan(o[:, 0, 9]).all())
+        for ws in (True, False):
+            got, nb = run_cached(hip, c, q, scale, ws)
+            close(got, o, bound, f"all={all_keys} ws={ws}")
