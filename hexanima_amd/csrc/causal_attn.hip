@@ -7,7 +7,8 @@
 //
 // Online softmax: over 64-key tiles S = K Q^T, p = 2^(c S - c m) with c = scale log2(e) and the running maximum m, l += p,
 // O^T = V^T P^T. O and l are rescaled only when m grows by more than 5.5 nats (p <= e^5.5 otherwise, well within fp16).
-// p is rounded to the input type, as the matrix product takes it; S, m, l and O stay in fp32.
+// p is rounded to the input type, as the matrix product takes it, and l adds it as rounded: equal values come out as they are, and a
+// weight's rounding costs at most half a step of it on |v - o|. S, m, l and O stay in fp32.
 //
 // Tiles move global -> LDS directly, rows of K and V as they lie in memory, double buffered, one barrier a tile. V is transposed
 // on its way out of LDS (ds_read_b64_tr_b16: 16 lanes that read 4 keys x 16 dims get 4 keys of one dim each), so no
@@ -707,10 +708,11 @@ HXA_DEV void few_item(const Keys<T> &s, const Item &it, const T *q, long ldq, in
       const float mb = mrun == -INFINITY ? 0.0f : mrun * c;
       v4 pf;
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(S[r], c, -mb));
-        pf[r] = (T)p;
-        lsum += p;
+      for (int r = 0; r < 4; r += 2) {
+        const typename HxaVec<T>::v2 h = {(T)__builtin_amdgcn_exp2f(fmaf(S[r], c, -mb)), (T)__builtin_amdgcn_exp2f(fmaf(S[r + 1], c, -mb))};
+        pf[r] = h[0];
+        pf[r + 1] = h[1];
+        lsum = sum2(h, lsum);
       }
 #pragma unroll
       for (int d = 0; d < ND; d++) {

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from tests._causal import BF16, F16, Cache, Packed, attend_bound, close, narrow
+from tests._causal import BF16, F16, Cache, Packed, attend_bound, close, narrow, widen
 from tests.test_gpu_causal import expect_causal, hip, queries, run_cached, run_causal, say  # noqa: F401 (hip is a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +72,54 @@ def test_cached_scores_of_minus_infinity_over_values_that_are_not_finite(hip, dt
         for ws in (True, False):
             got, nb = run_cached(hip, c, q, scale, ws)
             close(got, o, bound, f"all={all_keys} ws={ws}")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,Hq,H", [(64, 16, 8), (128, 16, 16), (256, 8, 2), (128, 64, 2)])
+def test_equal_values_come_out_as_they_are(hip, dtype, hd, Hq, H):
+    """the weights' sum is that of the weights as they are multiplied: rounded alike, they cancel. 64 scores of 0, then 64 of up to 5.4 (below the
+    growth that rescales, so weights are not near 1), over one value just below 2, where half a step of the result is half of what
+    a weight's rounding may be: the sums are off by 128 2^-24 of it, so every result is the value"""
+    say("equal values", dtype, hd, Hq, H)
+    v = bits(2, dtype) - 1
+    rng = np.random.default_rng(hd)
+    B = 12
+    q = np.zeros((B, Hq, hd))
+    q[:, :, 0] = rng.uniform(3.0, 5.4, (B, Hq))
+    q = widen(narrow(q, dtype), dtype)
+    c = Cache(hip, rng, [1] * B, [127] * B, 0, 16, H, hd, dtype)
+    c.k[:] = 0
+    for i in range(B):
+        c.k[c.table[i, 4:8], :, :, 0] = bits(1, dtype)
+        c.v[c.table[i, :8]] = v
+    for ws in (True, False):
+        got, _ = run_cached(hip, c, q, 1.0, ws)
+        assert (got == widen(np.uint16(v), dtype)).all(), (ws, np.unique(got))
+    b = Packed(hip, rng, [128], Hq, H, hd, dtype)
+    b.q[:b.n, :Hq * hd], b.k[:b.n, :H * hd], b.v[:b.n, :H * hd] = 0, 0, v
+    b.q[:b.n, np.arange(Hq) * hd] = narrow(rng.uniform(3.0, 5.4, (b.n, Hq)), dtype)
+    b.k[64:128, np.arange(H) * hd] = bits(1, dtype)
+    assert (run_causal(hip, b, 1.0) == widen(np.uint16(v), dtype)).all()
+
+
+@pytest.mark.parametrize("hd,Hq,H", [(64, 2, 1), (128, 4, 2), (256, 2, 1)])
+def test_many_small_weights_count(hip, hd, Hq, H):
+    """weights of 2^-15 (subnormal in fp16) beside one of 1: 3000 of them are a tenth of the sum"""
+    say("small weights", hd)
+    n = 3000
+    s = float(15 * np.log(2))
+    b = Packed(hip, np.random.default_rng(1), [n], Hq, H, hd, F16)
+    b.q[:n, :Hq * hd], b.k[:n, :H * hd] = 0, 0
+    b.q[:n, np.arange(Hq) * hd] = bits(s, F16)
+    b.k[0, np.arange(H) * hd] = bits(1, F16)
+    want, bound = expect_causal(b, 1.0)
+    close(run_causal(hip, b, 1.0), want, bound, "causal")
+    c = Cache(hip, np.random.default_rng(2), [1, 2], [n, 100], 0, 16, H, hd, F16)
+    c.k[:] = 0
+    for i in range(2):
+        c.k[c.table[i, 0], :, 0, 0] = bits(1, F16)
+    q = np.zeros((3, Hq, hd))
+    q[:, :, 0] = widen(np.array([bits(s, F16)]), F16)[0]
+    o, a, m, smax, vmax = c.expect(q, 1.0)
+    for ws in (True, False):
+        close(run_cached(hip, c, q, 1.0, ws)[0], o, attend_bound(o, a, vmax, m, hd, smax, F16), f"ws={ws}")
