@@ -1095,7 +1095,7 @@ extern "C" int hxa_attention_causal(int dtype, const void *q, long ldq, const vo
   if (!cu || (uintptr_t)cu % 4) return hxa_set_error(HXA_E_ARG, "attention_causal: cu");
   const int G = Hq / Hk;
   const long RT = (long)T * G;
-  CausalArgs p{q, k, v, o, ldq, ldk, ldv, ldo, cu, T, nseq, G, Hk, std::max(1, causal_ncu() / Hk), recip(G), scale * L2E};
+  CausalArgs p{q, k, v, o, ldq, ldk, ldv, ldo, cu, T, nseq, G, Hk, second_layer(hd, causal_ncu(), Hk), recip(G), scale * L2E};
   // 64 rows a workgroup while 128 would leave workgroup places free
   const int mode = (RT / 128 + nseq) * Hk < wg_slots(hd) ? 2 : 4;
   const int rb = mode == 2 ? 64 : 128;

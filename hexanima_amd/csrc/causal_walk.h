@@ -27,10 +27,8 @@ struct Block {
   int first;      // first row (token x G + head) of the block within the sequence; -1: none
 };
 // Block `blk` of the grid: sequence i has ceil(n_i G / RB) blocks, and a block's keys grow with its place in the sequence. Up to 16
-// sequences, places are dealt from the highest down over all of them (the longest first). Two workgroups share a CU: of the second layer (blocks
-// first .. 2 first - 1, `first` = CUs / key heads) the order is reversed, so that the longest block has the shortest of
-// them beside it (4096 tokens, 32 / 8 heads: 149 -> 143 us). More sequences: in their order, each from its end. cu's entries are
-// clamped into [0, T].
+// sequences, places are dealt from the highest down over all of them (the longest first); of blocks first .. 2 first - 1 the order is
+// reversed (second_layer below). More sequences: in their order, each from its end. cu's entries are clamped into [0, T].
 template <class W>
 HXA_ANY Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int RB, int blk, int first) {
   typedef typename W::I I;
@@ -89,6 +87,12 @@ HXA_ANY Block find_block(const int *__restrict__ cu, int nseq, int T, int G, int
   }
   return Block{0, 0, 0, -1};
 }
+
+// The first block of those that share the CUs with the first ones, of the same number. Where two workgroups run on a CU (heads of 64 and 128) it has
+// the shortest of them beside its longest block (heads of 128, 4096 tokens, 32 / 8 heads: 149 -> 143 us). Heads of 256 take a CU for one:
+// their second layer follows the first, longest first as well (2048 tokens, 32 / 8 heads: 95 -> 81 us against
+// the reversed order; 6500, 10 / 2: 252 -> 218; 8192, 16 / 4, five layers: 526, 530), so none of its blocks is reversed.
+inline int second_layer(int hd, int ncu, int Hk) { return hd == 256 ? 1 << 29 : imax(1, ncu / Hk); }
 
 // ---- over the cache ----
 // The keys of a sequence are one list: the prefix (P keys), then its own. The work of a key head, in grid order:

@@ -98,6 +98,8 @@ extern "C" long host_find_block(const int *cu, int nseq, int T, int G, int RB, i
   return g_bad;
 }
 
+extern "C" int host_second_layer(int hd, int ncu, int Hk) { return second_layer(hd, ncu, Hk); }
+
 // The items of a key head over the cache, as the library plans them: every tile of every block in one piece, its pieces in slots of their own,
 // the slots behind the last one filled, the prefix likewise; no work behind the grid. plan (if not null): the host's plan
 extern "C" long host_cached(int hd, int Hq, int H, int T, int nseq, const int *cu, const int *len, int page, int ldt, int prefix_len,

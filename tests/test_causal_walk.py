@@ -69,6 +69,20 @@ def test_every_block_of_long_batches_once(host, nseq):
                 assert bad == 0, (blocks, first)
 
 
+@pytest.mark.parametrize("hd,RB", [(64, 128), (128, 64), (128, 128), (256, 64), (256, 128)])
+@pytest.mark.parametrize("Hk", [1, 2, 8, 12, 300])
+def test_longest_blocks_first_with_a_reversed_layer_only_where_two_share_a_cu(host, hd, RB, Hk):
+    first = host.host_second_layer(hd, 256, Hk)
+    for lens in ([4096], [6500, 300, 1], [900] * 16):
+        bad, order = prompts(host, lens, 4, RB, first)
+        order = order[order >= 0]
+        assert bad == 0
+        if hd != 256:
+            assert first == max(1, 256 // Hk)
+            order[first:2 * first] = order[first:2 * first][::-1].copy()
+        assert (np.diff(order) <= 0).all()
+
+
 def test_prompts_past_the_rows(host):
     """entries of cu past T count as T"""
     for lens in ([100, 200], [50] * 20, [10] * 70):
