@@ -280,7 +280,9 @@ extern "C" int hxa_qk_norm_rope(int dtype, const void *q, long ldq, int Hq, cons
   if (((uintptr_t)gq | (uintptr_t)gk) % 16 || (uintptr_t)pos % 4)
     return hxa_set_error(HXA_E_ARG, "qk_norm_rope: gains or positions not aligned");
   const int groups = (Hq + Hk + 1024 / hd - 1) / (1024 / hd);
-  // one wave a token forms the angles once; few tokens are spread over more waves instead
+  // one wave a token forms the angles once; few tokens are spread over more waves instead, a wave a group of heads (kernel us, one wave a token /
+  // a wave a group: 32 + 8 heads of 128, 256 tokens 6.0 / 4.4, 1024 8.5 / 8.2, 2048 10.9 / 12.2; 10 + 2 of 256, 256 5.0 / 4.1, 1024 6.5 / 6.0, 1031
+  // 6.2 / 6.5, 2048 8.2 / 9.0; two waves a token are within 10% of the better one from 1024 tokens on)
   p.parts = T < 1024 ? groups : 1;
   p.per = (groups + p.parts - 1) / p.parts;
   const long wgs = ((long)T * p.parts + 3) / 4;
