@@ -5,6 +5,8 @@
 
 // rows and heads a call takes: grids of one wave a row and group of heads stay below 2^32 threads
 constexpr int HXA_MAX_ROWS = 1 << 25, HXA_MAX_HEADS = 4096;
+// sequences of a plan: wave_count_le's steps stay below 2^31
+constexpr int HXA_MAX_SEQS = 1 << 30;
 
 typedef __bf16 hxa_b;
 typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));

@@ -221,7 +221,8 @@ int hxa_kv_check(const hxa_kv_cache *c, int T, const char *who) {
   if (!c) return hxa_set_error(HXA_E_ARG, "%s: no cache", who);
   if (c->dtype != HXA_DT_F16 && c->dtype != HXA_DT_BF16) return hxa_set_error(HXA_E_MODE, "%s: dtype %d", who, c->dtype);
   if (c->hd != 64 && c->hd != 128 && c->hd != 256) return hxa_set_error(HXA_E_MODE, "%s: heads of %d", who, c->hd);
-  if (c->H <= 0 || c->H > HXA_MAX_HEADS || T > HXA_MAX_ROWS || c->page <= 0 || c->page > 65536 || c->npages <= 0 || T < 0 || c->nseq < 0 || c->ldt < 0 || c->prefix_len < 0)
+  if (c->H <= 0 || c->H > HXA_MAX_HEADS || T > HXA_MAX_ROWS || c->page <= 0 || c->page > 65536 || c->npages <= 0 || T < 0 || c->nseq < 0 ||
+      c->nseq > HXA_MAX_SEQS || c->ldt < 0 || c->prefix_len < 0)
     return hxa_set_error(HXA_E_ARG, "%s: H=%d page=%d npages=%d T=%d nseq=%d ldt=%d prefix_len=%d", who, c->H, c->page, c->npages, T,
                          c->nseq, c->ldt, c->prefix_len);
   if ((__int128)c->npages * c->H * c->page >= (__int128)1 << 32)

@@ -292,7 +292,7 @@ typedef struct {
   int ldt;           /* entries a sequence; ldt * page + prefix_len < 2^30 */
   const int *len;    /* device [nseq] */
   const int *cu;     /* device [nseq + 1] */
-  int nseq;
+  int nseq;          /* at most 2^30 */
 } hxa_kv_cache;
 /* The new tokens' keys and values into their sequences' own pages: k [T][ldk] with the norm gk (NULL: none) and the rotation rope
  * (NULL: none) at position prefix_len + own position, as hxa_qk_norm_rope, v [T][ldv] as it is. A token whose own position is
