@@ -21,7 +21,8 @@
 //   few rows:     16 rows, 16 keys of the tile to each wave (16x16 MFMAs), joined at the end; bound by reading the cache
 //
 // Bound, and measured (32 query heads on 8 key heads of 128, bf16):
-//   prompts: the matrix instructions, at the board's power limit from ~8000 tokens on (16384 tokens 1.92 ms, 1.15 PFLOP/s); a shorter batch by its
+//   prompts: the matrix instructions, at the board's power limit from ~8000 tokens on (16384 tokens 1.89 - 1.97 ms on five cards, 1.12 - 1.16 PFLOP/s, 2.19
+//            on a sixth); a shorter batch by its
 //            longest block, whose tiles follow each other (a tile of 128 rows 2300 cycles alone, 3050 with two workgroups a CU, of them 1024 MFMAs)
 //   single tokens: reading the keys (16 tokens over 90000 keys behind 32768 shared ones 99 us, 5.1 TB/s; 64 over 30000 behind 4096 40 us)
 // Two workgroups a CU, one's softmax beside the other's matrix products, did better than one that interleaves the tiles' phases itself.

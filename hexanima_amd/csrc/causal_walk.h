@@ -316,12 +316,13 @@ HXA_ANY bool first_work(const CachedWork &p, int q, typename W::Stash stash, Wal
 //   Rows a workgroup: 64 where the average sequence has no more, else 128 (at 65 .. 96 rows one workgroup of 128 takes 0.97 us a
 //   tile, two of 64 take 1.26); for what is left of a sequence 16 or 64 where that is enough, which is found on the device (a prompt of 1000
 //   tokens and 63 single ones over 800 each behind 500, 32 / 8 heads: 89 -> 60 us against 128 rows for all).
-//   Shared prefix: where sequences bring at most 16 rows, there are at least two of them and the prefix is worth four tiles. No more
-//   slots than ranges first_work's chunk can make.
+//   Shared prefix: where sequences bring at most 16 rows on average, there are at least two of them and the prefix is worth four tiles (prompts
+//   read it block by block). No more slots than ranges first_work's chunk can make.
 //   Not split where the table and the prefix hold at most 6 tiles of keys, or 16 where the blocks fill a quarter of the places: a second
 //   launch and what the ranges set up take longer than the tiles one after the other (single tokens, 16 / 8 heads of 128, us split, whole: one
 //   sequence of 4 tiles 8.9, 7.4, of 8 9.2, 10.0; 16 of 4 9.6, 7.7, of 8 13.6, 11.1, of 16 19.5, 18.4; 64 of 4 18.2, 14.9, of 16 48.5, 43.1).
-//   Ranges of keys: with few rows as many as run at once, but none that would bring the partials past 1 GB. With more rows a partial
+//   Ranges of keys: with few rows as many as run at once; where the partials would pass 1 GB fewer, down to two of the own keys beside two of the
+//   prefix (four times T Hq rows in fp32). With more rows a partial
 //   result is as wide as a row's output is in fp32, so keys are split only where the blocks fill less than 5/8 of the places (32 prompts of
 //   75 tokens behind 1000, 16 / 8 heads, 456 blocks of 512 places: split in two 65 us, whole 51).
 inline long cached_ws(const CachedPlan &p, const hxa_kv_cache &c, int T, int Hq) {

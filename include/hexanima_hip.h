@@ -237,7 +237,9 @@ int hxa_rows_to_x32(const float *x, float *tiles, int R, int C, void *stream);
  * ============================================================================================================
  * Rows are tokens; head h of a row is columns [h hd, (h + 1) hd). dtype HXA_DT_F16 or HXA_DT_BF16; hd 64, 128 or 256; row
  * strides in elements, multiples of 8 and at least the row's heads; pointers 16-byte aligned; at most 2^25 rows, 4096 heads. Sums, softmax statistics and
- * angles are held in 32 bits or more and every output is rounded once.
+ * angles are held in 32 bits or more and every output is rounded once. The attention's weights (relative to a row's largest, or up to e^5.5 of one) are
+ * rounded to dtype for their product with the values, and their sum is that of the rounded ones: beside the output's own rounding at most half a
+ * step of dtype of the weighted mean of |v - o|.
  *
  * A batch of sequences is packed: sequence i's tokens are rows cu[i] .. cu[i + 1] - 1 (cu: device, nseq + 1 ascending entries,
  * cu[0] = 0, a sequence may be empty; entries past T count as T). Rows outside every sequence are neither read into a result nor written. cu, len, the page
@@ -260,8 +262,9 @@ typedef struct {
  *   HXA_ROPE_LINEAR every position divided by factor
  *   HXA_ROPE_BASE   base * factor^(rot / (rot - 2)) in the place of base: the slowest pair turns factor times slower, the fastest as before
  *   HXA_ROPE_PARTS  by the turns r = orig_len freq[i] / (2 pi) a pair makes over the trained length: as they are from r = beta_fast on,
- *                   divided by factor up to r = beta_slow, between them mixed by the share of log(r) (as parts of the pair index);
- *                   *mscale = 0.1 ln(factor) + 1
+ *                   divided by factor up to r = beta_slow, between them mixed by the share of log(r), that is linearly in the pair index
+ *                   between the borders' exact places; *mscale = 0.1 ln(factor) + 1. A model that was trained with borders rounded to whole
+ *                   pairs, or with a mix linear in r, has other values between the borders: pass its own frequencies in hxa_rope
  * rot even and at least 2 (BASE: 4), base > 1, factor >= 1; orig_len > 0 and beta_fast > beta_slow > 0 for PARTS. Other modes set
  * *mscale = 1; mscale may be NULL. Computed in 64 bits, each frequency rounded once. */
 #define HXA_ROPE_PLAIN 0
@@ -310,7 +313,8 @@ int hxa_attention_causal(int dtype, const void *q, long ldq, const void *k, long
 /* Attention of the new tokens over the cache: the query at own position p sees the whole prefix and the own positions 0 .. p
  * that the cache holds (so append first). Keys of a page that is not in [0, npages) are left out; a query that sees no key, or
  * only scores of -infinity, gets zeros, as in hxa_attention_causal. q, o [T][ld.] of Hq heads (a multiple of c->H). ws: hxa_attention_cached_ws_bytes(c, T, Hq) bytes, 16-byte aligned, for
- * the partial results where the keys of few rows are split over the chip and where the prefix is read once for the whole batch; NULL or
+ * the partial results where the keys of few rows are split over the chip and where the prefix is read once for each 128 rows of the batch (256 tokens of it or
+ * more, two sequences or more, T Hq / c->H / nseq at most 16); at most 1 GB or 4 T Hq (4 hd + 8) bytes, whichever is more. NULL or
  * fewer bytes: one launch that splits nothing. The sums' order depends on the form, not on a run. Calls that
  * share ws must not overlap in time, graphs' replays included; o overlaps neither q, the pools nor ws. T * Hq < 2^30, and
  * (T Hq / c->H / 64 + nseq) c->H < 2^21. */
