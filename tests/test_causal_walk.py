@@ -90,11 +90,11 @@ def test_prompts_past_the_rows(host):
             assert prompts(host, lens, 3, 64, 32, T)[0] == 0
 
 
-def cached(host, hd, Hq, H, new, length, page, ldt, prefix, ws=1, places=None, rcp=0):
+def cached(host, hd, Hq, H, new, length, page, ldt, prefix, ws=1, places=None, rcp=0, behind=0):
     """mistakes in a key head's items over the cache, and the host's plan"""
     cu, ln = ints(np.cumsum([0] + list(new))), ints(length)
     plan = np.zeros(9, np.int32)
-    bad = host.host_cached(hd, Hq, H, int(cu[-1]), len(new), ptr(cu), ptr(ln), page, ldt, prefix, ws,
+    bad = host.host_cached(hd, Hq, H, int(cu[-1]) + behind, len(new), ptr(cu), ptr(ln), page, ldt, prefix, ws,
                            C.c_long(places or (256 if hd == 256 else 512)), rcp, ptr(plan))
     names = ("np_mode", "np_blocks", "sp_max", "rb_log", "s_max", "x_first", "budget", "least", "n_blocks")
     return bad, dict(zip(names, plan.tolist()))
@@ -145,3 +145,17 @@ def test_pieces_of_very_long_lists_fit_the_grid(host, seed):
                 assert bad == 0, (hd, H, G, nseq, tiles, prefix, rcp, plan)
         sizes.append((plan["s_max"] > 1, plan["n_blocks"] * tiles / plan["budget"]))
     assert any(x and n > 2 ** 21 for x, n in sizes) and any(not x and n > 2 ** 24 for x, n in sizes)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_plans_for_more_rows_than_there_are(host, seed):
+    """a launch captured for a full batch, replayed with fewer tokens, down to none"""
+    r = random.Random(200 + seed)
+    for _ in range(60):
+        nseq, H, G, hd = r.choice([1, 2, 40, 64, 65, 130]), r.choice([1, 2, 8, 40]), r.choice([1, 2, 8]), r.choice([64, 128, 256])
+        new = [r.choice([0, 0, 1, 3]) if r.random() < 0.7 else 0 for _ in range(nseq)] if r.random() < 0.7 else [0] * nseq
+        length = [n + r.randint(0, 3000) for n in new]
+        prefix, behind = r.choice([0, r.randint(256, 9000)]), r.choice([1, nseq, 700])
+        for rcp in (-1, 1):
+            bad, plan = cached(host, hd, G * H, H, new, length, 16, 300, prefix, r.random() < 0.8, rcp=rcp, behind=behind)
+            assert bad == 0, (hd, G, H, new, length, prefix, behind, rcp, plan)
