@@ -51,3 +51,4 @@ HXA_DEV long cache_row(int e, int npages, int H, int h, int page, int r) {
 
 // host side: hxa_kv_cache checks shared by the calls on it (HXA_OK or the error, with its message set)
 int hxa_kv_check(const hxa_kv_cache *c, int T, const char *who);
+int hxa_kv_check_q8(const hxa_kv_cache_q8 *c, int T, const char *who);

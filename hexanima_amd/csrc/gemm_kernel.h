@@ -22,6 +22,7 @@
 //  * The fp16-rounded output tile is staged through LDS for a coalesced epilogue (16-byte loads / stores).
 //  * The block index is remapped so each of the 8 XCDs (own L2) works on a rectangle of output tiles.
 #pragma once
+#include <atomic>
 #include <type_traits>
 
 #include "hxa_common.h"
@@ -203,6 +204,24 @@ HXA_DEV float situ_f(float u, float g) {
   return tu * gs;
 }
 
+// Format of a product of int8 activations and int8 weights (hxa_linear_i8), beside the public weight formats: rows of bytes that the loop moves as it
+// moves fp16, K counted in pairs of them (64 bytes are a "group"), v_mfma_i32_16x16x64_i8 in the place of the fp16 MFMA and int32 sums, which are exact.
+constexpr int HXG_I8 = 3;
+// formats whose W needs no dequantisation
+constexpr bool plain_fmt(int fmt) { return fmt == HXA_W_F16 || fmt == HXG_I8; }
+typedef int int4_t __attribute__((ext_vector_type(4)));
+template <int FMT>
+using acc_t = typename std::conditional<FMT == HXG_I8, int4_t, float4_t>::type;
+HXA_DEV float4_t mma_wa(half8_t w, half8_t a, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(w, a, c, 0, 0, 0); }
+HXA_DEV int4_t mma_wa(half8_t w, half8_t a, int4_t c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4_t, w), __builtin_bit_cast(int4_t, a), c, 0, 0, 0);
+}
+// HXG_I8: out = the sum times a scale of its row and one of its column, plus a bias of the column
+struct GemmParamsI8 : GemmParams {
+  const float *sa, *sw, *bias;
+  int dtype;  // of out
+};
+
 // ---- geometry of a tile's LDS ring ----
 // A stage holds 64 k of the tile (two quantisation groups): BM rows of 128 B of A, BN rows of W (fp16 128 B, int8 64 B,
 // int4 32 B) and the two groups' scale (and offset) vectors. 64 deep, because a row's 128 B is one cache line: 32-deep
@@ -210,10 +229,10 @@ HXA_DEV float situ_f(float u, float g) {
 // every line of A from L2 twice.
 template <int BM, int BN, int FMT>
 struct GemmGeo {
-  static constexpr int RBW = FMT == HXA_W_F16 ? 128 : FMT == HXA_W_Q8 ? 64 : 32;  // W bytes per row per stage
+  static constexpr int RBW = plain_fmt(FMT) ? 128 : FMT == HXA_W_Q8 ? 64 : 32;  // W bytes per row per stage
   static constexpr int A_BYTES = BM * 128;
   static constexpr int W_BYTES = BN * RBW;
-  static constexpr int S_BYTES = FMT == HXA_W_F16 ? 0 : BN * 4;      // one vector: 2 groups x BN fp16
+  static constexpr int S_BYTES = plain_fmt(FMT) ? 0 : BN * 4;      // one vector: 2 groups x BN fp16
   static constexpr int STAGE = A_BYTES + W_BYTES + 2 * S_BYTES;      // scale + optional offset vectors
   static constexpr int CROW = BN + 8;
   static constexpr int C_BYTES = BM * CROW * 2;
@@ -237,8 +256,8 @@ struct GemmGeo {
 // PARTIAL_F32: the K slice's fp32 sums straight from the accumulators (no fp16 rounding, no LDS staging). For block
 // (j, i) the lane holds row mrow + 16 i and columns ncol + 16 j + 0..3: one 16-byte store each, so a wave's store
 // fills 16 rows x 64 contiguous bytes. N % 8 == 0, so a chunk of 4 is inside N or past it.
-template <int MI, int NI>
-HXA_DEV void store_partial_f32(const GemmParams &p, const float4_t (&acc)[NI][MI], int mrow, int ncol, int z) {
+template <int MI, int NI, typename A>
+HXA_DEV void store_partial_f32(const GemmParams &p, const A (&acc)[NI][MI], int mrow, int ncol, int z) {
   float *base = p.out32 + (long)z * p.out_zstride;
 #pragma unroll
   for (int i = 0; i < MI; i++) {
@@ -247,7 +266,7 @@ HXA_DEV void store_partial_f32(const GemmParams &p, const float4_t (&acc)[NI][MI
 #pragma unroll
     for (int j = 0; j < NI; j++) {
       const int n = ncol + j * 16;
-      if (n < p.N) *(float4_t *)(base + (long)m * p.ldo + n) = acc[j][i];
+      if (n < p.N) *(A *)(base + (long)m * p.ldo + n) = acc[j][i];
     }
   }
 }
@@ -261,6 +280,30 @@ HXA_DEV void stage_tile(hxa_h *Cs, const float4_t (&acc)[NI][MI], int ml, int nl
     for (int i = 0; i < MI; i++)
       *(half4_t *)(Cs + (ml + i * 16) * CROW + nl + j * 16) =
           (half4_t){(hxa_h)acc[j][i][0], (hxa_h)acc[j][i][1], (hxa_h)acc[j][i][2], (hxa_h)acc[j][i][3]};
+}
+
+// four sums of a row and four columns to their 16-bit results: the sum, the row's scale, the columns' scales and biases, each in fp32
+template <typename T>
+HXA_DEV uint2_t scale_i8(int4_t s, float sa, float4_t sw, float4_t b) {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  v4 o;
+#pragma unroll
+  for (int e = 0; e < 4; e++) o[e] = (T)fmaf((float)s[e] * sa, sw[e], b[e]);
+  return __builtin_bit_cast(uint2_t, o);
+}
+// HXG_I8: the scaled tile as [BM][CROW] in LDS, as stage_tile
+template <int MI, int NI, int CROW, typename T>
+HXA_DEV void stage_tile_i8(const GemmParamsI8 &p, uint16_t *Cs, const int4_t (&acc)[NI][MI], int m0, int n0, int ml, int nl) {
+  float sa[MI];
+#pragma unroll
+  for (int i = 0; i < MI; i++) sa[i] = p.sa[min(m0 + ml + i * 16, p.M - 1)];
+#pragma unroll
+  for (int j = 0; j < NI; j++) {
+    const int n = min(n0 + nl + j * 16, p.N - 4);  // N % 8 == 0: four columns are inside N or past it
+    const float4_t sw = *(const float4_t *)(p.sw + n), b = p.bias ? *(const float4_t *)(p.bias + n) : (float4_t){};
+#pragma unroll
+    for (int i = 0; i < MI; i++) *(uint2_t *)(Cs + (ml + i * 16) * CROW + nl + j * 16) = scale_i8<T>(acc[j][i], sa[i], sw, b);
+  }
 }
 
 template <int BM, int BN, int NT, bool SPLIT2>
@@ -725,7 +768,7 @@ HXA_DEV void xattn_tail(const GemmParams &p, const float4_t (&acc)[NI][MI], int 
 template <int BM, int BN, int FMT, bool ASYM, bool SPLIT2, int NW, bool XATTN = false>
 HXA_DEV void gemm_body(const GemmParams &p, const int bid, const int z) {
   using G = GemmGeo<BM, BN, FMT>;
-  constexpr bool QW = FMT != HXA_W_F16;
+  constexpr bool QW = !plain_fmt(FMT);
   constexpr int NT = 64 * NW, WNW = NW / 2;
   constexpr int WTM = BM / 2, WTN = BN / WNW, MI = WTM / 16, NI = WTN / 16, NMF = MI * NI;
   constexpr bool DEEP = G::DEEP && !XATTN;
@@ -757,7 +800,7 @@ HXA_DEV void gemm_body(const GemmParams &p, const int bid, const int z) {
   // ---- loader. 1 KB instruction t of a stage: 8 rows of A (t < NA) or 8 / 16 / 32 rows of fp16 / int8 / int4 W, 16
   // bytes per lane, XOR-swizzled so that 16 rows' equal chunks fall in distinct banks. The per-lane
   // offsets from the tile corner are fixed; a stage moves the wave-uniform bases. Rows past M / N clamp to the last.
-  constexpr long ES = FMT == HXA_W_F16 ? 2 : 1;
+  constexpr long ES = plain_fmt(FMT) ? 2 : 1;
   // group (0, 1) of the stage that this lane's chunk of instruction t belongs to
   auto chunk_of = [&](int t, int &row, int &c) {
     if (t < NA) {
@@ -765,7 +808,7 @@ HXA_DEV void gemm_body(const GemmParams &p, const int bid, const int z) {
       c = (lane & 7) ^ ((row >> 1) & 7);
       return c >> 2;
     }
-    if constexpr (FMT == HXA_W_F16) {
+    if constexpr (plain_fmt(FMT)) {
       row = (t - NA) * 8 + (lane >> 3);
       c = (lane & 7) ^ ((row >> 1) & 7);
       return c >> 2;
@@ -788,7 +831,7 @@ HXA_DEV void gemm_body(const GemmParams &p, const int bid, const int z) {
     if (t < NA) off[l] = ((uint32_t)(min(m0 + row, p.M - 1) - m0) * (uint32_t)p.lda + g * 32 + (c & 3) * 8) * 2u;
     else {
       const uint32_t r = (uint32_t)(min(n0 + row, p.N - 1) - n0) * (uint32_t)p.w_rs + g * (uint32_t)p.w_gs;
-      off[l] = FMT == HXA_W_F16 ? (r + (c & 3) * 8) * 2u : FMT == HXA_W_Q8 ? r + (c & 1) * 16 : r;
+      off[l] = plain_fmt(FMT) ? (r + (c & 3) * 8) * 2u : FMT == HXA_W_Q8 ? r + (c & 1) * 16 : r;
     }
   }
   constexpr int CPW = QW ? BN / 4 / NW : 1;  // 16-byte chunks of the scale vectors per wave
@@ -886,11 +929,11 @@ HXA_DEV void gemm_body(const GemmParams &p, const int bid, const int z) {
     }
   };
 
-  float4_t acc[NI][MI];
+  acc_t<FMT> acc[NI][MI];
 #pragma unroll
   for (int j = 0; j < NI; j++)
 #pragma unroll
-    for (int i = 0; i < MI; i++) acc[j][i] = (float4_t){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < MI; i++) acc[j][i] = (acc_t<FMT>){};
 
   // ---- prologue: NS stages in flight (the last one's second half goes out with slice 0 when NS > 2), stage 0 landed
   constexpr int H1 = NS > 2 && !DEEP ? NL / 2 : NL;  // loads of a stage issued right after the barrier; the rest a slice later
@@ -952,7 +995,7 @@ HXA_DEV void gemm_body(const GemmParams &p, const int bid, const int z) {
     for (int q = 0; q < NMF; q++) {
       const int j = q / MI, i = q % MI;
       const half8_t w = fb[QW ? (KS * NI + j) & 1 : KS][QW ? 0 : j];
-      acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, fa[KS][i], acc[j][i], 0, 0, 0);
+      acc[j][i] = mma_wa(w, fa[KS][i], acc[j][i]);
       if constexpr (QW) {
         // raw fragment j of the next stage, once this stage's second slice of it is dequantised
         if (KS == 1 && i == 0) rd_raw(rs, 0, j);
@@ -995,7 +1038,7 @@ HXA_DEV void gemm_body(const GemmParams &p, const int bid, const int z) {
         // fp16: slice 0's blocks, then slice 1's; quantised: both slices of one W fragment after another
         const int j = QW ? q / (2 * MI) : q % NMF / MI, ks = QW ? q % (2 * MI) / MI : q / NMF, i = q % MI;
         const half8_t w = QW ? fb[j & 1][ks] : fb[c][ks * NI + j];
-        acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, fa[c][ks * MI + i], acc[j][i], 0, 0, 0);
+        acc[j][i] = mma_wa(w, fa[c][ks * MI + i], acc[j][i]);
 #pragma unroll
         for (int u = 0; u < RPS; u++) {
           const int x = q * RPS + u;
@@ -1075,6 +1118,23 @@ HXA_DEV void gemm_body(const GemmParams &p, const int bid, const int z) {
     return;
   }
   wait_vm<0>();  // the trailing (dummy) stage loads must land before the epilogue reuses the LDS ring
+  if constexpr (FMT == HXG_I8) {
+    if (p.epi == HXA_EPI_PARTIAL_F32) {  // the slice's int32 sums
+      store_partial_f32<MI, NI>(p, acc, m0 + ml, n0 + nl, z);
+      return;
+    }
+    __syncthreads();
+    const GemmParamsI8 &p8 = static_cast<const GemmParamsI8 &>(p);
+    uint16_t *Cs = (uint16_t *)lds8;
+    if (p8.dtype == HXA_DT_F16) stage_tile_i8<MI, NI, G::CROW, hxa_h>(p8, Cs, acc, m0, n0, ml, nl);
+    else stage_tile_i8<MI, NI, G::CROW, __bf16>(p8, Cs, acc, m0, n0, ml, nl);
+    __syncthreads();
+    for (int c = tid; c < BM * (BN / 8); c += NT) {
+      const int r = c / (BN / 8), n = (c % (BN / 8)) * 8;
+      if (m0 + r < p.M && n0 + n < p.N) *(uint4_t *)(p.out + (long)(m0 + r) * p.ldo + n0 + n) = *(const uint4_t *)(Cs + r * G::CROW + n);
+    }
+    return;
+  } else {
   if constexpr (!SPLIT2) {
     if (p.epi == HXA_EPI_PARTIAL_F32) {  // no LDS staging and no prefetch (gemm_prepare rejects pf with it)
       store_partial_f32<MI, NI>(p, acc, m0 + ml, n0 + nl, z);
@@ -1095,14 +1155,17 @@ HXA_DEV void gemm_body(const GemmParams &p, const int bid, const int z) {
   __syncthreads();
   gemm_epilogue<BM, BN, NT, SPLIT2>(p, Cs, m0, n0, tid, z);
   if (p.pf_bytes > 0) wait_vm<0>();
+  }
 }
 
 // At least two waves per SIMD also for 4-wave kernels, so that the accumulators stay in the 256 directly addressable
 // registers (with 512 the compiler kept them in AGPRs and copied them in and out around the MFMAs: 64x128 at 512 x 2048 x
 // 2048 17.2 -> 13.8 us)
+template <int FMT>
+using params_t = typename std::conditional<FMT == HXG_I8, GemmParamsI8, GemmParams>::type;
 template <int BM, int BN, int FMT, bool ASYM, bool SPLIT2, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void gemm_kernel(GemmParams p) {
-  if constexpr (NW == 8 && !SPLIT2) {
+__global__ __launch_bounds__(64 * NW, 2) void gemm_kernel(params_t<FMT> p) {
+  if constexpr (NW == 8 && !SPLIT2 && FMT != HXG_I8) {
     if ((int)blockIdx.x >= p.tiles_m * p.tiles_n) {  // an appended workgroup: side GEMV rows, no LDS and no barrier
       side_gemv<2>(p.side, (blockIdx.x - p.tiles_m * p.tiles_n) * 8 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
                    p.side_wgs * 8, threadIdx.x & 63);
@@ -1125,23 +1188,32 @@ __global__ __launch_bounds__(64 * NW) void gemm_group_kernel(const GemmParams *_
   gemm_body<BM, BN, FMT, ASYM, false, NW>(ps[blockIdx.y], blockIdx.x, 0);
 }
 
+// more than 64 KB of LDS for a kernel: allowed once a device (done: a bit for each, of the first 64)
+inline hipError_t allow_lds_once(const void *kern, int bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  const hipError_t d = hipGetDevice(&dev);
+  if (d != hipSuccess) return d;
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (done.load() & bit) return hipSuccess;
+  const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) done |= bit;
+  return e;
+}
+
 // ---- launches of one weight format (explicitly instantiated in that format's translation unit) ----
 template <int BM, int BN, int FMT, bool ASYM, bool SPLIT2, int NW>
-hipError_t launch_t(const GemmParams &p, int ksplit, hipStream_t st) {
+hipError_t launch_t(const params_t<FMT> &p, int ksplit, hipStream_t st) {
   auto kern = gemm_kernel<BM, BN, FMT, ASYM, SPLIT2, NW>;
   using G = GemmGeo<BM, BN, FMT>;
   constexpr int base = G::lds(G::NS), lds = SPLIT2 && 2 * G::C_BYTES > base ? 2 * G::C_BYTES : base;
   constexpr int most = !SPLIT2 && G::lds_erf(G::NS) > lds ? G::lds_erf(G::NS) : lds;
   static_assert(most <= 160 * 1024, "LDS");
-  static bool attr = false;
-  if (!attr) {
-    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e != hipSuccess) return e;
-    attr = true;
-  }
+  static std::atomic<uint64_t> attr{0};
+  const hipError_t a = allow_lds_once((const void *)kern, most, attr);
+  if (a != hipSuccess) return a;
   const dim3 grid(p.tiles_m * p.tiles_n + (NW == 8 && !SPLIT2 && ksplit == 1 ? p.side_wgs : 0), 1, ksplit);
   if (!SPLIT2 && p.epi == HXA_EPI_GELU_ERF && p.erf_t2 != nullptr) {  // the T2 table past the staged tile
-    GemmParams pe = p;
+    params_t<FMT> pe = p;
     pe.erf_lds = G::ERF_OFF;
     hxa_launch(kern, grid, dim3(64 * NW), most, st, pe);
   } else {
@@ -1171,11 +1243,11 @@ hipError_t launch_pair_t(const GemmParams &p0, const GemmParams &p1, hipStream_t
 constexpr int tile_nw(int bm, int bn, int fmt) {
   if (bm * bn > 128 * 128) return 8;
   if (bm * bn < 128 * 128 && bn == 64) return 4;
-  return fmt == HXA_W_F16 ? 4 : 8;
+  return plain_fmt(fmt) ? 4 : 8;
 }
 // a single GEMM on tile bm x bn (tile_built says which exist)
 template <int FMT, bool ASYM>
-hipError_t launch_fmt(int bm, int bn, const GemmParams &p, int ksplit, hipStream_t st) {
+hipError_t launch_fmt(int bm, int bn, const params_t<FMT> &p, int ksplit, hipStream_t st) {
 #define HXG_TILE(BM, BN) \
   if (bm == BM && bn == BN) return launch_t<BM, BN, FMT, ASYM, false, tile_nw(BM, BN, FMT)>(p, ksplit, st);
   HXG_TILE(256, 256)
@@ -1222,6 +1294,7 @@ hipError_t launch_group_fmt(const GemmParams *ps, int G, int tiles, hipStream_t 
 }
 hipError_t launch_xattn(const GemmParams &p, hipStream_t st);  // gemm_f16.hip
 hipError_t launch_skinny(int bm, int fmt, bool asym, const GemmParams &p, hipStream_t st);  // gemm_skinny.hip: bm 32, 64
+hipError_t launch_skinny_i8(int bm, const GemmParamsI8 &p, hipStream_t st);                 // gemm_skinny.hip
 
 #define HXG_LAUNCHES(X, FMT, ASYM)                                                                                   \
   X template hipError_t launch_fmt<FMT, ASYM>(int, int, const GemmParams &, int, hipStream_t);                       \

@@ -9,8 +9,8 @@ namespace hxg {
 template <int BM, int FMT>
 struct SkinnyGeo {
   static constexpr int BN = 32, NW = 4;
-  static constexpr int A_BYTES = BM * 128, W_BYTES = BN * (FMT == HXA_W_F16 ? 128 : FMT == HXA_W_Q8 ? 64 : 32);
-  static constexpr int S_BYTES = FMT == HXA_W_F16 ? 0 : BN * 4;
+  static constexpr int A_BYTES = BM * 128, W_BYTES = BN * (plain_fmt(FMT) ? 128 : FMT == HXA_W_Q8 ? 64 : 32);
+  static constexpr int S_BYTES = plain_fmt(FMT) ? 0 : BN * 4;
   static constexpr int STAGE = A_BYTES + W_BYTES + 2 * S_BYTES;
   static constexpr int NS = 160 * 1024 / (NW * STAGE) < 6 ? 160 * 1024 / (NW * STAGE) : 6;
   static constexpr int SROW = BN + 4;  // fp32 row stride of a wave's staged sums (spreads 16 rows' chunks over the banks)
@@ -28,10 +28,10 @@ struct SkinnyGeo {
 // 13.3 -> 7.7 us, 64 x 2048 x 2048 9.8 -> 6.9, 1562 x 3072 x 128 (M x K x N) 20.9 (one launch) -> 10.1, 1562 x 8192 x 128
 // 48.7 (one launch) -> 18.4; fp16 256 x 2048 x 2048 11.9 -> 9.4.
 template <int BM, int FMT, bool ASYM>
-__global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(GemmParams p) {
+__global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(params_t<FMT> p) {
   using G = SkinnyGeo<BM, FMT>;
   constexpr int BN = G::BN, NW = G::NW, NS = G::NS, MI = BM / 16, NI = BN / 16;
-  constexpr bool QW = FMT != HXA_W_F16;
+  constexpr bool QW = !plain_fmt(FMT);
   constexpr int NA = G::A_BYTES / 1024, NL = NA + G::W_BYTES / 1024, L = NL + (QW ? ASYM ? 2 : 1 : 0);
   static_assert(NS >= 3 && NS * L < 64, "ring");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(GemmParams p) {
   const int nt = p.tiles_m * p.tiles_n, x = blockIdx.x & 7, q = nt >> 3, r = nt & 7;
   const int tile = x * q + min(x, r) + (blockIdx.x >> 3);
   int tm, tn;
-  if ((long)p.M * 2 > (long)p.N * (FMT == HXA_W_F16 ? 2 : 1)) {
+  if ((long)p.M * 2 > (long)p.N * (plain_fmt(FMT) ? 2 : 1)) {
     tm = tile / p.tiles_n;
     tn = tile - tm * p.tiles_n;
   } else {
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(GemmParams p) {
 
   // loader: 1 KB instruction l of a stage, 8 rows of A (l < NA) or 8 / 16 / 32 rows of fp16 / int8 / int4 W; rows past M /
   // N clamp to the last
-  constexpr long ES = FMT == HXA_W_F16 ? 2 : 1;
+  constexpr long ES = plain_fmt(FMT) ? 2 : 1;
   uint32_t off[NL], soff = 0;
 #pragma unroll
   for (int l = 0; l < NL; l++) {
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(GemmParams p) {
       off[l] = ((uint32_t)(min(m0 + row, p.M - 1) - m0) * (uint32_t)p.lda + c * 8) * 2u;
     } else {
       int row, g, c;  // row, k group of the stage, 16-byte chunk of the group
-      if constexpr (FMT == HXA_W_F16) {
+      if constexpr (plain_fmt(FMT)) {
         row = (l - NA) * 8 + (lane >> 3);
         c = (lane & 7) ^ ((row >> 1) & 7);
         g = c >> 2, c &= 3;
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(GemmParams p) {
   };
 
   // fragments of a stage (two sets): lane (h4, r16) holds k 16 h4 .. + 15 of row r16, two MFMAs of 8 each
-  typedef typename std::conditional<FMT == HXA_W_F16, half8_t,
+  typedef typename std::conditional<plain_fmt(FMT), half8_t,
                                     typename std::conditional<FMT == HXA_W_Q8, uint4_t, uint2_t>::type>::type raw_t;
   half8_t fa[2][MI][2];
   raw_t fw[2][NI][QW ? 1 : 2];
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(GemmParams p) {
 #pragma unroll
     for (int j = 0; j < NI; j++) {
       const int row = j * 16 + r16;
-      if constexpr (FMT == HXA_W_F16) {
+      if constexpr (plain_fmt(FMT)) {
 #pragma unroll
         for (int k = 0; k < 2; k++)
           fw[u][j][k] = *(const half8_t *)(ws + row * 128 + (((2 * h4 + k) ^ ((row >> 1) & 7)) << 4));
@@ -130,18 +130,18 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(GemmParams p) {
         fa[u][i][k] = *(const half8_t *)(b + row * 128 + (((2 * h4 + k) ^ ((row >> 1) & 7)) << 4));
       }
   };
-  float4_t acc[NI][MI];
+  acc_t<FMT> acc[NI][MI];
 #pragma unroll
   for (int j = 0; j < NI; j++)
 #pragma unroll
-    for (int i = 0; i < MI; i++) acc[j][i] = (float4_t){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < MI; i++) acc[j][i] = (acc_t<FMT>){};
   auto mac = [&](int u) {
 #pragma unroll
     for (int k = 0; k < 2; k++)
 #pragma unroll
       for (int j = 0; j < NI; j++) {
         half8_t w;
-        if constexpr (FMT == HXA_W_F16) {
+        if constexpr (plain_fmt(FMT)) {
           w = fw[u][j][k];
         } else {
           const half2_t s2 = {sc[u][j], sc[u][j]};
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(GemmParams p) {
           w = __builtin_bit_cast(half8_t, (uint4_t){o[0], o[1], o[2], o[3]});
         }
 #pragma unroll
-        for (int i = 0; i < MI; i++) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, fa[u][i][k], acc[j][i], 0, 0, 0);
+        for (int i = 0; i < MI; i++) acc[j][i] = mma_wa(w, fa[u][i][k], acc[j][i]);
       }
   };
   // stage t has landed: the loads of the `newer` stages issued after it may still fly
@@ -207,34 +207,38 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(GemmParams p) {
 #pragma unroll
   for (int j = 0; j < NI; j++)
 #pragma unroll
-    for (int i = 0; i < MI; i++) *(float4_t *)(mine + (i * 16 + r16) * G::SROW + j * 16 + 4 * h4) = acc[j][i];
+    for (int i = 0; i < MI; i++) *(acc_t<FMT> *)(mine + (i * 16 + r16) * G::SROW + j * 16 + 4 * h4) = acc[j][i];
   __syncthreads();
 #pragma unroll
   for (int i = tid; i < BM * BN / 4; i += 64 * NW) {
     const int row = i >> 3, c = (i & 7) * 4;
     if (m0 + row >= p.M || n0 + c >= p.N) continue;  // N % 8 == 0: four columns are inside N or past it
-    float4_t s = *(const float4_t *)(part + row * G::SROW + c);
+    acc_t<FMT> s = *(const acc_t<FMT> *)(part + row * G::SROW + c);
 #pragma unroll
-    for (int w = 1; w < NW; w++) s += *(const float4_t *)(part + (w * BM + row) * G::SROW + c);
-    *(half4_t *)(p.out + (long)(m0 + row) * p.ldo + n0 + c) = (half4_t){(hxa_h)s[0], (hxa_h)s[1], (hxa_h)s[2], (hxa_h)s[3]};
+    for (int w = 1; w < NW; w++) s += *(const acc_t<FMT> *)(part + (w * BM + row) * G::SROW + c);
+    hxa_h *const out = p.out + (long)(m0 + row) * p.ldo + n0 + c;
+    if constexpr (FMT == HXG_I8) {
+      const float sa = p.sa[m0 + row];
+      const float4_t sw = *(const float4_t *)(p.sw + n0 + c), b = p.bias ? *(const float4_t *)(p.bias + n0 + c) : (float4_t){};
+      *(uint2_t *)out = p.dtype == HXA_DT_F16 ? scale_i8<hxa_h>(s, sa, sw, b) : scale_i8<__bf16>(s, sa, sw, b);
+    } else {
+      *(half4_t *)out = (half4_t){(hxa_h)s[0], (hxa_h)s[1], (hxa_h)s[2], (hxa_h)s[3]};
+    }
   }
 }
 
 template <int BM, int FMT, bool ASYM>
-static hipError_t launch_skinny_t(const GemmParams &p, hipStream_t st) {
+static hipError_t launch_skinny_t(const params_t<FMT> &p, hipStream_t st) {
   auto kern = gemm_skinny_kernel<BM, FMT, ASYM>;
   constexpr int lds = SkinnyGeo<BM, FMT>::LDS;
-  static bool attr = false;
-  if (!attr) {
-    const hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
-    attr = true;
-  }
+  static std::atomic<uint64_t> attr{0};
+  const hipError_t a = allow_lds_once((const void *)kern, lds, attr);
+  if (a != hipSuccess) return a;
   hxa_launch(kern, dim3(p.tiles_m * p.tiles_n), dim3(256), lds, st, p);
   return hipGetLastError();
 }
 template <int FMT, bool ASYM>
-static hipError_t launch_skinny_fmt(int bm, const GemmParams &p, hipStream_t st) {
+static hipError_t launch_skinny_fmt(int bm, const params_t<FMT> &p, hipStream_t st) {
   return bm == 32 ? launch_skinny_t<32, FMT, ASYM>(p, st) : launch_skinny_t<64, FMT, ASYM>(p, st);
 }
 hipError_t launch_skinny(int bm, int fmt, bool asym, const GemmParams &p, hipStream_t st) {
@@ -242,4 +246,5 @@ hipError_t launch_skinny(int bm, int fmt, bool asym, const GemmParams &p, hipStr
   if (fmt == HXA_W_Q8) return launch_skinny_fmt<HXA_W_Q8, false>(bm, p, st);
   return asym ? launch_skinny_fmt<HXA_W_Q4, true>(bm, p, st) : launch_skinny_fmt<HXA_W_Q4, false>(bm, p, st);
 }
+hipError_t launch_skinny_i8(int bm, const GemmParamsI8 &p, hipStream_t st) { return launch_skinny_fmt<HXG_I8, false>(bm, p, st); }
 }  // namespace hxg

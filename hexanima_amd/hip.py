@@ -21,6 +21,7 @@ W_F16, W_Q8, W_Q4 = 0, 1, 2
 W_KTILED = 16  # OR'ed into a format: matrix stored k-tiled, [K/32][N][chunk]
 EPI_STORE, EPI_GELU_TANH, EPI_GELU_ERF, EPI_RESADD, EPI_STORE_T, EPI_SITU, EPI_PARTIAL, EPI_RESADD_SPLIT2, EPI_PARTIAL_F32 = range(9)
 DT_F16, DT_BF16 = 1, 2
+I8_MAX_K = 130944
 ROPE_HALF, ROPE_PAIRS = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = range(4)
 KIND_WEIGHTS_ANIMA, KIND_BLOB, KIND_WEIGHTS_MOSS = 0, 1, 2
@@ -53,6 +54,11 @@ class KvCache(C.Structure):
     """hxa_kv_cache: a paged key / value cache and the plan of a call on it (device pointers)"""
     _fields_ = [("dtype", I), ("H", I), ("hd", I), ("page", I), ("npages", I), ("k", P), ("v", P), ("prefix", P),
                 ("prefix_len", I), ("table", P), ("ldt", I), ("len", P), ("cu", P), ("nseq", I)]
+
+
+class KvCacheQ8(C.Structure):
+    """hxa_kv_cache_q8: a KvCache whose pools hold int8, and the scales of its pages and heads (device pointers)"""
+    _fields_ = [("c", KvCache), ("kscale", P), ("vscale", P)]
 
 
 _SIGS = {
@@ -108,6 +114,13 @@ _SIGS = {
     "hxa_attention_causal": (I, [I, P, L, P, L, P, L, P, L, I, P, I, I, I, I, F, P]),
     "hxa_attention_cached": (I, [C.POINTER(KvCache), P, L, P, L, I, I, F, P, L, P]),
     "hxa_attention_cached_ws_bytes": (L, [C.POINTER(KvCache), I, I]),
+    "hxa_quantize_rows": (I, [I, P, L, I, I, P, L, P, P]),
+    "hxa_linear_i8": (I, [I, P, L, P, I, P, L, P, I, I, P, P, L, P, L, P]),
+    "hxa_linear_i8_ws_bytes": (L, [I, I, I]),
+    "hxa_linear_i8_tile": (I, [I, P, L, P, I, P, L, P, I, I, P, P, L, I, I, I, P, L, P]),
+    "hxa_kv_append_q8": (I, [C.POINTER(KvCacheQ8), P, L, P, L, I, P, F, C.POINTER(Rope), P]),
+    "hxa_attention_cached_q8": (I, [C.POINTER(KvCacheQ8), P, L, P, L, I, I, F, P, L, P]),
+    "hxa_attention_cached_q8_ws_bytes": (L, [C.POINTER(KvCacheQ8), I, I]),
     "hxa_fill_normal": (I, [P, I, SZ, U64, F, F, P]),
     "hxa_fill_uniform_int": (I, [P, I, SZ, U64, I, I, P]),
     "hxa_fill_const": (I, [P, I, SZ, F, P]),

@@ -323,6 +323,53 @@ int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long ldq, void *o
 long hxa_attention_cached_ws_bytes(const hxa_kv_cache *c, int T, int Hq); /* 0: the one-launch form is the best one */
 
 /* ============================================================================================================
+ * 3c. The text model in 8 bits: int8 rows with a scale each, their product, a paged cache of int8 and the attention over it
+ * ============================================================================================================
+ * Types, rows, sequences and plans are those of 3b. int8 values are two's complement; a value is its byte times a scale (fp32). Rounding to a byte
+ * is to the nearest integer, ties to even, within +-127; a NaN becomes 0 and an infinity +-127 (0 where every finite value is 0). Scales are
+ * max |x| / 127 over the finite values, at least 2^-64, or 0 where all of them are 0. */
+#define HXA_I8_MAX_K 130944 /* a multiple of 128, up to which int32 sums of products of bytes are exact */
+/* Rows to int8: x [M][ldx] (dtype, K values a row, ldx % 8 == 0) to q [M][ldq] with q = x * (127 / max |x|) rounded and scale[m] = max |x| / 127. Columns
+ * K .. ceil(K / 128) 128 - 1 of q are written as zeros (ldq at least that, a multiple of 16); columns behind them are left as they are. Rows of a
+ * weight [N][K] are its channels. M at most 2^25, K 1 .. HXA_I8_MAX_K; x and q 16-byte aligned, they do not overlap. */
+int hxa_quantize_rows(int dtype, const void *x, long ldx, int M, int K, void *q, long ldq, float *scale, void *stream);
+/* Product of int8 rows: out[m][n] = sa[m] * sw[n] * (sum over k of a[m][k] * w[n][k]) + bias[n], out [M][ldo] of dtype. a [M][lda] and w [N][ldw] are
+ * int8 rows that hold ceil(K / 128) 128 columns: those past K are multiplied too, so one of a and w has zeros there, as hxa_quantize_rows leaves them.
+ * The sum is exact (int32); scales and bias (NULL: none) are applied in fp32, one rounding. M any, N % 8 == 0, K 1 .. HXA_I8_MAX_K;
+ * lda, ldw multiples of 16 below 2^23, ldo % 8 == 0; pointers 16-byte aligned (sa: 4). out overlaps no operand. ws: hxa_linear_i8_ws_bytes(M, N,
+ * K) bytes, 16-byte aligned, for int32 partial sums where there are few output tiles; NULL or fewer bytes: one launch. The results
+ * are the same bits in every form. Calls that share ws must not overlap in time, graphs' replays included. */
+int hxa_linear_i8(int dtype, const void *a, long lda, const float *sa, int M, const void *w, long ldw, const float *sw, int N, int K,
+                  const float *bias, void *out, long ldo, void *ws, long ws_bytes, void *stream);
+long hxa_linear_i8_ws_bytes(int M, int N, int K);
+/* hxa_linear_i8 on a given tile (tuning, tests): bm x bn output tiles, ksplit slices of K, each a multiple of 128 (above 1: ksplit M N 4 bytes of
+ * ws). Tiles: 256 x 256, 256 x 192, 192 x 256, 192 x 192, 256 x 128, 128 x 256, 192 x 128, 128 x 128, 64 x 128, 128 x 64, 64 x 64, and with ksplit
+ * 1 64 x 32, 32 x 32. */
+int hxa_linear_i8_tile(int dtype, const void *a, long lda, const float *sa, int M, const void *w, long ldw, const float *sw, int N, int K,
+                       const float *bias, void *out, long ldo, int bm, int bn, int ksplit, void *ws, long ws_bytes, void *stream);
+/* A paged cache of int8: c as in 3b, but c.k and c.v are int8 pools [npages][H][page][hd] and c.dtype is the type of the rows that go in and come
+ * out; kscale, vscale [npages][H]: the scales of each page and head. */
+typedef struct {
+  hxa_kv_cache c;
+  float *kscale, *vscale;
+} hxa_kv_cache_q8;
+/* The new tokens' keys (norm and rotation in 32 bits as hxa_kv_append, not rounded in between) and values into their sequences' own pages. For each
+ * page and head: where the call writes the page's first row, its scale is that of the call's rows in it. Else the rows before them stay, and so
+ * does the scale s if the new rows fit (|x| <= 127 s); if not, it becomes the least s * 2^j that they fit, and the earlier rows' bytes become
+ * round(q / 2^j). (An earlier scale of 0 counts as a page of zeros.) A value is so off by less than one present scale of its page however many calls fill
+ * it, and by half of one where one call does. Rows behind the call's are left as they are. Tokens that are left out are those of hxa_kv_append. A page
+ * that is written may stand in one place of the table only. (T / page + 2 nseq) H < 2^24. */
+int hxa_kv_append_q8(const hxa_kv_cache_q8 *c, const void *k, long ldk, const void *v, long ldv, int T, const float *gk, float eps,
+                     const hxa_rope *rope, void *stream);
+/* hxa_attention_cached over such a cache: the same rows, masks, limits, workspace rules and forms. A scale that is not finite and positive counts as 0, its
+ * page's keys or values as zeros; so does a value scale of 2^-64 or less. Weights are rounded to fp16 for their product with the bytes, their sum
+ * is taken before that: beside the output's own rounding at most 2^-11 of the weighted mean of |v|. bf16 queries are brought to fp16 by a power of two
+ * of their row: what is below 2^-38 of the row's largest value is lost. Value scales of pages that one row sees may differ by up to 2^90. */
+int hxa_attention_cached_q8(const hxa_kv_cache_q8 *c, const void *q, long ldq, void *o, long ldo, int T, int Hq, float scale, void *ws,
+                            long ws_bytes, void *stream);
+long hxa_attention_cached_q8_ws_bytes(const hxa_kv_cache_q8 *c, int T, int Hq);
+
+/* ============================================================================================================
  * 4. GPU block packs and the device-level block (weights resident in HBM)
  * ============================================================================================================ */
 /* A pack is one device allocation holding every weight of one block in the GPU layouts above, at offsets
