@@ -8,8 +8,8 @@
 // in fp16. q in bf16 is brought to fp16 by a power of two of its row, whose largest value it puts near 2^14: the row's values down to 2^-28 of that stay exact.
 // t, m, both sums and O are held in fp32; the denominator adds the weights before they are rounded.
 //
-// Tiles of 64 keys go through registers: loaded while the tile before them is computed, then turned into fp16 rows in LDS once for all four
-// waves. A byte is finite whatever it holds, so that a masked key needs nothing but a weight of 0.
+// Rows modes: tiles of 64 keys go through registers, where they are turned into fp16 once for all four waves, into one of two places in LDS; that runs beside
+// the products of K of the tile before. A byte is finite whatever it holds, so that a masked key needs nothing but a weight of 0.
 #include "causal_attn.h"
 #include "int8_rows.h"
 
@@ -22,10 +22,13 @@ struct KeysQ8 : Keys<int8_t> {
 template <int HD>
 struct GeoQ8 {
   static constexpr int RB = HD * 2, TB = KT * RB;     // bytes of an fp16 row, of a tile
-  static constexpr int CST = 2 * TB;                  // c ks, log2 vs and 1 / vs of the tile's keys
-  static constexpr int LDS = 2 * TB + 2048;
+  static constexpr int CST = 4 * TB;                  // past K, K, V, V: twice c ks, log2 vs and 1 / vs of the tile's keys
+  static constexpr int LDS = 4 * TB + 2048;
   static constexpr int CH = HD / 16, N = KT * CH / 256;  // 16-byte chunks of a row of bytes; loads a thread, for K and for V each
 };
+
+// stands for a key scale of 0: scores are as good as 0, and -infinity stays what it is
+constexpr float NO_SCALE = 0x1p-110f;
 
 // four bytes to fp16: u = q + 128 under the exponent of 1024 is 1024 + u
 HXA_DEV uint2_t q8_halves(uint32_t d) {
@@ -35,11 +38,11 @@ HXA_DEV uint2_t q8_halves(uint32_t d) {
                    __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - c)};
 }
 
-// The tiles of a work item: row (PERM ? krow_key(j) : j) of LDS holds key j, in the orders of Swz
-template <int HD, bool PERM>
+// The tiles of a work item in the rows modes: row krow_key(j) of LDS holds key j, in the orders of Swz
+template <int HD>
 struct LoaderQ8 {
   typedef GeoQ8<HD> G_;
-  typedef Swz<hxa_h, HD, PERM> S_;
+  typedef Swz<hxa_h, HD, true> S_;
   const KeysQ8 &s;
   const Item &it;
   uint8_t *lds;
@@ -49,9 +52,16 @@ struct LoaderQ8 {
   unsigned in_page;
   uint4_t raw[2][G_::N];
   float ks, vs;  // of this lane's key
+  uint32_t to[2][2];  // where the two halves of this thread's first 16 bytes of K (V) go; its other ones are whole numbers of 16 rows behind
   HXA_DEV LoaderQ8(const KeysQ8 &s_, const Item &it_, uint8_t *lds_, float c_, int tid_)
       : s(s_), it(it_), lds(lds_), c(c_), tid(tid_), lane(tid_ & 63), ent(-1), in_page(0) {
     entry(0);
+    const int row = krow_key(tid / G_::CH), ch = tid % G_::CH;  // (krow_key is its own inverse)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      to[0][e] = row * G_::RB + (((2 * ch + e) ^ S_::fk(row)) << 4);
+      to[1][e] = row * G_::RB + (((2 * ch + e) ^ S_::fv(row)) << 4);
+    }
   }
   HXA_DEV void entry(int i) {  // the page of this lane's key of tile i
     const int x = it.x0 + i * KT + lane;
@@ -80,37 +90,39 @@ struct LoaderQ8 {
     }
     return mask;
   }
-  // the tile opened last into LDS
-  HXA_DEV void store() {
-    const uint64_t zero = __ballot(!(vs > HXA_Q8_LEAST && vs < INFINITY));
+  HXA_DEV uint8_t *kbuf(int i) const { return lds + (i & 1) * G_::TB; }
+  HXA_DEV uint8_t *vbuf(int i) const { return lds + (2 + (i & 1)) * G_::TB; }
+  HXA_DEV float *cst(int i) const { return (float *)(lds + G_::CST) + (i & 1) * 192; }
+  // the tile opened last, as tile i into LDS, in 2 N pieces; `begin` before them
+  HXA_DEV void begin(int i) {
+    const bool vok = vs > HXA_Q8_LEAST && vs < INFINITY;
+    const uint64_t zero = __ballot(!vok);
     if (zero) {  // keys without a scale (or without a page): values of 0, whatever the bytes
 #pragma unroll
       for (int n = 0; n < G_::N; n++)
         if ((zero >> ((n * 256 + tid) / G_::CH)) & 1) raw[1][n] = (uint4_t){0, 0, 0, 0};
     }
-#pragma unroll
-    for (int n = 0; n < G_::N; n++) {
-      const int u = n * 256 + tid, key = u / G_::CH, ch = u % G_::CH;
-      const int row = PERM ? krow_key(key) : key;  // (krow_key is its own inverse)
-#pragma unroll
-      for (int V = 0; V < 2; V++) {
-        uint8_t *to = lds + V * G_::TB + row * G_::RB;
-        const int f = V ? S_::fv(row) : S_::fk(row);
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const uint2_t a = q8_halves(raw[V][n][2 * e]), b = q8_halves(raw[V][n][2 * e + 1]);
-          *(uint4_t *)(to + (((2 * ch + e) ^ f) << 4)) = (uint4_t){a.x, a.y, b.x, b.y};
-        }
-      }
-    }
     if (tid < 64) {
-      float *cst = (float *)(lds + G_::CST);
-      const float a = ks > 0.0f && ks < INFINITY ? ks : 0.0f;
-      const float b = vs > HXA_Q8_LEAST && vs < INFINITY ? vs : HXA_Q8_LEAST;
-      cst[lane] = a * c;
-      cst[64 + lane] = __builtin_amdgcn_logf(b);
-      cst[128 + lane] = 1.0f / b;
+      const float b = vok ? vs : HXA_Q8_LEAST;
+      float *x = cst(i) + lane;
+      x[0] = ks > 0.0f && ks < INFINITY ? fmaxf(ks * c, NO_SCALE) : NO_SCALE;
+      x[64] = __builtin_amdgcn_logf(b);
+      x[128] = 1.0f / b;
     }
+  }
+  HXA_DEV void piece(int i, int p) {
+    const int V = p >= G_::N, n = V ? p - G_::N : p;
+    uint8_t *at = (V ? vbuf(i) : kbuf(i)) + n * (256 / G_::CH) * G_::RB;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const uint2_t a = q8_halves(raw[V][n][2 * e]), b = q8_halves(raw[V][n][2 * e + 1]);
+      *(uint4_t *)(at + to[V][e]) = (uint4_t){a.x, a.y, b.x, b.y};
+    }
+  }
+  HXA_DEV void store(int i) {
+    begin(i);
+#pragma unroll
+    for (int p = 0; p < 2 * G_::N; p++) piece(i, p);
   }
 };
 
@@ -122,11 +134,14 @@ HXA_DEV half8_t q_halves(bf8_t q, float f) {
   for (int e = 0; e < 8; e++) r[e] = (hxa_h)((float)q[e] * f);
   return r;
 }
-// 2^(14 - e) for a row whose largest magnitude is 2^e .. 2^(e + 1); 1 for one of zeros, and where it is not finite
+// 1 for a row whose largest magnitude is 1 .. 2^15, 0 or not finite, else 2^(14 - e) where it is 2^e .. 2^(e + 1)
 HXA_DEV float row_factor(float top) {
   const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
-  return top >= 0x1p-100f && top < INFINITY ? __builtin_bit_cast(float, (uint32_t)(127 + 14 - e) << 23) : 1.0f;
+  return top >= 0x1p-100f && top < INFINITY && !(top >= 1.0f && top < 0x1p15f) ? __builtin_bit_cast(float, (uint32_t)(127 + 14 - e) << 23) : 1.0f;
 }
+// a key's scale times what its row's queries were divided by, not below NO_SCALE
+template <bool BF>
+HXA_DEV float with_back(float k, float back) { return BF ? fmaxf(k * back, NO_SCALE) : k; }
 template <typename V, int N>
 HXA_DEV float most_of(const V (&q)[N]) {
   float m = 0.0f;
@@ -138,7 +153,9 @@ HXA_DEV float most_of(const V (&q)[N]) {
 }
 
 // ---- rows modes: as causal_attn.hip's rows_item; m and the sums in powers of two ----
-template <typename T, int HD, int W>
+// G8: eight keys of a lane (8 g + 0 .. 7 of every 16) lie on one page, so that they share its scales: the maximum is taken of the scores, the
+// scales go into one fma a score. (With constants for each key, three 16-byte reads of LDS for four of them, the LDS decides: @G8@.)
+template <typename T, int HD, int W, bool G8>
 HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, int head0, float c, uint8_t *lds, float16_t (&acc)[HD / 32],
                           float &mrun, float &lsum) {
   typedef GeoQ8<HD> G_;
@@ -174,9 +191,7 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
     for (int i = 0; i < HD / 16; i++) qf[i] = q_halves(raw[i], f);
   }
   const int lim = tok_limit(it, tok);
-  const int last = it.nrows - 1;
   const int lim_min = row_limit(it, it.r0);
-  const int wave_max = it.r0 + rw * 32 <= last ? row_limit(it, min(it.r0 + rw * 32 + 31, last)) : -1;
 
 #pragma unroll
   for (int d = 0; d < ND; d++) acc[d] = (float16_t){};
@@ -184,33 +199,32 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
   lsum = 0.0f;
   const int nt = (it.x1 - it.x0 + KT - 1) / KT;
   if (nt <= 0) return;
-  LoaderQ8<HD, true> ld(s, it, lds, c, tid);
-  uint64_t km_next = ld.open(0);
+  LoaderQ8<HD> ld(s, it, lds, c, tid);
+  uint64_t km = ld.open(0);
 
   const int vrow = 4 * g + ((lane & 15) >> 2);
   const int vlow = ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;
   uint32_t vat[ND];
 #pragma unroll
   for (int d = 0; d < ND; d++) vat[d] = vrow * G_::RB + (((d << 2) ^ S_::fv(vrow)) << 4) + vlow;
-  const uint8_t *kb = lds, *vb = lds + G_::TB;
-  const float *cst = (const float *)(lds + G_::CST) + 32 * kh + 8 * g;
-  auto kfrag = [&](int ds, int b) {
-    const int row = (b + kh) * 32 + ql, ch = 2 * ds + g;
-    return *(const half8_t *)(kb + row * G_::RB + ((ch ^ S_::fk(row)) << 4));
-  };
-  auto vfrag = [&](int n) {
-    const uint8_t *at = vb + vat[n % ND] + (kh * 32 + n / ND * 16) * G_::RB;
-    return __builtin_shufflevector(read_tr<half4_t>(at), read_tr<half4_t>(at + 8 * G_::RB), 0, 1, 2, 3, 4, 5, 6, 7);
-  };
+  ld.store(0);
+  uint64_t km_next = 0;
+  if (nt > 1) km_next = ld.open(1);
+  reads_done_barrier();  // tile 0 is in LDS
 
+  // Tile i: its products of K carry the next tile's way from registers into LDS; then the registers take the loads of the tile behind that.
   for (int i = 0; i < nt; i++) {
-    reads_done_barrier();  // every wave is done with tile i - 1
-    ld.store();
-    const uint64_t km = km_next;
     const int key0 = it.x0 + i * KT;
-    if (i + 1 < nt) km_next = ld.open(i + 1);
-    reads_done_barrier();  // tile i is in LDS
-    if (key0 + 32 * kh > wave_max) continue;  // no row of this wave sees it
+    const uint8_t *kb = ld.kbuf(i), *vb = ld.vbuf(i);
+    const float *cst = ld.cst(i) + 32 * kh + 8 * g;
+    auto kfrag = [&](int ds, int b) {
+      const int row = (b + kh) * 32 + ql, ch = 2 * ds + g;
+      return *(const half8_t *)(kb + row * G_::RB + ((ch ^ S_::fk(row)) << 4));
+    };
+    auto vfrag = [&](int n) {
+      const uint8_t *at = vb + vat[n % ND] + (kh * 32 + n / ND * 16) * G_::RB;
+      return __builtin_shufflevector(read_tr<half4_t>(at), read_tr<half4_t>(at + 8 * G_::RB), 0, 1, 2, 3, 4, 5, 6, 7);
+    };
     const bool cut = km != ~0ull || key0 + KT - 1 > lim_min;
     float16_t S[NB];
     half8_t kf[AK + 1][NB];
@@ -218,6 +232,12 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
     for (int ds = 0; ds < AK; ds++)
 #pragma unroll
       for (int b = 0; b < NB; b++) kf[ds][b] = kfrag(ds, b);
+    float kg[2 * NB], lg[2 * NB], ig[2 * NB];  // G8: of keys 16 u + 8 g .. + 7
+    if constexpr (G8) {
+#pragma unroll
+      for (int u = 0; u < 2 * NB; u++) kg[u] = with_back<BF>(cst[16 * u], back), lg[u] = cst[16 * u + 64], ig[u] = cst[16 * u + 128];
+    }
+    ld.begin(i + 1);  // (past the last tile: of what the registers hold, for nobody)
 #pragma unroll
     for (int ds = 0; ds < HD / 16; ds++) {
       __builtin_amdgcn_sched_barrier(0);
@@ -225,41 +245,61 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
 #pragma unroll
         for (int b = 0; b < NB; b++) kf[(ds + AK) % (AK + 1)][b] = kfrag(ds + AK, b);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if (ds % 2 == 0) ld.piece(i + 1, ds / 2);
 #pragma unroll
       for (int b = 0; b < NB; b++) S[b] = mma32(kf[ds % (AK + 1)][b], qf[ds], ds == 0 ? (float16_t){} : S[b]);
     }
     __builtin_amdgcn_sched_barrier(0);
+    const uint64_t km_i = km;
+    km = km_next;
+    if (i + 2 < nt) km_next = ld.open(i + 2);
     half8_t vf[AV + 1];
 #pragma unroll
     for (int n = 0; n < AV; n++) vf[n] = vfrag(n);
-    // scores to exponents: 8 keys of a lane lie side by side
+    if constexpr (!G8) {
+    // scores to exponents, four keys at a time (their constants two reads ahead: all of them at once are more registers than there are)
+      auto at = [&](int u) { return cst + 16 * (u >> 1) + 4 * (u & 1); };
+      float4_t k[2], lv[2];
+      k[0] = *(const float4_t *)at(0), lv[0] = *(const float4_t *)(at(0) + 64);
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+      for (int u = 0; u < 4 * NB; u++) {
+        if (u + 1 < 4 * NB) k[(u + 1) & 1] = *(const float4_t *)at(u + 1), lv[(u + 1) & 1] = *(const float4_t *)(at(u + 1) + 64);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const float *at = cst + 32 * b + 16 * (r >> 3) + (r & 7);
-        const float4_t k = *(const float4_t *)at, lv = *(const float4_t *)(at + 64);
-#pragma unroll
-        for (int e = 0; e < 4; e++) S[b][r + e] = fmaf(BF ? S[b][r + e] * back : S[b][r + e], k[e], lv[e]);
-      }
-    if (cut) {
-      const int n = lim - key0 - 32 * kh - 8 * g;
-      const uint64_t see = km >> (32 * kh + 8 * g);
-#pragma unroll
-      for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int k = 32 * b + 16 * (r >> 3) + (r & 7);
-          if (k > n || !((see >> k) & 1)) S[b][r] = -INFINITY;
+        for (int e = 0; e < 4; e++) {
+          const float x = S[u >> 2][4 * (u & 3) + e];
+          S[u >> 2][4 * (u & 3) + e] = fmaf(BF ? x * back : x, k[u & 1][e], lv[u & 1][e]);
         }
+      }
     }
-    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (cut) {
+      // a row's limit hides the keys past x1 too (a range that ends before it ends with a tile); pages that are not there need the mask
+      const int n = lim - key0 - 32 * kh - 8 * g, left = it.x1 - key0;
+      if (km_i == (left >= KT ? ~0ull : (1ull << left) - 1)) {
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) m4[r & 3] = fmaxf(m4[r & 3], S[b][r]);
-    float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          for (int r = 0; r < 16; r++)
+            if (32 * b + 16 * (r >> 3) + (r & 7) > n) S[b][r] = -INFINITY;
+      } else {
+        const uint64_t see = km_i >> (32 * kh + 8 * g);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int k = 32 * b + 16 * (r >> 3) + (r & 7);
+            if (k > n || !((see >> k) & 1)) S[b][r] = -INFINITY;
+          }
+      }
+    }
+    float mt = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2 * NB; u++) {
+      float m8 = S[u >> 1][8 * (u & 1)];
+#pragma unroll
+      for (int r = 1; r < 8; r++) m8 = fmaxf(m8, S[u >> 1][8 * (u & 1) + r]);
+      mt = fmaxf(mt, G8 ? fmaf(m8, kg[u], lg[u]) : m8);
+    }
     {
       float lo, hi;
       halves(mt, lo, hi);
@@ -275,14 +315,23 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
     }
     const float mb = mrun == -INFINITY ? 0.0f : mrun;
     half8_t pf[NB][2];
-    float ls[2] = {0.0f, 0.0f};
+    float ls[2 * NB] = {};
     auto expo2 = [&](int n) {
-      const float2_t inv = *(const float2_t *)(cst + 128 + 32 * (n >> 4) + 16 * ((n >> 3) & 1) + (n & 7));
-      const float p0 = __builtin_amdgcn_exp2f(S[n >> 4][n & 15] - mb);
-      const float p1 = __builtin_amdgcn_exp2f(S[n >> 4][(n & 15) + 1] - mb);
-      pf[n >> 4][(n >> 3) & 1][n & 7] = (hxa_h)p0;
-      pf[n >> 4][(n >> 3) & 1][(n & 7) + 1] = (hxa_h)p1;
-      ls[(n >> 1) & 1] = fmaf(p1, inv[1], fmaf(p0, inv[0], ls[(n >> 1) & 1]));
+      const int u = n >> 3;
+      float p0 = S[n >> 4][n & 15], p1 = S[n >> 4][(n & 15) + 1];
+      if constexpr (G8) {
+        p0 = __builtin_amdgcn_exp2f(fmaf(p0, kg[u], lg[u] - mb));
+        p1 = __builtin_amdgcn_exp2f(fmaf(p1, kg[u], lg[u] - mb));
+        ls[u] += p0;
+        ls[u] += p1;
+      } else {
+        const float2_t inv = *(const float2_t *)(cst + 128 + 16 * u + (n & 7));
+        p0 = __builtin_amdgcn_exp2f(p0 - mb);
+        p1 = __builtin_amdgcn_exp2f(p1 - mb);
+        ls[u] = fmaf(p1, inv[1], fmaf(p0, inv[0], ls[u]));
+      }
+      pf[n >> 4][u & 1][n & 7] = (hxa_h)p0;
+      pf[n >> 4][u & 1][(n & 7) + 1] = (hxa_h)p1;
     };
 #pragma unroll
     for (int n = 0; n < 16; n += 2) expo2(n);
@@ -296,7 +345,9 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    lsum += ls[0] + ls[1];
+#pragma unroll
+    for (int u = 0; u < 2 * NB; u++) lsum = G8 ? fmaf(ls[u], ig[u], lsum) : lsum + ls[u];
+    reads_done_barrier();  // every wave is done with tile i, and has its part of the next one in LDS
   }
   {
     float lo, hi;
@@ -337,48 +388,54 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
 }
 
 // ---- few rows: 16 rows, each wave 16 keys of every tile ----
-// Bound by reading the cache, so the tiles stay bytes until a wave needs its part of one: they go from memory straight into a ring of NS of them in LDS
-// (global_load_lds), NS - 1 ahead, one barrier a tile, and a wave turns its own 16 keys into fp16 fragments. What the addresses need, a page's place and its scales, is in LDS as well, for 512 pages at a time: a load of it inside the loop would
-// be waited for with all those behind it.
+// Bound by reading the cache, and in short items by what follows one after the other. So the tiles stay bytes until a wave needs its part of one, and
+// a wave fetches its own keys and waits for nobody: 16 keys of two tiles a step go from memory straight into its ring of RS steps in LDS
+// (global_load_lds), are read into registers and their place is loaded again before the step is computed. What addresses and exponents need of
+// the pages, their places and scales, is in LDS as well, for 512 pages at a time (a load of it inside the loop would be waited for with all
+// those behind it); the first steps take their places from the tables themselves.
 //
-// LDS row 4 b + a of a wave's 16 holds key 4 a + b. K: a lane takes 16 bytes of its key, two slices of 8 dims; q's dims follow that order. V: dword u of
+// Row 4 b + a of a wave's 16 holds key 4 a + b. K: a lane takes 16 bytes of its key, two slices of 8 dims; q's dims follow that order. V: dword u of
 // keys 4 gi .. + 3 is dims 4 u .. + 3 of four keys, transposed by byte permutations: product j of a 64-dim group has dims 4 u + j. Chunks are swizzled
 // so that the lanes of either read spread over the banks.
 template <int HD>
 struct FewQ8 {
-  static constexpr int NS = HD == 64 ? 6 : 4, TB = KT * HD;  // tiles in the ring; bytes of a tile of K, or of V
-  static constexpr int CH = HD / 16, RPL = 64 / CH;           // 16-byte chunks a row, rows of one wave-wide load
-  static constexpr int NLD = HD / 64;                         // loads a wave and tile, for K and for V each
-  static constexpr int PAGES = 512, TABLE = NS * 2 * TB;      // the pages' table, past the ring
+  static constexpr int RS = HD == 64 ? 4 : 2;          // steps in a wave's ring
+  static constexpr int TB = 16 * HD;                   // bytes of a wave's keys of a tile, and of its values
+  static constexpr int CH = HD / 16, RPL = 64 / CH;    // 16-byte chunks a row, rows of one wave-wide load
+  static constexpr int NLD = HD / 64;                  // loads of a tile's keys, and of its values
+  static constexpr int PAGES = 512, TABLE = 4 * RS * 4 * TB;  // the pages' table, past the four rings
   static constexpr int LDS = TABLE + PAGES * 16 + 16;
   static HXA_DEV int fk(int row) { return HD == 64 ? (row >> 2) & 3 : HD == 128 ? (row >> 1) & 7 : row & 15; }
   static HXA_DEV int fv(int row) { return HD == 64 ? 0 : HD == 128 ? (row << 1) & 4 : (row & 3) << 2; }
 };
 // row of LDS <-> key, within 16 (its own inverse)
-HXA_DEV int few_row(int key) { return (key & ~15) | (key & 3) << 2 | (key >> 2 & 3); }
+HXA_DEV int few_row(int key) { return (key & 3) << 2 | (key >> 2 & 3); }
 
-// The pages of keys x from `x0` on, PAGES of them: place in the pools (npages H page rows; ~0: not there) and scales
+// The pages of keys x from a first one on, PAGES of them: place in the pools (npages H page rows; ~0: not there) and scales
 template <int HD>
 struct PagesQ8 {
+  static constexpr int N = FewQ8<HD>::PAGES;
   const KeysQ8 &s;
   uint32_t *ph;
   float *ks, *lv, *iv;
-  int first, own;  // entry of page slot n of the prefix: n - first, of the sequence: n + own
+  int *flag;
+  int first, own;        // entry of page slot n of the prefix: n - first, of the sequence: n + own
+  int npre, pre_end, own_end;
   HXA_DEV PagesQ8(const KeysQ8 &s_, uint8_t *lds) : s(s_), first(0), own(0) {
     ph = (uint32_t *)(lds + FewQ8<HD>::TABLE);
-    ks = (float *)(ph + FewQ8<HD>::PAGES);
-    lv = ks + FewQ8<HD>::PAGES;
-    iv = lv + FewQ8<HD>::PAGES;
+    ks = (float *)(ph + N);
+    lv = ks + N;
+    iv = lv + N;
+    flag = (int *)(iv + N);
   }
   HXA_DEV int entry(int x, unsigned &in_page) const {
     const bool pre = x < s.P;
     return (int)s.slot(pre ? x : x - s.P, in_page) + (pre ? -first : own);
   }
-  // whole workgroup, between barriers; whether a page of [x0, x1) is not there (in the words behind the table, once the workgroup has met)
-  HXA_DEV void fill(int x0, int x1, float c, int tid) {
-    constexpr int N = FewQ8<HD>::PAGES;
+  // the entries from key x0 on, of keys below x1
+  HXA_DEV void start(int x0, int x1) {
     unsigned in;
-    int npre = 0;
+    npre = 0;
     if (x0 < s.P) {
       first = (int)s.slot(x0, in);
       npre = (int)s.slot(s.P - 1, in) - first + 1;
@@ -386,41 +443,47 @@ struct PagesQ8 {
     } else {
       own = -(int)s.slot(x0 - s.P, in);
     }
-    const int own_end = x1 > s.P ? (int)s.slot(x1 - 1 - s.P, in) + 1 + own : npre;  // entries of the sequence's pages end here
-    const int pre_end = x1 > s.P ? npre : x1 > x0 ? (int)s.slot(x1 - 1, in) - first + 1 : 0;
+    own_end = x1 > s.P ? (int)s.slot(x1 - 1 - s.P, in) + 1 + own : npre;
+    pre_end = x1 > s.P ? npre : (int)s.slot(x1 - 1, in) - first + 1;
+  }
+  HXA_DEV bool there(int j) const { return j < (j < npre ? pre_end : own_end); }
+  HXA_DEV int page_of(int j) const { return there(j) ? (j < npre ? s.prefix[first + j] : s.table[j - own]) : -1; }
+  // the workgroup's threads take two pages each, e[k] of entry 256 k + tid
+  HXA_DEV void fill(const int (&e)[2], float c, int tid) {
     bool hole = false;
+    float a[2], b[2];
+    uint32_t at[2];
 #pragma unroll
-    for (int k = 0; k < N / 256; k++) {
-      const int j = k * 256 + tid;
-      const bool pre = j < npre, there = j < (pre ? pre_end : own_end);
-      const int e = there ? (pre ? s.prefix[first + j] : s.table[j - own]) : -1;
-      const bool ok = (unsigned)e < (unsigned)s.npages;
-      hole |= there && !ok;
-      const uint32_t at = ok ? (uint32_t)e * s.H + s.h : 0;
-      const float a = ok ? s.ks[at] : 0.0f, b = ok ? s.vs[at] : 0.0f;
-      const bool vok = b > HXA_Q8_LEAST && b < INFINITY;
-      ph[j] = ok ? at : ~0u;
-      ks[j] = a > 0.0f && a < INFINITY ? a * c : 0.0f;
-      lv[j] = vok ? __builtin_amdgcn_logf(b) : -64.0f;
-      iv[j] = vok ? 1.0f / b : 1.0f / HXA_Q8_LEAST;
+    for (int k = 0; k < 2; k++) {
+      const bool ok = (unsigned)e[k] < (unsigned)s.npages;
+      hole |= !ok && there(k * 256 + tid);
+      at[k] = ok ? (uint32_t)e[k] * s.H + s.h : ~0u;
+      a[k] = ok ? s.ks[at[k]] : 0.0f;
+      b[k] = ok ? s.vs[at[k]] : 0.0f;
     }
-    int *flag = (int *)(iv + N);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int j = k * 256 + tid;
+      const bool vok = b[k] > HXA_Q8_LEAST && b[k] < INFINITY;
+      ph[j] = at[k];
+      ks[j] = a[k] > 0.0f && a[k] < INFINITY ? fmaxf(a[k] * c, NO_SCALE) : NO_SCALE;
+      lv[j] = vok ? __builtin_amdgcn_logf(b[k]) : -64.0f;
+      iv[j] = vok ? 1.0f / b[k] : 1.0f / HXA_Q8_LEAST;
+    }
     const bool any = __any(hole);
     if ((tid & 63) == 0) flag[tid >> 6] = any;
   }
-  HXA_DEV bool holes() const {
-    const int *flag = (const int *)(iv + FewQ8<HD>::PAGES);
-    return (flag[0] | flag[1] | flag[2] | flag[3]) != 0;
-  }
+  HXA_DEV bool holes() const { return (flag[0] | flag[1] | flag[2] | flag[3]) != 0; }
 };
 
-template <typename T, int HD>
+template <typename T, int HD, bool G8>
 HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, int head0, float c, uint8_t *lds, const Out<T> &out) {
   typedef FewQ8<HD> F;
   typedef typename HxaVec<T>::v8 v8;
   typedef typename HxaVec<T>::v4 v4;
   constexpr bool BF = std::is_same<T, hxa_b>::value;
-  constexpr int NG = HD / 64, NS = F::NS;  // groups of 64 dims
+  constexpr int NG = HD / 64, RS = F::RS;  // groups of 64 dims
+  constexpr int L = 4 * F::NLD;            // loads a step
   const int tid = this_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int gi = lane >> 4, ql = lane & 15;
   const int R = it.r0 + ql, last = it.nrows - 1, Rc = min(R, last);
@@ -430,19 +493,69 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
 #pragma unroll
     for (int j = 0; j < 4; j++) acc[g][j] = (float4_t){};
   float mrun = -INFINITY, lsum = 0.0f;
-  const int nt = (it.x1 - it.x0 + KT - 1) / KT;
-  if (nt > 0) {
+  const int ns = (it.x1 - it.x0 + 2 * KT - 1) / (2 * KT);  // steps of two tiles
+  if (ns > 0) {
     PagesQ8<HD> pages(s, lds);
+    uint8_t *const ring = lds + wave * (RS * 4 * F::TB);
+    uint32_t koff[F::NLD], voff[F::NLD];
+    int from[F::NLD];  // the lane that knows the row of this lane's part of load n
+#pragma unroll
+    for (int n = 0; n < F::NLD; n++) {
+      const int row = n * F::RPL + lane / F::CH, ch = lane % F::CH;
+      from[n] = few_row(row);
+      koff[n] = (uint32_t)((ch ^ F::fk(row)) << 4);
+      voff[n] = (uint32_t)((ch ^ F::fv(row)) << 4);
+    }
+    // lane (h, key) of the first 32: the key of a step
+    const int xlane = it.x0 + (lane >> 4 & 1) * KT + 16 * wave + ql;
+    auto pool_row = [&](uint32_t p, unsigned in) { return p == ~0u ? 0u : p * s.page + in; };  // < 2^32: checked on the host
+    auto row_of = [&](int st) {
+      const int x = xlane + st * 2 * KT;
+      unsigned in;
+      if (x >= it.x1) return 0u;
+      const uint32_t p = pages.ph[pages.entry(x, in)];
+      return pool_row(p, in);
+    };
+    // loads of a step, whose keys' rows `at` has, into its place of the ring
+    auto load = [&](int st, uint32_t at) {
+      uint8_t *to = ring + (st % RS) * 4 * F::TB;
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int n = 0; n < F::NLD; n++) {
+          const uint64_t row = (uint64_t)(uint32_t)__shfl((int)at, 16 * h + from[n]) * HD;
+          g2l16_opaque((const uint8_t *)s.k + row + koff[n], to + h * 2 * F::TB + n * 1024);
+          g2l16_opaque((const uint8_t *)s.v + row + voff[n], to + h * 2 * F::TB + F::TB + n * 1024);
+        }
+    };
+    // the first steps' places and the table's pages from memory side by side, then the keys and the scales
+    pages.start(it.x0, it.x1);
+    int e0[RS], e1[2];
+    unsigned in0[RS];
+#pragma unroll
+    for (int i = 0; i < RS; i++) {
+      const int x = xlane + i * 2 * KT;
+      e0[i] = x < it.x1 ? pages.page_of(pages.entry(x, in0[i])) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) e1[k] = pages.page_of(k * 256 + tid);
     // q: dims 16 (4 d + gi) + 8 e .. + 7 in qf[d][e]
     int rest;
     const int tok = row_tok(it, Rc, rest);
     const T *qp = q + (long)(it.tok0 + tok) * ldq + (long)(head0 + rest) * HD;
+    v8 raw[2 * NG];
+#pragma unroll
+    for (int i = 0; i < 2 * NG; i++) raw[i] = *(const v8 *)(qp + 16 * (4 * (i >> 1) + gi) + 8 * (i & 1));
+    uint32_t at0[RS];
+#pragma unroll
+    for (int i = 0; i < RS; i++) at0[i] = (unsigned)e0[i] < (unsigned)s.npages ? pool_row((uint32_t)e0[i] * s.H + s.h, in0[i]) : 0u;
+#pragma unroll
+    for (int i = 0; i < RS; i++)
+      if (i < ns) load(i, at0[i]);
+    pages.fill(e1, c, tid);
     half8_t qf[NG][2];
     float back = 1.0f;
     {
-      v8 raw[2 * NG];
-#pragma unroll
-      for (int i = 0; i < 2 * NG; i++) raw[i] = *(const v8 *)(qp + 16 * (4 * (i >> 1) + gi) + 8 * (i & 1));
       float f = 1.0f;
       if (BF) {
         f = row_factor(max16(most_of(raw)));
@@ -452,109 +565,113 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
       for (int i = 0; i < 2 * NG; i++) qf[i >> 1][i & 1] = q_halves(raw[i], f);
     }
     const int lim = tok_limit(it, tok), lim_min = row_limit(it, it.r0);
-    const bool four = ((s.page | s.P) & 3) == 0;  // keys 4 gi .. + 3 lie on one page
-    uint32_t koff[F::NLD], voff[F::NLD], key_of[F::NLD];
-#pragma unroll
-    for (int n = 0; n < F::NLD; n++) {
-      const int row = (n * 4 + wave) * F::RPL + lane / F::CH, ch = lane % F::CH;
-      key_of[n] = few_row(row);
-      koff[n] = (uint32_t)((ch ^ F::fk(row)) << 4);
-      voff[n] = (uint32_t)((ch ^ F::fv(row)) << 4);
-    }
-    const int krow = 16 * wave + few_row(ql);
-    const uint8_t *kat = lds + krow * HD, *vat = lds + F::TB + (16 * wave + gi) * HD;  // keys 4 gi + e: rows 16 w + 4 e + gi
+    const int krow = few_row(ql);
+    const uint8_t *kat = ring + krow * HD, *vat = ring + F::TB + gi * HD;  // values of key 4 gi + e: row 4 e + gi
     uint32_t vch[NG];
 #pragma unroll
     for (int g = 0; g < NG; g++) vch[g] = (uint32_t)((((4 * g + (ql >> 2)) ^ F::fv(gi)) << 4) + (ql & 3) * 4);
-    const int kstep = it.x0 + 16 * wave + 4 * gi;
 
-    // loads of tile i into its place of the ring
-    auto load = [&](int i) {
-      const int x = it.x0 + i * KT + lane;
-      uint32_t at = 0;
-      if (x < it.x1) {
-        unsigned in;
-        const uint32_t p = pages.ph[pages.entry(x, in)];
-        at = p == ~0u ? 0 : p * s.page + in;  // < 2^32: checked on the host
-      }
-      uint8_t *to = lds + (i % NS) * 2 * F::TB + wave * 1024;
+    for (int s0 = 0; s0 < ns;) {
+      if (s0 > 0) {  // the next 512 pages
+        reads_done_barrier();
+        pages.start(it.x0 + s0 * 2 * KT, it.x1);
 #pragma unroll
-      for (int n = 0; n < F::NLD; n++) {
-        const uint64_t row = (uint64_t)(uint32_t)__shfl((int)at, (int)key_of[n]) * HD;
-        g2l16_opaque((const uint8_t *)s.k + row + koff[n], to + n * 4096);
-        g2l16_opaque((const uint8_t *)s.v + row + voff[n], to + F::TB + n * 4096);
+        for (int k = 0; k < 2; k++) e1[k] = pages.page_of(k * 256 + tid);
+        pages.fill(e1, c, tid);
       }
-    };
-    for (int t0 = 0; t0 < nt;) {
-      // the pages from tile t0 on, and how many tiles they reach
-      if (t0 > 0) reads_done_barrier();
-      pages.fill(it.x0 + t0 * KT, it.x1, c, tid);
       reads_done_barrier();
       const bool holes = pages.holes();
-      int t1 = nt;
-      {
+      int s1 = ns;  // the steps whose pages are in the table
+      for (;;) {
         unsigned in;
-        // (an entry is a page of one key at least)
-        while (pages.entry(min(it.x0 + t1 * KT, it.x1) - 1, in) >= F::PAGES) {
-          const int over = pages.entry(min(it.x0 + t1 * KT, it.x1) - 1, in) - F::PAGES + 1;
-          t1 -= max(1, (int)min((long)(over - 1) * s.page / KT, (long)t1 - t0 - 1));
-        }
+        const int over = pages.entry(min(it.x0 + s1 * 2 * KT, it.x1) - 1, in) - F::PAGES + 1;
+        if (over <= 0) break;
+        s1 -= max(1, (int)min((long)(over - 1) * s.page / (2 * KT), (long)s1 - s0 - 1));
       }
+      if (s0 > 0) {
 #pragma unroll
-      for (int i = 0; i < NS - 1; i++)
-        if (t0 + i < t1) load(t0 + i);
-      for (int i = t0; i < t1; i++) {
-        // tile i has landed: the loads of the `newer` tiles behind it may still fly
-        const int newer = min(NS - 2, t1 - 1 - i);
-        constexpr int L = 2 * F::NLD;
-        if (newer >= NS - 2) wait_vm<(NS - 2) * L>();
-        else if (newer == 3) wait_vm<(NS > 5 ? 3 * L : 0)>();
-        else if (newer == 2) wait_vm<(NS > 4 ? 2 * L : 0)>();
+        for (int i = 0; i < RS; i++)
+          if (s0 + i < s1) load(s0 + i, row_of(s0 + i));
+      }
+      // (the first table holds the first RS steps: fewer than 512 pages of a key each)
+      uint32_t at_next = s0 + RS < s1 ? row_of(s0 + RS) : 0;
+      for (int st = s0; st < s1; st++) {
+        // this step has landed: the loads of the steps behind it may still fly
+        const int newer = min(RS, s1 - st) - 1;
+        if (newer == 0) wait_vm<0>();
         else if (newer == 1) wait_vm<L>();
-        else wait_vm<0>();
-        reads_done_barrier();  // for every wave; and every wave is done with tile i - 1
-        if (i + NS - 1 < t1) load(i + NS - 1);
-        const int at = (i % NS) * 2 * F::TB;
-        float4_t S = {};
+        else if (newer == 2) wait_vm<(RS > 2 ? 2 * L : 0)>();
+        else wait_vm<(RS > 3 ? 3 * L : 0)>();
+        asm volatile("" ::: "memory");
+        const int at = (st % RS) * 4 * F::TB;
+        uint4_t kr[2][NG];
+        uint32_t vr[2][NG][4];
+        float k4[2][G8 ? 1 : 4], l4[2][G8 ? 1 : 4], i4[2][G8 ? 1 : 4];  // G8: keys 4 gi .. + 3 lie on one page
+        const int x = it.x0 + st * 2 * KT + 16 * wave + 4 * gi;
 #pragma unroll
-        for (int d = 0; d < NG; d++) {
-          const uint4_t w = *(const uint4_t *)(kat + at + (((4 * d + gi) ^ F::fk(krow)) << 4));
+        for (int h = 0; h < 2; h++) {
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const uint2_t a = q8_halves(w[2 * e]), b = q8_halves(w[2 * e + 1]);
-            S = mma16(__builtin_bit_cast(half8_t, (uint4_t){a.x, a.y, b.x, b.y}), qf[d][e], S);
-          }
+          for (int d = 0; d < NG; d++) kr[h][d] = *(const uint4_t *)(kat + at + h * 2 * F::TB + (((4 * d + gi) ^ F::fk(krow)) << 4));
         }
-        const int x = kstep + i * KT;
-        float4_t k, lv, iv;
-        unsigned in;
-        if (four) {
-          const int p = min(pages.entry(min(x, it.x1 - 1), in), F::PAGES - 1);
-          k = pages.ks[p];
-          lv = pages.lv[p];
-          iv = pages.iv[p];
-        } else {
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const int p = min(pages.entry(min(x + r, it.x1 - 1), in), F::PAGES - 1);
-            k[r] = pages.ks[p];
-            lv[r] = pages.lv[p];
-            iv[r] = pages.iv[p];
+        for (int h = 0; h < 2; h++) {
+          unsigned in;
+#pragma unroll
+          for (int r = 0; r < (G8 ? 1 : 4); r++) {
+            const int p = pages.entry(min(x + h * KT + r, it.x1 - 1), in);
+            k4[h][r] = with_back<BF>(pages.ks[p], back), l4[h][r] = pages.lv[p], i4[h][r] = pages.iv[p];
           }
         }
 #pragma unroll
-        for (int r = 0; r < 4; r++) S[r] = fmaf(BF ? S[r] * back : S[r], k[r], lv[r]);
-        if (it.x0 + i * KT + KT - 1 > lim_min) {  // (a row's limit hides what lies past x1 too)
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int r = 0; r < 4; r++)
-            if (x + r > lim || x + r >= it.x1) S[r] = -INFINITY;
+          for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) vr[h][g][e] = *(const uint32_t *)(vat + at + h * 2 * F::TB + 4 * e * HD + vch[g]);
+        if (st + RS < s1) {
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the step is in registers, its place is free
+          asm volatile("" ::: "memory");
+          load(st + RS, at_next);
+          if (st + RS + 1 < s1) at_next = row_of(st + RS + 1);
+        }
+        float4_t S[2] = {};
+#pragma unroll
+        for (int d = 0; d < NG; d++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const uint2_t a = q8_halves(kr[h][d][2 * e]), b = q8_halves(kr[h][d][2 * e + 1]);
+              S[h] = mma16(__builtin_bit_cast(half8_t, (uint4_t){a.x, a.y, b.x, b.y}), qf[d][e], S[h]);
+            }
+        if (it.x0 + (st + 1) * 2 * KT - 1 > min(lim_min, it.x1 - 1)) {
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              if (x + h * KT + r > lim || x + h * KT + r >= it.x1) S[h][r] = -INFINITY;
         }
         if (holes) {
 #pragma unroll
-          for (int r = 0; r < 4; r++)
-            if (pages.ph[min(pages.entry(min(x + r, it.x1 - 1), in), F::PAGES - 1)] == ~0u) S[r] = -INFINITY;
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              unsigned in;
+              if (pages.ph[pages.entry(min(x + h * KT + r, it.x1 - 1), in)] == ~0u) S[h][r] = -INFINITY;
+            }
         }
-        const float mt = max16(fmaxf(fmaxf(S[0], S[1]), fmaxf(S[2], S[3])));
+        float mt;
+        if constexpr (G8) {
+          mt = fmaxf(fmaf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])), k4[0][0], l4[0][0]),
+                     fmaf(fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])), k4[1][0], l4[1][0]));
+        } else {
+          mt = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) mt = fmaxf(mt, fmaf(S[h][r], k4[h][r], l4[h][r]));
+        }
+        mt = max16(mt);
         const bool need = mt - mrun > RESCALE2;
         if (__any(need)) {
           const float alpha = need ? __builtin_amdgcn_exp2f(mrun - mt) : 1.0f;
@@ -566,32 +683,44 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
             for (int j = 0; j < 4; j++) acc[g][j] *= alpha;
         }
         const float mb = mrun == -INFINITY ? 0.0f : mrun;
-        half4_t pf;
+        half8_t pf;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const float p = __builtin_amdgcn_exp2f(S[r] - mb);
-          pf[r] = (hxa_h)(iv[r] < 1.0f / HXA_Q8_LEAST ? p : p == p ? 0.0f : p);  // a page without a scale: values of 0, whatever the bytes
-          lsum = fmaf(p, iv[r], lsum);
+        for (int h = 0; h < 2; h++) {
+          float l = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            constexpr int one = G8 ? 0 : ~0;
+            const float iv = i4[h][r & one], p = __builtin_amdgcn_exp2f(fmaf(S[h][r], k4[h][r & one], l4[h][r & one] - mb));
+            pf[4 * h + r] = (hxa_h)(iv < 1.0f / HXA_Q8_LEAST ? p : p == p ? 0.0f : p);  // a page without a scale: values of 0, whatever the bytes
+            l = G8 ? l + p : fmaf(p, iv, l);
+          }
+          lsum = G8 ? fmaf(l, i4[h][0], lsum) : lsum + l;
         }
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-          uint32_t w[4];
+          // bytes of two keys side by side, dims 0, 1 (w[..][0]) and 2, 3
+          uint32_t w[4][2];
 #pragma unroll
-          for (int e = 0; e < 4; e++) w[e] = *(const uint32_t *)(vat + at + 4 * e * HD + vch[g]) ^ 0x80808080u;
-          // bytes of two keys side by side, dims 0, 1 and 2, 3
-          const uint32_t a0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), a1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
-          const uint32_t b0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), b1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+          for (int y = 0; y < 4; y++) {
+            const uint32_t lo = vr[y >> 1][g][2 * (y & 1)] ^ 0x80808080u, hi = vr[y >> 1][g][2 * (y & 1) + 1] ^ 0x80808080u;
+            w[y][0] = __builtin_amdgcn_perm(hi, lo, 0x05010400u);
+            w[y][1] = __builtin_amdgcn_perm(hi, lo, 0x07030602u);
+          }
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            const uint32_t sel = j & 1 ? 0x04030402u : 0x04010400u;
             const half2_t bias = {(hxa_h)1152.0f, (hxa_h)1152.0f};
-            const half2_t lo = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, j < 2 ? a0 : a1, sel)) - bias;
-            const half2_t hi = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, j < 2 ? b0 : b1, sel)) - bias;
-            acc[g][j] = mma16h(__builtin_shufflevector(lo, hi, 0, 1, 2, 3), pf, acc[g][j]);
+            half8_t v;
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+              const half2_t z = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[y][j >> 1], j & 1 ? 0x04030402u : 0x04010400u)) - bias;
+              v[2 * y] = z[0];
+              v[2 * y + 1] = z[1];
+            }
+            acc[g][j] = mma16(v, pf, acc[g][j]);
           }
         }
       }
-      t0 = t1;
+      s0 = s1;
     }
     lsum = add16(lsum);
   }
@@ -651,23 +780,23 @@ constexpr int lds_q8() { return std::max(GeoQ8<HD>::LDS, FewQ8<HD>::LDS); }
 struct CachedQ8Args : CachedArgs {
   const float *ks, *vs;
 };
-template <typename T, int HD>
+template <typename T, int HD, bool G8>
 HXA_DEV void any_item_q8(int mode, const KeysQ8 &s, const Item &it, const CachedQ8Args &p, int head0, uint8_t *lds, const Out<T> &out) {
   if (mode == 1) {
-    few_item_q8<T, HD>(s, it, (const T *)p.q, p.ldq, head0, p.cs, lds, out);
+    few_item_q8<T, HD, G8>(s, it, (const T *)p.q, p.ldq, head0, p.cs, lds, out);
     return;
   }
   float16_t acc[HD / 32];
   float m, l;
   if (mode == 2) {
-    rows_item_q8<T, HD, 2>(s, it, (const T *)p.q, p.ldq, head0, p.cs, lds, acc, m, l);
+    rows_item_q8<T, HD, 2, G8>(s, it, (const T *)p.q, p.ldq, head0, p.cs, lds, acc, m, l);
     rows_out<T, HD, 2>(out, it, head0, 1.0f, lds, acc, m, l);
   } else {
-    rows_item_q8<T, HD, 4>(s, it, (const T *)p.q, p.ldq, head0, p.cs, lds, acc, m, l);
+    rows_item_q8<T, HD, 4, G8>(s, it, (const T *)p.q, p.ldq, head0, p.cs, lds, acc, m, l);
     rows_out<T, HD, 4>(out, it, head0, 1.0f, lds, acc, m, l);
   }
 }
-template <typename T, int HD>
+template <typename T, int HD, bool G8>
 __global__ HXA_CAUSAL_BOUNDS void cached_q8_kernel(CachedQ8Args p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int h = blockIdx.x % p.c.H;
@@ -676,7 +805,7 @@ __global__ HXA_CAUSAL_BOUNDS void cached_q8_kernel(CachedQ8Args p) {
   s.v = (const int8_t *)p.c.v;
   s.ks = p.ks;
   s.vs = p.vs;
-  walk_cache<T, lds_q8<HD>()>(p, h, s, lds, [&](int mode, const Item &it, const Out<T> &out) { any_item_q8<T, HD>(mode, s, it, p, h * p.G, lds, out); });
+  walk_cache<T, lds_q8<HD>()>(p, h, s, lds, [&](int mode, const Item &it, const Out<T> &out) { any_item_q8<T, HD, G8>(mode, s, it, p, h * p.G, lds, out); });
 }
 
 int q8_check(const hxa_kv_cache_q8 *c, int T, int Hq) {
@@ -688,7 +817,7 @@ int q8_check(const hxa_kv_cache_q8 *c, int T, int Hq) {
 
 extern "C" long hxa_attention_cached_q8_ws_bytes(const hxa_kv_cache_q8 *c, int T, int Hq) {
   if (q8_check(c, T, Hq) != HXA_OK || T == 0 || c->c.nseq == 0) return 0;
-  return cached_ws(cached_plan(c->c, T, Hq, true, wg_slots(c->c.hd)), c->c, T, Hq);
+  return cached_ws(cached_plan(c->c, T, Hq, true, wg_slots(c->c.hd), true), c->c, T, Hq);
 }
 
 extern "C" int hxa_attention_cached_q8(const hxa_kv_cache_q8 *cache, const void *q, long ldq, void *o, long ldo, int T, int Hq, float scale,
@@ -699,9 +828,11 @@ extern "C" int hxa_attention_cached_q8(const hxa_kv_cache_q8 *cache, const void 
   p.ks = cache->kscale;
   p.vs = cache->vscale;
   return cached_call(
-      p, cache->c, q, ldq, o, ldo, T, Hq, scale, ws, ws_bytes, (hipStream_t)stream, "attention_cached_q8",
-      [](auto ty, auto hdc) {
+      p, cache->c, q, ldq, o, ldo, T, Hq, scale, ws, ws_bytes, (hipStream_t)stream, "attention_cached_q8", true,
+      [](auto ty, auto hdc, const CachedPlan &pl, const hxa_kv_cache &d) {
         constexpr int HD = decltype(hdc)::value;
-        return std::make_pair(cached_q8_kernel<decltype(ty), HD>, lds_q8<HD>() + 4096);
+        // pages hold whole groups of eight keys, counted from where a range may begin
+        const bool g8 = d.page % 8 == 0 && (d.prefix_len % 8 == 0 || pl.x_first == d.prefix_len);
+        return std::make_tuple(g8 ? cached_q8_kernel<decltype(ty), HD, true> : cached_q8_kernel<decltype(ty), HD, false>, lds_q8<HD>() + 4096, g8 ? 6 : 0);
       });
 }

@@ -5,7 +5,7 @@
 #include <cmath>
 #include <mutex>
 #include <type_traits>
-#include <utility>
+#include <tuple>
 
 #include "causal.h"
 #include "causal_walk.h"
@@ -327,16 +327,17 @@ HXA_DEV void walk_cache(const CachedArgs &p, int h, K &s, uint8_t *lds, F run) {
       it.x1 = (int)min((long)end, p.p.x_first + (long)w.t1 * KT);
       slot_end = p.p.sp_max + p.p.s_max;
     }
-    if (p.part != nullptr && w.last) {  // slots that no range fills: sums of nothing
+    const bool none = p.part != nullptr && !w.shared && it.x1 <= it.x0;  // a piece that ends before the block's first tile
+    if (p.part != nullptr && (w.last || none)) {  // slots that no range fills: sums of nothing
       const int rows = min(mode_rows(mode), it.nrows - it.r0);
-      const int free = slot_end - w.slot - 1;
+      const int from = none ? w.slot : w.slot + 1, free = (w.last ? slot_end : w.slot + 1) - from;
       for (int j = threadIdx.x; j < rows * free; j += 256) {
         int head;
         const int row = j / free, tok = row_tok(it, it.r0 + row, head);
-        p.ml[((long)(it.tok0 + tok) * p.Hq + h * p.G + head) * (p.p.sp_max + p.p.s_max) + w.slot + 1 + j - row * free] = (float2_t){-INFINITY, 0.0f};
+        p.ml[((long)(it.tok0 + tok) * p.Hq + h * p.G + head) * (p.p.sp_max + p.p.s_max) + from + j - row * free] = (float2_t){-INFINITY, 0.0f};
       }
     }
-    run(mode, it, Out<T>{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, w.slot, p.p.sp_max + p.p.s_max, p.Hq});
+    if (!none) run(mode, it, Out<T>{(T *)p.o, p.ldo, p.part, p.ml, (long)p.T * p.Hq, w.slot, p.p.sp_max + p.p.s_max, p.Hq});
     if (k.pos >= k.end) return;
     reads_done_barrier();  // every wave is done with the LDS
     if (!further_work<Wave>(p, k, stash, w)) return;
@@ -446,18 +447,19 @@ int cached_limits(const hxa_kv_cache &c, int T, int Hq, const char *who) {
     return hxa_set_error(HXA_E_ARG, "%s: T=%d nseq=%d H=%d are too many blocks", who, T, c.nseq, c.H);
   return HXA_OK;
 }
-// the call, after its checks of the cache; f gives the kernel of a type and head width and its bytes of LDS
+// the call, after its checks of the cache; f gives the kernel of a type and head width, its bytes of LDS, and 0 or, for a second kernel of the same type
+// and width, 6
 template <typename A, typename F>
 int cached_call(A &p, const hxa_kv_cache &c, const void *q, long ldq, void *o, long ldo, int T, int Hq, float scale, void *ws, long ws_bytes,
-                hipStream_t st, const char *who, F f) {
+                hipStream_t st, const char *who, bool q8, F f) {
   if (!(scale > 0.0f) || !std::isfinite(scale)) return hxa_set_error(HXA_E_ARG, "%s: scale %g", who, (double)scale);
   if (T == 0 || c.nseq == 0) return HXA_OK;
   if (!rows_ok(q, ldq, Hq, c.hd) || !rows_ok(o, ldo, Hq, c.hd))
     return hxa_set_error(HXA_E_ARG, "%s: pointers null or not 16-byte aligned, or strides (%ld %ld)", who, ldq, ldo);
   if ((uintptr_t)ws % 16) return hxa_set_error(HXA_E_ARG, "%s: workspace not aligned", who);
-  CachedPlan pl = cached_plan(c, T, Hq, true, wg_slots(c.hd));
+  CachedPlan pl = cached_plan(c, T, Hq, true, wg_slots(c.hd), q8);
   const long need = cached_ws(pl, c, T, Hq);
-  if (need > 0 && (ws == nullptr || ws_bytes < need)) pl = cached_plan(c, T, Hq, false, wg_slots(c.hd));
+  if (need > 0 && (ws == nullptr || ws_bytes < need)) pl = cached_plan(c, T, Hq, false, wg_slots(c.hd), q8);
   const int nslots = pl.sp_max + pl.s_max;
   static_cast<CachedArgs &>(p) = CachedArgs{{c, T, Hq / c.H, pl}, q, o, ldq, ldo, Hq, recip(Hq / c.H), recip(c.page), scale * L2E, nullptr, nullptr};
   if (nslots > 1) {
@@ -466,10 +468,10 @@ int cached_call(A &p, const hxa_kv_cache &c, const void *q, long ldq, void *o, l
   }
   const long wgs = cached_items(pl) * c.H;
   return by_type(c.dtype, c.hd, [&](auto ty, auto hdc, int id) -> int {
-    const auto k = f(ty, hdc);
-    const int a = allow_lds((const void *)k.first, k.second, 12 + id);
-    if (a != HXA_OK) return hxa_set_error(a, "%s: %d bytes of LDS", who, k.second);
-    hxa_launch(k.first, dim3((unsigned)wgs), dim3(256), k.second, st, p);
+    const auto [k, lds, more] = f(ty, hdc, pl, c);
+    const int a = allow_lds((const void *)k, lds, 12 + id + more);
+    if (a != HXA_OK) return hxa_set_error(a, "%s: %d bytes of LDS", who, lds);
+    hxa_launch(k, dim3((unsigned)wgs), dim3(256), lds, st, p);
     if (nslots > 1)
       hxa_launch(cached_merge_kernel<decltype(ty), decltype(hdc)::value>, dim3((unsigned)ceil_div((long)T * Hq, 4)), dim3(256), 0, st,
                  static_cast<const CachedArgs &>(p));

@@ -705,9 +705,9 @@ extern "C" int hxa_attention_cached(const hxa_kv_cache *c, const void *q, long l
   const int r = cached_check(c, T, Hq);
   if (r != HXA_OK) return r;
   CachedArgs p{};
-  return cached_call(p, *c, q, ldq, o, ldo, T, Hq, scale, ws, ws_bytes, (hipStream_t)stream, "attention_cached", [](auto ty, auto hdc) {
+  return cached_call(p, *c, q, ldq, o, ldo, T, Hq, scale, ws, ws_bytes, (hipStream_t)stream, "attention_cached", false, [](auto ty, auto hdc, const CachedPlan &, const hxa_kv_cache &) {
     typedef decltype(ty) T_;
     constexpr int HD = decltype(hdc)::value;
-    return std::make_pair(cached_kernel<T_, HD>, Geo<T_, HD>::LDS + 4096);
+    return std::make_tuple(cached_kernel<T_, HD>, Geo<T_, HD>::LDS + 4096, 0);
   });
 }

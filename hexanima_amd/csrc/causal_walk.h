@@ -107,7 +107,9 @@ inline int second_layer(int hd, int ncu, int Hk) { return hd == 256 ? 1 << 29 : 
 // neither one long sequence among short ones nor a few items more than places decide the time (128 sequences, 32 / 8 heads, 500 keys behind 300:
 // 71 -> 65 us against pieces in their own blocks, 1024 of 300 behind 600: 458 -> 315; 16 of 1000: 18.8 us so, 20.2 cut anywhere).
 // Not split, an item is a block.
-constexpr int SEG = 2;
+// Over a cache of int8 a tile of few rows takes a third of the time that its setup and result take for the same keys, and its way to fp16 makes a tile of the prefix
+// dearer: the plan has both numbers (SEG and 5/4 where keys are 16 bits).
+constexpr int SEG = 2, PRE4 = 5, Q8_SEG = 6, Q8_PRE4 = 8;
 // what the host decides, from sizes that it knows
 struct CachedPlan {
   int np_mode, np_blocks, sp_max;  // sp_max 0: nothing is shared
@@ -116,6 +118,7 @@ struct CachedPlan {
   int budget;     // items a key head that run at once
   int least;      // tiles an item is worth
   int n_blocks;   // at most, of a key head
+  int seg, pre4;  // what a block counts beside its tiles, and four tiles of the prefix, in tiles of few rows
 };
 struct CachedWork {
   hxa_kv_cache c;
@@ -176,8 +179,8 @@ struct Walk {
   bool own_pieces;  // a block is a whole number of pieces in the list
 };
 template <class W>
-HXA_ANY typename W::I list_tiles(const Walk &k, const Lanes<W> &s) {
-  return W::map([&](int t) { return k.own_pieces ? (int)ceil_of<W>(imax(t, 1), k.chunk) * k.chunk : t + SEG; }, s.tiles);
+HXA_ANY typename W::I list_tiles(const Walk &k, const Lanes<W> &s, int seg) {
+  return W::map([&](int t) { return k.own_pieces ? (int)ceil_of<W>(imax(t, 1), k.chunk) * k.chunk : t + seg; }, s.tiles);
 }
 template <class W>
 HXA_ANY typename W::I list_ends(const Lanes<W> &s, const typename W::I &each) {
@@ -231,11 +234,11 @@ HXA_ANY bool next_work(const CachedWork &p, Walk &k, Lanes<W> &s, typename W::I 
     k.base += 64;
     if (k.base >= p.c.nseq) return false;
     s.load(p, k.base);
-    each = list_tiles<W>(k, s);
+    each = list_tiles<W>(k, s, p.p.seg);
     inc = list_ends<W>(s, each);
   }
   W::keep(stash, s.b, s.n, s.len, inc);
-  const int l = __builtin_ctzll(hit), seg = k.own_pieces ? 0 : SEG;
+  const int l = __builtin_ctzll(hit), seg = k.own_pieces ? 0 : p.p.seg;
   take(w, s, l, k.base);
   const int eff = W::get(each, l), nb = W::get(s.nb, l);
   int at = k.pos - (k.seen + W::get(inc, l) - nb * eff);
@@ -256,7 +259,7 @@ HXA_ANY bool further_work(const CachedWork &p, Walk &k, typename W::Stash stash,
   typename W::I inc;
   W::kept(stash, s.b, s.n, s.len, inc);
   s.sizes(p);
-  return next_work<W>(p, k, s, list_tiles<W>(k, s), inc, stash, w);
+  return next_work<W>(p, k, s, list_tiles<W>(k, s, p.p.seg), inc, stash, w);
 }
 // the first work of item `q` of a key head, split
 template <class W>
@@ -272,21 +275,21 @@ HXA_ANY bool first_work(const CachedWork &p, int q, typename W::Stash stash, Wal
                                                              : __builtin_popcountll(W::ballot([](int nb) { return nb > 0; }, s.nb));
     longest = imax(longest, W::most(s.tiles));
   }
-  // a tile of 128 rows takes about 5/4 of one of 16 (4600 cycles, 3800)
-  const uint32_t pre = (uint32_t)a.np_blocks * pt * 5 / 4;
-  uint32_t chunk = umax(ceil_of<W>(own + SEG * blocks + pre, a.budget), (uint32_t)a.least);
+  // (16-bit keys: a tile of 128 rows takes about 5/4 of one of 16, 4600 cycles, 3800)
+  const uint32_t pre = (uint32_t)a.np_blocks * pt * a.pre4 / 4;
+  uint32_t chunk = umax(ceil_of<W>(own + a.seg * blocks + pre, a.budget), (uint32_t)a.least);
   // no more pieces of a block than slots
-  if (longest + SEG - 1 > (long)chunk * (a.s_max - 1)) chunk = ceil_of<W>(longest + SEG - 1, a.s_max - 1);
+  if (longest + a.seg - 1 > (long)chunk * (a.s_max - 1)) chunk = ceil_of<W>(longest + a.seg - 1, a.s_max - 1);
   k.own_pieces = false;
   const int taken = blocks + a.np_blocks;  // every block has one piece that is not full
   if (2 * taken <= a.budget) {
     uint32_t whole = umax(ceil_of<W>(own + pre, a.budget - taken), (uint32_t)a.least);
     if (longest > (long)whole * a.s_max) whole = ceil_of<W>(longest, a.s_max);
-    k.own_pieces = whole < chunk + SEG;
+    k.own_pieces = whole < chunk + a.seg;
     if (k.own_pieces) chunk = whole;
   }
   if (a.sp_max) {
-    const uint32_t cp = umax((chunk * 4 + 4) / 5, ceil_of<W>(pt, a.sp_max));
+    const uint32_t cp = umax((chunk * 4 + a.pre4 - 1) / a.pre4, ceil_of<W>(pt, a.sp_max));
     const int ns = (int)ceil_of<W>(pt, cp);
     if (q < ns * a.np_blocks) {
       w.shared = true;
@@ -300,14 +303,14 @@ HXA_ANY bool first_work(const CachedWork &p, int q, typename W::Stash stash, Wal
     }
     q -= ns * a.np_blocks;
   }
-  const int total = k.own_pieces ? 1 << 30 : own + SEG * blocks;
+  const int total = k.own_pieces ? 1 << 30 : own + a.seg * blocks;
   if ((uint64_t)q * chunk >= (uint32_t)total) return false;
   k.chunk = (int)chunk;
   k.pos = q * (int)chunk;
   k.end = imin(k.pos + (int)chunk, total);
   k.base = k.seen = 0;
   w.shared = false;
-  const typename W::I each = list_tiles<W>(k, s);
+  const typename W::I each = list_tiles<W>(k, s, p.p.seg);
   return next_work<W>(p, k, s, each, list_ends<W>(s, each), stash, w);
 }
 
@@ -330,11 +333,13 @@ inline long cached_ws(const CachedPlan &p, const hxa_kv_cache &c, int T, int Hq)
   return slots == 1 ? 0 : slots * T * Hq * (c.hd * 4L + 8);
 }
 // places: workgroups that run at once
-inline CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws, long places) {
+inline CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws, long places, bool q8 = false) {
   const auto least = [](long a, long b) { return a < b ? a : b; };
   const int G = Hq / c.H;
   const long RT = (long)T * G, P = c.prefix_len, cap = (long)c.ldt * c.page;
   CachedPlan p{};
+  p.seg = q8 ? Q8_SEG : SEG;
+  p.pre4 = q8 ? Q8_PRE4 : PRE4;
   const int mode = rows_mode(ceil_div(RT, c.nseq));
   p.rb_log = mode == 4 ? 7 : 6;
   p.n_blocks = (int)((RT >> p.rb_log) + c.nseq);
@@ -349,6 +354,8 @@ inline CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws, lon
     p.sp_max = (int)least(32, least(ceil_div(P, KT), ceil_div(p.budget, p.np_blocks) + 1));
     p.x_first = (int)P;
   }
+  // (int8: ranges and pieces, roundings included, are no more than places: one that began when the first have ended would end last)
+  if (q8) p.budget = imax(1, p.budget - p.np_blocks - 1);
   // a list that is cut anywhere: a block of so many ranges touches one workgroup more
   const long tiles = ceil_div(cap + P - p.x_first, KT);
   if (mode == 1) p.s_max = most <= 16 && blocks * c.H * 4 >= places && p.sp_max == 0 ? 1 : (int)least(31, tiles);
@@ -357,7 +364,7 @@ inline CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws, lon
   if (p.s_max > 1 || p.sp_max > 0) p.s_max++;
   while (p.s_max > 2 && cached_ws(p, c, T, Hq) > 1L << 30) p.s_max = p.s_max / 2 + 1;
   // a piece stays below 2^24 tiles (all tiles / half the budget at the most), so that its keys are counted in 31 bits, and the list below 2^29
-  const long list = p.n_blocks * (tiles + SEG) + ceil_div(P, KT) * p.np_blocks * 2;
+  const long list = p.n_blocks * (tiles + p.seg) + ceil_div(P, KT) * p.np_blocks * (q8 ? 4 : 2);
   if (list >= least(1L << 29, (long)p.budget << 23)) p.sp_max = p.np_blocks = p.x_first = 0, p.s_max = 1;
   return p;
 }

@@ -1,7 +1,7 @@
 """Helpers of the 8-bit text model's tests: the operators' definitions in 64 bits (32 where a definition names a 32-bit step), and caches of int8."""
 import numpy as np
 
-from tests._causal import HALF_STEP, TINY, U24, Cache, narrow, norm_rope, widen
+from tests._causal import BF16, HALF_STEP, TINY, U24, Cache, narrow, norm_rope, widen
 
 LEAST = np.float32(2.0 ** -64)
 
@@ -47,11 +47,12 @@ def linear_bound(dot, want, dtype):
     return HALF_STEP[dtype] * np.abs(want) + 3 * U24 * (np.abs(dot) + np.abs(want)) + TINY[dtype]
 
 
-def attend_q8_bound(o, a, vtop, n, hd, smax, lmax, dtype):
+def attend_q8_bound(o, a, vtop, n, hd, smax, lmax, kmax, dtype):
     """As attend_bound: the output's own rounding; the weights' rounding to fp16 (relative 2^-11 of the mean of |v|; 2^-25 where they are subnormal, of
     weights of which the largest is at least 1 before its byte, so n 2^-25 127 of the largest scale); the fp32 sums; the exponent's terms, the score
-    (smax) and the logarithm of the value's scale (lmax), each with a few half steps of its own."""
-    return HALF_STEP[dtype] * np.abs(o) + (2.0 ** -11 + (n + (hd + 8) * smax + 8 * lmax + 256) * U24) * a + n * 2.0 ** -25 * vtop + TINY[dtype]
+    (smax) and the logarithm of the value's scale (lmax), each with a few half steps of its own; of bf16 queries what fp16 loses beside a largest value of 1 or more, 2^-25 a
+    dim, times the largest key (kmax, scaled)."""
+    return HALF_STEP[dtype] * np.abs(o) + (2.0 ** -11 + (n + (hd + 8) * smax + 8 * lmax + 256) * U24 + hd * 2.0 ** -25 * kmax) * a + n * 2.0 ** -25 * vtop + TINY[dtype]
 
 
 class CacheQ8(Cache):
@@ -97,10 +98,12 @@ class CacheQ8(Cache):
                 out[x], ok[x] = val[e, :, y % self.page], True
         return out, ok
 
-    def bound(self, o, a, n, smax):
+    def bound(self, o, a, n, smax, scale):
         good = self.vs[np.isfinite(self.vs) & (self.vs > 0)].astype(np.float64)
         lmax = np.abs(np.log2(good)).max(initial=64.0)
-        return attend_q8_bound(o, a, 127 * good.max(initial=0.0), n, self.hd, smax, lmax, self.dtype)
+        ks = self.ks[np.isfinite(self.ks) & (self.ks > 0)].astype(np.float64)
+        kmax = 127 * ks.max(initial=0.0) * scale if self.dtype == BF16 else 0.0
+        return attend_q8_bound(o, a, 127 * good.max(initial=0.0), n, self.hd, smax, lmax, kmax, self.dtype)
 
 
 def append(c, k, v, gain, eps, freq, layout, T):

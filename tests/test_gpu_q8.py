@@ -317,7 +317,7 @@ def run_cached(hip, c, q, scale, with_ws=True, stream=None):
 def check_cached(hip, c, q, scale, with_ws, what):
     got = run_cached(hip, c, q, scale, with_ws)
     o, a, n, smax, _ = c.expect(q, scale)
-    close(got, o, c.bound(o, a, n, smax), what)
+    close(got, o, c.bound(o, a, n, smax, scale), what)
     return got
 
 
@@ -436,7 +436,7 @@ def test_cached_q8_lengths_out_of_range(hip):
         o, a, n, smax, _ = held.expect(q, hd ** -0.5)
         for ws in (True, False):
             got = run_cached(hip, c, q, hd ** -0.5, ws)
-            close(got, o, held.bound(o, a, n, smax), "lengths")
+            close(got, o, held.bound(o, a, n, smax, hd ** -0.5), "lengths")
             assert prefix or (got[:2] == 0).all()
     c = CacheQ8(hip, rng, [1, 2], [0, 0], 300, page, H, hd, F16)
     q = queries(rng, 3, Hq, hd, F16)
@@ -446,7 +446,7 @@ def test_cached_q8_lengths_out_of_range(hip):
     none.lens, none.past = [0, 0], [10 ** 6] * 2
     o, a, n, smax, _ = none.expect(q, hd ** -0.5)
     for ws in (True, False):
-        close(run_cached(hip, c, q, hd ** -0.5, ws), o, none.bound(o, a, n, smax), "prefix alone")
+        close(run_cached(hip, c, q, hd ** -0.5, ws), o, none.bound(o, a, n, smax, hd ** -0.5), "prefix alone")
 
 
 def test_q8_offsets_past_32_bits(hip):
@@ -478,7 +478,7 @@ def test_q8_offsets_past_32_bits(hip):
         s = (c.ks if pool is c.k else c.vs).max()
         assert np.abs(got - widen(rows, F16).reshape(n, H, hd)).max() <= s * 0.5001
     o, a, m, smax, _ = c.expect(widen(q, F16).reshape(n, Hq, hd), hd ** -0.5)
-    close(widen(x[3].numpy(), F16).reshape(n, Hq, hd), o, c.bound(o, a, m, smax), "cached")
+    close(widen(x[3].numpy(), F16).reshape(n, Hq, hd), o, c.bound(o, a, m, smax, hd ** -0.5), "cached")
 
 
 def test_q8_two_streams_at_once(hip):
@@ -602,7 +602,7 @@ def test_a_layer_in_8_bits(hip, dtype):
                      what + " append")
         qh = widen(g["q"], dtype).reshape(n, Hq, hd)
         o, a, m, smax, _ = c.expect(qh, scale)
-        close(widen(g["o"], dtype).reshape(n, Hq, hd), o, c.bound(o, a, m, smax), what + " attention")
+        close(widen(g["o"], dtype).reshape(n, Hq, hd), o, c.bound(o, a, m, smax, scale), what + " attention")
 
     states = [narrow(rng.standard_normal((n + steps, 504)), dtype) for n in rest]
     b = buffers(sum(rest))
