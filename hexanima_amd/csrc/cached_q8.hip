@@ -154,7 +154,8 @@ HXA_DEV float most_of(const V (&q)[N]) {
 
 // ---- rows modes: as causal_attn.hip's rows_item; m and the sums in powers of two ----
 // G8: eight keys of a lane (8 g + 0 .. 7 of every 16) lie on one page, so that they share its scales: the maximum is taken of the scores, the
-// scales go into one fma a score. (With constants for each key, three 16-byte reads of LDS for four of them, the LDS decides: @G8@.)
+// scales go into one fma a score. (With constants for each key, 24 more 16-byte reads of
+// LDS a tile: 32 prompts of 75 behind 4000 186 us against 168.)
 template <typename T, int HD, int W, bool G8>
 HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, int head0, float c, uint8_t *lds, float16_t (&acc)[HD / 32],
                           float &mrun, float &lsum) {

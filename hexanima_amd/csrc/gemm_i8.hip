@@ -44,16 +44,21 @@ __global__ __launch_bounds__(256) void sum_i8_kernel(GemmParamsI8 p, const int *
   *(uint4_t *)(p.out + (long)m * p.ldo + n) = (uint4_t){x.x, x.y, y.x, y.y};
 }
 
-// Cost of a form, as gemm.hip's: rounds of workgroups over the CUs x (a BM BN K + b) + c us; bn 32: gemm_skinny.hip's tiles
+// Cost of a form, as gemm.hip's: rounds of workgroups over the CUs x (a BM BN K + b) + c us, and for K slices the sum's launch and its bytes. bn 32, 16: gemm_skinny.hip's
+// tiles (2048 x 8192 weights, one token: 16 x 16 over 8 waves 6.5, 32 x 32 over 4 9.6; 64 tokens: 32 x 16 9.4, 32 x 32 11.8, 64 x 64 in four slices 12.3).
+// Fitted to every tile timed, weights from HBM, on 174 (M, N, K) of 1 - 6500 rows x 10 weights of 1 - 34 MB, in one to eight slices; the
+// choice is 1.0% above the fastest form (geometric mean).
 struct Cost {
   int bm, bn;
   float a, b, c;  // a per 2^20 BM BN K
 };
 constexpr Cost kCost[] = {
-    {256, 256, 0.15f, 7.8f, 0.0f}, {256, 192, 0.155f, 6.7f, 0.0f}, {192, 256, 0.155f, 6.9f, 0.0f}, {192, 192, 0.17f, 6.3f, 0.0f},
-    {256, 128, 0.165f, 5.9f, 0.0f}, {128, 256, 0.17f, 6.1f, 0.0f}, {192, 128, 0.18f, 5.6f, 0.0f}, {128, 128, 0.20f, 5.0f, 0.0f},
-    {64, 128, 0.27f, 1.6f, 2.3f}, {128, 64, 0.28f, 1.7f, 2.0f}, {64, 64, 0.36f, 1.1f, 2.4f}, {64, 32, 0.51f, 3.2f, 0.0f}, {32, 32, 0.73f, 2.5f, 0.6f},
+    {256, 256, 0.1647f, 9.89f, 3.83f}, {256, 192, 0.1936f, 7.32f, 3.54f}, {192, 256, 0.1934f, 7.97f, 2.80f}, {192, 192, 0.1765f, 8.45f, 1.19f},
+    {256, 128, 0.1776f, 7.63f, 1.56f}, {128, 256, 0.1922f, 7.32f, 1.94f}, {192, 128, 0.1991f, 6.88f, 0.76f}, {128, 128, 0.2513f, 5.51f, 0.47f},
+    {64, 128, 0.3865f, 1.03f, 3.17f}, {128, 64, 0.3898f, 0.26f, 4.05f}, {64, 64, 0.4510f, 1.20f, 2.92f}, {64, 32, 0.5902f, 2.01f, 1.97f},
+    {32, 32, 0.8709f, 1.43f, 2.45f}, {32, 16, 0.9046f, 1.10f, 3.31f}, {16, 16, 1.3548f, 0.47f, 4.06f},
 };
+constexpr double kSumUs = 3.0, kSumBytesPerUs = 12.0e6;
 struct Form {
   int bm, bn, ksplit;
 };
@@ -73,9 +78,9 @@ Form form_of(int M, int N, int K, bool split) {
   double best = 1e30;
   for (int S = 1; S <= (split ? 8 : 1); S *= 2) {
     if (K % (128 * S) || (S > 1 && K / S < 512)) continue;
-    const double sum = S == 1 ? 0.0 : 2.0 + (8.0 * S + 2.0) * M * (double)N / 12.0e6;
+    const double sum = S == 1 ? 0.0 : kSumUs + (8.0 * S + 2.0) * M * (double)N / kSumBytesPerUs;
     for (const Cost &c : kCost) {
-      if (c.bn == 32 && S > 1) continue;
+      if (c.bn <= 32 && S > 1) continue;
       const double t = cost_of(c, M, N, K, S) + sum;
       if (t < best) best = t, f = Form{c.bm, c.bn, S};
     }
@@ -127,8 +132,8 @@ int launch(GemmParamsI8 &p, const Form &f, void *ws, hipStream_t st, const char 
     if (best < 0 || bytes < best) best = bytes, p.xcd_gm = gm;
   }
   hipError_t e;
-  if (f.bn == 32) {
-    e = launch_skinny_i8(f.bm, p, st);
+  if (f.bn <= 32) {
+    e = launch_skinny_i8(f.bm, f.bn, p, st);
   } else if (!split) {
     e = launch_fmt<HXG_I8, false>(f.bm, f.bn, p, 1, st);
   } else {
@@ -172,7 +177,7 @@ extern "C" int hxa_linear_i8_tile(int dtype, const void *a, long lda, const floa
   const int r = prepare(p, dtype, a, lda, sa, M, w, ldw, sw, N, K, bias, out, ldo, "linear_i8_tile");
   if (r != HXA_OK || M == 0 || N == 0) return r;
   const Form f{bm, bn, ksplit};
-  if (!built(bm, bn) || ksplit < 1 || ksplit > 64 || padded(K) % (128 * ksplit) || (bn == 32 && ksplit > 1))
+  if (!built(bm, bn) || ksplit < 1 || ksplit > 64 || padded(K) % (128 * ksplit) || (bn <= 32 && ksplit > 1))
     return hxa_set_error(HXA_E_ARG, "linear_i8_tile: tile %d x %d, %d slices of K=%d", bm, bn, ksplit, K);
   if (ksplit > 1 && (ws == nullptr || (uintptr_t)ws % 16 || ws_bytes < ws_of(f, M, N)))
     return hxa_set_error(HXA_E_ARG, "linear_i8_tile: workspace");

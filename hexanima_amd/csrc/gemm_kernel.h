@@ -1294,7 +1294,7 @@ hipError_t launch_group_fmt(const GemmParams *ps, int G, int tiles, hipStream_t 
 }
 hipError_t launch_xattn(const GemmParams &p, hipStream_t st);  // gemm_f16.hip
 hipError_t launch_skinny(int bm, int fmt, bool asym, const GemmParams &p, hipStream_t st);  // gemm_skinny.hip: bm 32, 64
-hipError_t launch_skinny_i8(int bm, const GemmParamsI8 &p, hipStream_t st);                 // gemm_skinny.hip
+hipError_t launch_skinny_i8(int bm, int bn, const GemmParamsI8 &p, hipStream_t st);         // gemm_skinny.hip: bm 32, 64 with bn 32, 16, 32 with 16
 
 #define HXG_LAUNCHES(X, FMT, ASYM)                                                                                   \
   X template hipError_t launch_fmt<FMT, ASYM>(int, int, const GemmParams &, int, hipStream_t);                       \

@@ -6,9 +6,8 @@ namespace hxg {
 
 // Stage (64 k) of one wave: A rows of 128 B, W rows (fp16 128 B, int8 64 B, int4 32 B), the two groups' scale (and offset)
 // vectors; swizzled like gemm_body's stages.
-template <int BM, int FMT>
+template <int BM, int FMT, int BN = 32, int NW = 4>
 struct SkinnyGeo {
-  static constexpr int BN = 32, NW = 4;
   static constexpr int A_BYTES = BM * 128, W_BYTES = BN * (plain_fmt(FMT) ? 128 : FMT == HXA_W_Q8 ? 64 : 32);
   static constexpr int S_BYTES = plain_fmt(FMT) ? 0 : BN * 4;
   static constexpr int STAGE = A_BYTES + W_BYTES + 2 * S_BYTES;
@@ -27,10 +26,10 @@ struct SkinnyGeo {
 // Measured (cold weights, back to back; before: the fastest of one launch and split-K with a sum): int8 256 x 2048 x 2048
 // 13.3 -> 7.7 us, 64 x 2048 x 2048 9.8 -> 6.9, 1562 x 3072 x 128 (M x K x N) 20.9 (one launch) -> 10.1, 1562 x 8192 x 128
 // 48.7 (one launch) -> 18.4; fp16 256 x 2048 x 2048 11.9 -> 9.4.
-template <int BM, int FMT, bool ASYM>
-__global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(params_t<FMT> p) {
-  using G = SkinnyGeo<BM, FMT>;
-  constexpr int BN = G::BN, NW = G::NW, NS = G::NS, MI = BM / 16, NI = BN / 16;
+template <int BM, int FMT, bool ASYM, int BN = 32, int NW = 4>
+__global__ __launch_bounds__(64 * NW, 2) void gemm_skinny_kernel(params_t<FMT> p) {
+  using G = SkinnyGeo<BM, FMT, BN, NW>;
+  constexpr int NS = G::NS, MI = BM / 16, NI = BN / 16;
   constexpr bool QW = !plain_fmt(FMT);
   constexpr int NA = G::A_BYTES / 1024, NL = NA + G::W_BYTES / 1024, L = NL + (QW ? ASYM ? 2 : 1 : 0);
   static_assert(NS >= 3 && NS * L < 64, "ring");
@@ -211,7 +210,7 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(params_t<FMT> p) {
   __syncthreads();
 #pragma unroll
   for (int i = tid; i < BM * BN / 4; i += 64 * NW) {
-    const int row = i >> 3, c = (i & 7) * 4;
+    const int row = i / (BN / 4), c = i % (BN / 4) * 4;
     if (m0 + row >= p.M || n0 + c >= p.N) continue;  // N % 8 == 0: four columns are inside N or past it
     acc_t<FMT> s = *(const acc_t<FMT> *)(part + row * G::SROW + c);
 #pragma unroll
@@ -227,14 +226,14 @@ __global__ __launch_bounds__(256, 2) void gemm_skinny_kernel(params_t<FMT> p) {
   }
 }
 
-template <int BM, int FMT, bool ASYM>
+template <int BM, int FMT, bool ASYM, int BN = 32, int NW = 4>
 static hipError_t launch_skinny_t(const params_t<FMT> &p, hipStream_t st) {
-  auto kern = gemm_skinny_kernel<BM, FMT, ASYM>;
-  constexpr int lds = SkinnyGeo<BM, FMT>::LDS;
+  auto kern = gemm_skinny_kernel<BM, FMT, ASYM, BN, NW>;
+  constexpr int lds = SkinnyGeo<BM, FMT, BN, NW>::LDS;
   static std::atomic<uint64_t> attr{0};
   const hipError_t a = allow_lds_once((const void *)kern, lds, attr);
   if (a != hipSuccess) return a;
-  hxa_launch(kern, dim3(p.tiles_m * p.tiles_n), dim3(256), lds, st, p);
+  hxa_launch(kern, dim3(p.tiles_m * p.tiles_n), dim3(64 * NW), lds, st, p);
   return hipGetLastError();
 }
 template <int FMT, bool ASYM>
@@ -246,5 +245,9 @@ hipError_t launch_skinny(int bm, int fmt, bool asym, const GemmParams &p, hipStr
   if (fmt == HXA_W_Q8) return launch_skinny_fmt<HXA_W_Q8, false>(bm, p, st);
   return asym ? launch_skinny_fmt<HXA_W_Q4, true>(bm, p, st) : launch_skinny_fmt<HXA_W_Q4, false>(bm, p, st);
 }
-hipError_t launch_skinny_i8(int bm, const GemmParamsI8 &p, hipStream_t st) { return launch_skinny_fmt<HXG_I8, false>(bm, p, st); }
+// int8: 32 columns as the other formats, and for a decoding step 16 columns of 16 or 32 rows, K over 8 waves
+hipError_t launch_skinny_i8(int bm, int bn, const GemmParamsI8 &p, hipStream_t st) {
+  if (bn == 32) return launch_skinny_fmt<HXG_I8, false>(bm, p, st);
+  return bm == 16 ? launch_skinny_t<16, HXG_I8, false, 16, 8>(p, st) : launch_skinny_t<32, HXG_I8, false, 16, 8>(p, st);
+}
 }  // namespace hxg

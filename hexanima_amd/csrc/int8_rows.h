@@ -5,8 +5,8 @@
 // the least scale of values that are not all 0: scales of one cache stay within 2^-64 .. 2^121, so that the attention can hold their ratios in 32 bits
 constexpr float HXA_Q8_LEAST = 0x1p-64f;
 
-// the scale of values whose largest finite magnitude is top
-HXA_DEV float q8_scale(float top) { return top > 0.0f ? fmaxf(top / 127.0f, HXA_Q8_LEAST) : 0.0f; }
+// the scale of values whose largest finite magnitude is top (by the rounded 1 / 127: at most an ulp beside the quotient, without a division)
+HXA_DEV float q8_scale(float top) { return top > 0.0f ? fmaxf(top * (1.0f / 127.0f), HXA_Q8_LEAST) : 0.0f; }
 // |x|, 0 where it is not finite
 HXA_DEV float finite_abs(float x) {
   const float a = fabsf(x);

@@ -1,4 +1,4 @@
-// Rows of 16-bit values to int8 with a scale each (hxa_quantize_rows): s = max |x| / 127, q = x (127 / max |x|) rounded to the nearest integer.
+// Rows of 16-bit values to int8 with a scale each (hxa_quantize_rows): s = max |x| / 127, q = x (1 / max |x| * 127) rounded to the nearest integer.
 //
 // Bound by HBM: 2 bytes read and 1 written per value. A row is held in registers between its maximum and its rounding, so it is read once: by one
 // wave where rows are short and many (no barrier), else by the four waves of a workgroup; rows of more than 16384 values are read a second time.
@@ -19,7 +19,7 @@ struct QuantArgs {
 // W waves a row, N chunks of 8 values a thread at a time
 template <typename T, int W, int N>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs p) {
-  typedef typename HxaVec<T>::v8 v8;
+  typedef typename HxaVec<T>::v8 v8 __attribute__((aligned(2)));  // rows begin anywhere (a contiguous matrix of an odd number of columns)
   constexpr int TPR = 64 * W;
   const int t = threadIdx.x % TPR;
   const long m = (long)blockIdx.x * (4 / W) + threadIdx.x / TPR;
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs p) {
     top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   }
   const float least = fmaxf(top, 127.0f * HXA_Q8_LEAST);
-  const float inv = top > 0.0f ? 127.0f / least : 0.0f;
+  const float inv = top > 0.0f ? 1.0f / least * 127.0f : 0.0f;
   if (t == 0) p.s[m] = q8_scale(top);
   const bool again = chunks > N * TPR;
   for (int base = 0; base < chunks; base += N * TPR) {
@@ -78,9 +78,9 @@ extern "C" int hxa_quantize_rows(int dtype, const void *x, long ldx, int M, int 
   if (dtype != HXA_DT_F16 && dtype != HXA_DT_BF16) return hxa_set_error(HXA_E_MODE, "quantize_rows: dtype %d", dtype);
   if (M < 0 || M > HXA_MAX_ROWS || K < 1 || K > HXA_I8_MAX_K) return hxa_set_error(HXA_E_ARG, "quantize_rows: M=%d K=%d", M, K);
   if (M == 0) return HXA_OK;
-  if (!x || (uintptr_t)x % 16 || !q || (uintptr_t)q % 16) return hxa_set_error(HXA_E_ARG, "quantize_rows: pointers null or not 16-byte aligned");
+  if (!x || (uintptr_t)x % 2 || !q || (uintptr_t)q % 16) return hxa_set_error(HXA_E_ARG, "quantize_rows: pointers null or not aligned");
   if (!scale || (uintptr_t)scale % 4) return hxa_set_error(HXA_E_ARG, "quantize_rows: scales null or not aligned");
-  if (ldx % 8 || ldx < K || ldq % 16 || ldq < (K + 127) / 128 * 128)
+  if (ldx < K || ldq % 16 || ldq < (K + 127) / 128 * 128)
     return hxa_set_error(HXA_E_ARG, "quantize_rows: strides (%ld %ld) for K=%d", ldx, ldq, K);
   const QuantArgs p{x, ldx, ldq, M, K, (int8_t *)q, scale};
   const hipStream_t st = (hipStream_t)stream;

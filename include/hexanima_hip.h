@@ -327,11 +327,12 @@ long hxa_attention_cached_ws_bytes(const hxa_kv_cache *c, int T, int Hq); /* 0: 
  * ============================================================================================================
  * Types, rows, sequences and plans are those of 3b. int8 values are two's complement; a value is its byte times a scale (fp32). Rounding to a byte
  * is to the nearest integer, ties to even, within +-127; a NaN becomes 0 and an infinity +-127 (0 where every finite value is 0). Scales are
- * max |x| / 127 over the finite values, at least 2^-64, or 0 where all of them are 0. */
+ * max |x| / 127 over the finite values (within an ulp), at least 2^-64, or 0 where all of them are 0. */
 #define HXA_I8_MAX_K 130944 /* a multiple of 128, up to which int32 sums of products of bytes are exact */
-/* Rows to int8: x [M][ldx] (dtype, K values a row, ldx % 8 == 0) to q [M][ldq] with q = x * (127 / max |x|) rounded and scale[m] = max |x| / 127. Columns
+/* Rows to int8: x [M][ldx] (dtype, K values a row, ldx >= K) to q [M][ldq] with q = x * (1 / max |x| * 127) rounded, in 32 bits, and scale[m] = max |x| / 127. Columns
  * K .. ceil(K / 128) 128 - 1 of q are written as zeros (ldq at least that, a multiple of 16); columns behind them are left as they are. Rows of a
- * weight [N][K] are its channels. M at most 2^25, K 1 .. HXA_I8_MAX_K; x and q 16-byte aligned, they do not overlap. */
+ * weight [N][K] are its channels. M at most 2^25, K 1 .. HXA_I8_MAX_K; x on whole values, q 16-byte
+ * aligned, they do not overlap. */
 int hxa_quantize_rows(int dtype, const void *x, long ldx, int M, int K, void *q, long ldq, float *scale, void *stream);
 /* Product of int8 rows: out[m][n] = sa[m] * sw[n] * (sum over k of a[m][k] * w[n][k]) + bias[n], out [M][ldo] of dtype. a [M][lda] and w [N][ldw] are
  * int8 rows that hold ceil(K / 128) 128 columns: those past K are multiplied too, so one of a and w has zeros there, as hxa_quantize_rows leaves them.
@@ -344,7 +345,7 @@ int hxa_linear_i8(int dtype, const void *a, long lda, const float *sa, int M, co
 long hxa_linear_i8_ws_bytes(int M, int N, int K);
 /* hxa_linear_i8 on a given tile (tuning, tests): bm x bn output tiles, ksplit slices of K, each a multiple of 128 (above 1: ksplit M N 4 bytes of
  * ws). Tiles: 256 x 256, 256 x 192, 192 x 256, 192 x 192, 256 x 128, 128 x 256, 192 x 128, 128 x 128, 64 x 128, 128 x 64, 64 x 64, and with ksplit
- * 1 64 x 32, 32 x 32. */
+ * 1 64 x 32, 32 x 32, 32 x 16, 16 x 16. */
 int hxa_linear_i8_tile(int dtype, const void *a, long lda, const float *sa, int M, const void *w, long ldw, const float *sw, int N, int K,
                        const float *bias, void *out, long ldo, int bm, int bn, int ksplit, void *ws, long ws_bytes, void *stream);
 /* A paged cache of int8: c as in 3b, but c.k and c.v are int8 pools [npages][H][page][hd] and c.dtype is the type of the rows that go in and come

@@ -16,8 +16,8 @@ def quantize(x):
         x = x.astype(np.float32)
         top = np.where(np.isfinite(x), np.abs(x), 0).max(-1).astype(np.float32)
         t = np.maximum(top, np.float32(127) * LEAST)
-        scale = np.where(top > 0, np.maximum(top / np.float32(127), LEAST), np.float32(0)).astype(np.float32)
-        inv = np.where(top > 0, np.float32(127) / t, np.float32(0)).astype(np.float32)
+        scale = page_scale(top)
+        inv = np.where(top > 0, np.float32(1) / t * np.float32(127), np.float32(0)).astype(np.float32)
         r = x * inv[..., None]
     return to_byte(r), scale
 
@@ -29,7 +29,7 @@ def to_byte(r):
 def page_scale(top):
     """the scale of values whose largest finite magnitude is top (fp32)"""
     top = np.asarray(top, np.float32)
-    return np.where(top > 0, np.maximum(top / np.float32(127), LEAST), np.float32(0)).astype(np.float32)
+    return np.where(top > 0, np.maximum(top * np.float32(1 / 127), LEAST), np.float32(0)).astype(np.float32)
 
 
 def grow(old, need):

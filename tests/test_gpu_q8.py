@@ -51,6 +51,20 @@ def test_quantize_rows(hip, dtype, M, K):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,K,ldx,off", [(5, 1003, 1003, 0), (1100, 229, 229, 1), (3, 8191, 8195, 3), (4, 16, 17, 5), (2, 20001, 20001, 7)])
+def test_quantize_rows_that_begin_anywhere(hip, dtype, M, K, ldx, off):
+    """row strides and first values of no alignment, the last row ending with the buffer"""
+    say("quant", dtype, M, K, ldx, off)
+    b = narrow(np.random.default_rng(K).standard_normal(off + (M - 1) * ldx + K), dtype)
+    rows = np.stack([b[off + m * ldx:off + m * ldx + K] for m in range(M)])
+    d = [dev(hip, b), dev(hip, np.full((M, round128(K)), 85, np.int8)), dev(hip, np.zeros(M, np.float32))]
+    hip.check(hip.lib().hxa_quantize_rows(dtype, d[0].at(2 * off), ldx, M, K, d[1].ptr, round128(K), d[2].ptr, None), "quantize_rows")
+    hip.sync()
+    wq, ws = quantize(widen(rows, dtype))
+    assert np.array_equal(d[2].numpy(), ws) and np.array_equal(d[1].numpy()[:, :K], wq) and not d[1].numpy()[:, K:].any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("M,K", [(6, 300), (1100, 96)])
 def test_quantize_special_rows(hip, dtype, M, K):
     """zeros, infinities, NaN, subnormal and largest values, ties"""
@@ -143,7 +157,7 @@ def test_linear_i8(hip, dtype, M, N, K):
         assert np.array_equal(p.run(dtype, with_ws=False), got)  # the same bits in every form
 
 
-TILES = [(256, 256), (256, 192), (192, 256), (192, 192), (256, 128), (128, 256), (192, 128), (128, 128), (64, 128), (128, 64), (64, 64), (64, 32), (32, 32)]
+TILES = [(256, 256), (256, 192), (192, 256), (192, 192), (256, 128), (128, 256), (192, 128), (128, 128), (64, 128), (128, 64), (64, 64), (64, 32), (32, 32), (32, 16), (16, 16)]
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 8, 128), (70, 200, 640), (300, 520, 1280), (513, 264, 256), (40, 40, 5120)])
@@ -155,7 +169,7 @@ def test_linear_i8_tiles(hip, M, N, K):
     close(widen(first, BF16), want, bound, "linear")
     for bm, bn in TILES:
         for S in (1, 2, 5):
-            if K % (128 * S) or (bn == 32 and S > 1):
+            if K % (128 * S) or (bn <= 32 and S > 1):
                 continue
             say("tile", bm, bn, S)
             assert np.array_equal(p.run(BF16, tile=(bm, bn, S)), first), (bm, bn, S)

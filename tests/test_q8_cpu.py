@@ -18,8 +18,8 @@ def quant(hip, **kw):
 
 @pytest.mark.parametrize("kw,rc", [
     (dict(dtype=0), -11), (dict(dtype=3), -11), (dict(M=-1), -12), (dict(M=2 ** 25 + 1), -12), (dict(K=0), -12), (dict(K=-5), -12),
-    (dict(K=130945, ldx=140000, ldq=140032), -12), (dict(x=None), -12), (dict(q=None), -12), (dict(scale=None), -12), (dict(x=FAKE + 8), -12),
-    (dict(q=FAKE + 8), -12), (dict(scale=FAKE + 2), -12), (dict(ldx=128), -12), (dict(ldx=132), -12), (dict(ldq=240), -12), (dict(ldq=264), -12)])
+    (dict(K=130945, ldx=140000, ldq=140032), -12), (dict(x=None), -12), (dict(q=None), -12), (dict(scale=None), -12), (dict(x=FAKE + 1), -12),
+    (dict(q=FAKE + 8), -12), (dict(scale=FAKE + 2), -12), (dict(ldx=128), -12), (dict(ldx=129), -12), (dict(ldq=240), -12), (dict(ldq=264), -12)])
 def test_quantize_rows_refuses(hip, kw, rc):
     assert quant(hip, **kw) == rc and hip.last_error().startswith("quantize_rows")
 
