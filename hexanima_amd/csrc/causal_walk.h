@@ -107,9 +107,11 @@ inline int second_layer(int hd, int ncu, int Hk) { return hd == 256 ? 1 << 29 : 
 // neither one long sequence among short ones nor a few items more than places decide the time (128 sequences, 32 / 8 heads, 500 keys behind 300:
 // 71 -> 65 us against pieces in their own blocks, 1024 of 300 behind 600: 458 -> 315; 16 of 1000: 18.8 us so, 20.2 cut anywhere).
 // Not split, an item is a block.
-// Over a cache of int8 a tile of few rows takes a third of the time that its setup and result take for the same keys, and its way to fp16 makes a tile of the prefix
-// dearer: the plan has both numbers (SEG and 5/4 where keys are 16 bits).
+// Over a cache of int8 a tile of few rows takes half the time or less, its setup and result as long as over 16 bits, and a tile of the prefix, which goes through fp16,
+// longer: counted as 6 and 2 (64 sequences of 1900 behind 4096, 32 / 8 heads: 74 -> 67 us; 16 of 5600 behind 32768: 72 -> 66).
 constexpr int SEG = 2, PRE4 = 5, Q8_SEG = 6, Q8_PRE4 = 8;
+// tiles up to which nothing is split: any batch, blocks that fill a quarter of the places
+constexpr int WHOLE = 6, WHOLE_MANY = 16, Q8_WHOLE = 10, Q8_WHOLE_MANY = 32;
 // what the host decides, from sizes that it knows
 struct CachedPlan {
   int np_mode, np_blocks, sp_max;  // sp_max 0: nothing is shared
@@ -323,7 +325,7 @@ HXA_ANY bool first_work(const CachedWork &p, int q, typename W::Stash stash, Wal
 //   read it block by block). No more slots than ranges first_work's chunk can make.
 //   Not split where the table and the prefix hold at most 6 tiles of keys, or 16 where the blocks fill a quarter of the places: a second
 //   launch and what the ranges set up take longer than the tiles one after the other (single tokens, 16 / 8 heads of 128, us split, whole: one
-//   sequence of 4 tiles 8.9, 7.4, of 8 9.2, 10.0; 16 of 4 9.6, 7.7, of 8 13.6, 11.1, of 16 19.5, 18.4; 64 of 4 18.2, 14.9, of 16 48.5, 43.1).
+//   sequence of 4 tiles 8.9, 7.4, of 8 9.2, 10.0; 16 of 4 9.6, 7.7, of 8 13.6, 11.1, of 16 19.5, 18.4; 64 of 4 18.2, 14.9, of 16 48.5, 43.1). int8: 10 tiles, 32 where the blocks are many (16 of 5: 13.1, 11.3; one of 13: 11.7, 14.0; 128 of 11, 32 / 8 heads: 33.7, 28.8; 16 of 20: 13.1, 16.4).
 //   Ranges of keys: with few rows as many as run at once; where the partials would pass 1 GB fewer, down to two of the own keys beside two of the
 //   prefix (four times T Hq rows in fp32). With more rows a partial
 //   result is as wide as a row's output is in fp32, so keys are split only where the blocks fill less than 5/8 of the places (32 prompts of
@@ -347,7 +349,7 @@ inline CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws, lon
   p.least = mode == 1 ? 1 : 4;
   p.s_max = 1;
   const long blocks = ceil_div(RT, mode_rows(mode)) + c.nseq / 2, most = ceil_div(cap + P, KT);
-  if (!ws || most <= 6) return p;
+  if (!ws || most <= (q8 ? Q8_WHOLE : WHOLE)) return p;
   if (mode == 1 && c.nseq >= 2 && P >= 4 * KT) {
     p.np_mode = rows_mode(RT);
     p.np_blocks = (int)ceil_div(RT, mode_rows(p.np_mode));
@@ -358,7 +360,7 @@ inline CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws, lon
   if (q8) p.budget = imax(1, p.budget - p.np_blocks - 1);
   // a list that is cut anywhere: a block of so many ranges touches one workgroup more
   const long tiles = ceil_div(cap + P - p.x_first, KT);
-  if (mode == 1) p.s_max = most <= 16 && blocks * c.H * 4 >= places && p.sp_max == 0 ? 1 : (int)least(31, tiles);
+  if (mode == 1) p.s_max = most <= (q8 ? Q8_WHOLE_MANY : WHOLE_MANY) && blocks * c.H * 4 >= places && p.sp_max == 0 ? 1 : (int)least(31, tiles);
   else if (blocks * c.H * 8 < places * 5) p.s_max = (int)least(8, least(tiles / p.least, ceil_div(places, blocks * c.H)));
   p.s_max = imax(1, p.s_max);
   if (p.s_max > 1 || p.sp_max > 0) p.s_max++;
