@@ -5,11 +5,11 @@
 //   t_j = (q . qk_j) (c ks_j) + log2(vs_j),   w_j = 2^(t_j - m),   o = sum w_j qv_j / sum w_j / vs_j
 // The values' scale is folded into the exponent, so that one running maximum m bounds what is rounded to fp16, the weight as it stands before its
 // byte: a key whose page has small values loses no bits to one whose page has large ones, and the products take the bytes as they are. A byte is exact
-// in fp16. q in bf16 is brought to fp16 by a power of two of its row, whose largest value it puts near 2^14: the row's values down to 2^-28 of that stay exact.
+// in fp16. q in bf16 becomes fp16 as it is where its row's largest magnitude is 1 .. 2^15, otherwise times the power of two that puts the largest near
+// 2^14: what is then 2^-17 or more stays exact, anything smaller is off by 2^-25 at most.
 // t, m, both sums and O are held in fp32; the denominator adds the weights before they are rounded.
 //
-// Rows modes: tiles of 64 keys go through registers, where they are turned into fp16 once for all four waves, into one of two places in LDS; that runs beside
-// the products of K of the tile before. A byte is finite whatever it holds, so that a masked key needs nothing but a weight of 0.
+// A byte is finite whatever it holds, so that a masked key needs nothing but a weight of 0.
 #include "causal_attn.h"
 #include "int8_rows.h"
 
@@ -21,10 +21,14 @@ struct KeysQ8 : Keys<int8_t> {
 
 template <int HD>
 struct GeoQ8 {
-  static constexpr int RB = HD * 2, TB = KT * RB;     // bytes of an fp16 row, of a tile
-  static constexpr int CST = 4 * TB;                  // past K, K, V, V: twice c ks, log2 vs and 1 / vs of the tile's keys
-  static constexpr int LDS = 4 * TB + 2048;
-  static constexpr int CH = HD / 16, N = KT * CH / 256;  // 16-byte chunks of a row of bytes; loads a thread, for K and for V each
+  static constexpr int RB = HD * 2, TB = KT * RB;    // bytes of an fp16 row, of a tile
+  static constexpr int CH = HD / 16, RPL = 64 / CH;  // 16-byte chunks of a row of bytes, rows of one wave-wide load
+  static constexpr int NLD = HD / 64;                // loads of a wave's keys of a tile, and of its values
+  static constexpr int WB = 16 * HD;                 // bytes of a wave's keys of a tile, and of its values
+  static constexpr int RAW = 2 * TB;                 // past K and V in fp16: each wave's bytes of two tiles
+  static constexpr int CST = RAW + 4 * 4 * WB;       // c ks, log2 vs and 1 / vs of the tile's keys
+  static constexpr int TABLE = CST + 768;            // the pages' table
+  static constexpr int LDS = TABLE + 512 * 16 + 16;
 };
 
 // stands for a key scale of 0: scores are as good as 0, and -infinity stays what it is
@@ -37,94 +41,6 @@ HXA_DEV uint2_t q8_halves(uint32_t d) {
   return (uint2_t){__builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - c),
                    __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - c)};
 }
-
-// The tiles of a work item in the rows modes: row krow_key(j) of LDS holds key j, in the orders of Swz
-template <int HD>
-struct LoaderQ8 {
-  typedef GeoQ8<HD> G_;
-  typedef Swz<hxa_h, HD, true> S_;
-  const KeysQ8 &s;
-  const Item &it;
-  uint8_t *lds;
-  const float c;
-  int tid, lane;
-  int ent;
-  unsigned in_page;
-  uint4_t raw[2][G_::N];
-  float ks, vs;  // of this lane's key
-  uint32_t to[2][2];  // where the two halves of this thread's first 16 bytes of K (V) go; its other ones are whole numbers of 16 rows behind
-  HXA_DEV LoaderQ8(const KeysQ8 &s_, const Item &it_, uint8_t *lds_, float c_, int tid_)
-      : s(s_), it(it_), lds(lds_), c(c_), tid(tid_), lane(tid_ & 63), ent(-1), in_page(0) {
-    entry(0);
-    const int row = krow_key(tid / G_::CH), ch = tid % G_::CH;  // (krow_key is its own inverse)
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      to[0][e] = row * G_::RB + (((2 * ch + e) ^ S_::fk(row)) << 4);
-      to[1][e] = row * G_::RB + (((2 * ch + e) ^ S_::fv(row)) << 4);
-    }
-  }
-  HXA_DEV void entry(int i) {  // the page of this lane's key of tile i
-    const int x = it.x0 + i * KT + lane;
-    ent = -1;
-    if (x < it.x1) {
-      const bool pre = x < s.P;
-      const unsigned y = pre ? x : x - s.P;
-      ent = (pre ? s.prefix : s.table)[s.slot(y, in_page)];
-    }
-  }
-  // begins the loads of tile i; the mask of its keys that are there
-  HXA_DEV uint64_t open(int i) {
-    const bool ok = (unsigned)ent < (unsigned)s.npages;  // (-1 past x1)
-    const uint32_t ph = ok ? (uint32_t)ent * s.H + s.h : 0;
-    const uint32_t at = ok ? ph * s.page + in_page : 0;  // < 2^32: checked on the host
-    const uint64_t mask = __ballot(ok);
-    ks = ok ? s.ks[ph] : 0.0f;
-    vs = ok ? s.vs[ph] : 0.0f;
-    if (it.x0 + i * KT + KT < it.x1) entry(i + 1);
-#pragma unroll
-    for (int n = 0; n < G_::N; n++) {
-      const int u = n * 256 + tid, key = u / G_::CH, ch = u % G_::CH;
-      const uint64_t row = (uint64_t)(uint32_t)__shfl((int)at, key) * HD + ch * 16;
-      raw[0][n] = *(const uint4_t *)(s.k + row);
-      raw[1][n] = *(const uint4_t *)(s.v + row);
-    }
-    return mask;
-  }
-  HXA_DEV uint8_t *kbuf(int i) const { return lds + (i & 1) * G_::TB; }
-  HXA_DEV uint8_t *vbuf(int i) const { return lds + (2 + (i & 1)) * G_::TB; }
-  HXA_DEV float *cst(int i) const { return (float *)(lds + G_::CST) + (i & 1) * 192; }
-  // the tile opened last, as tile i into LDS, in 2 N pieces; `begin` before them
-  HXA_DEV void begin(int i) {
-    const bool vok = vs > HXA_Q8_LEAST && vs < INFINITY;
-    const uint64_t zero = __ballot(!vok);
-    if (zero) {  // keys without a scale (or without a page): values of 0, whatever the bytes
-#pragma unroll
-      for (int n = 0; n < G_::N; n++)
-        if ((zero >> ((n * 256 + tid) / G_::CH)) & 1) raw[1][n] = (uint4_t){0, 0, 0, 0};
-    }
-    if (tid < 64) {
-      const float b = vok ? vs : HXA_Q8_LEAST;
-      float *x = cst(i) + lane;
-      x[0] = ks > 0.0f && ks < INFINITY ? fmaxf(ks * c, NO_SCALE) : NO_SCALE;
-      x[64] = __builtin_amdgcn_logf(b);
-      x[128] = 1.0f / b;
-    }
-  }
-  HXA_DEV void piece(int i, int p) {
-    const int V = p >= G_::N, n = V ? p - G_::N : p;
-    uint8_t *at = (V ? vbuf(i) : kbuf(i)) + n * (256 / G_::CH) * G_::RB;
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const uint2_t a = q8_halves(raw[V][n][2 * e]), b = q8_halves(raw[V][n][2 * e + 1]);
-      *(uint4_t *)(at + to[V][e]) = (uint4_t){a.x, a.y, b.x, b.y};
-    }
-  }
-  HXA_DEV void store(int i) {
-    begin(i);
-#pragma unroll
-    for (int p = 0; p < 2 * G_::N; p++) piece(i, p);
-  }
-};
 
 // q's eight values as fp16; bf16: times a power of two, whose inverse the caller keeps
 HXA_DEV half8_t q_halves(half8_t q, float) { return q; }
@@ -152,10 +68,91 @@ HXA_DEV float most_of(const V (&q)[N]) {
   return m;
 }
 
+// The pages of keys x from a first one on, 512 of them: place in the pools (npages H page rows; ~0: not there) and scales
+struct PagesQ8 {
+  static constexpr int N = 512;
+  const KeysQ8 &s;
+  uint32_t *ph;
+  float *ks, *lv, *iv;
+  int *flag;
+  int first, own;        // entry of page slot n of the prefix: n - first, of the sequence: n + own
+  int npre, pre_end, own_end;
+  HXA_DEV PagesQ8(const KeysQ8 &s_, uint8_t *table) : s(s_), first(0), own(0) {
+    ph = (uint32_t *)table;
+    ks = (float *)(ph + N);
+    lv = ks + N;
+    iv = lv + N;
+    flag = (int *)(iv + N);
+  }
+  HXA_DEV int entry(int x, unsigned &in_page) const {
+    const bool pre = x < s.P;
+    return (int)s.slot(pre ? x : x - s.P, in_page) + (pre ? -first : own);
+  }
+  // the entries from key x0 on, of keys below x1
+  HXA_DEV void start(int x0, int x1) {
+    unsigned in;
+    npre = 0;
+    if (x0 < s.P) {
+      first = (int)s.slot(x0, in);
+      npre = (int)s.slot(s.P - 1, in) - first + 1;
+      own = npre;
+    } else {
+      own = -(int)s.slot(x0 - s.P, in);
+    }
+    own_end = x1 > s.P ? (int)s.slot(x1 - 1 - s.P, in) + 1 + own : npre;
+    pre_end = x1 > s.P ? npre : (int)s.slot(x1 - 1, in) - first + 1;
+  }
+  HXA_DEV bool there(int j) const { return j < (j < npre ? pre_end : own_end); }
+  HXA_DEV int page_of(int j) const { return there(j) ? (j < npre ? s.prefix[first + j] : s.table[j - own]) : -1; }
+  // the workgroup's threads take two pages each, e[k] of entry 256 k + tid
+  HXA_DEV void fill(const int (&e)[2], float c, int tid) {
+    bool hole = false, bare = false;
+    float a[2], b[2];
+    uint32_t at[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const bool ok = (unsigned)e[k] < (unsigned)s.npages;
+      hole |= !ok && there(k * 256 + tid);
+      at[k] = ok ? (uint32_t)e[k] * s.H + s.h : ~0u;
+      a[k] = ok ? s.ks[at[k]] : 0.0f;
+      b[k] = ok ? s.vs[at[k]] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int j = k * 256 + tid;
+      const bool vok = b[k] > HXA_Q8_LEAST && b[k] < INFINITY;
+      bare |= at[k] != ~0u && !vok;
+      ph[j] = at[k];
+      ks[j] = a[k] > 0.0f && a[k] < INFINITY ? fmaxf(a[k] * c, NO_SCALE) : NO_SCALE;
+      lv[j] = vok ? __builtin_amdgcn_logf(b[k]) : -64.0f;
+      iv[j] = vok ? 1.0f / b[k] : 1.0f / HXA_Q8_LEAST;
+    }
+    const int any = (__any(hole) ? 1 : 0) | (__any(bare) ? 2 : 0);
+    if ((tid & 63) == 0) flag[tid >> 6] = any;
+  }
+  // once the workgroup has met: 1: a page is not there; 2: one is without a value scale
+  HXA_DEV int flags() const { return __builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3]); }
+  HXA_DEV bool holes() const { return flags() & 1; }
+  // where the steps [s0, s1) of `span` keys from x0 on, below x1, that the table reaches end
+  HXA_DEV int reach(int s0, int s1, int span, int x0, int x1) const {
+    for (;;) {
+      unsigned in;
+      const int over = entry(min(x0 + s1 * span, x1) - 1, in) - N + 1;
+      if (over <= 0) return s1;
+      s1 -= max(1, (int)min((long)(over - 1) * s.page / span, (long)s1 - s0 - 1));
+    }
+  }
+};
+
 // ---- rows modes: as causal_attn.hip's rows_item; m and the sums in powers of two ----
+// A tile's bytes go straight into LDS two tiles ahead (each wave its 16 keys), from there through registers, where they become fp16 once for all four
+// waves, into the tile that the products read. Pages' places and scales come from the table in LDS, as a load of them would be waited for with the keys'.
+// Bound by the conversions, which the other workgroup's products hide in part. 64 decoding tokens with 470 keys each behind a prefix of 4096 36.1 us and 32 prompts of 75
+// 57.1; with the tile ahead held in registers and converted beside K's products 37.4 and 56.7 (128 tokens behind 200 keys each 29.0, here 27.3); with
+// V converted beside K's products and K beside V's 40.1 and 68.3.
+//
 // G8: eight keys of a lane (8 g + 0 .. 7 of every 16) lie on one page, so that they share its scales: the maximum is taken of the scores, the
-// scales go into one fma a score. (With constants for each key, 24 more 16-byte reads of
-// LDS a tile: 32 prompts of 75 behind 4000 186 us against 168.)
+// scales go into one fma a score. (With constants for each key, 24 more 16-byte reads of LDS a tile: 32 prompts of 75 behind 4000 186 us against 168.)
 template <typename T, int HD, int W, bool G8>
 HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, int head0, float c, uint8_t *lds, float16_t (&acc)[HD / 32],
                           float &mrun, float &lsum) {
@@ -175,180 +172,280 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
   int rest;
   const int tok = row_tok(it, Rc, rest);
   const T *qp = q + (long)(it.tok0 + tok) * ldq + (long)(head0 + rest) * HD;
-  half8_t qf[HD / 16];
-  float back = 1.0f;  // what q was divided by
-  {
-    v8 raw[HD / 16];
-#pragma unroll
-    for (int i = 0; i < HD / 16; i++) raw[i] = *(const v8 *)(qp + i * 16 + 8 * g);
-    float f = 1.0f;
-    if (BF) {
-      float lo, hi;
-      halves(most_of(raw), lo, hi);
-      f = row_factor(fmaxf(lo, hi));
-      back = 1.0f / f;
-    }
-#pragma unroll
-    for (int i = 0; i < HD / 16; i++) qf[i] = q_halves(raw[i], f);
-  }
-  const int lim = tok_limit(it, tok);
-  const int lim_min = row_limit(it, it.r0);
-
+  const int lim = tok_limit(it, tok), lim_min = row_limit(it, it.r0);
 #pragma unroll
   for (int d = 0; d < ND; d++) acc[d] = (float16_t){};
   mrun = -INFINITY;
   lsum = 0.0f;
   const int nt = (it.x1 - it.x0 + KT - 1) / KT;
   if (nt <= 0) return;
-  LoaderQ8<HD> ld(s, it, lds, c, tid);
-  uint64_t km = ld.open(0);
+
+  // the wave's part of a tile: keys 16 wave .. + 15, as they come into one of two places, then as fp16 rows for all waves
+  PagesQ8 pages(s, lds + G_::TABLE);
+  constexpr int L = 2 * G_::NLD;  // loads a tile
+  uint8_t *const raw = lds + G_::RAW + wave * (4 * G_::WB);
+  const int xlane = it.x0 + 16 * wave + (lane & 15), ch = lane % G_::CH;
+  auto pool_row = [&](uint32_t p, unsigned in) { return p == ~0u ? 0u : p * s.page + in; };  // < 2^32: checked on the host
+  auto row_of = [&](int i) {
+    const int x = xlane + i * KT;
+    unsigned in;
+    if (x >= it.x1) return 0u;
+    const uint32_t p = pages.ph[pages.entry(x, in)];
+    return pool_row(p, in);
+  };
+  auto load = [&](int i, uint32_t at) {
+    uint8_t *to = raw + (i & 1) * 2 * G_::WB;
+#pragma unroll
+    for (int n = 0; n < G_::NLD; n++) {
+      const uint64_t from = (uint64_t)(uint32_t)__shfl((int)at, n * G_::RPL + lane / G_::CH) * HD + ch * 16;
+      g2l16_opaque((const uint8_t *)s.k + from, to + n * 1024);
+      g2l16_opaque((const uint8_t *)s.v + from, to + G_::WB + n * 1024);
+    }
+  };
+  // the first tiles' places and the table's pages from memory side by side, then the keys and the scales
+  pages.start(it.x0, it.x1);
+  int e0[2], e1[2];
+  unsigned in0[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) e0[i] = xlane + i * KT < it.x1 ? pages.page_of(pages.entry(xlane + i * KT, in0[i])) : -1;
+#pragma unroll
+  for (int k = 0; k < 2; k++) e1[k] = pages.page_of(k * 256 + tid);
+  half8_t qf[HD / 16];
+  float back = 1.0f;  // what q was divided by
+  {
+    v8 x[HD / 16];
+#pragma unroll
+    for (int i = 0; i < HD / 16; i++) x[i] = *(const v8 *)(qp + i * 16 + 8 * g);
+    uint32_t at0[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) at0[i] = (unsigned)e0[i] < (unsigned)s.npages ? pool_row((uint32_t)e0[i] * s.H + s.h, in0[i]) : 0u;
+    load(0, at0[0]);
+    if (nt > 1) load(1, at0[1]);
+    pages.fill(e1, c, tid);
+    float f = 1.0f;
+    if (BF) {
+      float lo, hi;
+      halves(most_of(x), lo, hi);
+      f = row_factor(fmaxf(lo, hi));
+      back = 1.0f / f;
+    }
+#pragma unroll
+    for (int i = 0; i < HD / 16; i++) qf[i] = q_halves(x[i], f);
+  }
 
   const int vrow = 4 * g + ((lane & 15) >> 2);
   const int vlow = ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;
   uint32_t vat[ND];
 #pragma unroll
   for (int d = 0; d < ND; d++) vat[d] = vrow * G_::RB + (((d << 2) ^ S_::fv(vrow)) << 4) + vlow;
-  ld.store(0);
-  uint64_t km_next = 0;
-  if (nt > 1) km_next = ld.open(1);
-  reads_done_barrier();  // tile 0 is in LDS
+  const uint8_t *const kb = lds, *const vb = lds + G_::TB;
+  const float *const cst = (const float *)(lds + G_::CST) + 32 * kh + 8 * g;
 
-  // Tile i: its products of K carry the next tile's way from registers into LDS; then the registers take the loads of the tile behind that.
-  for (int i = 0; i < nt; i++) {
-    const int key0 = it.x0 + i * KT;
-    const uint8_t *kb = ld.kbuf(i), *vb = ld.vbuf(i);
-    const float *cst = ld.cst(i) + 32 * kh + 8 * g;
-    auto kfrag = [&](int ds, int b) {
-      const int row = (b + kh) * 32 + ql, ch = 2 * ds + g;
-      return *(const half8_t *)(kb + row * G_::RB + ((ch ^ S_::fk(row)) << 4));
-    };
-    auto vfrag = [&](int n) {
-      const uint8_t *at = vb + vat[n % ND] + (kh * 32 + n / ND * 16) * G_::RB;
-      return __builtin_shufflevector(read_tr<half4_t>(at), read_tr<half4_t>(at + 8 * G_::RB), 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    const bool cut = km != ~0ull || key0 + KT - 1 > lim_min;
-    float16_t S[NB];
-    half8_t kf[AK + 1][NB];
+  for (int s0 = 0; s0 < nt;) {
+    if (s0 > 0) {  // the next 512 pages
+      reads_done_barrier();
+      pages.start(it.x0 + s0 * KT, it.x1);
 #pragma unroll
-    for (int ds = 0; ds < AK; ds++)
-#pragma unroll
-      for (int b = 0; b < NB; b++) kf[ds][b] = kfrag(ds, b);
-    float kg[2 * NB], lg[2 * NB], ig[2 * NB];  // G8: of keys 16 u + 8 g .. + 7
-    if constexpr (G8) {
-#pragma unroll
-      for (int u = 0; u < 2 * NB; u++) kg[u] = with_back<BF>(cst[16 * u], back), lg[u] = cst[16 * u + 64], ig[u] = cst[16 * u + 128];
+      for (int k = 0; k < 2; k++) e1[k] = pages.page_of(k * 256 + tid);
+      pages.fill(e1, c, tid);
     }
-    ld.begin(i + 1);  // (past the last tile: of what the registers hold, for nobody)
-#pragma unroll
-    for (int ds = 0; ds < HD / 16; ds++) {
-      __builtin_amdgcn_sched_barrier(0);
-      if (ds + AK < HD / 16) {
-#pragma unroll
-        for (int b = 0; b < NB; b++) kf[(ds + AK) % (AK + 1)][b] = kfrag(ds + AK, b);
-      }
-      if (ds % 2 == 0) ld.piece(i + 1, ds / 2);
-#pragma unroll
-      for (int b = 0; b < NB; b++) S[b] = mma32(kf[ds % (AK + 1)][b], qf[ds], ds == 0 ? (float16_t){} : S[b]);
+    reads_done_barrier();
+    const int flags = pages.flags();
+    const int s1 = pages.reach(s0, nt, KT, it.x0, it.x1);  // the tiles whose pages are in the table
+    if (s0 > 0) {
+      load(s0, row_of(s0));
+      if (s0 + 1 < s1) load(s0 + 1, row_of(s0 + 1));
     }
-    __builtin_amdgcn_sched_barrier(0);
-    const uint64_t km_i = km;
-    km = km_next;
-    if (i + 2 < nt) km_next = ld.open(i + 2);
-    half8_t vf[AV + 1];
+    uint32_t at_next = s0 + 2 < s1 ? row_of(s0 + 2) : 0;
+    for (int i = s0; i < s1; i++) {
+      const int key0 = it.x0 + i * KT;
+      __builtin_amdgcn_s_setprio(0);
+      if (i + 1 < s1) wait_vm<L>();  // the wave's part of tile i has landed
+      else wait_vm<0>();
+      asm volatile("" ::: "memory");
+      uint4_t w[2][G_::NLD];
+      {
+        const uint8_t *from = raw + (i & 1) * 2 * G_::WB + lane * 16;
 #pragma unroll
-    for (int n = 0; n < AV; n++) vf[n] = vfrag(n);
-    if constexpr (!G8) {
-    // scores to exponents, four keys at a time (their constants two reads ahead: all of them at once are more registers than there are)
-      auto at = [&](int u) { return cst + 16 * (u >> 1) + 4 * (u & 1); };
-      float4_t k[2], lv[2];
-      k[0] = *(const float4_t *)at(0), lv[0] = *(const float4_t *)(at(0) + 64);
-#pragma unroll
-      for (int u = 0; u < 4 * NB; u++) {
-        if (u + 1 < 4 * NB) k[(u + 1) & 1] = *(const float4_t *)at(u + 1), lv[(u + 1) & 1] = *(const float4_t *)(at(u + 1) + 64);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float x = S[u >> 2][4 * (u & 3) + e];
-          S[u >> 2][4 * (u & 3) + e] = fmaf(BF ? x * back : x, k[u & 1][e], lv[u & 1][e]);
+        for (int n = 0; n < G_::NLD; n++) {
+          w[0][n] = *(const uint4_t *)(from + n * 1024);
+          w[1][n] = *(const uint4_t *)(from + G_::WB + n * 1024);
         }
       }
-    }
-    if (cut) {
-      // a row's limit hides the keys past x1 too (a range that ends before it ends with a tile); pages that are not there need the mask
-      const int n = lim - key0 - 32 * kh - 8 * g, left = it.x1 - key0;
-      if (km_i == (left >= KT ? ~0ull : (1ull << left) - 1)) {
+      reads_done_barrier();  // it is in registers; every wave is done with tile i - 1
+      if (i + 2 < s1) {
+        load(i + 2, at_next);
+        if (i + 3 < s1) at_next = row_of(i + 3);
+      }
+      if (flags & 2) {  // pages without a value scale: values of 0, whatever the bytes
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+        for (int n = 0; n < G_::NLD; n++) {
+          unsigned in;
+          const int x = min(key0 + 16 * wave + n * G_::RPL + lane / G_::CH, it.x1 - 1);
+          if (pages.iv[pages.entry(x, in)] >= 1.0f / HXA_Q8_LEAST) w[1][n] = (uint4_t){0, 0, 0, 0};
+        }
+      }
+      uint64_t km = ~0ull;
+      {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));  // opaque: the loop keeps none of these addresses in registers
 #pragma unroll
-          for (int r = 0; r < 16; r++)
-            if (32 * b + 16 * (r >> 3) + (r & 7) > n) S[b][r] = -INFINITY;
-      } else {
-        const uint64_t see = km_i >> (32 * kh + 8 * g);
+        for (int n = 0; n < G_::NLD; n++) {
+          const int row = krow_key(16 * wave + n * G_::RPL + ln / G_::CH), c2 = 2 * (ln % G_::CH);  // (its own inverse)
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+          for (int V = 0; V < 2; V++) {
+            uint8_t *to = lds + V * G_::TB + row * G_::RB;
+            const int f = V ? S_::fv(row) : S_::fk(row);
 #pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const int k = 32 * b + 16 * (r >> 3) + (r & 7);
-            if (k > n || !((see >> k) & 1)) S[b][r] = -INFINITY;
+            for (int e = 0; e < 2; e++) {
+              const uint2_t a = q8_halves(w[V][n][2 * e]), b = q8_halves(w[V][n][2 * e + 1]);
+              *(uint4_t *)(to + (((c2 + e) ^ f) << 4)) = (uint4_t){a.x, a.y, b.x, b.y};
+            }
           }
+        }
+        if (wave == 0 || (flags & 1)) {
+          unsigned in;
+          const int x = key0 + ln, e = pages.entry(min(x, it.x1 - 1), in);
+          if (flags & 1) km = __ballot(x < it.x1 && pages.ph[e] != ~0u);
+          if (wave == 0) {
+            float *to = (float *)(lds + G_::CST) + ln;
+            to[0] = pages.ks[e];
+            to[64] = pages.lv[e];
+            to[128] = pages.iv[e];
+          }
+        }
       }
-    }
-    float mt = -INFINITY;
+      reads_done_barrier();  // tile i is in LDS
+      __builtin_amdgcn_s_setprio(1);  // products before the other workgroup's conversions (32 prompts 57.1 us against 60.3)
+      auto kfrag = [&](int ds, int b) {
+        const int row = (b + kh) * 32 + ql, ch = 2 * ds + g;
+        return *(const half8_t *)(kb + row * G_::RB + ((ch ^ S_::fk(row)) << 4));
+      };
+      auto vfrag = [&](int n) {
+        const uint8_t *at = vb + vat[n % ND] + (kh * 32 + n / ND * 16) * G_::RB;
+        return __builtin_shufflevector(read_tr<half4_t>(at), read_tr<half4_t>(at + 8 * G_::RB), 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      const bool cut = km != ~0ull || key0 + KT - 1 > min(lim_min, it.x1 - 1);
+      float16_t S[NB];
+      half8_t kf[AK + 1][NB];
 #pragma unroll
-    for (int u = 0; u < 2 * NB; u++) {
-      float m8 = S[u >> 1][8 * (u & 1)];
+      for (int ds = 0; ds < AK; ds++)
 #pragma unroll
-      for (int r = 1; r < 8; r++) m8 = fmaxf(m8, S[u >> 1][8 * (u & 1) + r]);
-      mt = fmaxf(mt, G8 ? fmaf(m8, kg[u], lg[u]) : m8);
-    }
-    {
-      float lo, hi;
-      halves(mt, lo, hi);
-      mt = fmaxf(lo, hi);
-    }
-    const bool need = mt - mrun > RESCALE2;  // also when mrun is still -inf
-    if (__any(need)) {
-      const float alpha = need ? __builtin_amdgcn_exp2f(mrun - mt) : 1.0f;
-      if (need) mrun = mt;
-      lsum *= alpha;
-#pragma unroll
-      for (int d = 0; d < ND; d++) acc[d] *= alpha;
-    }
-    const float mb = mrun == -INFINITY ? 0.0f : mrun;
-    half8_t pf[NB][2];
-    float ls[2 * NB] = {};
-    auto expo2 = [&](int n) {
-      const int u = n >> 3;
-      float p0 = S[n >> 4][n & 15], p1 = S[n >> 4][(n & 15) + 1];
+        for (int b = 0; b < NB; b++) kf[ds][b] = kfrag(ds, b);
+      float kg[2 * NB], lg[2 * NB], ig[2 * NB];  // G8: of keys 16 u + 8 g .. + 7
       if constexpr (G8) {
-        p0 = __builtin_amdgcn_exp2f(fmaf(p0, kg[u], lg[u] - mb));
-        p1 = __builtin_amdgcn_exp2f(fmaf(p1, kg[u], lg[u] - mb));
-        ls[u] += p0;
-        ls[u] += p1;
-      } else {
-        const float2_t inv = *(const float2_t *)(cst + 128 + 16 * u + (n & 7));
-        p0 = __builtin_amdgcn_exp2f(p0 - mb);
-        p1 = __builtin_amdgcn_exp2f(p1 - mb);
-        ls[u] = fmaf(p1, inv[1], fmaf(p0, inv[0], ls[u]));
+#pragma unroll
+        for (int u = 0; u < 2 * NB; u++) kg[u] = with_back<BF>(cst[16 * u], back), lg[u] = cst[16 * u + 64], ig[u] = cst[16 * u + 128];
       }
-      pf[n >> 4][u & 1][n & 7] = (hxa_h)p0;
-      pf[n >> 4][u & 1][(n & 7) + 1] = (hxa_h)p1;
-    };
 #pragma unroll
-    for (int n = 0; n < 16; n += 2) expo2(n);
+      for (int ds = 0; ds < HD / 16; ds++) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (ds + AK < HD / 16) {
 #pragma unroll
-    for (int n = 0; n < 2 * NB * ND; n++) {
-      if (n + AV < 2 * NB * ND) vf[(n + AV) % (AV + 1)] = vfrag(n + AV);
-      acc[n % ND] = mma32(vf[n % (AV + 1)], pf[n / (2 * ND)][n / ND & 1], acc[n % ND]);
-      if (NB == 2 && n < 2 * ND && (ND < 8 || n % 2 == 0)) {
+          for (int b = 0; b < NB; b++) kf[(ds + AK) % (AK + 1)][b] = kfrag(ds + AK, b);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int e = 0; e < (ND < 8 ? 8 / ND : 2); e += 2) expo2(16 + n * 8 / ND + e);
+        for (int b = 0; b < NB; b++) S[b] = mma32(kf[ds % (AK + 1)][b], qf[ds], ds == 0 ? (float16_t){} : S[b]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      half8_t vf[AV + 1];
+#pragma unroll
+      for (int n = 0; n < AV; n++) vf[n] = vfrag(n);
+      if constexpr (!G8) {
+        // scores to exponents, four keys at a time (their constants two reads ahead: all of them at once are more registers than there are)
+        auto at = [&](int u) { return cst + 16 * (u >> 1) + 4 * (u & 1); };
+        float4_t k[2], lv[2];
+        k[0] = *(const float4_t *)at(0), lv[0] = *(const float4_t *)(at(0) + 64);
+#pragma unroll
+        for (int u = 0; u < 4 * NB; u++) {
+          if (u + 1 < 4 * NB) k[(u + 1) & 1] = *(const float4_t *)at(u + 1), lv[(u + 1) & 1] = *(const float4_t *)(at(u + 1) + 64);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float x = S[u >> 2][4 * (u & 3) + e];
+            S[u >> 2][4 * (u & 3) + e] = fmaf(BF ? x * back : x, k[u & 1][e], lv[u & 1][e]);
+          }
+        }
+      }
+      if (cut) {
+        // a row's limit hides the keys past x1 too (a range that ends before it ends with a tile); pages that are not there need the mask
+        const int n = lim - key0 - 32 * kh - 8 * g, left = it.x1 - key0;
+        if (km == ~0ull || km == (left >= KT ? ~0ull : (1ull << left) - 1)) {
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+              if (32 * b + 16 * (r >> 3) + (r & 7) > n) S[b][r] = -INFINITY;
+        } else {
+          const uint64_t see = km >> (32 * kh + 8 * g);
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+              const int k = 32 * b + 16 * (r >> 3) + (r & 7);
+              if (k > n || !((see >> k) & 1)) S[b][r] = -INFINITY;
+            }
+        }
+      }
+      float mt = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2 * NB; u++) {
+        float m8 = S[u >> 1][8 * (u & 1)];
+#pragma unroll
+        for (int r = 1; r < 8; r++) m8 = fmaxf(m8, S[u >> 1][8 * (u & 1) + r]);
+        mt = fmaxf(mt, G8 ? fmaf(m8, kg[u], lg[u]) : m8);
+      }
+      {
+        float lo, hi;
+        halves(mt, lo, hi);
+        mt = fmaxf(lo, hi);
+      }
+      const bool need = mt - mrun > RESCALE2;  // also when mrun is still -inf
+      if (__any(need)) {
+        const float alpha = need ? __builtin_amdgcn_exp2f(mrun - mt) : 1.0f;
+        if (need) mrun = mt;
+        lsum *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; d++) acc[d] *= alpha;
+      }
+      const float mb = mrun == -INFINITY ? 0.0f : mrun;
+      half8_t pf[NB][2];
+      float ls[2 * NB] = {};
+      auto expo2 = [&](int n) {
+        const int u = n >> 3;
+        float p0 = S[n >> 4][n & 15], p1 = S[n >> 4][(n & 15) + 1];
+        if constexpr (G8) {
+          p0 = __builtin_amdgcn_exp2f(fmaf(p0, kg[u], lg[u] - mb));
+          p1 = __builtin_amdgcn_exp2f(fmaf(p1, kg[u], lg[u] - mb));
+          ls[u] += p0;
+          ls[u] += p1;
+        } else {
+          const float2_t inv = *(const float2_t *)(cst + 128 + 16 * u + (n & 7));
+          p0 = __builtin_amdgcn_exp2f(p0 - mb);
+          p1 = __builtin_amdgcn_exp2f(p1 - mb);
+          ls[u] = fmaf(p1, inv[1], fmaf(p0, inv[0], ls[u]));
+        }
+        pf[n >> 4][u & 1][n & 7] = (hxa_h)p0;
+        pf[n >> 4][u & 1][(n & 7) + 1] = (hxa_h)p1;
+      };
+#pragma unroll
+      for (int n = 0; n < 16; n += 2) expo2(n);
+#pragma unroll
+      for (int n = 0; n < 2 * NB * ND; n++) {
+        if (n + AV < 2 * NB * ND) vf[(n + AV) % (AV + 1)] = vfrag(n + AV);
+        acc[n % ND] = mma32(vf[n % (AV + 1)], pf[n / (2 * ND)][n / ND & 1], acc[n % ND]);
+        if (NB == 2 && n < 2 * ND && (ND < 8 || n % 2 == 0)) {
+#pragma unroll
+          for (int e = 0; e < (ND < 8 ? 8 / ND : 2); e += 2) expo2(16 + n * 8 / ND + e);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 2 * NB; u++) lsum = G8 ? fmaf(ls[u], ig[u], lsum) : lsum + ls[u];
     }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int u = 0; u < 2 * NB; u++) lsum = G8 ? fmaf(ls[u], ig[u], lsum) : lsum + ls[u];
-    reads_done_barrier();  // every wave is done with tile i, and has its part of the next one in LDS
+    s0 = s1;
+    __builtin_amdgcn_s_setprio(0);
   }
   {
     float lo, hi;
@@ -404,78 +501,13 @@ struct FewQ8 {
   static constexpr int TB = 16 * HD;                   // bytes of a wave's keys of a tile, and of its values
   static constexpr int CH = HD / 16, RPL = 64 / CH;    // 16-byte chunks a row, rows of one wave-wide load
   static constexpr int NLD = HD / 64;                  // loads of a tile's keys, and of its values
-  static constexpr int PAGES = 512, TABLE = 4 * RS * 4 * TB;  // the pages' table, past the four rings
-  static constexpr int LDS = TABLE + PAGES * 16 + 16;
+  static constexpr int TABLE = 4 * RS * 4 * TB;         // the pages' table, past the four rings
+  static constexpr int LDS = TABLE + 512 * 16 + 16;
   static HXA_DEV int fk(int row) { return HD == 64 ? (row >> 2) & 3 : HD == 128 ? (row >> 1) & 7 : row & 15; }
   static HXA_DEV int fv(int row) { return HD == 64 ? 0 : HD == 128 ? (row << 1) & 4 : (row & 3) << 2; }
 };
 // row of LDS <-> key, within 16 (its own inverse)
 HXA_DEV int few_row(int key) { return (key & 3) << 2 | (key >> 2 & 3); }
-
-// The pages of keys x from a first one on, PAGES of them: place in the pools (npages H page rows; ~0: not there) and scales
-template <int HD>
-struct PagesQ8 {
-  static constexpr int N = FewQ8<HD>::PAGES;
-  const KeysQ8 &s;
-  uint32_t *ph;
-  float *ks, *lv, *iv;
-  int *flag;
-  int first, own;        // entry of page slot n of the prefix: n - first, of the sequence: n + own
-  int npre, pre_end, own_end;
-  HXA_DEV PagesQ8(const KeysQ8 &s_, uint8_t *lds) : s(s_), first(0), own(0) {
-    ph = (uint32_t *)(lds + FewQ8<HD>::TABLE);
-    ks = (float *)(ph + N);
-    lv = ks + N;
-    iv = lv + N;
-    flag = (int *)(iv + N);
-  }
-  HXA_DEV int entry(int x, unsigned &in_page) const {
-    const bool pre = x < s.P;
-    return (int)s.slot(pre ? x : x - s.P, in_page) + (pre ? -first : own);
-  }
-  // the entries from key x0 on, of keys below x1
-  HXA_DEV void start(int x0, int x1) {
-    unsigned in;
-    npre = 0;
-    if (x0 < s.P) {
-      first = (int)s.slot(x0, in);
-      npre = (int)s.slot(s.P - 1, in) - first + 1;
-      own = npre;
-    } else {
-      own = -(int)s.slot(x0 - s.P, in);
-    }
-    own_end = x1 > s.P ? (int)s.slot(x1 - 1 - s.P, in) + 1 + own : npre;
-    pre_end = x1 > s.P ? npre : (int)s.slot(x1 - 1, in) - first + 1;
-  }
-  HXA_DEV bool there(int j) const { return j < (j < npre ? pre_end : own_end); }
-  HXA_DEV int page_of(int j) const { return there(j) ? (j < npre ? s.prefix[first + j] : s.table[j - own]) : -1; }
-  // the workgroup's threads take two pages each, e[k] of entry 256 k + tid
-  HXA_DEV void fill(const int (&e)[2], float c, int tid) {
-    bool hole = false;
-    float a[2], b[2];
-    uint32_t at[2];
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      const bool ok = (unsigned)e[k] < (unsigned)s.npages;
-      hole |= !ok && there(k * 256 + tid);
-      at[k] = ok ? (uint32_t)e[k] * s.H + s.h : ~0u;
-      a[k] = ok ? s.ks[at[k]] : 0.0f;
-      b[k] = ok ? s.vs[at[k]] : 0.0f;
-    }
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      const int j = k * 256 + tid;
-      const bool vok = b[k] > HXA_Q8_LEAST && b[k] < INFINITY;
-      ph[j] = at[k];
-      ks[j] = a[k] > 0.0f && a[k] < INFINITY ? fmaxf(a[k] * c, NO_SCALE) : NO_SCALE;
-      lv[j] = vok ? __builtin_amdgcn_logf(b[k]) : -64.0f;
-      iv[j] = vok ? 1.0f / b[k] : 1.0f / HXA_Q8_LEAST;
-    }
-    const bool any = __any(hole);
-    if ((tid & 63) == 0) flag[tid >> 6] = any;
-  }
-  HXA_DEV bool holes() const { return (flag[0] | flag[1] | flag[2] | flag[3]) != 0; }
-};
 
 template <typename T, int HD, bool G8>
 HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, int head0, float c, uint8_t *lds, const Out<T> &out) {
@@ -496,7 +528,7 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
   float mrun = -INFINITY, lsum = 0.0f;
   const int ns = (it.x1 - it.x0 + 2 * KT - 1) / (2 * KT);  // steps of two tiles
   if (ns > 0) {
-    PagesQ8<HD> pages(s, lds);
+    PagesQ8 pages(s, lds + F::TABLE);
     uint8_t *const ring = lds + wave * (RS * 4 * F::TB);
     uint32_t koff[F::NLD], voff[F::NLD];
     int from[F::NLD];  // the lane that knows the row of this lane's part of load n
@@ -582,13 +614,7 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
       }
       reads_done_barrier();
       const bool holes = pages.holes();
-      int s1 = ns;  // the steps whose pages are in the table
-      for (;;) {
-        unsigned in;
-        const int over = pages.entry(min(it.x0 + s1 * 2 * KT, it.x1) - 1, in) - F::PAGES + 1;
-        if (over <= 0) break;
-        s1 -= max(1, (int)min((long)(over - 1) * s.page / (2 * KT), (long)s1 - s0 - 1));
-      }
+      const int s1 = pages.reach(s0, ns, 2 * KT, it.x0, it.x1);  // the steps whose pages are in the table
       if (s0 > 0) {
 #pragma unroll
         for (int i = 0; i < RS; i++)
@@ -722,6 +748,7 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
         }
       }
       s0 = s1;
+    __builtin_amdgcn_s_setprio(0);
     }
     lsum = add16(lsum);
   }
