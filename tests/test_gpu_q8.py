@@ -103,6 +103,24 @@ def test_quantize_offsets_past_32_bits(hip):
     assert np.array_equal(got, wq) and np.array_equal(s.numpy(), ws)
 
 
+def test_quantize_more_rows_than_a_grid_holds(hip):
+    """2^24 + 3 rows of a workgroup each"""
+    M, K, ldq = 2 ** 24 + 3, 2056, 2176
+    x, q, s = hip.DeviceArray((M, K), np.uint16), hip.DeviceArray((M, ldq), np.int8), hip.DeviceArray((M,), np.float32)
+    at = [0, 1, 2 ** 23 - 1, 2 ** 23, 2 ** 24 - 1, 2 ** 24, M - 1]
+    rows = narrow(np.random.default_rng(1).standard_normal((len(at), K)), F16)
+    for i, m in enumerate(at):
+        hip.check(hip.lib().hxa_h2d(x.at(m * K * 2), rows[i].ctypes.data, 2 * K))
+    hip.check(hip.lib().hxa_quantize_rows(F16, x.ptr, K, M, K, q.ptr, ldq, s.ptr, None))
+    hip.sync()
+    wq, ws = quantize(widen(rows, F16))
+    got, gs = np.zeros((len(at), ldq), np.int8), np.zeros(len(at), np.float32)
+    for i, m in enumerate(at):
+        hip.check(hip.lib().hxa_d2h(got[i].ctypes.data, q.at(m * ldq), ldq))
+        hip.check(hip.lib().hxa_d2h(gs[i:].ctypes.data, s.at(m * 4), 4))
+    assert np.array_equal(got[:, :K], wq) and not got[:, K:].any() and np.array_equal(gs, ws)
+
+
 # ------------------------------------------------------------------------------------------------------------- product
 class Linear:
     def __init__(self, hip, M, N, K, bias=True, seed=0, junk="a", gap=(16, 48, 8)):
