@@ -123,7 +123,8 @@ int launch(GemmParamsI8 &p, const Form &f, void *ws, hipStream_t st, const char 
   p.epi = split ? HXA_EPI_PARTIAL_F32 : HXA_EPI_STORE;
   p.tiles_m = (p.M + f.bm - 1) / f.bm;
   p.tiles_n = (p.N + f.bn - 1) / f.bn;
-  if ((long)p.tiles_m * p.tiles_n >= 1L << 24) return hxa_set_error(HXA_E_ARG, "%s: M=%d N=%d are too many tiles", who, p.M, p.N);
+  const int waves = f.bn <= 32 ? f.bn == 16 ? 8 : 4 : tile_nw(f.bm, f.bn, HXG_I8);
+  if ((long)p.tiles_m * p.tiles_n * 64 * waves >= 1L << 32) return hxa_set_error(HXA_E_ARG, "%s: M=%d N=%d are too many tiles", who, p.M, p.N);
   // 8 XCD rectangles of the fewest A + W bytes, as gemm_prepare's
   long best = -1;
   for (int gm = 1; gm <= 8; gm *= 2) {

@@ -115,3 +115,7 @@ def test_the_tests_own_definitions():
     q, s = quantize(widen(narrow(x, BF16), BF16))
     assert (np.abs(q * s[:, None] - widen(narrow(x, BF16), BF16)) <= s[:, None] * 0.50001).all() and (np.abs(q).max(1) == 127).all()
     assert (np.abs(x - widen(narrow(x, F16), F16)) <= 2.0 ** -11 * np.abs(x)).all()
+
+
+def test_linear_i8_refuses_grids_past_32_bits(hip):
+    assert linear(hip, (16, 16, 1), M=1 << 27, N=8, ldo=8) == -12 and "too many tiles" in hip.last_error()
