@@ -748,7 +748,6 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
         }
       }
       s0 = s1;
-    __builtin_amdgcn_s_setprio(0);
     }
     lsum = add16(lsum);
   }

@@ -336,7 +336,7 @@ long hxa_attention_cached_ws_bytes(const hxa_kv_cache *c, int T, int Hq); /* 0: 
 int hxa_quantize_rows(int dtype, const void *x, long ldx, int M, int K, void *q, long ldq, float *scale, void *stream);
 /* Product of int8 rows: out[m][n] = sa[m] * sw[n] * (sum over k of a[m][k] * w[n][k]) + bias[n], out [M][ldo] of dtype. a [M][lda] and w [N][ldw] are
  * int8 rows that hold ceil(K / 128) 128 columns: those past K are multiplied too, so one of a and w has zeros there, as hxa_quantize_rows leaves them.
- * The sum is exact (int32); scales and bias (NULL: none) are applied in fp32, one rounding. M any, N % 8 == 0, K 1 .. HXA_I8_MAX_K;
+ * The sum is exact (int32); scales and bias (NULL: none) are applied in fp32, one rounding. M any (fewer than 2^23 output tiles), N % 8 == 0, K 1 .. HXA_I8_MAX_K;
  * lda, ldw multiples of 16 below 2^23, ldo % 8 == 0; pointers 16-byte aligned (sa: 4). out overlaps no operand. ws: hxa_linear_i8_ws_bytes(M, N,
  * K) bytes, 16-byte aligned, for int32 partial sums where there are few output tiles; NULL or fewer bytes: one launch. The results
  * are the same bits in every form. Calls that share ws must not overlap in time, graphs' replays included. */
@@ -357,15 +357,18 @@ typedef struct {
 /* The new tokens' keys (norm and rotation in 32 bits as hxa_kv_append, not rounded in between) and values into their sequences' own pages. For each
  * page and head: where the call writes the page's first row, its scale is that of the call's rows in it. Else the rows before them stay, and so
  * does the scale s if the new rows fit (|x| <= 127 s); if not, it becomes the least s * 2^j that they fit, and the earlier rows' bytes become
- * round(q / 2^j). (An earlier scale of 0 counts as a page of zeros.) A value is so off by less than one present scale of its page however many calls fill
+ * round(q / 2^j). (An earlier scale that is not finite and positive, as that of rows of zeros, gives way to the new rows'; the bytes stay.) A value is so off by less than one present scale of its page however many calls fill
  * it, and by half of one where one call does. Rows behind the call's are left as they are. Tokens that are left out are those of hxa_kv_append. A page
  * that is written may stand in one place of the table only. (T / page + 2 nseq) H < 2^24. */
 int hxa_kv_append_q8(const hxa_kv_cache_q8 *c, const void *k, long ldk, const void *v, long ldv, int T, const float *gk, float eps,
                      const hxa_rope *rope, void *stream);
 /* hxa_attention_cached over such a cache: the same rows, masks, limits, workspace rules and forms. A scale that is not finite and positive counts as 0, its
- * page's keys or values as zeros; so does a value scale of 2^-64 or less. Weights are rounded to fp16 for their product with the bytes, their sum
- * is taken before that: beside the output's own rounding at most 2^-11 of the weighted mean of |v|. bf16 queries are brought to fp16 by a power of two
- * of their row: what is below 2^-38 of the row's largest value is lost. Value scales of pages that one row sees may differ by up to 2^90. */
+ * page's keys or values as zeros; so does a value scale of 2^-64 or less. Weights times their value scales are rounded to fp16 for the product with the
+ * bytes, the sum of the weights is taken before that: beside the output's own rounding an error of 2^-11 of the weighted mean of |v| or, where that is
+ * more, 2^-25 of the largest such product for each key. bf16 queries are brought to fp16: a row whose largest magnitude is 1 .. 2^15 as it is, values
+ * below 2^-17 rounded to multiples of 2^-24; another one by a power of two, values
+ * below 2^-31 of the largest rounded alike (a row that stays below 2^-100: zeros). Value scales of pages that one
+ * row sees may differ by up to 2^90. */
 int hxa_attention_cached_q8(const hxa_kv_cache_q8 *c, const void *q, long ldq, void *o, long ldo, int T, int Hq, float scale, void *ws,
                             long ws_bytes, void *stream);
 long hxa_attention_cached_q8_ws_bytes(const hxa_kv_cache_q8 *c, int T, int Hq);

@@ -436,6 +436,23 @@ def test_cached_q8_steep_scores_and_wide_queries(hip, dtype, hd, Hq, H, new, pas
     check_cached(hip, c, q, 1.0, with_ws, "a query of zeros")
 
 
+@pytest.mark.parametrize("with_ws", [True, False])
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix,page", [
+    (128, 4, 2, [100, 3], [1500, 700], 600, 1), (64, 8, 2, [40, 90], [1300, 0], 1111, 2), (256, 2, 1, [64, 1, 30], [1700, 5, 64], 0, 3),
+    (128, 8, 1, [17, 1], [5000, 4200], 40, 8)])
+def test_cached_q8_more_pages_than_the_table(hip, hd, Hq, H, new, past, prefix, page, with_ws):
+    """ranges of several times 512 pages, of the prefix and of the sequences, in every mode; pages that are not there and scales that are none in the later ones"""
+    say("many pages", hd, page, with_ws)
+    rng = np.random.default_rng(hd + page)
+    c = CacheQ8(hip, rng, new, past, prefix, page, H, hd, F16)
+    q = queries(rng, int(c.cu[-1]), Hq, hd, F16)
+    check_cached(hip, c, q, hd ** -0.5, with_ws, "many pages")
+    c = CacheQ8(hip, rng, new, past, prefix, page, H, hd, F16, bad={(0, 513): -1, (0, 514): 10 ** 6, (0, 580): 2 ** 31 - 1})
+    c.vs[rng.random(c.vs.shape) < 0.1] = 0
+    c.ks[rng.random(c.ks.shape) < 0.1] = np.nan
+    check_cached(hip, c, q, hd ** -0.5, with_ws, "many pages, some bad")
+
+
 def test_cached_q8_queries_not_finite(hip):
     """a NaN or infinite query makes its own row NaN and no other"""
     rng = np.random.default_rng(3)
