@@ -1,5 +1,5 @@
 // The GEMM kernels' device code: O[M][N] = A[M][K] . W[N][K]^T with fused epilogues, instantiated per weight format in
-// gemm_f16.hip, gemm_q8.hip and gemm_q4.hip (one translation unit each); gemm.hip holds the host side.
+// gemm_f16.hip, gemm_q8.hip, gemm_q4.hip and, int8 operands on both sides, gemm_i8.hip (one translation unit each); gemm.hip holds the host side.
 //
 // Replaces the reference's HMX GEMM engine (hexagon/mega/gemm2.c:96-137, gemm_run_geo) including its q8 tile
 // dequantisation (gemm2.c:19-35 dq_tile), the MOSS q4a dequantisation (moss/hexagon/mega/gemm2.c:39-56) and the
