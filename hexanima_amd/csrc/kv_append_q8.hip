@@ -8,9 +8,9 @@
 // A workgroup takes one page of one sequence and one head: its rows' maxima come first, so that the page is written once, and a page is nobody else's.
 // hd / 16 lanes hold a row (causal_heads.h).
 //
-// Bound by HBM: 4 bytes read and 2 written per value of k and v, and for prompts nearly as much by the angles, which each head's workgroup forms again: 9001 tokens
+// Bound by HBM: 4 bytes read and 2 written per value of k and v, and for prompts by a workgroup's chain (lengths, rows, angles, maxima, bytes) with four of them a CU: 9001 tokens
 // of 8 heads of 128 into pages of 64 21 us (2.6 TB/s; 26 with the library's sine and cosine; with an angle for a few heads at a time, in registers, 30: two workgroups
-// a CU), 64000 tokens 109 us (3.6 TB/s; a large copy 5.1). Few tokens take the launch and three dependent loads: lengths, then pages beside the rows, then scales.
+// a CU; for two heads, in LDS, 20, and 64 single tokens 8.7 for 7.1), 64000 tokens 109 us (3.6 TB/s; a large copy 5.1). Few tokens take the launch and three dependent loads: lengths, then pages beside the rows, then scales.
 #include <algorithm>
 #include <type_traits>
 
