@@ -175,6 +175,27 @@ def test_linear_i8(hip, dtype, M, N, K):
         assert np.array_equal(p.run(dtype, with_ws=False), got)  # the same bits in every form
 
 
+def test_linear_i8_widest_strides(hip):
+    """rows just below 2^23 bytes apart, of the result 2^23 values: the tiles' offsets in 32 bits, all others past them"""
+    M, N, K, ld, ldo = 300, 264, 256, 2 ** 23 - 16, 2 ** 23
+    p = Linear(hip, M, N, K)
+    want, bound = p.expect(F16)
+    a, w, o = hip.DeviceArray((M, ld), np.int8), hip.DeviceArray((N, ld), np.int8), hip.DeviceArray((M, ldo), np.uint16)
+    for d, rows in ((a, p.a), (w, p.w)):
+        for i in range(len(rows)):
+            hip.check(hip.lib().hxa_h2d(d.at(i * ld), rows[i].ctypes.data, K))
+    for tile in ((256, 256), (192, 192), (128, 128), (64, 64), (64, 32), (32, 16), (16, 16)):
+        for i in range(M):
+            hip.check(hip.lib().hxa_memset(o.at(i * ldo * 2), 0x55, (N + 8) * 2))
+        hip.check(hip.lib().hxa_linear_i8_tile(F16, a.ptr, ld, p.d[1].ptr, M, w.ptr, ld, p.d[3].ptr, N, K, p.db.ptr, o.ptr, ldo, *tile, 1, None, 0, None))
+        hip.sync()
+        got = np.zeros((M, N + 8), np.uint16)
+        for i in range(M):
+            hip.check(hip.lib().hxa_d2h(got[i].ctypes.data, o.at(i * ldo * 2), (N + 8) * 2))
+        assert (got[:, N:] == 0x5555).all()
+        close(widen(got[:, :N], F16), want, bound, f"strides {tile}")
+
+
 TILES = [(256, 256), (256, 192), (192, 256), (192, 192), (256, 128), (128, 256), (192, 128), (128, 128), (64, 128), (128, 64), (64, 64), (64, 32), (32, 32), (32, 16), (16, 16)]
 
 
