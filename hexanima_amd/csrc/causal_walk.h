@@ -356,8 +356,10 @@ inline CachedPlan cached_plan(const hxa_kv_cache &c, int T, int Hq, bool ws, lon
     p.sp_max = (int)least(32, least(ceil_div(P, KT), ceil_div(p.budget, p.np_blocks) + 1));
     p.x_first = (int)P;
   }
-  // (int8: ranges and pieces, roundings included, are no more than places: one that began when the first have ended would end last)
-  if (q8) p.budget = imax(1, p.budget - p.np_blocks - 1);
+  // int8, while the prefix's blocks are less than half the places: ranges and pieces, roundings included, are no more than places, as one that begins when the
+  // first have ended ends last. More blocks are whole ranges, beside which the pieces need all places (us, places kept for the blocks / not, 32 / 8 heads of
+  // 128: 64 sequences behind 4096 35.6, 40.9; 512 212, 258; 1024 504, 433; 2048, where the blocks are as many as the places, 20400, 830)
+  if (q8 && 2 * (p.np_blocks + 1) <= p.budget) p.budget -= p.np_blocks + 1;
   // a list that is cut anywhere: a block of so many ranges touches one workgroup more
   const long tiles = ceil_div(cap + P - p.x_first, KT);
   if (mode == 1) p.s_max = most <= (q8 ? Q8_WHOLE_MANY : WHOLE_MANY) && blocks * c.H * 4 >= places && p.sp_max == 0 ? 1 : (int)least(31, tiles);
