@@ -1,0 +1,100 @@
+"""Attention over the int8 cache where scales, queries and weights are far apart, against its definition in 64 bits, with a bound for each row and head."""
+import numpy as np
+import pytest
+
+from tests._causal import BF16, F16, HALF_STEP, TINY, U24, close
+from tests._q8 import CacheQ8
+from tests.test_gpu_causal import queries, say
+from tests.test_gpu_q8 import FORMS, run_cached
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from hexanima_amd import hip as h
+    h.init(0)
+    return h
+
+
+def scales_of(c, i):
+    """(key scales, value scales) [keys][H] of sequence i's keys, 0 where they count as none"""
+    pages = [int((c.prefix if x < c.P else c.table[i])[(x if x < c.P else x - c.P) // c.page]) for x in range(c.P + c.lens[i])]
+    at = [e if 0 <= e < c.npages else -1 for e in pages]
+    with np.errstate(invalid="ignore"):
+        return [np.where((np.array(at) >= 0)[:, None] & np.isfinite(s[at]) & (s[at] > 0), s[at], 0).astype(np.float64) for s in (c.ks, c.vs)]
+
+
+def rows_of(c, q, scale):
+    """(o, bound) per row, head and dim, in 64 bits. In natural units of the score, with w the softmax's weights, vs a key's value scale:
+      - every weight carries the same relative error rel at most, of numerator and denominator: the score's 32-bit sum of hd products and its scaling ((hd + 8)
+        half steps of the sum of |q k|), the logarithm of vs (8 half steps of it), exponential, rescales and joins (256); the sums themselves n;
+      - the numerator's weights are rounded to fp16, half a step 2^-11, or 2^-25 below 2^-14, where the largest w vs of the row is 2^-25 / FLOOR at least (a
+        page without a scale stands there with 2^-64, the least scale): n keys of bytes up to 127;
+      - bf16 queries lose at most 2^-25 a dim where the row's largest is 1 or more (2^-39 of it otherwise, which the 256 hold);
+      - the output's own rounding."""
+    n_q, Hq, hd = q.shape
+    G = Hq // c.H
+    o, bound = np.zeros_like(q), np.zeros_like(q)
+    for i, b in enumerate(c.cu[:-1]):
+        n = c.new[i]
+        if n == 0 or c.P + c.lens[i] == 0:
+            continue
+        (k, ok), (v, _), (_, vs) = c.keys(c.k, i), c.keys(c.v, i), scales_of(c, i)
+        seen = (np.arange(len(k))[None] <= c.P + c.past[i] + np.arange(n)[:, None]) & ok[None]
+        for h in range(Hq):
+            kh, vh, qh = k[:, h // G], v[:, h // G], q[b:b + n, h]
+            s = np.where(seen, qh @ kh.T * scale, -np.inf)
+            p = np.exp(s - s.max(1, keepdims=True))
+            w = p / p.sum(1, keepdims=True)
+            keys = seen.sum(1)[:, None]
+            size = (np.where(seen, np.abs(qh) @ np.abs(kh).T, 0).max(1) * scale)[:, None]
+            lmax = np.abs(np.log2(vs[:, h // G], out=np.full(len(vs), -64.0), where=vs[:, h // G] > 0)).max()
+            rel = (keys + (hd + 8) * size + 8 * lmax + 256) * U24
+            if c.dtype == BF16:
+                rel = rel + hd * 2.0 ** -25 * np.abs(kh).max() * scale
+            a = w @ np.abs(vh)
+            o[b:b + n, h] = w @ vh
+            bound[b:b + n, h] = (HALF_STEP[c.dtype] * np.abs(o[b:b + n, h]) + (2.0 ** -11 + 2 * rel) * a +
+                                 keys * FLOOR * 127 * (w * np.maximum(vs[:, h // G], 2.0 ** -64)).max(1)[:, None] + TINY[c.dtype])
+    if c.dtype == F16:  # from 65520 on the nearest fp16 value is infinity
+        o = np.where(np.abs(o) >= 65520, np.copysign(np.inf, o), o)
+    return o, bound
+
+
+FLOOR = 2.0 ** -25
+
+
+@pytest.mark.parametrize("with_ws", [True, False])
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix", FORMS)
+def test_small_values_keep_their_bits(hip, hd, Hq, H, new, past, prefix, page, with_ws):
+    """rows whose weight lies on pages of small values, beside pages of values 10^5 times as large: the bound is well below most results"""
+    say("small values", hd, page, with_ws)
+    rng = np.random.default_rng(6)
+    c = CacheQ8(hip, rng, new, past, prefix, page, H, hd, F16, spread=0.0)
+    c.vs[:] = np.where(rng.random(c.vs.shape) < 0.5, 0.01, 1000.0)
+    big = c.vs > 1
+    c.k[big], c.k[~big] = np.clip(c.k[big], -127, 0), np.clip(c.k[~big], 0, 127)
+    q = np.abs(queries(rng, int(c.cu[-1]), Hq, hd, F16))
+    o, bound = rows_of(c, q, 2.0 * hd ** -0.5)
+    few = [r for i, b in enumerate(c.cu[:-1]) for r in range(b, c.cu[i + 1])]
+    assert (bound[few] < np.abs(o[few]) / 8).mean() > 0.8
+    close(run_cached(hip, c, q, 2.0 * hd ** -0.5, with_ws), o, bound, "small values")
+
+
+@pytest.mark.parametrize("with_ws", [True, False])
+@pytest.mark.parametrize("dtype,page", [(F16, 16), (BF16, 16), (BF16, 5)])
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix", FORMS)
+def test_wide_value_scales_row_by_row(hip, dtype, hd, Hq, H, new, past, prefix, page, with_ws):
+    """value scales from 2^-40 to 2^8 side by side, some of none: each row by the largest scale that it gives weight to"""
+    say("wide value scales", dtype, hd, page, with_ws)
+    rng = np.random.default_rng(9)
+    c = CacheQ8(hip, rng, new, past, prefix, page, H, hd, dtype)
+    c.vs[:] = np.exp2(rng.uniform(-40, 8, c.vs.shape))
+    q = queries(rng, int(c.cu[-1]), Hq, hd, dtype, std=6.0)
+    close(run_cached(hip, c, q, hd ** -0.5, with_ws), *rows_of(c, q, hd ** -0.5), "wide value scales")
+    kinds = rng.integers(0, 12, c.vs.shape)
+    for n, none in enumerate((0.0, -1.0, np.inf, np.nan)):
+        c.vs[kinds == n] = none
+    close(run_cached(hip, c, q, hd ** -0.5, with_ws), *rows_of(c, q, hd ** -0.5), "some without")
