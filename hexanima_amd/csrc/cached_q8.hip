@@ -31,8 +31,11 @@ struct GeoQ8 {
   static constexpr int LDS = TABLE + 512 * 16 + 16;
 };
 
-// stands for a key scale of 0: scores are as good as 0, and -infinity stays what it is
+// the least factor of a score, and what stands for a key scale of 0: scores are as good as 0, and -infinity stays what it is
 constexpr float NO_SCALE = 0x1p-110f;
+// the least key scale in the pages' table: a bf16 row's factor, up to 2^113, comes to it first, so there it is 0, which that factor leaves 0
+template <bool BF>
+constexpr float LEAST_KS = BF ? 0.0f : NO_SCALE;
 
 // four bytes to fp16: u = q + 128 under the exponent of 1024 is 1024 + u
 HXA_DEV uint2_t q8_halves(uint32_t d) {
@@ -104,8 +107,8 @@ struct PagesQ8 {
   }
   HXA_DEV bool there(int j) const { return j < (j < npre ? pre_end : own_end); }
   HXA_DEV int page_of(int j) const { return there(j) ? (j < npre ? s.prefix[first + j] : s.table[j - own]) : -1; }
-  // the workgroup's threads take two pages each, e[k] of entry 256 k + tid
-  HXA_DEV void fill(const int (&e)[2], float c, int tid) {
+  // the workgroup's threads take two pages each, e[k] of entry 256 k + tid; least: of a key scale
+  HXA_DEV void fill(const int (&e)[2], float c, float least, int tid) {
     bool hole = false, bare = false;
     float a[2], b[2];
     uint32_t at[2];
@@ -123,7 +126,7 @@ struct PagesQ8 {
       const bool vok = b[k] > HXA_Q8_LEAST && b[k] < INFINITY;
       bare |= at[k] != ~0u && !vok;
       ph[j] = at[k];
-      ks[j] = a[k] > 0.0f && a[k] < INFINITY ? fmaxf(a[k] * c, NO_SCALE) : NO_SCALE;
+      ks[j] = a[k] > 0.0f && a[k] < INFINITY ? fmaxf(a[k] * c, least) : least;
       lv[j] = vok ? __builtin_amdgcn_logf(b[k]) : -64.0f;
       iv[j] = vok ? 1.0f / b[k] : 1.0f / HXA_Q8_LEAST;
     }
@@ -221,7 +224,7 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
     for (int i = 0; i < 2; i++) at0[i] = (unsigned)e0[i] < (unsigned)s.npages ? pool_row((uint32_t)e0[i] * s.H + s.h, in0[i]) : 0u;
     load(0, at0[0]);
     if (nt > 1) load(1, at0[1]);
-    pages.fill(e1, c, tid);
+    pages.fill(e1, c, LEAST_KS<BF>, tid);
     float f = 1.0f;
     if (BF) {
       float lo, hi;
@@ -247,7 +250,7 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
       pages.start(it.x0 + s0 * KT, it.x1);
 #pragma unroll
       for (int k = 0; k < 2; k++) e1[k] = pages.page_of(k * 256 + tid);
-      pages.fill(e1, c, tid);
+      pages.fill(e1, c, LEAST_KS<BF>, tid);
     }
     reads_done_barrier();
     const int flags = pages.flags();
@@ -364,7 +367,7 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float x = S[u >> 2][4 * (u & 3) + e];
-            S[u >> 2][4 * (u & 3) + e] = fmaf(BF ? x * back : x, k[u & 1][e], lv[u & 1][e]);
+            S[u >> 2][4 * (u & 3) + e] = fmaf(x, BF ? k[u & 1][e] * back : k[u & 1][e], lv[u & 1][e]);
           }
         }
       }
@@ -585,7 +588,7 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
 #pragma unroll
     for (int i = 0; i < RS; i++)
       if (i < ns) load(i, at0[i]);
-    pages.fill(e1, c, tid);
+    pages.fill(e1, c, LEAST_KS<BF>, tid);
     half8_t qf[NG][2];
     float back = 1.0f;
     {
@@ -610,7 +613,7 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
         pages.start(it.x0 + s0 * 2 * KT, it.x1);
 #pragma unroll
         for (int k = 0; k < 2; k++) e1[k] = pages.page_of(k * 256 + tid);
-        pages.fill(e1, c, tid);
+        pages.fill(e1, c, LEAST_KS<BF>, tid);
       }
       reads_done_barrier();
       const bool holes = pages.holes();

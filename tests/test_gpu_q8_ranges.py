@@ -98,3 +98,23 @@ def test_wide_value_scales_row_by_row(hip, dtype, hd, Hq, H, new, past, prefix, 
     for n, none in enumerate((0.0, -1.0, np.inf, np.nan)):
         c.vs[kinds == n] = none
     close(run_cached(hip, c, q, hd ** -0.5, with_ws), *rows_of(c, q, hd ** -0.5), "some without")
+
+
+@pytest.mark.parametrize("with_ws", [True, False])
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix", FORMS)
+@pytest.mark.parametrize("power", [92, 112, 122])
+def test_wide_queries_beside_pages_without_a_key_scale(hip, power, hd, Hq, H, new, past, prefix, page, with_ws):
+    """bf16 queries of about 2^power over keys of about 2^-power: keys whose scale is 0, negative, infinite or NaN score 0, whatever their bytes"""
+    say("wide queries, no key scale", power, hd, page, with_ws)
+    rng = np.random.default_rng(power)
+    c = CacheQ8(hip, rng, new, past, prefix, page, H, hd, BF16, spread=0.0)
+    c.k[:] = np.clip(np.rint(c.k / 32.0), -4, 4)
+    c.ks[:] = np.float32(2.0 ** -power)
+    kinds = rng.integers(0, 12, c.ks.shape)
+    for n, none in enumerate((0.0, -1.0, np.inf, np.nan)):
+        c.ks[kinds == n] = none
+    c.k[kinds < 4] = rng.integers(-128, 128, c.k[kinds < 4].shape)
+    q = queries(rng, int(c.cu[-1]), Hq, hd, BF16) * 2.0 ** power
+    o, bound = rows_of(c, q, hd ** -0.5)
+    close(run_cached(hip, c, q, hd ** -0.5, with_ws), o, bound, "wide queries")
