@@ -61,6 +61,13 @@ HXA_DEV float row_factor(float top) {
 // a key's scale times what its row's queries were divided by, not below NO_SCALE
 template <bool BF>
 HXA_DEV float with_back(float k, float back) { return BF ? fmaxf(k * back, NO_SCALE) : k; }
+// An exponent t - m is one fma of the score with the key's scale and log2(vs) - m: t is not rounded by itself, as m, the largest rounded t, was. Below 2^18 the two
+// differ by less than 2^-5. Whether some row of the wave has a (finite) maximum farther out: then t is rounded first, so that no exponent passes
+// what the running maximum leaves unscaled, at 64 steps and single ones 1% at most.
+HXA_DEV bool far_scores(float mt) {
+  constexpr uint32_t FAR = 0x48800000u;  // 2^18
+  return __any((__builtin_bit_cast(uint32_t, mt) & 0x7fffffffu) - FAR < 0x7f800000u - FAR);
+}
 template <typename V, int N>
 HXA_DEV float most_of(const V (&q)[N]) {
   float m = 0.0f;
@@ -335,7 +342,7 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
       for (int ds = 0; ds < AK; ds++)
 #pragma unroll
         for (int b = 0; b < NB; b++) kf[ds][b] = kfrag(ds, b);
-      float kg[2 * NB], lg[2 * NB], ig[2 * NB];  // G8: of keys 16 u + 8 g .. + 7
+      float kg[2 * NB], lg[2 * NB], ig[2 * NB], lm[2 * NB];  // G8: of keys 16 u + 8 g .. + 7
       if constexpr (G8) {
 #pragma unroll
         for (int u = 0; u < 2 * NB; u++) kg[u] = with_back<BF>(cst[16 * u], back), lg[u] = cst[16 * u + 64], ig[u] = cst[16 * u + 128];
@@ -412,15 +419,28 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
 #pragma unroll
         for (int d = 0; d < ND; d++) acc[d] *= alpha;
       }
-      const float mb = mrun == -INFINITY ? 0.0f : mrun;
+      float mb = mrun == -INFINITY ? 0.0f : mrun;
+      if constexpr (G8) {
+#pragma unroll
+        for (int u = 0; u < 2 * NB; u++) lm[u] = lg[u] - mb;
+      }
+      if (far_scores(mt)) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) S[b][r] = (G8 ? fmaf(S[b][r], kg[2 * b + (r >> 3)], lg[2 * b + (r >> 3)]) : S[b][r]) - mb;
+#pragma unroll
+        for (int u = 0; u < 2 * NB; u++) kg[u] = 1.0f, lm[u] = 0.0f;
+        mb = 0.0f;
+      }
       half8_t pf[NB][2];
       float ls[2 * NB] = {};
       auto expo2 = [&](int n) {
         const int u = n >> 3;
         float p0 = S[n >> 4][n & 15], p1 = S[n >> 4][(n & 15) + 1];
         if constexpr (G8) {
-          p0 = __builtin_amdgcn_exp2f(fmaf(p0, kg[u], lg[u] - mb));
-          p1 = __builtin_amdgcn_exp2f(fmaf(p1, kg[u], lg[u] - mb));
+          p0 = __builtin_amdgcn_exp2f(fmaf(p0, kg[u], lm[u]));
+          p1 = __builtin_amdgcn_exp2f(fmaf(p1, kg[u], lm[u]));
           ls[u] += p0;
           ls[u] += p1;
         } else {
@@ -713,6 +733,24 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
             for (int j = 0; j < 4; j++) acc[g][j] *= alpha;
         }
         const float mb = mrun == -INFINITY ? 0.0f : mrun;
+        float lm[2][G8 ? 1 : 4];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int r = 0; r < (G8 ? 1 : 4); r++) lm[h][r] = l4[h][r] - mb;
+        if (far_scores(mt)) {
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              constexpr int one = G8 ? 0 : ~0;
+              S[h][r] = fmaf(S[h][r], k4[h][r & one], l4[h][r & one]) - mb;
+            }
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < (G8 ? 1 : 4); r++) k4[h][r] = 1.0f, lm[h][r] = 0.0f;
+        }
         half8_t pf;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -720,7 +758,7 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
 #pragma unroll
           for (int r = 0; r < 4; r++) {
             constexpr int one = G8 ? 0 : ~0;
-            const float iv = i4[h][r & one], p = __builtin_amdgcn_exp2f(fmaf(S[h][r], k4[h][r & one], l4[h][r & one] - mb));
+            const float iv = i4[h][r & one], p = __builtin_amdgcn_exp2f(fmaf(S[h][r], k4[h][r & one], lm[h][r & one]));
             pf[4 * h + r] = (hxa_h)(iv < 1.0f / HXA_Q8_LEAST ? p : p == p ? 0.0f : p);  // a page without a scale: values of 0, whatever the bytes
             l = G8 ? l + p : fmaf(p, iv, l);
           }

@@ -118,3 +118,33 @@ def test_wide_queries_beside_pages_without_a_key_scale(hip, power, hd, Hq, H, ne
     q = queries(rng, int(c.cu[-1]), Hq, hd, BF16) * 2.0 ** power
     o, bound = rows_of(c, q, hd ** -0.5)
     close(run_cached(hip, c, q, hd ** -0.5, with_ws), o, bound, "wide queries")
+
+
+LONG = [(128, 8, 4, [1, 1], [3000, 2500], 0), (64, 4, 4, [40], [2000], 0), (256, 2, 1, [1] * 3, [1500] * 3, 300), (128, 2, 2, [130], [1500], 0),
+        (128, 8, 2, [1] * 20, [700] * 20, 1000)]
+
+
+@pytest.mark.parametrize("with_ws", [True, False])
+@pytest.mark.parametrize("dtype,page", [(F16, 16), (BF16, 16), (F16, 5)])
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix", LONG)
+@pytest.mark.parametrize("power", [10, 19, 26, 40, 80])
+def test_scores_far_from_zero(hip, power, hd, Hq, H, new, past, prefix, dtype, page, with_ws):
+    """The largest score is about 2^power in powers of two and the others at most 4/5 of it, or (of the other sign) -2^power and the others 5/4 of it: the key's value and
+    nothing else. The sums of products are multiples of 2^10 below 2^25, exact; whatever is rounded after them is the key's weight, the same above and
+    below the line but for its rounding to fp16. The others' weights are 2^-190 or less."""
+    say("far scores", power, dtype, hd, page, with_ws)
+    rng = np.random.default_rng(14)
+    for sign in (1, -1):
+        c = CacheQ8(hip, rng, new, past, prefix, page, H, hd, dtype, spread=0.0)
+        c.k[:] = rng.integers(0, 101, c.k.shape) if sign > 0 else rng.integers(125, 128, c.k.shape)
+        c.v[:] = rng.integers(-127, 128, c.v.shape)
+        c.ks[:], c.vs[:] = 1.0, np.exp2(rng.uniform(-3, 3, c.vs.shape))
+        want = np.zeros((int(c.cu[-1]), Hq, hd))
+        for i, b in enumerate(c.cu[:-1]):
+            x = int(rng.integers(0, past[i] + 1))
+            pg = c.table[i, x // page]
+            c.k[pg, :, x % page] = 127 if sign > 0 else 100
+            want[b:b + new[i]] = np.repeat(c.v[pg, :, x % page] * c.vs[pg, :, None].astype(np.float64), Hq // H, 0)
+        q = np.full(want.shape, sign * 1024.0)
+        got = run_cached(hip, c, q, 2.0 ** power / (1024 * 127 * hd * np.log2(np.e)), with_ws)
+        close(got, want, (HALF_STEP[dtype] + 2.0 ** -11 + 256 * U24) * np.abs(want) + TINY[dtype], "far scores")
