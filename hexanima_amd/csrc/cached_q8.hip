@@ -2,7 +2,7 @@
 // heads of 64, 128 or 256, grouped heads, a prefix that the batch shares. Rows, work items and modes are those of causal_attn.hip.
 //
 // With k = ks qk and v = vs qv (qk, qv the bytes, ks, vs the scales of their pages), in powers of two and with c = scale log2(e):
-//   t_j = (q . qk_j) (c ks_j) + log2(vs_j),   w_j = 2^(t_j - m),   o = sum w_j qv_j / sum w_j / vs_j
+//   t_j = (q . qk_j) (c ks_j) + log2(vs_j),   w_j = 2^(t_j - m + 7),   o = sum w_j qv_j / sum w_j / vs_j
 // The values' scale is folded into the exponent, so that one running maximum m bounds what is rounded to fp16, the weight as it stands before its
 // byte: a key whose page has small values loses no bits to one whose page has large ones, and the products take the bytes as they are. A byte is exact
 // in fp16. q in bf16 becomes fp16 as it is where its row's largest magnitude is 1 .. 2^15, otherwise times the power of two that puts the largest near
@@ -14,6 +14,10 @@
 #include "int8_rows.h"
 
 namespace {
+
+// A row's weights are 2^7 times 2^(t - m), so up to 2^15 before their bytes: what fp16 keeps below 2^-14 in multiples of 2^-24 are weights below 2^-21 of
+// the largest one, in multiples of 2^-31 of it (without it 5000 keys of 2^-27 the largest one's weight are nothing).
+constexpr float LIFT = 7.0f;
 
 struct KeysQ8 : Keys<int8_t> {
   const float *ks, *vs;
@@ -422,7 +426,7 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
       float mb = mrun == -INFINITY ? 0.0f : mrun;
       if constexpr (G8) {
 #pragma unroll
-        for (int u = 0; u < 2 * NB; u++) lm[u] = lg[u] - mb;
+        for (int u = 0; u < 2 * NB; u++) lm[u] = lg[u] - (mb - LIFT);
       }
       if (far_scores(mt)) {
 #pragma unroll
@@ -430,7 +434,7 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
 #pragma unroll
           for (int r = 0; r < 16; r++) S[b][r] = (G8 ? fmaf(S[b][r], kg[2 * b + (r >> 3)], lg[2 * b + (r >> 3)]) : S[b][r]) - mb;
 #pragma unroll
-        for (int u = 0; u < 2 * NB; u++) kg[u] = 1.0f, lm[u] = 0.0f;
+        for (int u = 0; u < 2 * NB; u++) kg[u] = 1.0f, lm[u] = LIFT;
         mb = 0.0f;
       }
       half8_t pf[NB][2];
@@ -445,8 +449,8 @@ HXA_DEV void rows_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq,
           ls[u] += p1;
         } else {
           const float2_t inv = *(const float2_t *)(cst + 128 + 16 * u + (n & 7));
-          p0 = __builtin_amdgcn_exp2f(p0 - mb);
-          p1 = __builtin_amdgcn_exp2f(p1 - mb);
+          p0 = __builtin_amdgcn_exp2f(p0 - (mb - LIFT));
+          p1 = __builtin_amdgcn_exp2f(p1 - (mb - LIFT));
           ls[u] = fmaf(p1, inv[1], fmaf(p0, inv[0], ls[u]));
         }
         pf[n >> 4][u & 1][n & 7] = (hxa_h)p0;
@@ -737,7 +741,7 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int r = 0; r < (G8 ? 1 : 4); r++) lm[h][r] = l4[h][r] - mb;
+          for (int r = 0; r < (G8 ? 1 : 4); r++) lm[h][r] = l4[h][r] - (mb - LIFT);
         if (far_scores(mt)) {
 #pragma unroll
           for (int h = 0; h < 2; h++)
@@ -749,7 +753,7 @@ HXA_DEV void few_item_q8(const KeysQ8 &s, const Item &it, const T *q, long ldq, 
 #pragma unroll
           for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int r = 0; r < (G8 ? 1 : 4); r++) k4[h][r] = 1.0f, lm[h][r] = 0.0f;
+            for (int r = 0; r < (G8 ? 1 : 4); r++) k4[h][r] = 1.0f, lm[h][r] = LIFT;
         }
         half8_t pf;
 #pragma unroll

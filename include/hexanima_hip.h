@@ -365,7 +365,7 @@ int hxa_kv_append_q8(const hxa_kv_cache_q8 *c, const void *k, long ldk, const vo
 /* hxa_attention_cached over such a cache: the same rows, masks, limits, workspace rules and forms. A scale that is not finite and positive counts as 0, its
  * page's keys or values as zeros; so does a value scale of 2^-64 or less. Weights times their value scales are rounded to fp16 for the product with the
  * bytes, the sum of the weights is taken before that: beside the output's own rounding an error of 2^-11 of the weighted mean of |v| or, where that is
- * more, 2^-25 of the largest such product for each key. bf16 queries are brought to fp16: a row whose largest magnitude is 1 .. 2^15 as it is, values
+ * more, 127 2^-32 of the row's largest such product (a scale that counts as 0: 2^-64) for each key. bf16 queries are brought to fp16: a row whose largest magnitude is 1 .. 2^15 as it is, values
  * below 2^-17 rounded to multiples of 2^-24; another one by a power of two, values
  * below 2^-31 of the largest rounded alike (a row that stays below 2^-100: zeros). Value scales of pages that one
  * row sees may differ by up to 2^90. */

@@ -62,7 +62,7 @@ def rows_of(c, q, scale):
     return o, bound
 
 
-FLOOR = 2.0 ** -25
+FLOOR = 2.0 ** -32  # the largest weight of a row stands as 2^7 or more before its byte
 
 
 @pytest.mark.parametrize("with_ws", [True, False])
@@ -122,6 +122,25 @@ def test_wide_queries_beside_pages_without_a_key_scale(hip, power, hd, Hq, H, ne
 
 LONG = [(128, 8, 4, [1, 1], [3000, 2500], 0), (64, 4, 4, [40], [2000], 0), (256, 2, 1, [1] * 3, [1500] * 3, 300), (128, 2, 2, [130], [1500], 0),
         (128, 8, 2, [1] * 20, [700] * 20, 1000)]
+
+
+@pytest.mark.parametrize("with_ws", [True, False])
+@pytest.mark.parametrize("dtype,page", [(F16, 16), (BF16, 16), (F16, 5)])
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix", LONG)
+def test_a_long_tail_of_small_weights(hip, dtype, hd, Hq, H, new, past, prefix, page, with_ws):
+    """the first key, whose value is 0, has nearly all the weight; thousands behind it have 2^-27 of it each and make up the result"""
+    say("tail", dtype, hd, page, with_ws)
+    rng = np.random.default_rng(13)
+    c = CacheQ8(hip, rng, new, past, prefix, page, H, hd, dtype, spread=0.0)
+    c.k[:], c.v[:] = rng.integers(-8, 9, c.k.shape), rng.integers(64, 128, c.v.shape)
+    for pg in [c.prefix[0]] if prefix else c.table[:, 0]:
+        c.k[pg, :, 0], c.v[pg, :, 0] = 127, 0
+    c.ks[:], c.vs[:] = 1 / 127, 1.0
+    q = 1 + queries(rng, int(c.cu[-1]), Hq, hd, dtype, std=0.0)
+    scale = 27 * np.log(2) / hd
+    o, bound = rows_of(c, q, scale)
+    assert (bound < np.abs(o) / 8).mean() > 0.9
+    close(run_cached(hip, c, q, scale, with_ws), o, bound, "tail")
 
 
 @pytest.mark.parametrize("with_ws", [True, False])
