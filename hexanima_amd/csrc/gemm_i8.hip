@@ -6,8 +6,6 @@
 // Bound by the matrix cores from about a thousand rows on: 6500 x 2048 -> 16384 228 us (1.92 POP/s in 6.5 rounds of 256 x 256 tiles), 8192 cubed
 // 2.22 - 2.28 POP/s; below by the weights' bytes and a tile's chain of stages (64 x 8192 -> 2048 7.7 us, 1000 x 8192 -> 2048 24.8).
 #define HXG_INSTANTIATE
-#include <mutex>
-
 #include "gemm_kernel.h"
 
 namespace hxg {
@@ -69,9 +67,10 @@ bool built(int bm, int bn) {
     if (c.bm == bm && c.bn == bn) return true;
   return false;
 }
+long tiles_of(int n, int b) { return ((long)n + b - 1) / b; }
 int padded(int K) { return (K + 127) / 128 * 128; }
 double cost_of(const Cost &c, int M, int N, int K, int S) {
-  const long ncu = ncu_i8(), tiles = (long)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn) * S;
+  const long ncu = ncu_i8(), tiles = tiles_of(M, c.bm) * tiles_of(N, c.bn) * S;
   return (double)((tiles + ncu - 1) / ncu) * (c.a / 1048576.0 * c.bm * c.bn * (K / S) + c.b) + c.c;
 }
 Form form_of(int M, int N, int K, bool split) {
@@ -123,8 +122,8 @@ int launch(GemmParamsI8 &p, const Form &f, void *ws, hipStream_t st, const char 
   const bool split = f.ksplit > 1;
   p.Kslice = p.Ktot / f.ksplit;
   p.epi = split ? HXA_EPI_PARTIAL_F32 : HXA_EPI_STORE;
-  p.tiles_m = (p.M + f.bm - 1) / f.bm;
-  p.tiles_n = (p.N + f.bn - 1) / f.bn;
+  p.tiles_m = (int)tiles_of(p.M, f.bm);
+  p.tiles_n = (int)tiles_of(p.N, f.bn);
   const int waves = f.bn <= 32 ? f.bn == 16 ? 8 : 4 : tile_nw(f.bm, f.bn, HXG_I8);
   if ((long)p.tiles_m * p.tiles_n * 64 * waves >= 1L << 32) return hxa_set_error(HXA_E_ARG, "%s: M=%d N=%d are too many tiles", who, p.M, p.N);
   // 8 XCD rectangles of the fewest A + W bytes, as gemm_prepare's

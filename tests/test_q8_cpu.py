@@ -119,3 +119,19 @@ def test_the_tests_own_definitions():
 
 def test_linear_i8_refuses_grids_past_32_bits(hip):
     assert linear(hip, (16, 16, 1), M=1 << 27, N=8, ldo=8) == -12 and "too many tiles" in hip.last_error()
+
+
+@pytest.mark.parametrize("M,N,tiles", [
+    (2 ** 31 - 1, 8, (None, (256, 256, 1), (128, 64, 1), (64, 64, 1), (16, 16, 1))), (8, 2 ** 31 - 8, ((256, 256, 1), (64, 128, 1), (16, 16, 1))),
+    (2 ** 31 - 128, 8, ((256, 256, 1), (192, 128, 1), (16, 16, 1))), (2 ** 31 - 255, 8, ((256, 256, 1),)), (17, 2 ** 31 - 128, ((256, 256, 1),))])
+def test_linear_i8_refuses_rows_and_columns_near_2_31(hip, M, N, tiles):
+    """rounding them up to whole tiles passes 32 bits (threads: 512 a tile, 256 up to 128 x 128 and 64 columns)"""
+    for tile in tiles:
+        rc = linear(hip, tile, M=M, N=N, ldo=N)
+        assert rc == -12 and "too many tiles" in hip.last_error(), (tile, hip.last_error())
+
+
+def test_linear_i8_workspaces_of_large_products(hip):
+    """the K slices that pay for no product of many tiles, up to the largest sizes"""
+    for p in range(13, 31):
+        assert hip.lib().hxa_linear_i8_ws_bytes(2 ** p + 77, 4096, 8192) == 0 and hip.lib().hxa_linear_i8_ws_bytes(4096, 2 ** p + 8, 8192) == 0
