@@ -743,21 +743,14 @@ int hxa_attn_launch(const HxaAttn &p, hipStream_t st) {
   constexpr int LDS = LDS_BYTES + SINK_BYTES;
   constexpr int LDS6 = 6 * (66 * 64 * 4 + 8192);  // the merge and the output staging of 12 waves: more than the tiles
   static_assert(LDS6 >= LDS && LDS6 <= 160 * 1024, "LDS");
-  static bool attr = false;
-  if (!attr) {
-    const struct {
-      const void *f;
-      int lds;
-    } kerns[] = {{(const void *)attn_kernel<4, false, false>, LDS},    {(const void *)attn_kernel<4, false, true>, LDS},
-                 {(const void *)attn_kernel<4, true, false>, LDS},     {(const void *)attn_kernel<4, true, true>, LDS},
-                 {(const void *)attn_kernel<4, true, false, 1>, LDS},  {(const void *)attn_kernel<4, true, true, 1>, LDS},
-                 {(const void *)attn_kernel<2, true, false, 1>, LDS},  {(const void *)attn_kernel<2, true, true, 1>, LDS},
-                 {(const void *)attn_kernel<6, false, false, 2>, LDS6}, {(const void *)attn_kernel<6, false, true, 2>, LDS6},
-                 {(const void *)attn_short_kernel, SK_LDS}};
-    for (const auto &k : kerns)
-      if (hipFuncSetAttribute(k.f, hipFuncAttributeMaxDynamicSharedMemorySize, k.lds) != hipSuccess) return HXA_E_HIP;
-    attr = true;
-  }
+  const KernelLds kerns[] = {{(const void *)attn_kernel<4, false, false>, LDS},    {(const void *)attn_kernel<4, false, true>, LDS},
+                             {(const void *)attn_kernel<4, true, false>, LDS},     {(const void *)attn_kernel<4, true, true>, LDS},
+                             {(const void *)attn_kernel<4, true, false, 1>, LDS},  {(const void *)attn_kernel<4, true, true, 1>, LDS},
+                             {(const void *)attn_kernel<2, true, false, 1>, LDS},  {(const void *)attn_kernel<2, true, true, 1>, LDS},
+                             {(const void *)attn_kernel<6, false, false, 2>, LDS6}, {(const void *)attn_kernel<6, false, true, 2>, LDS6},
+                             {(const void *)attn_short_kernel, SK_LDS}};
+  static std::atomic<uint64_t> attr{0};
+  if (allow_lds_once(kerns, attr) != hipSuccess) return HXA_E_HIP;
   HxaAttn pk = p;
   pk.clk = g_hxa_clk_attn;
 #ifndef HXA_ATTN_SHORT

@@ -875,17 +875,10 @@ int final_launch(const float *x, int B, int T, int xrows, int D, const float *sh
     return HXA_E_ARG;
   // partial sums + statistics: 16 x 16 x 64, 16 x 16 x 128 or 8 x 16 x 256 floats (64 / 128 / 128 KB)
   auto bytes = [](int nw, int no) { return (int)sizeof(float) * (nw * FT * no + 2 * FT); };
-  static bool attr = false;
-  if (!attr) {
-    if (hipFuncSetAttribute((const void *)final_kernel<4, 16, W32>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                            bytes(16, 64)) != hipSuccess ||
-        hipFuncSetAttribute((const void *)final_kernel<8, 16, W32>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                            bytes(16, 128)) != hipSuccess ||
-        hipFuncSetAttribute((const void *)final_kernel<16, 8, W32>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                            bytes(8, 256)) != hipSuccess)
-      return HXA_E_HIP;
-    attr = true;
-  }
+  const KernelLds kerns[] = {{(const void *)final_kernel<4, 16, W32>, bytes(16, 64)}, {(const void *)final_kernel<8, 16, W32>, bytes(16, 128)},
+                             {(const void *)final_kernel<16, 8, W32>, bytes(8, 256)}};
+  static std::atomic<uint64_t> attr{0};
+  if (allow_lds_once(kerns, attr) != hipSuccess) return HXA_E_HIP;
   const int ntok = B * T;
   const dim3 grid((ntok + FT - 1) / FT);
   if (NO == 64)

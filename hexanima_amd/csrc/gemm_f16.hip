@@ -11,12 +11,9 @@ __global__ __launch_bounds__(256, 2) void gemm_xattn_kernel(GemmParams p) {
 }
 hipError_t launch_xattn(const GemmParams &p, hipStream_t st) {
   constexpr int lds = XA_LDS;
-  static bool attr = false;
-  if (!attr) {
-    const hipError_t e = hipFuncSetAttribute((const void *)gemm_xattn_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
-    attr = true;
-  }
+  static std::atomic<uint64_t> attr{0};
+  const hipError_t a = allow_lds_once((const void *)gemm_xattn_kernel, lds, attr);
+  if (a != hipSuccess) return a;
   hxa_launch(gemm_xattn_kernel, dim3(p.tiles_m * p.tiles_n), dim3(256), lds, st, p);
   return hipGetLastError();
 }

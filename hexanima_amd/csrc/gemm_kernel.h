@@ -22,7 +22,6 @@
 //  * The fp16-rounded output tile is staged through LDS for a coalesced epilogue (16-byte loads / stores).
 //  * The block index is remapped so each of the 8 XCDs (own L2) works on a rectangle of output tiles.
 #pragma once
-#include <atomic>
 #include <type_traits>
 
 #include "hxa_common.h"
@@ -1188,18 +1187,6 @@ __global__ __launch_bounds__(64 * NW) void gemm_group_kernel(const GemmParams *_
   gemm_body<BM, BN, FMT, ASYM, false, NW>(ps[blockIdx.y], blockIdx.x, 0);
 }
 
-// more than 64 KB of LDS for a kernel: allowed once a device (done: a bit for each, of the first 64)
-inline hipError_t allow_lds_once(const void *kern, int bytes, std::atomic<uint64_t> &done) {
-  int dev = 0;
-  const hipError_t d = hipGetDevice(&dev);
-  if (d != hipSuccess) return d;
-  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
-  if (done.load() & bit) return hipSuccess;
-  const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == hipSuccess) done |= bit;
-  return e;
-}
-
 // ---- launches of one weight format (explicitly instantiated in that format's translation unit) ----
 template <int BM, int BN, int FMT, bool ASYM, bool SPLIT2, int NW>
 hipError_t launch_t(const params_t<FMT> &p, int ksplit, hipStream_t st) {
@@ -1225,12 +1212,9 @@ template <int BM, int BN, int FMT, bool ASYM, int NW>
 hipError_t launch_pair_t(const GemmParams &p0, const GemmParams &p1, hipStream_t st) {
   auto kern = gemm_pair_kernel<BM, BN, FMT, ASYM, NW>;
   constexpr int lds = GemmGeo<BM, BN, FMT>::lds(GemmGeo<BM, BN, FMT>::NS);
-  static bool attr = false;
-  if (!attr) {
-    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
-    attr = true;
-  }
+  static std::atomic<uint64_t> attr{0};
+  const hipError_t a = allow_lds_once((const void *)kern, lds, attr);
+  if (a != hipSuccess) return a;
   const int n0 = p0.tiles_m * p0.tiles_n;
   hxa_launch(kern, dim3(n0 + p1.tiles_m * p1.tiles_n), dim3(64 * NW), lds, st, p0, p1, n0);
   return hipGetLastError();
@@ -1283,12 +1267,9 @@ template <int FMT, bool ASYM>
 hipError_t launch_group_fmt(const GemmParams *ps, int G, int tiles, hipStream_t st) {
   auto kern = gemm_group_kernel<192, 256, FMT, ASYM, 8>;
   constexpr int lds = GemmGeo<192, 256, FMT>::lds(GemmGeo<192, 256, FMT>::NS);
-  static bool attr = false;
-  if (!attr) {
-    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
-    attr = true;
-  }
+  static std::atomic<uint64_t> attr{0};
+  const hipError_t a = allow_lds_once((const void *)kern, lds, attr);
+  if (a != hipSuccess) return a;
   hxa_launch(kern, dim3(tiles, G), dim3(512), lds, st, ps);
   return hipGetLastError();
 }

@@ -40,6 +40,7 @@ constexpr int HXA_MAX_DEVICES = 64;
 
 // status codes, weight formats (HXA_W_*) and GEMM epilogues (HXA_EPI_*) are those of the public C-ABI
 #include "../../include/hexanima_hip.h"
+#include "lds_once.h"
 
 struct HxaWeight {
   int fmt;            // HXA_W_*
