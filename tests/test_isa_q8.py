@@ -9,3 +9,11 @@ def test_no_barrier_is_passed_with_a_read_in_flight(tmp_path):
     assert len(kernels) >= 4 + 3 + 3
     bad = {n: [r for r in _reads_at_barriers(ins) if r[1] > 0] for n, ins in kernels.items()}
     assert not {n: r for n, r in bad.items() if r}
+
+
+def test_no_barrier_is_passed_with_a_read_in_flight_in_the_other_widths(tmp_path):
+    kernels = _kernels(r"cached_q8_kernel\w*Li(64|256)E|kv_append_q8_kernel|quant_rows_kernel", str(tmp_path))
+    names = " ".join(kernels)
+    assert sum("cached_q8" in n for n in kernels) == 8 and sum("kv_append_q8" in n for n in kernels) == 18 and "quant_rows" in names
+    bad = {n: [r for r in _reads_at_barriers(ins) if r[1] > 0] for n, ins in kernels.items()}
+    assert not {n: r for n, r in bad.items() if r}
