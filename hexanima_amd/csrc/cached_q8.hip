@@ -162,7 +162,7 @@ struct PagesQ8 {
 // A tile's bytes go straight into LDS two tiles ahead (each wave its 16 keys), from there through registers, where they become fp16 once for all four
 // waves, into the tile that the products read. Pages' places and scales come from the table in LDS, as a load of them would be waited for with the keys'.
 // Bound by the conversions, which the other workgroup's products hide in part. 64 decoding tokens with 470 keys each behind a prefix of 4096 36.1 us and 32 prompts of 75
-// 57.1; with the tile ahead held in registers and converted beside K's products 37.4 and 56.7 (128 tokens behind 200 keys each 29.0, here 27.3); with
+// 57.1 (both 1% more since far scores are looked for); with the tile ahead held in registers and converted beside K's products 37.4 and 56.7 (128 tokens behind 200 keys each 29.0, here 27.3); with
 // V converted beside K's products and K beside V's 40.1 and 68.3.
 //
 // G8: eight keys of a lane (8 g + 0 .. 7 of every 16) lie on one page, so that they share its scales: the maximum is taken of the scores, the

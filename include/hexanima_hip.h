@@ -336,7 +336,7 @@ long hxa_attention_cached_ws_bytes(const hxa_kv_cache *c, int T, int Hq); /* 0: 
 int hxa_quantize_rows(int dtype, const void *x, long ldx, int M, int K, void *q, long ldq, float *scale, void *stream);
 /* Product of int8 rows: out[m][n] = sa[m] * sw[n] * (sum over k of a[m][k] * w[n][k]) + bias[n], out [M][ldo] of dtype. a [M][lda] and w [N][ldw] are
  * int8 rows that hold ceil(K / 128) 128 columns: those past K are multiplied too, so one of a and w has zeros there, as hxa_quantize_rows leaves them.
- * The sum is exact (int32); scales and bias (NULL: none) are applied in fp32, one rounding. M any (fewer than 2^23 output tiles), N % 8 == 0, K 1 .. HXA_I8_MAX_K;
+ * The sum is exact (int32); sa, then sw, then bias (NULL: none) are applied in fp32, one rounding (the sum times sa stays below 2^128). M any (fewer than 2^23 output tiles), N % 8 == 0, K 1 .. HXA_I8_MAX_K;
  * lda, ldw multiples of 16 below 2^23, ldo % 8 == 0; pointers 16-byte aligned (sa: 4). out overlaps no operand. ws: hxa_linear_i8_ws_bytes(M, N,
  * K) bytes, 16-byte aligned, for int32 partial sums where there are few output tiles; NULL or fewer bytes: one launch. The results
  * are the same bits in every form. Calls that share ws must not overlap in time, graphs' replays included. */
