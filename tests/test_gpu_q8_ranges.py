@@ -36,6 +36,8 @@ def rows_of(c, q, scale):
     n_q, Hq, hd = q.shape
     G = Hq // c.H
     o, bound = np.zeros_like(q), np.zeros_like(q)
+    pools = c.values(c.k), c.values(c.v)
+    c.values = lambda pool: pools[pool is c.v]  # once for all sequences
     for i, b in enumerate(c.cu[:-1]):
         n = c.new[i]
         if n == 0 or c.P + c.lens[i] == 0:
@@ -45,8 +47,8 @@ def rows_of(c, q, scale):
         for h in range(Hq):
             kh, vh, qh = k[:, h // G], v[:, h // G], q[b:b + n, h]
             s = np.where(seen, qh @ kh.T * scale, -np.inf)
-            p = np.exp(s - s.max(1, keepdims=True))
-            w = p / p.sum(1, keepdims=True)
+            p = np.exp(s - np.where(seen.any(1), s.max(1), 0)[:, None])
+            w = p / np.maximum(p.sum(1, keepdims=True), 1e-300)  # a row that sees nothing: zeros
             keys = seen.sum(1)[:, None]
             size = (np.where(seen, np.abs(qh) @ np.abs(kh).T, 0).max(1) * scale)[:, None]
             lmax = np.abs(np.log2(vs[:, h // G], out=np.full(len(vs), -64.0), where=vs[:, h // G] > 0)).max()
@@ -57,6 +59,7 @@ def rows_of(c, q, scale):
             o[b:b + n, h] = w @ vh
             bound[b:b + n, h] = (HALF_STEP[c.dtype] * np.abs(o[b:b + n, h]) + (2.0 ** -11 + 2 * rel) * a +
                                  keys * FLOOR * 127 * (w * np.maximum(vs[:, h // G], 2.0 ** -64)).max(1)[:, None] + TINY[c.dtype])
+    del c.values
     if c.dtype == F16:  # from 65520 on the nearest fp16 value is infinity
         o = np.where(np.abs(o) >= 65520, np.copysign(np.inf, o), o)
     return o, bound
@@ -167,3 +170,15 @@ def test_scores_far_from_zero(hip, power, hd, Hq, H, new, past, prefix, dtype, p
         q = np.full(want.shape, sign * 1024.0)
         got = run_cached(hip, c, q, 2.0 ** power / (1024 * 127 * hd * np.log2(np.e)), with_ws)
         close(got, want, (HALF_STEP[dtype] + 2.0 ** -11 + 256 * U24) * np.abs(want) + TINY[dtype], "far scores")
+
+
+@pytest.mark.parametrize("hd,Hq,H,new,past,prefix,page", [
+    (64, 80, 40, [1] * 420, [(7 * i) % 90 for i in range(420)], 300, 16), (128, 160, 40, [1, 3, 2, 0, 4] * 20, [(11 * i) % 200 for i in range(100)], 520, 64),
+    (256, 64, 32, [2] * 130, [(5 * i) % 130 for i in range(130)], 260, 5)])
+def test_large_batches_behind_a_prefix(hip, hd, Hq, H, new, past, prefix, page):
+    """the prefix's blocks are half the places of a key head and more"""
+    say("large batch", hd, Hq, len(new))
+    rng = np.random.default_rng(hd)
+    c = CacheQ8(hip, rng, new, past, prefix, page, H, hd, BF16)
+    q = queries(rng, int(c.cu[-1]), Hq, hd, BF16)
+    close(run_cached(hip, c, q, hd ** -0.5), *rows_of(c, q, hd ** -0.5), "large batch")
